@@ -1,0 +1,636 @@
+// Paged decode attention (one query token per sequence, GQA) over the 8-bit
+// KV cache on tcgen05: the cached e4m3 codes are the tensor core's operands as
+// they lie in memory, nothing is converted per cached byte.
+//
+//   S^T[128 keys, 16]  = K_tile . Q^T     (kind::f8f6f4, A = K codes, K-major)
+//   O^T[128 dims, N]   = V_tile^T . W     (A = V codes, MN-major)
+//
+// Both operands of an f8f6f4 product are 8-bit, so the bf16 query and the fp32
+// weights are split into e4m3 digits that stand in columns of their own:
+//   q * 2^s = hi + lo / 16            exact: bf16 has 8 significant bits, a
+//                                     digit 4; s brings the head's largest
+//                                     element to [2^7, 2^8)
+//   w       = hi + mid / 32 + lo / 1024  14 significant bits (bf16 has 8): each
+//                                     digit is rounded to nearest, so what is
+//                                     left of it is half a step, 5 bits further
+// The 16 columns of S hold both digits of up to 8 heads, so the split costs no
+// matrix instruction, and the N columns of O three digits of them.
+//
+// Scales (one power of two per page and head): K's multiplies a key's scores.
+// V's goes into the weight: w = 2^(s - m) * 2^6 * 2^(vsf - R), with R the
+// largest V exponent seen so far in this split and m the running maximum that
+// may lag by 2^2, so that w <= 2^8 < 448; a weight is off by at most
+// max(2^-14 w, 2^-20), 2^-26 of the largest one. The sum of the softmax takes
+// the undigited fp32 weight. When m or R grows, O^T is rescaled in TMEM.
+//
+// One CTA handles (sequence, KV head, KV split) and walks its share of the
+// sequence in tiles of 128 keys (8 pages), 32 KB for K and V:
+//   warp 0      TMA producer: lane 0 K tiles, lane 1 V tiles
+//   warp 1      MMA issuer
+//   warps 2..5  thread <-> key row for the softmax; they also stage Q
+// Pages that a sequence does not have are not loaded. V rows of the last tile
+// behind the sequence are zeroed in shared memory: a stale code there may be a
+// NaN, which a zero weight does not cancel (stale K rows only give masked
+// scores).
+// Split partials (output normalised by its own sum, LSE in log2 units) are
+// merged by a combine kernel.
+//
+// Bound by HBM: two 8-bit codes per key, dim and KV head.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "sm100.cuh"
+#include "tma_host.h"
+
+namespace ib200 {
+namespace dq8 {
+
+constexpr int D = 128;
+constexpr int BKV = 128;
+constexpr int PAGE = 16;
+constexpr int STAGES = 3;
+constexpr int BLK = 128 * 128;      // 128 rows x 128 codes
+constexpr int NS = 16;              // columns of S
+constexpr int QBLK = NS * 128;
+constexpr int NUM_THREADS = 192;
+constexpr float kLagLog2 = 2.0f;    // the running maximum may lag by this much
+constexpr int kTopLog2 = 6;         // weight of a key at the running maximum
+
+// columns of O^T: three digits of GP heads
+__host__ __device__ constexpr int cols_o(int gp) { return 3 * gp <= 16 ? 16 : 32; }
+__host__ __device__ constexpr int smem_bytes(int gp) {
+  return 1024 + STAGES * 2 * BLK + QBLK + 2 * cols_o(gp) * 128 + 1024;
+}
+constexpr uint32_t TMEM_COLS = 64;  // S0 [0,16) S1 [16,32) O [32,64)
+constexpr uint32_t O_COL = 32;
+
+struct Params {
+  const __nv_bfloat16* q;
+  int ldq;
+  const uint8_t* ksf;
+  const uint8_t* vsf;
+  int num_pages;
+  const int* block_table;
+  const int* bt_rows;
+  const int* seq_lens;
+  int max_pages, ld_table;  // places of a block-table row, and its pitch
+  int hq, hkv, G;
+  int splits;
+  int tiles_per_split;  // split s covers tiles [s * this, (s + 1) * this) of every sequence
+  float scale_log2;
+  float* o_part;    // [B, hq, splits, D]
+  float* lse_part;  // [B, hq, splits]
+  __nv_bfloat16* out;
+  int ldo;
+  int* status;
+};
+
+__device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<uint16_t>(v), __NV_E4M3)));
+}
+// byte offset of (row, byte k) in a K-major block of 128-byte rows, 128-byte swizzle
+__device__ __forceinline__ uint32_t sw_offset(int row, int k) {
+  return static_cast<uint32_t>(row * 128 + (((k >> 4) ^ (row & 7)) << 4) + (k & 15));
+}
+// The leading e4m3 digit of x, |x| <= 256: rounded to its top 4 bits, 0 where
+// that would be subnormal in e4m3 (the next digit, 32 times finer, takes it).
+__device__ __forceinline__ float digit(float x) {
+  return fabsf(x) >= 0.015625f ? __uint_as_float((__float_as_uint(x) + 0x80000u) & 0xFFF00000u) : 0.f;
+}
+
+template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
+__global__ void __launch_bounds__(NUM_THREADS, 2)
+    decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmK8, const __grid_constant__ CUtensorMap tmV8,
+                  const Params p) {
+  constexpr int NO = cols_o(GP);
+  constexpr int PBLK = NO * 128;
+  constexpr int ND = 3 * GP;            // digits of a key's weights
+  pdl_trigger();
+  pdl_wait();
+  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+  const int G = p.G;
+  int len = max(p.seq_lens[b], 0);
+  if (len > p.max_pages * PAGE) {  // more keys than the page table has places for
+    if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, b, len);
+    len = p.max_pages * PAGE;
+  }
+  const int n_tiles = (len + BKV - 1) / BKV;
+  const int t0 = split * p.tiles_per_split;
+  const int t1 = min(n_tiles, t0 + p.tiles_per_split);
+  if (t0 >= t1) {  // nothing in this split
+    if (p.splits > 1) {
+      if (threadIdx.x < G)
+        p.lse_part[(static_cast<size_t>(b) * p.hq + kvh * G + threadIdx.x) * p.splits + split] = -INFINITY;
+    } else {
+      for (int i = threadIdx.x; i < G * D; i += blockDim.x)
+        p.out[static_cast<size_t>(b) * p.ldo + kvh * G * D + i] = __float2bfloat16(0.f);
+    }
+    return;
+  }
+  const int nt = t1 - t0;
+  const int n_pages = (len + PAGE - 1) / PAGE;
+  const int* bt = p.block_table + static_cast<size_t>(p.bt_rows != nullptr ? p.bt_rows[b] : b) * p.ld_table;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sKV = smem;                        // stage s: K, V
+  uint8_t* sQ = smem + STAGES * 2 * BLK;      // rows: hi digits of GP heads, lo digits
+  uint8_t* sP = sQ + QBLK;                    // [2] rows: digit d of head h at d * GP + h
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * PBLK);
+  uint64_t* k_full = bars;
+  uint64_t* v_full = k_full + STAGES;
+  uint64_t* k_empty = v_full + STAGES;
+  uint64_t* v_empty = k_empty + STAGES;
+  uint64_t* s_full = v_empty + STAGES;        // [2]
+  uint64_t* p_full = s_full + 2;              // [2] one per P buffer
+  uint64_t* pv_done = p_full + 2;             // [2] PV of tile j commits to pv_done[j & 1]
+  uint64_t* q_ready = pv_done + 2;
+  uint64_t* grp = q_ready + 1;                // bounded barrier of the 128 softmax threads
+  uint64_t* drain = grp + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* red = reinterpret_cast<float*>(tmem_slot + 4);     // [2][4][GP] tile maxima
+  int* redv = reinterpret_cast<int*>(red + 2 * 4 * GP);     // [2][4] V exponents
+  float* lred = reinterpret_cast<float*>(redv + 8);         // [4][GP]
+  float* qsc = lred + 4 * GP;                               // [GP] scale_log2 * 2^-s
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_ready, 128);
+    mbar_init(grp, 128);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmK8);
+    tma_prefetch_desc(&tmV8);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane < 2) {
+      const bool is_v = lane == 1;
+      const CUtensorMap* tm1 = is_v ? &tmV : &tmK;
+      const CUtensorMap* tm8 = is_v ? &tmV8 : &tmK8;
+      uint64_t* full = is_v ? v_full : k_full;
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      uint8_t* dst0 = sKV + (is_v ? BLK : 0);
+      const uint64_t pol = policy_evict_first();
+      int issued = 0;
+      int nxt[8];
+      load_tile_pages(bt, t0, n_pages, nxt);
+      for (int j = 0; j < nt; ++j) {
+        const int st = j % STAGES;
+        int cur[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cur[i] = nxt[i];
+        if (j + 1 < nt) load_tile_pages(bt, t0 + j + 1, n_pages, nxt);  // in flight while we wait
+        if (!mbar_wait(&empty[st], static_cast<uint32_t>(((j / STAGES) & 1) ^ 1), abort_flag, p.status,
+                       kStatusTimeoutEmpty))
+          break;
+        uint8_t* dst = dst0 + st * 2 * BLK;
+        // eight consecutive pages are one 128-row box (the swizzle repeats
+        // every 8 rows: the same image as eight page boxes)
+        bool run = true;
+#pragma unroll
+        for (int pg = 1; pg < BKV / PAGE; ++pg) run = run && cur[pg] == cur[0] + pg;
+        const int n = min(BKV / PAGE, n_pages - (t0 + j) * (BKV / PAGE));  // pages that the sequence has here
+        mbar_expect_tx(&full[st], n * PAGE * 128);
+        if (run && n == BKV / PAGE) {
+          tma_load_2d(dst, tm8, &full[st], kvh * D, cur[0] * PAGE, pol);
+        } else {
+#pragma unroll
+          for (int pg = 0; pg < BKV / PAGE; ++pg)
+            if (pg < n) tma_load_2d(dst + pg * PAGE * 128, tm1, &full[st], kvh * D, cur[pg] * PAGE, pol);
+        }
+        ++issued;
+      }
+      for (int i = max(0, issued - STAGES); i < issued; ++i)
+        mbar_wait(&full[i % STAGES], static_cast<uint32_t>((i / STAGES) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc_s = make_idesc_e4m3(128, NS);
+      const uint32_t idesc_o = make_idesc_e4m3(128, NO) | (1u << 15);  // A = V^T, MN-major
+      const uint32_t q_addr = smem_u32(sQ);
+      const uint32_t p_addr = smem_u32(sP);
+      bool ok = mbar_wait(q_ready, 0, abort_flag, p.status, kStatusTimeoutFull);
+      tc_fence_after();
+      auto issue_pv = [&](int jj) -> bool {
+        const int st = jj % STAGES;
+        if (!mbar_wait(&p_full[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
+                       kStatusTimeoutTmemEmpty))
+          return false;
+        if (!mbar_wait(&v_full[st], static_cast<uint32_t>((jj / STAGES) & 1), abort_flag, p.status,
+                       kStatusTimeoutFull))
+          return false;
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(sKV + st * 2 * BLK + BLK);
+        const uint32_t pb = p_addr + static_cast<uint32_t>((jj & 1) * PBLK);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          // 32 keys: four groups of 8 rows, 1024 bytes apart (the stride);
+          // all 128 dims are one 128-byte row, so the leading offset is unused
+          const uint64_t ad = make_sw128_desc(v_addr + s * 4096, BLK, 1024);
+          const uint64_t bd = make_sw128_desc(pb + s * 32, 16, 1024);
+          umma_e4m3(tmem + O_COL, ad, bd, idesc_o, (jj > 0 || s > 0) ? 1u : 0u);
+        }
+        umma_commit(&pv_done[jj & 1]);
+        umma_commit(&v_empty[st]);
+        return true;
+      };
+      for (int j = 0; j < nt && ok; ++j) {
+        const int st = j % STAGES;
+        if (!mbar_wait(&k_full[st], static_cast<uint32_t>((j / STAGES) & 1), abort_flag, p.status,
+                       kStatusTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sKV + st * 2 * BLK);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          umma_e4m3(tmem + ((j & 1) ? NS : 0), make_sw128_desc(k_addr + s * 32, 16, 1024),
+                    make_sw128_desc(q_addr + s * 32, 16, 1024), idesc_s, s > 0 ? 1u : 0u);
+        umma_commit(&s_full[j & 1]);
+        umma_commit(&k_empty[st]);
+        if (j > 0 && !issue_pv(j - 1)) {
+          ok = false;
+          break;
+        }
+      }
+      if (ok) issue_pv(nt - 1);
+      umma_commit(drain);
+      mbar_wait(drain, 0, nullptr, p.status, kStatusTimeoutFull);
+    }
+  } else {
+    const int t = threadIdx.x - 64;   // 0..127
+    const int q4 = warp & 3;
+    const int r = q4 * 32 + lane;     // key row of S, dim row of O
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    uint32_t gph = 0;
+    bool ok = true;
+    auto group_sync = [&]() {
+      mbar_arrive(grp);
+      ok = mbar_wait_warp(grp, gph & 1u, abort_flag, p.status, kStatusTimeoutTmemFull) && ok;
+      ++gph;
+    };
+    // exponents of this row's page; a page id outside the cache (bad table)
+    // loads zeros through the tensor map and takes the smallest exponent here
+    auto page_of = [&](int j) -> int {
+      const int lp = (t0 + j) * (BKV / PAGE) + (r >> 4);
+      return lp < n_pages ? __ldg(bt + lp) : -1;
+    };
+    auto load_sf = [&](int page, int& ke, int& ve) {
+      const bool in = page >= 0 && page < p.num_pages;
+      const size_t at = static_cast<size_t>(in ? page : 0) * p.hkv + kvh;
+      ke = in ? p.ksf[at] : 1;
+      ve = in ? p.vsf[at] : 1;
+    };
+    int ke_n, ve_n;                   // of the next tile
+    int page_n2 = page_of(0);         // of the one after it
+    load_sf(page_n2, ke_n, ve_n);
+    page_n2 = nt > 1 ? page_of(1) : -1;
+
+    // stage Q: unused rows of Q and P are zero
+    for (int i = t; i < (QBLK + 2 * PBLK) / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    group_sync();
+    for (int h = q4; h < G; h += 4) {
+      const uint32_t* src =
+          reinterpret_cast<const uint32_t*>(p.q + static_cast<size_t>(b) * p.ldq + (kvh * G + h) * D) + lane * 2;
+      const uint32_t u0 = src[0], u1 = src[1];
+      float x[4] = {bf16_lo(u0), bf16_hi(u0), bf16_lo(u1), bf16_hi(u1)};
+      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+      const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+      const int s = min(100, 134 - static_cast<int>(mb >> 23));
+      const float f = two_to(s);
+      float hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) <= 3.4e38f ? x[i] * f : NAN;
+      const uint32_t h01 = to_e4m3x2(x[0], x[1]), h23 = to_e4m3x2(x[2], x[3]);
+      const float2 a = from_e4m3x2(h01), c = from_e4m3x2(h23);
+      hi[0] = a.x, hi[1] = a.y, hi[2] = c.x, hi[3] = c.y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lo[i] = (x[i] - hi[i]) * 16.f;
+      *reinterpret_cast<uint32_t*>(sQ + sw_offset(h, lane * 4)) = h01 | (h23 << 16);
+      *reinterpret_cast<uint32_t*>(sQ + sw_offset(GP + h, lane * 4)) =
+          to_e4m3x2(lo[0], lo[1]) | (to_e4m3x2(lo[2], lo[3]) << 16);
+      if (lane == 0) qsc[h] = p.scale_log2 * two_to(-s);
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_ready);
+    group_sync();  // qsc
+
+    float m_run[GP], l_part[GP], c_h[GP];
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      m_run[h] = -INFINITY;
+      l_part[h] = 0.f;
+      c_h[h] = h < G ? qsc[h] : 0.f;
+    }
+    int R = 0;  // largest V exponent so far
+    // the PV of tile jj has completed: its commit is completion (jj >> 1) + 1
+    // of pv_done[jj & 1], and no later PV on that barrier can have been issued
+    auto wait_pv = [&](int jj) -> bool {
+      if (!mbar_wait_warp(&pv_done[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
+                          kStatusTimeoutTmemFull))
+        return false;
+      tc_fence_after();
+      return true;
+    };
+    for (int j = 0; j < nt && ok; ++j) {
+      const int ke = ke_n, ve = ve_n;
+      if (j + 1 < nt) {
+        load_sf(page_n2, ke_n, ve_n);
+        page_n2 = j + 2 < nt ? page_of(j + 2) : -1;
+      }
+      if (!mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
+                          kStatusTimeoutTmemFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sv[16];
+      tmem_ld16(lane_addr + ((j & 1) ? NS : 0), sv);
+      tmem_ld_wait();
+      const int key = (t0 + j) * BKV + r;
+      const bool valid = key < len;
+      const float kf = two_to(max(ke, 1) - 127);
+      float s[GP];
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        const float raw = fmaf(__uint_as_float(sv[GP + h]), 0.0625f, __uint_as_float(sv[h]));
+        s[h] = valid && h < G ? raw * (c_h[h] * kf) : -INFINITY;
+        float mx = s[h];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (lane == 0) red[((j & 1) * 4 + q4) * GP + h] = mx;
+      }
+      const int vmax = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(valid ? max(ve, 1) : 1)));
+      if (lane == 0) redv[(j & 1) * 4 + q4] = vmax;
+      group_sync();
+      if (!ok) break;
+      // every thread derives the same maxima, so the decision is uniform over the CTA
+      const int* rv = redv + (j & 1) * 4;
+      const int tile_v = max(max(rv[0], rv[1]), max(rv[2], rv[3]));
+      float alpha[GP];
+      bool rescale = false;
+      float fR = 1.f;
+      if (tile_v > R) {
+        if (R > 0) {
+          fR = two_to(max(R - tile_v, -126));
+          rescale = true;
+        }
+        R = tile_v;
+      }
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        const float* rr = red + (j & 1) * 4 * GP;
+        const float tmax = fmaxf(fmaxf(rr[h], rr[GP + h]), fmaxf(rr[2 * GP + h], rr[3 * GP + h]));
+        alpha[h] = 1.f;
+        if (m_run[h] == -INFINITY) {
+          m_run[h] = tmax;  // nothing accumulated yet
+        } else if (tmax > m_run[h] + kLagLog2) {
+          alpha[h] = exp2f(m_run[h] - tmax);
+          m_run[h] = tmax;
+          rescale = true;
+        }
+      }
+      if (rescale && j > 0) {
+        if (!wait_pv(j - 1)) {
+          ok = false;
+          break;
+        }
+        uint32_t ov[NO];
+        if constexpr (NO == 16)
+          tmem_ld16(lane_addr + O_COL, ov);
+        else
+          tmem_ld32(lane_addr + O_COL, ov);
+        tmem_ld_wait();
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+          ov[n] = __float_as_uint(__uint_as_float(ov[n]) * (alpha[n % GP] * fR));
+        if constexpr (NO == 16)
+          tmem_st16(lane_addr + O_COL, ov);
+        else
+          tmem_st32(lane_addr + O_COL, ov);
+        tmem_st_wait();
+      }
+      float dg[ND + 1];
+      dg[ND] = 0.f;
+      const float vf = two_to(max(kTopLog2 + max(ve, 1) - R, -126));
+#pragma unroll
+      for (int h = 0; h < GP; ++h) {
+        // a head whose every key scored -inf has no maximum yet
+        const float pw = s[h] == -INFINITY ? 0.f : exp2f(s[h] - (m_run[h] == -INFINITY ? 0.f : m_run[h]));
+        l_part[h] = l_part[h] * alpha[h] + pw;
+        const float w = valid ? pw * vf : 0.f;
+        dg[h] = digit(w);
+        const float w1 = (w - dg[h]) * 32.f;
+        dg[GP + h] = digit(w1);
+        dg[2 * GP + h] = (w1 - dg[GP + h]) * 32.f;
+      }
+      // P buffer j & 1 was last read by the PV of tile j - 2
+      if (j >= 2 && !wait_pv(j - 2)) {
+        ok = false;
+        break;
+      }
+      uint8_t* pbuf = sP + (j & 1) * PBLK;
+#pragma unroll
+      for (int n = 0; n < ND; n += 2) {
+        const uint32_t u = to_e4m3x2(dg[n], dg[n + 1]);
+        pbuf[sw_offset(n, r)] = static_cast<uint8_t>(u);
+        if (n + 1 < ND) pbuf[sw_offset(n + 1, r)] = static_cast<uint8_t>(u >> 8);
+      }
+      if ((t0 + j + 1) * BKV > len) {
+        // the last tile: no stale V code behind the sequence reaches the product
+        const int st = j % STAGES;
+        if (!mbar_wait_warp(&v_full[st], static_cast<uint32_t>((j / STAGES) & 1), abort_flag, p.status,
+                            kStatusTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        if (!valid) {
+          uint4* row = reinterpret_cast<uint4*>(sKV + st * 2 * BLK + BLK + r * 128);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) row[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      mbar_arrive(&p_full[j & 1]);
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    uint32_t ov[NO];
+#pragma unroll
+    for (int n = 0; n < NO; ++n) ov[n] = 0u;
+    if (ok && wait_pv(nt - 1)) {
+      if constexpr (NO == 16)
+        tmem_ld16(lane_addr + O_COL, ov);
+      else
+        tmem_ld32(lane_addr + O_COL, ov);
+      tmem_ld_wait();
+    }
+    // sum of the softmax: the per-key partials over the 128 rows
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      float v = l_part[h];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) lred[q4 * GP + h] = v;
+    }
+    group_sync();
+    const float back = two_to(max(R, 1) - 127) * (1.f / (1 << kTopLog2));
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      if (h >= G || !ok) break;
+      const float l = lred[h] + lred[GP + h] + lred[2 * GP + h] + lred[3 * GP + h];
+      const float acc = fmaf(fmaf(__uint_as_float(ov[2 * GP + h]), 0.03125f, __uint_as_float(ov[GP + h])), 0.03125f,
+                             __uint_as_float(ov[h]));
+      const float o = l == 0.f ? 0.f : acc / l * back;
+      const int head = kvh * G + h;
+      if (p.splits == 1) {
+        p.out[static_cast<size_t>(b) * p.ldo + head * D + r] = __float2bfloat16(o);
+      } else {
+        const size_t slot = (static_cast<size_t>(b) * p.hq + head) * p.splits + split;
+        p.o_part[slot * D + r] = o;
+        if (r == 0) p.lse_part[slot] = l == 0.f ? -INFINITY : m_run[h] + log2f(l);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M); a NaN in a share stays one
+__global__ void __launch_bounds__(D) combine_kernel(const Params p) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+  const size_t base = (static_cast<size_t>(b) * p.hq + h) * p.splits;
+  float mx = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.lse_part[base + s]);
+  if (mx == -INFINITY) mx = 0.f;
+  float num = 0.f, den = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float lse = p.lse_part[base + s];
+    if (lse == -INFINITY) continue;
+    const float w = exp2f(lse - mx);
+    den += w;
+    num += p.o_part[(base + s) * D + d] * w;
+  }
+  p.out[static_cast<size_t>(b) * p.ldo + h * D + d] = __float2bfloat16(den == 0.f ? 0.f : num / den);
+}
+
+using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const Params);
+
+}  // namespace dq8
+}  // namespace ib200
+
+using namespace ib200;
+
+// q [B, ldq] bf16 (head h at columns h*128); kq / vq e4m3 [num_slots, hkv*128]
+// and ksf / vsf [num_slots/16, hkv]; block_table rows of max_pages places
+// (pitch ld_table), row bt_rows[b] (null: b); split s covers the 128-key tiles
+// [s*tiles_per_split, (s+1)*tiles_per_split) of every sequence
+// (splits*tiles_per_split*128 must cover the longest one); o_part / lse_part:
+// fp32 [B*hq*splits*128] / [B*hq*splits], only touched when splits > 1.
+extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const void* ksf, const void* vq,
+                                  const void* vsf, long long num_slots, const int* block_table, const int* bt_rows,
+                                  const int* seq_lens, int max_pages, int ld_table, int B, int hq, int hkv,
+                                  int splits, int tiles_per_split, float scale, float* o_part, float* lse_part, void* out,
+                                  int ldo, int* status, cudaStream_t stream) {
+  using namespace ib200::dq8;
+  if (B <= 0) return 0;
+  if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 8 || splits < 1 || tiles_per_split < 1 || (ldq % 2) != 0 ||
+      B > 65535 || splits > 65535 || num_slots < PAGE || num_slots % PAGE != 0 || max_pages < 0 ||
+      (reinterpret_cast<uintptr_t>(q) & 3) != 0)
+    return -1;
+  if (splits > 1 && (o_part == nullptr || lse_part == nullptr)) return -1;
+  const int kvw = hkv * D;
+  CUtensorMap tk, tv, tk8, tv8;
+  const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  if (!cached_tmap_2d(&tk, kq, u8, 1, num_slots, kvw, kvw, 16, 128)) return -2;
+  if (!cached_tmap_2d(&tv, vq, u8, 1, num_slots, kvw, kvw, 16, 128)) return -2;
+  if (!cached_tmap_2d(&tk8, kq, u8, 1, num_slots, kvw, kvw, 128, 128)) return -2;
+  if (!cached_tmap_2d(&tv8, vq, u8, 1, num_slots, kvw, kvw, 128, 128)) return -2;
+  Params p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.ldq = ldq;
+  p.ksf = static_cast<const uint8_t*>(ksf);
+  p.vsf = static_cast<const uint8_t*>(vsf);
+  p.num_pages = static_cast<int>(num_slots / PAGE);
+  p.block_table = block_table;
+  p.bt_rows = bt_rows;
+  p.seq_lens = seq_lens;
+  p.max_pages = max_pages;
+  p.ld_table = ld_table;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.G = hq / hkv;
+  p.splits = splits;
+  p.tiles_per_split = tiles_per_split;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.o_part = o_part;
+  p.lse_part = lse_part;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ldo = ldo;
+  p.status = status;
+  const int gp = p.G <= 1 ? 1 : (p.G <= 2 ? 2 : (p.G <= 4 ? 4 : 8));
+  const Kernel k = gp == 1 ? decode_kernel<1> : (gp == 2 ? decode_kernel<2> : (gp == 4 ? decode_kernel<4> : decode_kernel<8>));
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    cudaFuncSetAttribute(decode_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(1));
+    cudaFuncSetAttribute(decode_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(2));
+    cudaFuncSetAttribute(decode_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(4));
+    cudaFuncSetAttribute(decode_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(8));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  launch_pdl(k, dim3(hkv, B, splits), NUM_THREADS, smem_bytes(gp), stream, tk, tv, tk8, tv8, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (splits > 1) {
+    launch_pdl(combine_kernel, dim3(B, hq), D, 0, stream, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  return 0;
+}

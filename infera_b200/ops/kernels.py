@@ -345,7 +345,14 @@ def rope_cos_sin(max_pos: int, head_dim: int, theta: float, scaling: dict | None
 def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_sin: torch.Tensor, hq: int,
                  hkv: int, head_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
     """Rotate q/k of ``qkv`` in place and store k, v at ``slots`` of the
-    caches ([num_slots, hkv*head_dim]); slot -1 skips the store."""
+    caches ([num_slots, hkv*head_dim]); slot -1 skips the store. With 8-bit
+    caches (:class:`infera_b200.ops.kv8.KV8Cache`) only q is rotated in
+    place (:func:`infera_b200.ops.kv8.rope_kvwrite`)."""
+    if not isinstance(k_cache, torch.Tensor):
+        from infera_b200.ops import kv8
+
+        kv8.rope_kvwrite(qkv, pos, slots, cos_sin, hq, hkv, head_dim, k_cache, v_cache)
+        return
     T = qkv.shape[0]
     if not qkv.is_cuda:
         half = head_dim // 2
@@ -526,7 +533,13 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     ``tiles_per_split`` > 0: split s covers 128-key tiles [s*T, (s+1)*T) of
     every sequence (``splits * T * 128`` must cover the longest), so CTAs
     reading a shared prefix run together; ``l2_policy`` 0/1/2: K/V loads
-    evict_first / evict_normal / evict_last."""
+    evict_first / evict_normal / evict_last. 8-bit caches go to
+    :func:`infera_b200.ops.kv8.attn_decode`."""
+    if not isinstance(k_cache, torch.Tensor):
+        from infera_b200.ops import kv8
+
+        return kv8.attn_decode(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, splits=splits, out=out,
+                               bt_rows=bt_rows, tiles_per_split=tiles_per_split)
     B = seq_lens.shape[0]
     D = k_cache.shape[1] // hkv
     if not q.is_cuda:
@@ -612,7 +625,13 @@ def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     tiles: int32 [num_tiles, 2] from :func:`prefill_tiles` with the same
     ``tile_rows`` (None: ``PREFILL_TILE_ROWS``). ``kv_splits``: key shares
     per tile (None: :func:`prefill_kv_splits` from ``host_meta``, 1 without
-    it)."""
+    it). 8-bit caches go to :func:`infera_b200.ops.kv8.attn_prefill`."""
+    if not isinstance(k_cache, torch.Tensor):
+        from infera_b200.ops import kv8
+
+        return kv8.attn_prefill(q, k_cache, v_cache, block_table, q_start, q_len, ctx_len, tiles, hq, hkv, scale,
+                                out=out, host_meta=host_meta, bt_rows=bt_rows, kv_splits=kv_splits,
+                                tile_rows=tile_rows)
     T = q.shape[0]
     D = k_cache.shape[1] // hkv
     if not q.is_cuda:

@@ -1,0 +1,381 @@
+"""An 8-bit paged KV cache and the attention that reads it.
+
+One channel (K or V) of a layer holds
+
+* ``q``  [slots, hkv*128] float8_e4m3fn, slot = page*16 + offset, and
+* ``sf`` [slots/16, hkv] uint8: one scale 2^(sf-127) for each page of 16
+  tokens and KV head (0 counts as 1, so a zeroed cache holds zeros).
+
+A key or value element is ``q * 2^(sf-127)``: half the bytes of the bf16 cache
+plus 1/2048 for the scales. A power of two keeps both conversions exact: a
+page whose scale grows keeps its codes' values (only codes that become
+subnormal round again), and code times scale is exact in bf16.
+
+* :func:`rope_kvwrite` rotates q, and writes k (rotated) and v of an engine
+  step's rows. A page's scale is the smallest that holds every finite value
+  of the rows written to it (largest code 448). Writing a page's first slot
+  starts the page anew: its scale comes from this call's rows alone, and its
+  other slots hold nothing until they are written. Any other write keeps at
+  least the page's scale and brings the page's other rows to a grown one.
+  An infinity or a NaN is stored as NaN. Two rows with the same slot: the
+  later one stays.
+* :func:`attn_decode` attends with one query token per sequence.
+* :func:`attn_prefill` attends causally with chunks of new tokens.
+
+:mod:`infera_b200.ops.kernels`'s ``rope_kvwrite``, ``attn_decode`` and
+``attn_prefill`` come here for :class:`KV8Cache` caches. On CPU every
+function computes the same values with PyTorch in fp32.
+
+Reference counterpart: the reference's engines serve with fp8 KV caches
+(their stock workers' default); the kernels are not in its tree.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from infera_b200.ops import _native
+from infera_b200.ops import kernels as K
+
+E4M3_MAX = 448.0
+PAGE = 16
+HEAD_DIM = 128
+
+
+@dataclass
+class KV8Cache:
+    """One channel (K or V) of one layer, or of all layers with a leading dimension."""
+
+    q: torch.Tensor   # [(layers,) slots, hkv*128] float8_e4m3fn
+    sf: torch.Tensor  # [(layers,) slots/16, hkv] uint8
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.q.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.q.is_cuda
+
+    @property
+    def nbytes(self) -> int:
+        return self.q.numel() + self.sf.numel()
+
+    def __getitem__(self, layer: int) -> "KV8Cache":
+        return KV8Cache(self.q[layer], self.sf[layer])
+
+    def to(self, device) -> "KV8Cache":
+        return KV8Cache(self.q.to(device), self.sf.to(device))
+
+    def dequant(self) -> torch.Tensor:
+        """fp32 [.., slots, hkv*128]."""
+        s = _pow2(self.sf.to(torch.int32).clamp_min(1) - 127)
+        x = self.q.float().unflatten(-1, (self.sf.shape[-1], -1)).unflatten(-3, (-1, PAGE))
+        return (x * s[..., :, None, :, None]).flatten(-4, -3).flatten(-2)
+
+
+def alloc(slots: int, hkv: int, layers: int | None = None, device: torch.device | str = "cuda") -> KV8Cache:
+    """One zeroed channel of ``slots`` slots (a multiple of 16) and ``hkv`` heads of 128."""
+    if slots < PAGE or slots % PAGE or hkv < 1:
+        raise ValueError(f"{slots} slots x {hkv} heads: whole pages of {PAGE} slots and at least one head")
+    lead = () if layers is None else (layers,)
+    return KV8Cache(torch.zeros(*lead, slots, hkv * HEAD_DIM, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                    torch.zeros(*lead, slots // PAGE, hkv, dtype=torch.uint8, device=device))
+
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32, e a whole number in [-126, 127], from its bits."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _scale_exp(amax: torch.Tensor) -> torch.Tensor:
+    """Smallest biased exponent e in [1, 254] with amax <= 448 * 2^(e-127)."""
+    m, e = torch.frexp(amax.double() / E4M3_MAX)
+    e = torch.where(m == 0.5, e - 1, e) + 127
+    return torch.where(amax > 0, e, torch.ones_like(e)).clamp(1, 254).to(torch.int32)
+
+
+# ---------------------------------------------------------------- checks
+
+
+def _check_cache(name: str, c: KV8Cache, hkv: int, dev: torch.device) -> None:
+    if not isinstance(c, KV8Cache):
+        raise TypeError(f"{name} is a {type(c).__name__}, not a KV8Cache (K and V are both 8-bit, or neither)")
+    if c.q.dim() != 2 or c.q.dtype != torch.float8_e4m3fn or c.sf.dtype != torch.uint8:
+        raise ValueError(f"{name}: one layer's e4m3 codes [slots, hkv*128] and uint8 scales, not "
+                         f"{tuple(c.q.shape)} {c.q.dtype} / {c.sf.dtype}")
+    slots = c.q.shape[0]
+    if slots % PAGE or c.q.shape[1] != hkv * HEAD_DIM or tuple(c.sf.shape) != (slots // PAGE, hkv):
+        raise ValueError(f"{name}: codes {tuple(c.q.shape)} and scales {tuple(c.sf.shape)} do not hold whole pages "
+                         f"of {PAGE} slots with {hkv} heads of {HEAD_DIM}")
+    if not (c.q.is_contiguous() and c.sf.is_contiguous()):
+        raise ValueError(f"{name}: the cache has to be contiguous")
+    _check_dev(name, c.q, dev)
+    _check_dev(name, c.sf, dev)
+
+
+def _check_dev(name: str, t: torch.Tensor, dev: torch.device) -> None:
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the queries on {dev}")
+
+
+def _check_i32(name: str, t: torch.Tensor, n: int | None, dev: torch.device) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name}: a contiguous int32 vector{'' if n is None else f' of {n}'}, not "
+                         f"{tuple(t.shape)} {t.dtype}")
+    _check_dev(name, t, dev)
+
+
+def _check_heads(hq: int, hkv: int, most: int) -> None:
+    if hkv < 1 or hq < 1 or hq % hkv or hq // hkv > most:
+        raise ValueError(f"{hq} query heads over {hkv} KV heads: a whole number of at most {most} to one")
+
+
+def _check_rows(name: str, t: torch.Tensor, width: int) -> None:
+    if t.dim() != 2 or t.dtype != torch.bfloat16 or t.shape[1] < width or (t.shape[0] and t.stride(1) != 1):
+        raise ValueError(f"{name}: bf16 rows of at least {width} adjacent elements, not {tuple(t.shape)} {t.dtype}, "
+                         f"strides {t.stride()}")
+
+
+def _check_aligned(name: str, t: torch.Tensor, nbytes: int) -> None:
+    if t.is_cuda and (t.data_ptr() % nbytes or (t.shape[0] > 1 and t.stride(0) * t.element_size() % nbytes)):
+        raise ValueError(f"{name}: rows have to start on multiples of {nbytes} bytes")
+
+
+def _check_table(block_table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev: torch.device) -> None:
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise ValueError("block_table: int32 [rows, pages] with adjacent pages")
+    _check_dev("block_table", block_table, dev)
+    if bt_rows is not None:
+        _check_i32("bt_rows", bt_rows, n, dev)
+    elif block_table.shape[0] < n:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {n} sequences")
+
+
+# ---------------------------------------------------------------- append
+
+
+def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_sin: torch.Tensor, hq: int,
+                 hkv: int, head_dim: int, k_cache: KV8Cache, v_cache: KV8Cache,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate the q heads of ``qkv`` [T, >=(hq+2*hkv)*128] (bf16; q, k, v side
+    by side) into ``q_out`` [T, >=hq*128] (None: in place) and append the rotated
+    k and the v to the caches at ``slots`` (int32; -1: not stored). ``qkv``'s
+    k and v are left as they are. Returns ``q_out``."""
+    if head_dim != HEAD_DIM:
+        raise ValueError(f"head_dim {head_dim}: the 8-bit cache holds heads of {HEAD_DIM}")
+    _check_heads(hq, hkv, hq)
+    _check_rows("qkv", qkv, (hq + 2 * hkv) * HEAD_DIM)
+    if q_out is None:
+        q_out = qkv
+    _check_rows("q_out", q_out, hq * HEAD_DIM)
+    T, dev = qkv.shape[0], qkv.device
+    if q_out.shape[0] < T:
+        raise ValueError(f"q_out has {q_out.shape[0]} rows for {T}")
+    _check_dev("q_out", q_out, dev)
+    _check_i32("pos", pos, T, dev)
+    _check_i32("slots", slots, T, dev)
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or tuple(cos_sin.shape[1:]) != (HEAD_DIM // 2, 2) \
+            or not cos_sin.is_contiguous():
+        raise ValueError(f"cos_sin: contiguous fp32 [positions, {HEAD_DIM // 2}, 2]")
+    _check_dev("cos_sin", cos_sin, dev)
+    _check_cache("k_cache", k_cache, hkv, dev)
+    _check_cache("v_cache", v_cache, hkv, dev)
+    if k_cache.q.shape != v_cache.q.shape:
+        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+    if T == 0:
+        return q_out
+    if not qkv.is_cuda:
+        _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out)
+        return q_out
+    _check_aligned("qkv", qkv, 16)
+    _check_aligned("q_out", q_out, 16)
+    _check_aligned("cos_sin", cos_sin, 16)
+    rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, qkv.stride(0), q_out.data_ptr(), q_out.stride(0),
+                                         pos.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), hq, hkv,
+                                         k_cache.q.data_ptr(), k_cache.sf.data_ptr(), v_cache.q.data_ptr(),
+                                         v_cache.sf.data_ptr(), k_cache.q.shape[0], cos_sin.shape[0],
+                                         K.scratch(dev).status.data_ptr(), K._stream())
+    _native.check(rc, "ib_kv8_append")
+    K._count()
+    return q_out
+
+
+def _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out) -> None:
+    T, half = qkv.shape[0], HEAD_DIM // 2
+    ok = (pos >= 0) & (pos < cos_sin.shape[0])
+    cs = cos_sin[pos.long().clamp(0, cos_sin.shape[0] - 1)][:, None]
+    c, s = cs[..., 0], cs[..., 1]
+    x = qkv[:, : (hq + 2 * hkv) * HEAD_DIM].float().view(T, hq + 2 * hkv, HEAD_DIM)
+    a, b = x[:, : hq + hkv, :half], x[:, : hq + hkv, half:]
+    rot = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+    q_out[:T, : hq * HEAD_DIM][ok] = rot[:, :hq].to(qkv.dtype).reshape(T, -1)[ok]
+    live = ok & (slots >= 0) & (slots < k_cache.q.shape[0])
+    for cache, rows in ((k_cache, rot[:, hq:]), (v_cache, x[:, hq + hkv:])):
+        codes = cache.q.view(-1, PAGE, hkv, HEAD_DIM)
+        on: dict[int, dict[int, int]] = {}
+        for t in torch.nonzero(live).flatten().tolist():
+            on.setdefault(int(slots[t]) // PAGE, {})[int(slots[t]) % PAGE] = t
+        for page, at in on.items():
+            offs = list(at)
+            new = rows[list(at.values())]
+            new = torch.where(new.isfinite(), new, float("nan"))
+            e = _scale_exp(torch.nan_to_num(new, nan=0.0).abs().amax(dim=(0, 2)))
+            if 0 not in at:
+                old = cache.sf[page].to(torch.int32)
+                e = torch.maximum(e, old)
+                shift = _pow2((old - e).clamp_min(-60))
+                codes[page] = (codes[page].float() * shift[None, :, None]).to(torch.float8_e4m3fn)
+            codes[page, offs] = (new * _pow2(127 - e)[None, :, None]).to(torch.float8_e4m3fn)
+            cache.sf[page] = e.to(torch.uint8)
+
+
+# ---------------------------------------------------------------- decode attention
+
+
+def decode_plan(batch: int, hkv: int, max_len: int, num_sms: int = 148) -> tuple[int, int]:
+    """(splits, 128-key tiles per split) of :func:`attn_decode` for ``batch``
+    sequences whose longest has ``max_len`` keys."""
+    tiles = max(1, -(-max_len // 128))
+    tps = min(16, max(1, -(-batch * hkv * tiles // (2 * num_sms))))
+    return -(-tiles // tps), tps
+
+
+def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, hq: int, hkv: int, scale: float, splits: int = 1,
+                out: torch.Tensor | None = None, bt_rows: torch.Tensor | None = None,
+                tiles_per_split: int = 0) -> torch.Tensor:
+    """Single-token attention per sequence over the 8-bit cache. q: [B,
+    >=hq*128] bf16 (row stride free), seq_lens: int32 [B] (keys including the
+    current token; 0 gives a row of zeros). Up to 8 query heads per KV head.
+
+    ``splits`` and ``tiles_per_split`` come from :func:`decode_plan`: split s
+    covers the 128-key tiles [s*T, (s+1)*T) of every sequence, so ``splits *
+    tiles_per_split * 128`` must cover the longest one (``tiles_per_split=0``:
+    enough tiles for every key that the page table has room for)."""
+    _check_heads(hq, hkv, 8)
+    _check_rows("q", q, hq * HEAD_DIM)
+    B, dev = seq_lens.shape[0], q.device
+    if q.shape[0] < B:
+        raise ValueError(f"q has {q.shape[0]} rows for {B} sequences")
+    _check_i32("seq_lens", seq_lens, None, dev)
+    _check_cache("k_cache", k_cache, hkv, dev)
+    _check_cache("v_cache", v_cache, hkv, dev)
+    if k_cache.q.shape != v_cache.q.shape:
+        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+    _check_table(block_table, bt_rows, B, dev)
+    if splits < 1 or tiles_per_split < 0:
+        raise ValueError(f"splits {splits}, tiles_per_split {tiles_per_split}")
+    if out is not None:
+        _check_rows("out", out, hq * HEAD_DIM)
+        _check_dev("out", out, dev)
+        if out.shape[0] < B:
+            raise ValueError(f"out has {out.shape[0]} rows for {B} sequences")
+    if not q.is_cuda:
+        lens = [int(x) for x in seq_lens.tolist()]
+        bt = block_table if bt_rows is None else block_table[bt_rows.long()]
+        y = torch.zeros(B, hq * HEAD_DIM, dtype=q.dtype)
+        some = [b for b, n in enumerate(lens) if n > 0]
+        if some:
+            kept = [lens[b] for b in some]
+            outs = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
+                                    [[n - 1] for n in kept], kept, hq, hkv, scale)
+            y[some] = torch.cat(outs, 0).to(q.dtype)
+        if out is None:
+            return y
+        out[:B, : hq * HEAD_DIM].copy_(y)
+        return out
+    _check_aligned("q", q, 4)
+    if out is None:
+        out = torch.empty(B, hq * HEAD_DIM, dtype=q.dtype, device=dev)
+    if B == 0:
+        return out
+    if tiles_per_split == 0:
+        tiles_per_split = max(1, -(-(-(-block_table.shape[1] * PAGE // 128)) // splits))
+    st = K.scratch(dev).status
+    part = lse = None
+    if splits > 1:
+        # partials of this call: its own memory, so that calls on several
+        # streams and captured graphs share none
+        n = B * hq * splits
+        ws = torch.empty(n * (HEAD_DIM + 1), dtype=torch.float32, device=dev)
+        part, lse = ws.data_ptr(), ws.data_ptr() + 4 * n * HEAD_DIM
+    rc = _native.kernels().ib_attn_decode_kv8(q.data_ptr(), q.stride(0), k_cache.q.data_ptr(),
+                                              k_cache.sf.data_ptr(), v_cache.q.data_ptr(), v_cache.sf.data_ptr(),
+                                              k_cache.q.shape[0], block_table.data_ptr(), K._ptr(bt_rows),
+                                              seq_lens.data_ptr(), block_table.shape[1], block_table.stride(0), B,
+                                              hq, hkv, splits, tiles_per_split, scale, part, lse, out.data_ptr(),
+                                              out.stride(0), st.data_ptr(), K._stream())
+    _native.check(rc, "ib_attn_decode_kv8")
+    K._count(2 if splits > 1 else 1)
+    return out
+
+
+# ---------------------------------------------------------------- prompt attention
+
+
+def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_table: torch.Tensor,
+                 q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, tiles: torch.Tensor, hq: int,
+                 hkv: int, scale: float, out: torch.Tensor | None = None,
+                 host_meta: tuple[list[int], list[int]] | None = None, bt_rows: torch.Tensor | None = None,
+                 kv_splits: int | None = None, tile_rows: int | None = None) -> torch.Tensor:
+    """Causal attention for chunks of new tokens whose K/V already sit in the
+    8-bit cache; arguments as of :func:`infera_b200.ops.kernels.attn_prefill`.
+    ``host_meta`` (q lengths, context lengths on the host; read back from the
+    device without it) sizes the workspace.
+
+    Each sequence's pages are expanded to bf16 once (code times power of two is
+    exact there) and the flash-attention kernel reads those: its work is
+    bound by the softmax and the bf16 tensor core, so the expansion's bytes
+    cost less than conversions inside the kernel, which every query tile and
+    every query head of a group would repeat."""
+    _check_heads(hq, hkv, hq)
+    _check_rows("q", q, hq * HEAD_DIM)
+    n, dev = q_len.shape[0], q.device
+    for name, t in (("q_start", q_start), ("q_len", q_len), ("ctx_len", ctx_len)):
+        _check_i32(name, t, n, dev)
+    _check_cache("k_cache", k_cache, hkv, dev)
+    _check_cache("v_cache", v_cache, hkv, dev)
+    if k_cache.q.shape != v_cache.q.shape:
+        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+    _check_table(block_table, bt_rows, n, dev)
+    if host_meta is None:
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attn_prefill over an 8-bit cache needs host_meta during capture")
+        host_meta = (q_len.tolist(), ctx_len.tolist())
+    if len(host_meta[0]) != n or len(host_meta[1]) != n:
+        raise ValueError(f"host_meta is of {len(host_meta[0])} / {len(host_meta[1])} sequences, q_len of {n}")
+    if not q.is_cuda:
+        return K.attn_prefill(q, k_cache.dequant(), v_cache.dequant(), block_table, q_start, q_len, ctx_len, tiles,
+                              hq, hkv, scale, out=out, host_meta=host_meta, bt_rows=bt_rows)
+    _check_aligned("q", q, 16)
+    if out is not None:
+        _check_rows("out", out, hq * HEAD_DIM)
+        _check_dev("out", out, dev)
+        _check_aligned("out", out, 16)
+    pages = [-(-max(c, 0) // PAGE) for c in host_meta[1]]
+    total, most = sum(pages), max(pages, default=0)
+    if total == 0 or q.shape[0] == 0:
+        return out if out is not None else torch.empty(q.shape[0], hq * HEAD_DIM, dtype=q.dtype, device=dev)
+    if most > block_table.shape[1]:
+        raise ValueError(f"a context of {max(host_meta[1])} keys needs {most} pages, block_table has room for "
+                         f"{block_table.shape[1]}")
+    st = K.scratch(dev).status
+    # this call's own workspace, as in attn_decode
+    kv = torch.empty(2, total * PAGE, hkv * HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    table = torch.empty(n, most, dtype=torch.int32, device=dev)
+    rc = _native.kernels().ib_kv8_expand(k_cache.q.data_ptr(), k_cache.sf.data_ptr(), v_cache.q.data_ptr(),
+                                         v_cache.sf.data_ptr(), k_cache.sf.shape[0], hkv, block_table.data_ptr(),
+                                         K._ptr(bt_rows), block_table.stride(0), ctx_len.data_ptr(), n, most, total,
+                                         kv[0].data_ptr(), kv[1].data_ptr(), table.data_ptr(), st.data_ptr(),
+                                         K._stream())
+    _native.check(rc, "ib_kv8_expand")
+    K._count()
+    return K.attn_prefill(q, kv[0], kv[1], table, q_start, q_len, ctx_len, tiles, hq, hkv, scale, out=out,
+                          host_meta=host_meta, kv_splits=kv_splits, tile_rows=tile_rows)
