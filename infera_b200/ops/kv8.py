@@ -32,8 +32,6 @@ Reference counterpart: the reference's engines serve with fp8 KV caches
 
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from infera_b200.ops import _native
@@ -44,12 +42,31 @@ PAGE = 16
 HEAD_DIM = 128
 
 
-@dataclass
 class KV8Cache:
-    """One channel (K or V) of one layer, or of all layers with a leading dimension."""
+    """One channel (K or V) of one layer, or of all layers with a leading
+    dimension; ``cache[layer]`` is one layer's. The tensors are checked here,
+    once, and stay what they are."""
 
-    q: torch.Tensor   # [(layers,) slots, hkv*128] float8_e4m3fn
-    sf: torch.Tensor  # [(layers,) slots/16, hkv] uint8
+    __slots__ = ("q", "sf", "slots", "hkv", "dev", "_layers")
+
+    def __init__(self, q: torch.Tensor, sf: torch.Tensor):
+        self.q = q    # [(layers,) slots, hkv*128] float8_e4m3fn
+        self.sf = sf  # [(layers,) slots/16, hkv] uint8
+        qs, ss = q.shape, sf.shape
+        if q.dtype is not torch.float8_e4m3fn or sf.dtype is not torch.uint8:
+            raise ValueError(f"a KV8Cache holds float8_e4m3fn codes and uint8 scales, not {q.dtype} and {sf.dtype}")
+        if not 2 <= len(qs) == len(ss) <= 3 or qs[-2] != ss[-2] * PAGE or qs[-1] != ss[-1] * HEAD_DIM \
+                or qs[:-2] != ss[:-2] or ss[-1] < 1 or ss[-2] < 1:
+            raise ValueError(f"codes {tuple(qs)} and scales {tuple(ss)} do not hold whole pages of {PAGE} slots with "
+                             f"heads of {HEAD_DIM}")
+        if not (q.is_contiguous() and sf.is_contiguous()):
+            raise ValueError("a KV8Cache's tensors have to be contiguous")
+        self.slots, self.hkv, self.dev = qs[-2], ss[-1], q.get_device()
+        if sf.get_device() != self.dev:
+            raise ValueError(f"codes on {q.device}, scales on {sf.device}")
+        if self.dev >= 0 and q.data_ptr() % 16:
+            raise ValueError("a KV8Cache's codes have to start on a multiple of 16 bytes")
+        self._layers = [KV8Cache(q[i], sf[i]) for i in range(qs[0])] if len(qs) == 3 else None
 
     @property
     def shape(self) -> torch.Size:
@@ -68,7 +85,9 @@ class KV8Cache:
         return self.q.numel() + self.sf.numel()
 
     def __getitem__(self, layer: int) -> "KV8Cache":
-        return KV8Cache(self.q[layer], self.sf[layer])
+        if self._layers is None:
+            raise TypeError("this KV8Cache is one layer's")
+        return self._layers[layer]
 
     def to(self, device) -> "KV8Cache":
         return KV8Cache(self.q.to(device), self.sf.to(device))
@@ -76,7 +95,7 @@ class KV8Cache:
     def dequant(self) -> torch.Tensor:
         """fp32 [.., slots, hkv*128]."""
         s = _pow2(self.sf.to(torch.int32).clamp_min(1) - 127)
-        x = self.q.float().unflatten(-1, (self.sf.shape[-1], -1)).unflatten(-3, (-1, PAGE))
+        x = self.q.float().unflatten(-1, (self.hkv, -1)).unflatten(-3, (-1, PAGE))
         return (x * s[..., :, None, :, None]).flatten(-4, -3).flatten(-2)
 
 
@@ -102,34 +121,35 @@ def _scale_exp(amax: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- checks
+# The calls take some 10 us of host time, a small batch's kernel less: each
+# check is one comparison of plain attributes, and words its error only after
+# it failed.
+
+_BF16, _I32 = torch.bfloat16, torch.int32
 
 
-def _check_cache(name: str, c: KV8Cache, hkv: int, dev: torch.device) -> None:
-    if not isinstance(c, KV8Cache):
-        raise TypeError(f"{name} is a {type(c).__name__}, not a KV8Cache (K and V are both 8-bit, or neither)")
-    if c.q.dim() != 2 or c.q.dtype != torch.float8_e4m3fn or c.sf.dtype != torch.uint8:
-        raise ValueError(f"{name}: one layer's e4m3 codes [slots, hkv*128] and uint8 scales, not "
-                         f"{tuple(c.q.shape)} {c.q.dtype} / {c.sf.dtype}")
-    slots = c.q.shape[0]
-    if slots % PAGE or c.q.shape[1] != hkv * HEAD_DIM or tuple(c.sf.shape) != (slots // PAGE, hkv):
-        raise ValueError(f"{name}: codes {tuple(c.q.shape)} and scales {tuple(c.sf.shape)} do not hold whole pages "
-                         f"of {PAGE} slots with {hkv} heads of {HEAD_DIM}")
-    if not (c.q.is_contiguous() and c.sf.is_contiguous()):
-        raise ValueError(f"{name}: the cache has to be contiguous")
-    _check_dev(name, c.q, dev)
-    _check_dev(name, c.sf, dev)
+def _check_caches(k: KV8Cache, v: KV8Cache, hkv: int, dev: int) -> None:
+    if type(k) is not KV8Cache or type(v) is not KV8Cache:
+        raise TypeError(f"caches of {type(k).__name__} and {type(v).__name__}: K and V are both KV8Cache, or neither")
+    if k._layers is not None or v._layers is not None:
+        raise ValueError("the caches hold all layers: pass one layer's, cache[layer]")
+    if k.hkv != hkv or v.hkv != hkv:
+        raise ValueError(f"the caches hold {k.hkv} and {v.hkv} heads, not {hkv}")
+    if k.slots != v.slots:
+        raise ValueError(f"the caches hold {k.slots} and {v.slots} slots")
+    if k.dev != dev or v.dev != dev:
+        raise ValueError(f"caches on {k.device} and {v.device}, queries on {_name(dev)}")
 
 
-def _check_dev(name: str, t: torch.Tensor, dev: torch.device) -> None:
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the queries on {dev}")
+def _name(dev: int) -> str:
+    return "cpu" if dev < 0 else f"cuda:{dev}"
 
 
-def _check_i32(name: str, t: torch.Tensor, n: int | None, dev: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name}: a contiguous int32 vector{'' if n is None else f' of {n}'}, not "
-                         f"{tuple(t.shape)} {t.dtype}")
-    _check_dev(name, t, dev)
+def _check_i32(name: str, t: torch.Tensor, n: int, dev: int) -> None:
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 vector of {n}, not {tuple(t.shape)} {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the queries on {_name(dev)}")
 
 
 def _check_heads(hq: int, hkv: int, most: int) -> None:
@@ -137,25 +157,30 @@ def _check_heads(hq: int, hkv: int, most: int) -> None:
         raise ValueError(f"{hq} query heads over {hkv} KV heads: a whole number of at most {most} to one")
 
 
-def _check_rows(name: str, t: torch.Tensor, width: int) -> None:
-    if t.dim() != 2 or t.dtype != torch.bfloat16 or t.shape[1] < width or (t.shape[0] and t.stride(1) != 1):
-        raise ValueError(f"{name}: bf16 rows of at least {width} adjacent elements, not {tuple(t.shape)} {t.dtype}, "
-                         f"strides {t.stride()}")
+def _check_rows(name: str, t: torch.Tensor, rows: int, width: int, dev: int, align: int) -> int:
+    """Rows of ``width`` adjacent bf16 elements; returns their pitch."""
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] < rows or shape[1] < width:
+        raise ValueError(f"{name}: bf16 [{rows} or more, {width} or more], not {tuple(shape)} {t.dtype}")
+    pitch, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{name}: a row's elements have to be adjacent, not {one} apart")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the queries on {_name(dev)}")
+    if dev >= 0 and (t.data_ptr() | (2 * pitch if shape[0] > 1 else 0)) & (align - 1):
+        raise ValueError(f"{name}: rows have to start on multiples of {align} bytes")
+    return pitch
 
 
-def _check_aligned(name: str, t: torch.Tensor, nbytes: int) -> None:
-    if t.is_cuda and (t.data_ptr() % nbytes or (t.shape[0] > 1 and t.stride(0) * t.element_size() % nbytes)):
-        raise ValueError(f"{name}: rows have to start on multiples of {nbytes} bytes")
-
-
-def _check_table(block_table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev: torch.device) -> None:
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+def _check_table(table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev: int) -> None:
+    if table.dtype is not _I32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError("block_table: int32 [rows, pages] with adjacent pages")
-    _check_dev("block_table", block_table, dev)
+    if table.get_device() != dev:
+        raise ValueError(f"block_table is on {table.device}, the queries on {_name(dev)}")
     if bt_rows is not None:
         _check_i32("bt_rows", bt_rows, n, dev)
-    elif block_table.shape[0] < n:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows for {n} sequences")
+    elif table.shape[0] < n:
+        raise ValueError(f"block_table has {table.shape[0]} rows for {n} sequences")
 
 
 # ---------------------------------------------------------------- append
@@ -171,37 +196,32 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
     if head_dim != HEAD_DIM:
         raise ValueError(f"head_dim {head_dim}: the 8-bit cache holds heads of {HEAD_DIM}")
     _check_heads(hq, hkv, hq)
-    _check_rows("qkv", qkv, (hq + 2 * hkv) * HEAD_DIM)
+    T, dev = qkv.shape[0], qkv.get_device()
+    ld = _check_rows("qkv", qkv, T, (hq + 2 * hkv) * HEAD_DIM, dev, 16)
     if q_out is None:
-        q_out = qkv
-    _check_rows("q_out", q_out, hq * HEAD_DIM)
-    T, dev = qkv.shape[0], qkv.device
-    if q_out.shape[0] < T:
-        raise ValueError(f"q_out has {q_out.shape[0]} rows for {T}")
-    _check_dev("q_out", q_out, dev)
+        q_out, ldq = qkv, ld
+    else:
+        ldq = _check_rows("q_out", q_out, T, hq * HEAD_DIM, dev, 16)
     _check_i32("pos", pos, T, dev)
     _check_i32("slots", slots, T, dev)
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or tuple(cos_sin.shape[1:]) != (HEAD_DIM // 2, 2) \
+    _check_caches(k_cache, v_cache, hkv, dev)
+    max_pos = cos_sin.shape[0]
+    if cos_sin.dtype is not torch.float32 or cos_sin.shape != (max_pos, HEAD_DIM // 2, 2) \
             or not cos_sin.is_contiguous():
-        raise ValueError(f"cos_sin: contiguous fp32 [positions, {HEAD_DIM // 2}, 2]")
-    _check_dev("cos_sin", cos_sin, dev)
-    _check_cache("k_cache", k_cache, hkv, dev)
-    _check_cache("v_cache", v_cache, hkv, dev)
-    if k_cache.q.shape != v_cache.q.shape:
-        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+        raise ValueError(f"cos_sin: contiguous fp32 [positions, {HEAD_DIM // 2}, 2], not {tuple(cos_sin.shape)} "
+                         f"{cos_sin.dtype}")
+    if cos_sin.get_device() != dev or (dev >= 0 and cos_sin.data_ptr() & 15):
+        raise ValueError(f"cos_sin on {cos_sin.device} at {cos_sin.data_ptr():#x}: on the queries' device, at a "
+                         "multiple of 16 bytes")
     if T == 0:
         return q_out
-    if not qkv.is_cuda:
+    if dev < 0:
         _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out)
         return q_out
-    _check_aligned("qkv", qkv, 16)
-    _check_aligned("q_out", q_out, 16)
-    _check_aligned("cos_sin", cos_sin, 16)
-    rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, qkv.stride(0), q_out.data_ptr(), q_out.stride(0),
-                                         pos.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), hq, hkv,
-                                         k_cache.q.data_ptr(), k_cache.sf.data_ptr(), v_cache.q.data_ptr(),
-                                         v_cache.sf.data_ptr(), k_cache.q.shape[0], cos_sin.shape[0],
-                                         K.scratch(dev).status.data_ptr(), K._stream())
+    rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, ld, q_out.data_ptr(), ldq, pos.data_ptr(),
+                                         slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, k_cache.q.data_ptr(),
+                                         k_cache.sf.data_ptr(), v_cache.q.data_ptr(), v_cache.sf.data_ptr(),
+                                         k_cache.slots, max_pos, K.scratch(dev).status.data_ptr(), K._stream())
     _native.check(rc, "ib_kv8_append")
     K._count()
     return q_out
@@ -260,61 +280,56 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
     tiles_per_split * 128`` must cover the longest one (``tiles_per_split=0``:
     enough tiles for every key that the page table has room for)."""
     _check_heads(hq, hkv, 8)
-    _check_rows("q", q, hq * HEAD_DIM)
-    B, dev = seq_lens.shape[0], q.device
-    if q.shape[0] < B:
-        raise ValueError(f"q has {q.shape[0]} rows for {B} sequences")
-    _check_i32("seq_lens", seq_lens, None, dev)
-    _check_cache("k_cache", k_cache, hkv, dev)
-    _check_cache("v_cache", v_cache, hkv, dev)
-    if k_cache.q.shape != v_cache.q.shape:
-        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+    B, dev = seq_lens.shape[0], q.get_device()
+    ldq = _check_rows("q", q, B, hq * HEAD_DIM, dev, 4)
+    _check_i32("seq_lens", seq_lens, B, dev)
+    _check_caches(k_cache, v_cache, hkv, dev)
     _check_table(block_table, bt_rows, B, dev)
     if splits < 1 or tiles_per_split < 0:
         raise ValueError(f"splits {splits}, tiles_per_split {tiles_per_split}")
-    if out is not None:
-        _check_rows("out", out, hq * HEAD_DIM)
-        _check_dev("out", out, dev)
-        if out.shape[0] < B:
-            raise ValueError(f"out has {out.shape[0]} rows for {B} sequences")
-    if not q.is_cuda:
-        lens = [int(x) for x in seq_lens.tolist()]
-        bt = block_table if bt_rows is None else block_table[bt_rows.long()]
-        y = torch.zeros(B, hq * HEAD_DIM, dtype=q.dtype)
-        some = [b for b, n in enumerate(lens) if n > 0]
-        if some:
-            kept = [lens[b] for b in some]
-            outs = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
-                                    [[n - 1] for n in kept], kept, hq, hkv, scale)
-            y[some] = torch.cat(outs, 0).to(q.dtype)
-        if out is None:
-            return y
-        out[:B, : hq * HEAD_DIM].copy_(y)
-        return out
-    _check_aligned("q", q, 4)
     if out is None:
-        out = torch.empty(B, hq * HEAD_DIM, dtype=q.dtype, device=dev)
+        out = torch.empty(B, hq * HEAD_DIM, dtype=_BF16, device=q.device)
+        ldo = hq * HEAD_DIM
+    else:
+        ldo = _check_rows("out", out, B, hq * HEAD_DIM, dev, 2)
     if B == 0:
         return out
+    if dev < 0:
+        _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, out, bt_rows)
+        return out
+    places = block_table.shape[1]
     if tiles_per_split == 0:
-        tiles_per_split = max(1, -(-(-(-block_table.shape[1] * PAGE // 128)) // splits))
-    st = K.scratch(dev).status
+        tiles_per_split = max(1, -(-(-(-places * PAGE // 128)) // splits))
     part = lse = None
     if splits > 1:
         # partials of this call: its own memory, so that calls on several
         # streams and captured graphs share none
         n = B * hq * splits
-        ws = torch.empty(n * (HEAD_DIM + 1), dtype=torch.float32, device=dev)
-        part, lse = ws.data_ptr(), ws.data_ptr() + 4 * n * HEAD_DIM
-    rc = _native.kernels().ib_attn_decode_kv8(q.data_ptr(), q.stride(0), k_cache.q.data_ptr(),
-                                              k_cache.sf.data_ptr(), v_cache.q.data_ptr(), v_cache.sf.data_ptr(),
-                                              k_cache.q.shape[0], block_table.data_ptr(), K._ptr(bt_rows),
-                                              seq_lens.data_ptr(), block_table.shape[1], block_table.stride(0), B,
-                                              hq, hkv, splits, tiles_per_split, scale, part, lse, out.data_ptr(),
-                                              out.stride(0), st.data_ptr(), K._stream())
+        ws = torch.empty(n * (HEAD_DIM + 1), dtype=torch.float32, device=q.device)
+        part = ws.data_ptr()
+        lse = part + 4 * n * HEAD_DIM
+    rc = _native.kernels().ib_attn_decode_kv8(q.data_ptr(), ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
+                                              v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
+                                              block_table.data_ptr(), K._ptr(bt_rows), seq_lens.data_ptr(), places,
+                                              block_table.stride(0), B, hq, hkv, splits, tiles_per_split, scale,
+                                              part, lse, out.data_ptr(), ldo, K.scratch(dev).status.data_ptr(),
+                                              K._stream())
     _native.check(rc, "ib_attn_decode_kv8")
     K._count(2 if splits > 1 else 1)
     return out
+
+
+def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, out, bt_rows) -> None:
+    lens = [int(x) for x in seq_lens.tolist()]
+    bt = block_table if bt_rows is None else block_table[bt_rows.long()]
+    y = out[: len(lens), : hq * HEAD_DIM]
+    y.zero_()
+    some = [b for b, n in enumerate(lens) if n > 0]
+    if some:
+        kept = [lens[b] for b in some]
+        outs = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
+                                [[n - 1] for n in kept], kept, hq, hkv, scale)
+        y[some] = torch.cat(outs, 0).to(q.dtype)
 
 
 # ---------------------------------------------------------------- prompt attention
@@ -336,46 +351,42 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     cost less than conversions inside the kernel, which every query tile and
     every query head of a group would repeat."""
     _check_heads(hq, hkv, hq)
-    _check_rows("q", q, hq * HEAD_DIM)
-    n, dev = q_len.shape[0], q.device
-    for name, t in (("q_start", q_start), ("q_len", q_len), ("ctx_len", ctx_len)):
-        _check_i32(name, t, n, dev)
-    _check_cache("k_cache", k_cache, hkv, dev)
-    _check_cache("v_cache", v_cache, hkv, dev)
-    if k_cache.q.shape != v_cache.q.shape:
-        raise ValueError(f"k_cache and v_cache hold {k_cache.q.shape[0]} and {v_cache.q.shape[0]} slots")
+    n, T, dev = q_len.shape[0], q.shape[0], q.get_device()
+    _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
+    _check_i32("q_start", q_start, n, dev)
+    _check_i32("q_len", q_len, n, dev)
+    _check_i32("ctx_len", ctx_len, n, dev)
+    _check_caches(k_cache, v_cache, hkv, dev)
     _check_table(block_table, bt_rows, n, dev)
     if host_meta is None:
-        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+        if dev >= 0 and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attn_prefill over an 8-bit cache needs host_meta during capture")
         host_meta = (q_len.tolist(), ctx_len.tolist())
     if len(host_meta[0]) != n or len(host_meta[1]) != n:
         raise ValueError(f"host_meta is of {len(host_meta[0])} / {len(host_meta[1])} sequences, q_len of {n}")
-    if not q.is_cuda:
+    if out is not None:
+        _check_rows("out", out, T, hq * HEAD_DIM, dev, 16)
+    if dev < 0:
         return K.attn_prefill(q, k_cache.dequant(), v_cache.dequant(), block_table, q_start, q_len, ctx_len, tiles,
                               hq, hkv, scale, out=out, host_meta=host_meta, bt_rows=bt_rows)
-    _check_aligned("q", q, 16)
-    if out is not None:
-        _check_rows("out", out, hq * HEAD_DIM)
-        _check_dev("out", out, dev)
-        _check_aligned("out", out, 16)
     pages = [-(-max(c, 0) // PAGE) for c in host_meta[1]]
     total, most = sum(pages), max(pages, default=0)
-    if total == 0 or q.shape[0] == 0:
-        return out if out is not None else torch.empty(q.shape[0], hq * HEAD_DIM, dtype=q.dtype, device=dev)
     if most > block_table.shape[1]:
         raise ValueError(f"a context of {max(host_meta[1])} keys needs {most} pages, block_table has room for "
                          f"{block_table.shape[1]}")
-    st = K.scratch(dev).status
+    if total == 0 or T == 0:
+        return out if out is not None else torch.empty(T, hq * HEAD_DIM, dtype=_BF16, device=q.device)
     # this call's own workspace, as in attn_decode
-    kv = torch.empty(2, total * PAGE, hkv * HEAD_DIM, dtype=torch.bfloat16, device=dev)
-    table = torch.empty(n, most, dtype=torch.int32, device=dev)
+    width = hkv * HEAD_DIM
+    kv = torch.empty(2 * total * PAGE, width, dtype=_BF16, device=q.device)
+    kb, vb = kv.split(total * PAGE)
+    table = torch.empty(n, most, dtype=_I32, device=q.device)
     rc = _native.kernels().ib_kv8_expand(k_cache.q.data_ptr(), k_cache.sf.data_ptr(), v_cache.q.data_ptr(),
-                                         v_cache.sf.data_ptr(), k_cache.sf.shape[0], hkv, block_table.data_ptr(),
+                                         v_cache.sf.data_ptr(), k_cache.slots // PAGE, hkv, block_table.data_ptr(),
                                          K._ptr(bt_rows), block_table.stride(0), ctx_len.data_ptr(), n, most, total,
-                                         kv[0].data_ptr(), kv[1].data_ptr(), table.data_ptr(), st.data_ptr(),
-                                         K._stream())
+                                         kb.data_ptr(), vb.data_ptr(), table.data_ptr(),
+                                         K.scratch(dev).status.data_ptr(), K._stream())
     _native.check(rc, "ib_kv8_expand")
     K._count()
-    return K.attn_prefill(q, kv[0], kv[1], table, q_start, q_len, ctx_len, tiles, hq, hkv, scale, out=out,
+    return K.attn_prefill(q, kb, vb, table, q_start, q_len, ctx_len, tiles, hq, hkv, scale, out=out,
                           host_meta=host_meta, kv_splits=kv_splits, tile_rows=tile_rows)

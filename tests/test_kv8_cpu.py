@@ -222,12 +222,7 @@ APPEND_REFUSALS = {
     "mixed caches": dict(v_cache=torch.zeros(32, 2 * D, dtype=torch.bfloat16)),
     "slots of K and V": dict(v_cache=kv8.alloc(48, 2, device="cpu")),
     "cache heads": dict(k_cache=kv8.alloc(32, 4, device="cpu"), v_cache=kv8.alloc(32, 4, device="cpu")),
-    "cache type": dict(k_cache=kv8.KV8Cache(torch.zeros(32, 2 * D, dtype=torch.float8_e5m2),
-                                            torch.zeros(2, 2, dtype=torch.uint8))),
-    "scales shape": dict(k_cache=kv8.KV8Cache(kv8.alloc(32, 2, device="cpu").q, torch.zeros(2, 3, dtype=torch.uint8))),
     "all layers": dict(k_cache=kv8.alloc(32, 2, layers=2, device="cpu")),
-    "strided cache": dict(k_cache=kv8.KV8Cache(kv8.alloc(32, 4, device="cpu").q[:, : 2 * D],
-                                               torch.zeros(2, 2, dtype=torch.uint8))),
     "q_out rows": dict(q_out=torch.zeros(2, 4 * D, dtype=torch.bfloat16)),
     "q_out width": dict(q_out=torch.zeros(3, 3 * D, dtype=torch.bfloat16)),
     "q_out type": dict(q_out=torch.zeros(3, 4 * D)),
@@ -238,6 +233,22 @@ APPEND_REFUSALS = {
 def test_append_refuses(name):
     with pytest.raises((ValueError, TypeError)):
         kv8.rope_kvwrite(**append_args(**APPEND_REFUSALS[name]))
+
+
+def test_cache_refuses():
+    e4m3, u8 = torch.float8_e4m3fn, torch.uint8
+    q, sf = torch.zeros(32, 2 * D, dtype=u8).view(e4m3), torch.zeros(2, 2, dtype=u8)
+    kv8.KV8Cache(q, sf)
+    wide = torch.zeros(32, 4 * D, dtype=u8).view(e4m3)
+    for bad in ((q.view(torch.float8_e5m2), sf), (q, sf.int()), (q, sf[:1]), (q[:31], sf), (q, torch.zeros(2, 3, dtype=u8)),
+                (wide[:, : 2 * D], sf), (q, torch.zeros(2, 4, dtype=u8)[:, :2]), (q[None], sf), (q[:0], sf[:0]),
+                (q.view(-1), sf.view(-1)), (q[None, None], sf[None, None])):
+        with pytest.raises(ValueError):
+            kv8.KV8Cache(*bad)
+    with pytest.raises(TypeError):
+        kv8.KV8Cache(q, sf)[0]
+    both = kv8.alloc(32, 2, layers=3, device="cpu")
+    assert both[2] is both[2] and both[2].q.data_ptr() == both.q[2].data_ptr()
 
 
 def attend_args(**over):
