@@ -5,23 +5,33 @@
 //   S^T[128 keys, 16]  = K_tile . Q^T     (kind::f8f6f4, A = K codes, K-major)
 //   O^T[128 dims, N]   = V_tile^T . W     (A = V codes, MN-major)
 //
-// Both operands of an f8f6f4 product are 8-bit, so the bf16 query and the fp32
+// Both operands of an f8f6f4 product are 8-bit, so the bf16 query and the
 // weights are split into e4m3 digits that stand in columns of their own:
 //   q * 2^s = hi + lo / 16            exact: bf16 has 8 significant bits, a
 //                                     digit 4; s brings the head's largest
 //                                     element to [2^7, 2^8)
-//   w       = hi + mid / 32 + lo / 1024  14 significant bits (bf16 has 8): each
-//                                     digit is rounded to nearest, so what is
-//                                     left of it is half a step, 5 bits further
+//   w       = hi + mid / 32 + lo / 1024  a weight rounded to f16 (11 bits; bf16
+//                                     has 8): each digit is rounded to nearest,
+//                                     so what is left of it is at most half a
+//                                     step, 5 bits further; the last one ends
+//                                     at 2^-19
 // The 16 columns of S hold both digits of up to 8 heads, so the split costs no
 // matrix instruction, and the N columns of O three digits of them.
 //
 // Scales (one power of two per page and head): K's multiplies a key's scores.
 // V's goes into the weight: w = 2^(s - m) * 2^6 * 2^(vsf - R), with R the
-// largest V exponent seen so far in this split and m the running maximum that
-// may lag by 2^2, so that w <= 2^8 < 448; a weight is off by at most
-// max(2^-14 w, 2^-20), 2^-26 of the largest one. The sum of the softmax takes
-// the undigited fp32 weight. When m or R grows, O^T is rescaled in TMEM.
+// largest V exponent of the split's pages so far and m the running maximum
+// that may lag by 2^2, so that w <= 2^8 < 448; a weight is off by at most
+// max(2^-12 w, 2^-20), the latter 2^-26 of the largest one. The sum of the
+// softmax takes the fp32 weight. When m or R grows, O^T is rescaled in TMEM.
+//
+// A tile costs few instructions per score, because 4 warps have to keep up
+// with 32 KB of K and V: a tile first only asks whether any score is above its
+// head's running maximum by more than the lag (one compare per score, one
+// barrier with an OR); the maxima themselves are reduced when one is, in the
+// first tile and rarely after it. The digits are made in packed f16, and a
+// key's digits of all heads are one or two 16-byte stores (the weights' tile
+// has the columns adjacent, an MN-major operand).
 //
 // One CTA handles (sequence, KV head, KV split) and walks its share of the
 // sequence in tiles of 128 keys (8 pages), 32 KB for K and V:
@@ -59,8 +69,9 @@ constexpr int kTopLog2 = 6;         // weight of a key at the running maximum
 // columns of O^T: three digits of GP heads
 __host__ __device__ constexpr int cols_o(int gp) { return 3 * gp <= 16 ? 16 : 32; }
 __host__ __device__ constexpr int smem_bytes(int gp) {
-  return 1024 + STAGES * 2 * BLK + QBLK + 2 * cols_o(gp) * 128 + 1024;
+  return 1024 + STAGES * 2 * BLK + QBLK + 2 * cols_o(gp) * 128 + 2048;
 }
+constexpr int SF_TILES = 16;        // tiles whose page exponents are staged at a time: a page per softmax thread
 constexpr uint32_t TMEM_COLS = 64;  // S0 [0,16) S1 [16,32) O [32,64)
 constexpr uint32_t O_COL = 32;
 
@@ -77,7 +88,8 @@ struct Params {
   int hq, hkv, G;
   int splits;
   int tiles_per_split;  // split s covers tiles [s * this, (s + 1) * this) of every sequence
-  float scale_log2;
+  float scale_log2;  // |scale| * log2(e)
+  float q_sign;      // sign of the scale (0: every score is 0)
   float* o_part;    // [B, hq, splits, D]
   float* lse_part;  // [B, hq, splits]
   __nv_bfloat16* out;
@@ -98,10 +110,45 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
 __device__ __forceinline__ uint32_t sw_offset(int row, int k) {
   return static_cast<uint32_t>(row * 128 + (((k >> 4) ^ (row & 7)) << 4) + (k & 15));
 }
-// The leading e4m3 digit of x, |x| <= 256: rounded to its top 4 bits, 0 where
-// that would be subnormal in e4m3 (the next digit, 32 times finer, takes it).
-__device__ __forceinline__ float digit(float x) {
-  return fabsf(x) >= 0.015625f ? __uint_as_float((__float_as_uint(x) + 0x80000u) & 0xFFF00000u) : 0.f;
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// The leading e4m3 digits of two f16 values (|x| <= 256), and the rest of the
+// values after it, 32 times larger (exact in f16).
+__device__ __forceinline__ uint32_t digit2(__half2& x) {
+  const __half2_raw raw = x;
+  const uint32_t d = __nv_cvt_halfraw2_to_fp8x2(raw, __NV_SATFINITE, __NV_E4M3);
+  const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(d), __NV_E4M3));
+  x = __hmul2(__hsub2(x, back), __float2half2_rn(32.f));
+  return d;
+}
+__device__ __forceinline__ float max_over_warp(float x) {  // a NaN counts as nothing
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Barrier of the four softmax warps that ORs a predicate. Every one of them
+// passes the same number of these, whatever a bounded wait in between gave,
+// so none is left waiting.
+__device__ __forceinline__ bool barrier_or(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return r != 0;
+}
+// MN-major descriptor without swizzle: cores of 16 bytes (columns) x 8 keys,
+// `mn` bytes between cores along the columns, `k` along the keys.
+__device__ __forceinline__ uint64_t make_mn_desc(uint32_t smem_addr, uint32_t mn, uint32_t k) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((k >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((mn >> 4) & 0x3FFFu) << 32;
+  d |= 1ull << 46;
+  return d;
 }
 
 template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
@@ -110,6 +157,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
                   const __grid_constant__ CUtensorMap tmK8, const __grid_constant__ CUtensorMap tmV8,
                   const Params p) {
   constexpr int NO = cols_o(GP);
+  constexpr int NC = NO / 16;           // 16-byte pieces of a key's digits
   constexpr int PBLK = NO * 128;
   constexpr int ND = 3 * GP;            // digits of a key's weights
   pdl_trigger();
@@ -142,7 +190,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sKV = smem;                        // stage s: K, V
   uint8_t* sQ = smem + STAGES * 2 * BLK;      // rows: hi digits of GP heads, lo digits
-  uint8_t* sP = sQ + QBLK;                    // [2] rows: digit d of head h at d * GP + h
+  uint8_t* sP = sQ + QBLK;                    // [2] columns: digit d of head h at d * GP + h
   uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * PBLK);
   uint64_t* k_full = bars;
   uint64_t* v_full = k_full + STAGES;
@@ -152,14 +200,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   uint64_t* p_full = s_full + 2;              // [2] one per P buffer
   uint64_t* pv_done = p_full + 2;             // [2] PV of tile j commits to pv_done[j & 1]
   uint64_t* q_ready = pv_done + 2;
-  uint64_t* grp = q_ready + 1;                // bounded barrier of the 128 softmax threads
-  uint64_t* drain = grp + 1;
+  uint64_t* drain = q_ready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* red = reinterpret_cast<float*>(tmem_slot + 4);     // [2][4][GP] tile maxima
-  int* redv = reinterpret_cast<int*>(red + 2 * 4 * GP);     // [2][4] V exponents
-  float* lred = reinterpret_cast<float*>(redv + 8);         // [4][GP]
-  float* qsc = lred + 4 * GP;                               // [GP] scale_log2 * 2^-s
+  float* red = reinterpret_cast<float*>(tmem_slot + 4);     // [4][GP] tile maxima, then sums
+  int* redv = reinterpret_cast<int*>(red + 4 * GP);         // [4] V exponents
+  float* qsc = reinterpret_cast<float*>(redv + 4);          // [GP] scale_log2 * 2^-s
+  uint16_t* sSf = reinterpret_cast<uint16_t*>(qsc + GP);    // [2][128] exponents (K low byte, V high) of a batch's pages
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -177,7 +224,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_ready, 128);
-    mbar_init(grp, 128);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -241,7 +287,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc_s = make_idesc_e4m3(128, NS);
-      const uint32_t idesc_o = make_idesc_e4m3(128, NO) | (1u << 15);  // A = V^T, MN-major
+      const uint32_t idesc_o = make_idesc_e4m3(128, NO) | (1u << 15) | (1u << 16);  // both MN-major
       const uint32_t q_addr = smem_u32(sQ);
       const uint32_t p_addr = smem_u32(sP);
       bool ok = mbar_wait(q_ready, 0, abort_flag, p.status, kStatusTimeoutFull);
@@ -262,7 +308,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           // 32 keys: four groups of 8 rows, 1024 bytes apart (the stride);
           // all 128 dims are one 128-byte row, so the leading offset is unused
           const uint64_t ad = make_sw128_desc(v_addr + s * 4096, BLK, 1024);
-          const uint64_t bd = make_sw128_desc(pb + s * 32, 16, 1024);
+          const uint64_t bd = make_mn_desc(pb + s * 4 * NC * 128, 128, NC * 128);
           umma_e4m3(tmem + O_COL, ad, bd, idesc_o, (jj > 0 || s > 0) ? 1u : 0u);
         }
         umma_commit(&pv_done[jj & 1]);
@@ -298,33 +344,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const int q4 = warp & 3;
     const int r = q4 * 32 + lane;     // key row of S, dim row of O
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
-    uint32_t gph = 0;
     bool ok = true;
-    auto group_sync = [&]() {
-      mbar_arrive(grp);
-      ok = mbar_wait_warp(grp, gph & 1u, abort_flag, p.status, kStatusTimeoutTmemFull) && ok;
-      ++gph;
-    };
-    // exponents of this row's page; a page id outside the cache (bad table)
-    // loads zeros through the tensor map and takes the smallest exponent here
+    // Exponents of the pages of 16 tiles: one page per thread. A page id
+    // outside the cache (a bad table) loads zeros through the tensor map and
+    // takes the smallest exponents here, as do places behind the sequence.
     auto page_of = [&](int j) -> int {
-      const int lp = (t0 + j) * (BKV / PAGE) + (r >> 4);
-      return lp < n_pages ? __ldg(bt + lp) : -1;
+      const int lp = (t0 + j) * (BKV / PAGE) + t;
+      return lp < n_pages && j < nt ? __ldg(bt + lp) : -1;
     };
-    auto load_sf = [&](int page, int& ke, int& ve) {
-      const bool in = page >= 0 && page < p.num_pages;
-      const size_t at = static_cast<size_t>(in ? page : 0) * p.hkv + kvh;
-      ke = in ? p.ksf[at] : 1;
-      ve = in ? p.vsf[at] : 1;
+    auto load_sf = [&](int page) -> uint32_t {
+      if (page < 0 || page >= p.num_pages) return 0x0101u;
+      const size_t at = static_cast<size_t>(page) * p.hkv + kvh;
+      return max(static_cast<uint32_t>(p.ksf[at]), 1u) | max(static_cast<uint32_t>(p.vsf[at]), 1u) << 8;
     };
-    int ke_n, ve_n;                   // of the next tile
-    int page_n2 = page_of(0);         // of the one after it
-    load_sf(page_n2, ke_n, ve_n);
-    page_n2 = nt > 1 ? page_of(1) : -1;
+    uint32_t sf_next = load_sf(page_of(0));  // this thread's page of the next batch
+    int page_next = -1;
 
-    // stage Q: unused rows of Q and P are zero
-    for (int i = t; i < (QBLK + 2 * PBLK) / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
-    group_sync();
+    // stage Q: unused rows of Q are zero
+    for (int i = t; i < QBLK / 16; i += 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    barrier_or(false);
     for (int h = q4; h < G; h += 4) {
       const uint32_t* src =
           reinterpret_cast<const uint32_t*>(p.q + static_cast<size_t>(b) * p.ldq + (kvh * G + h) * D) + lane * 2;
@@ -333,153 +371,152 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
       const uint32_t mb = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
       const int s = min(100, 134 - static_cast<int>(mb >> 23));
-      const float f = two_to(s);
-      float hi[4], lo[4];
+      const float f = two_to(s) * p.q_sign;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) <= 3.4e38f ? x[i] * f : NAN;
       const uint32_t h01 = to_e4m3x2(x[0], x[1]), h23 = to_e4m3x2(x[2], x[3]);
       const float2 a = from_e4m3x2(h01), c = from_e4m3x2(h23);
-      hi[0] = a.x, hi[1] = a.y, hi[2] = c.x, hi[3] = c.y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lo[i] = (x[i] - hi[i]) * 16.f;
       *reinterpret_cast<uint32_t*>(sQ + sw_offset(h, lane * 4)) = h01 | (h23 << 16);
       *reinterpret_cast<uint32_t*>(sQ + sw_offset(GP + h, lane * 4)) =
-          to_e4m3x2(lo[0], lo[1]) | (to_e4m3x2(lo[2], lo[3]) << 16);
-      if (lane == 0) qsc[h] = p.scale_log2 * two_to(-s);
+          to_e4m3x2((x[0] - a.x) * 16.f, (x[1] - a.y) * 16.f) |
+          (to_e4m3x2((x[2] - c.x) * 16.f, (x[3] - c.y) * 16.f) << 16);
+      if (lane == 0) qsc[h] = fmaxf(p.scale_log2 * two_to(-s), 1.2e-38f);  // positive: masked scores are -inf times it
     }
     fence_proxy_async_smem();
     mbar_arrive(q_ready);
-    group_sync();  // qsc
+    barrier_or(false);  // qsc
 
-    float m_run[GP], l_part[GP], c_h[GP];
+    // a head's scores are c * x, its running maximum m; a score above `limit`
+    // is above the maximum by more than the lag
+    float m_run[GP], limit[GP], l_part[GP], c_h[GP];
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
-      m_run[h] = -INFINITY;
+      m_run[h] = 0.f;
+      limit[h] = h < G ? -INFINITY : INFINITY;
       l_part[h] = 0.f;
       c_h[h] = h < G ? qsc[h] : 0.f;
     }
-    int R = 0;  // largest V exponent so far
+    int R = 1;  // largest V exponent of the batches so far
     // the PV of tile jj has completed: its commit is completion (jj >> 1) + 1
     // of pv_done[jj & 1], and no later PV on that barrier can have been issued
-    auto wait_pv = [&](int jj) -> bool {
-      if (!mbar_wait_warp(&pv_done[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
-                          kStatusTimeoutTmemFull))
-        return false;
+    auto wait_pv = [&](int jj) {
+      if (ok) ok = mbar_wait_warp(&pv_done[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
+                                  kStatusTimeoutTmemFull);
       tc_fence_after();
-      return true;
     };
-    for (int j = 0; j < nt && ok; ++j) {
-      const int ke = ke_n, ve = ve_n;
-      if (j + 1 < nt) {
-        load_sf(page_n2, ke_n, ve_n);
-        page_n2 = j + 2 < nt ? page_of(j + 2) : -1;
+    // O^T *= f, a factor per head, once the PV of tile jj has landed
+    auto rescale = [&](int jj, const float (&f)[GP]) {
+      wait_pv(jj);
+      uint32_t ov[NO];
+      if constexpr (NO == 16)
+        tmem_ld16(lane_addr + O_COL, ov);
+      else
+        tmem_ld32(lane_addr + O_COL, ov);
+      tmem_ld_wait();
+#pragma unroll
+      for (int n = 0; n < ND; ++n) ov[n] = __float_as_uint(__uint_as_float(ov[n]) * f[n % GP]);
+      if constexpr (NO == 16)
+        tmem_st16(lane_addr + O_COL, ov);
+      else
+        tmem_st32(lane_addr + O_COL, ov);
+      tmem_st_wait();
+    };
+    for (int j = 0; j < nt; ++j) {
+      const int in_batch = j % SF_TILES;
+      uint16_t* sf = sSf + ((j / SF_TILES) & 1) * 128;
+      if (in_batch == 0) {
+        sf[t] = static_cast<uint16_t>(sf_next);
+        const uint32_t v = __reduce_max_sync(0xffffffffu, sf_next >> 8);
+        if (lane == 0) redv[q4] = static_cast<int>(v);
+        barrier_or(false);
+        const int batch_v = max(max(redv[0], redv[1]), max(redv[2], redv[3]));
+        if (batch_v > R) {
+          if (j > 0) {
+            float f[GP];
+#pragma unroll
+            for (int h = 0; h < GP; ++h) f[h] = two_to(max(R - batch_v, -126));
+            rescale(j - 1, f);
+          }
+          R = batch_v;
+        }
+        page_next = page_of(j + SF_TILES);
+      } else if (in_batch == 4) {
+        sf_next = load_sf(page_next);
       }
-      if (!mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
-                          kStatusTimeoutTmemFull)) {
-        ok = false;
-        break;
-      }
+      if (ok) ok = mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
+                                  kStatusTimeoutTmemFull);
       tc_fence_after();
       uint32_t sv[16];
       tmem_ld16(lane_addr + ((j & 1) ? NS : 0), sv);
+      const uint32_t e = sf[in_batch * (BKV / PAGE) + (r >> 4)];
+      const float kf = two_to(static_cast<int>(e & 255) - 127);
+      const float vf = two_to(max(kTopLog2 + static_cast<int>(e >> 8) - R, -126));
+      const bool last = (t0 + j + 1) * BKV > len;  // only here are rows masked
+      const bool valid = !last || (t0 + j) * BKV + r < len;
       tmem_ld_wait();
-      const int key = (t0 + j) * BKV + r;
-      const bool valid = key < len;
-      const float kf = two_to(max(ke, 1) - 127);
-      float s[GP];
+      float x[GP];
+      bool above = false;
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
-        const float raw = fmaf(__uint_as_float(sv[GP + h]), 0.0625f, __uint_as_float(sv[h]));
-        s[h] = valid && h < G ? raw * (c_h[h] * kf) : -INFINITY;
-        float mx = s[h];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (lane == 0) red[((j & 1) * 4 + q4) * GP + h] = mx;
+        x[h] = fmaf(__uint_as_float(sv[GP + h]), 0.0625f, __uint_as_float(sv[h])) * kf;
+        if (!valid) x[h] = -INFINITY;
+        above = above || x[h] > limit[h];
       }
-      const int vmax = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(valid ? max(ve, 1) : 1)));
-      if (lane == 0) redv[(j & 1) * 4 + q4] = vmax;
-      group_sync();
-      if (!ok) break;
-      // every thread derives the same maxima, so the decision is uniform over the CTA
-      const int* rv = redv + (j & 1) * 4;
-      const int tile_v = max(max(rv[0], rv[1]), max(rv[2], rv[3]));
-      float alpha[GP];
-      bool rescale = false;
-      float fR = 1.f;
-      if (tile_v > R) {
-        if (R > 0) {
-          fR = two_to(max(R - tile_v, -126));
-          rescale = true;
+      if (barrier_or(above)) {
+        // uniform over the CTA: every thread derives the same maxima
+#pragma unroll
+        for (int h = 0; h < GP; ++h) {
+          const float mx = max_over_warp(x[h]);
+          if (lane == 0) red[q4 * GP + h] = mx;
         }
-        R = tile_v;
-      }
+        barrier_or(false);
+        float f[GP];
 #pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        const float* rr = red + (j & 1) * 4 * GP;
-        const float tmax = fmaxf(fmaxf(rr[h], rr[GP + h]), fmaxf(rr[2 * GP + h], rr[3 * GP + h]));
-        alpha[h] = 1.f;
-        if (m_run[h] == -INFINITY) {
-          m_run[h] = tmax;  // nothing accumulated yet
-        } else if (tmax > m_run[h] + kLagLog2) {
-          alpha[h] = exp2f(m_run[h] - tmax);
-          m_run[h] = tmax;
-          rescale = true;
+        for (int h = 0; h < GP; ++h) {
+          const float tmax = fmaxf(fmaxf(red[h], red[GP + h]), fmaxf(red[2 * GP + h], red[3 * GP + h]));
+          f[h] = 1.f;
+          if (tmax > limit[h]) {
+            const float m = tmax * c_h[h];
+            f[h] = limit[h] == -INFINITY ? 0.f : exp2f(m_run[h] - m);  // nothing before it: all zeros
+            m_run[h] = m;
+            limit[h] = (m + kLagLog2) / c_h[h];
+            l_part[h] *= f[h];
+          }
         }
+        if (j > 0) rescale(j - 1, f);
+        barrier_or(false);  // red is read
       }
-      if (rescale && j > 0) {
-        if (!wait_pv(j - 1)) {
-          ok = false;
-          break;
+      uint32_t d[NO / 4];  // digit bytes by column
+#pragma unroll
+      for (int i = 0; i < NO / 4; ++i) d[i] = 0u;
+#pragma unroll
+      for (int h = 0; h < GP; h += 2) {
+        const float p0 = exp2f(fmaf(x[h], c_h[h], -m_run[h]));
+        l_part[h] += p0;
+        float p1 = 0.f;
+        if (h + 1 < GP) {
+          p1 = exp2f(fmaf(x[h + (GP > 1)], c_h[h + (GP > 1)], -m_run[h + (GP > 1)]));
+          l_part[h + (GP > 1)] += p1;
         }
-        uint32_t ov[NO];
-        if constexpr (NO == 16)
-          tmem_ld16(lane_addr + O_COL, ov);
-        else
-          tmem_ld32(lane_addr + O_COL, ov);
-        tmem_ld_wait();
+        __half2 w = __floats2half2_rn(p0 * vf, p1 * vf);
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-          ov[n] = __float_as_uint(__uint_as_float(ov[n]) * (alpha[n % GP] * fR));
-        if constexpr (NO == 16)
-          tmem_st16(lane_addr + O_COL, ov);
-        else
-          tmem_st32(lane_addr + O_COL, ov);
-        tmem_st_wait();
-      }
-      float dg[ND + 1];
-      dg[ND] = 0.f;
-      const float vf = two_to(max(kTopLog2 + max(ve, 1) - R, -126));
-#pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        // a head whose every key scored -inf has no maximum yet
-        const float pw = s[h] == -INFINITY ? 0.f : exp2f(s[h] - (m_run[h] == -INFINITY ? 0.f : m_run[h]));
-        l_part[h] = l_part[h] * alpha[h] + pw;
-        const float w = valid ? pw * vf : 0.f;
-        dg[h] = digit(w);
-        const float w1 = (w - dg[h]) * 32.f;
-        dg[GP + h] = digit(w1);
-        dg[2 * GP + h] = (w1 - dg[GP + h]) * 32.f;
+        for (int k = 0; k < 3; ++k) {
+          const int n = k * GP + h;
+          const uint32_t u = k < 2 ? digit2(w) : __nv_cvt_halfraw2_to_fp8x2(w, __NV_SATFINITE, __NV_E4M3);
+          d[n / 4] |= (GP > 1 ? u : (u & 0xffu)) << (8 * (n % 4));
+        }
       }
       // P buffer j & 1 was last read by the PV of tile j - 2
-      if (j >= 2 && !wait_pv(j - 2)) {
-        ok = false;
-        break;
-      }
-      uint8_t* pbuf = sP + (j & 1) * PBLK;
+      if (j >= 2) wait_pv(j - 2);
+      uint8_t* pbuf = sP + (j & 1) * PBLK + (r >> 3) * (NC * 128) + (r & 7) * 16;
 #pragma unroll
-      for (int n = 0; n < ND; n += 2) {
-        const uint32_t u = to_e4m3x2(dg[n], dg[n + 1]);
-        pbuf[sw_offset(n, r)] = static_cast<uint8_t>(u);
-        if (n + 1 < ND) pbuf[sw_offset(n + 1, r)] = static_cast<uint8_t>(u >> 8);
-      }
-      if ((t0 + j + 1) * BKV > len) {
-        // the last tile: no stale V code behind the sequence reaches the product
+      for (int c = 0; c < NC; ++c)
+        *reinterpret_cast<uint4*>(pbuf + c * 128) = make_uint4(d[4 * c], d[4 * c + 1], d[4 * c + 2], d[4 * c + 3]);
+      if (last) {
+        // no stale V code behind the sequence reaches the product
         const int st = j % STAGES;
-        if (!mbar_wait_warp(&v_full[st], static_cast<uint32_t>((j / STAGES) & 1), abort_flag, p.status,
-                            kStatusTimeoutFull)) {
-          ok = false;
-          break;
-        }
+        if (ok) ok = mbar_wait_warp(&v_full[st], static_cast<uint32_t>((j / STAGES) & 1), abort_flag, p.status,
+                                    kStatusTimeoutFull);
         if (!valid) {
           uint4* row = reinterpret_cast<uint4*>(sKV + st * 2 * BLK + BLK + r * 128);
 #pragma unroll
@@ -490,31 +527,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       tc_fence_before();
       mbar_arrive(&p_full[j & 1]);
     }
-    ok = __all_sync(0xffffffffu, ok);
+    wait_pv(nt - 1);
     uint32_t ov[NO];
-#pragma unroll
-    for (int n = 0; n < NO; ++n) ov[n] = 0u;
-    if (ok && wait_pv(nt - 1)) {
-      if constexpr (NO == 16)
-        tmem_ld16(lane_addr + O_COL, ov);
-      else
-        tmem_ld32(lane_addr + O_COL, ov);
-      tmem_ld_wait();
-    }
+    if constexpr (NO == 16)
+      tmem_ld16(lane_addr + O_COL, ov);
+    else
+      tmem_ld32(lane_addr + O_COL, ov);
+    tmem_ld_wait();
     // sum of the softmax: the per-key partials over the 128 rows
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
       float v = l_part[h];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) lred[q4 * GP + h] = v;
+      if (lane == 0) red[q4 * GP + h] = v;
     }
-    group_sync();
-    const float back = two_to(max(R, 1) - 127) * (1.f / (1 << kTopLog2));
+    barrier_or(false);
+    const float back = two_to(R - 127) * (1.f / (1 << kTopLog2));
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
       if (h >= G || !ok) break;
-      const float l = lred[h] + lred[GP + h] + lred[2 * GP + h] + lred[3 * GP + h];
+      const float l = red[h] + red[GP + h] + red[2 * GP + h] + red[3 * GP + h];
       const float acc = fmaf(fmaf(__uint_as_float(ov[2 * GP + h]), 0.03125f, __uint_as_float(ov[GP + h])), 0.03125f,
                              __uint_as_float(ov[h]));
       const float o = l == 0.f ? 0.f : acc / l * back;
@@ -538,22 +571,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M); a NaN in a share stays one
+// o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M); a NaN in a share stays
+// one. The weights are made once per block, a thread per share, and the loads
+// of the shares' outputs do not wait for one another.
 __global__ void __launch_bounds__(D) combine_kernel(const Params p) {
+  __shared__ float wgt[D], red[4];
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
   const size_t base = (static_cast<size_t>(b) * p.hq + h) * p.splits;
   float mx = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.lse_part[base + s]);
+  for (int s = d; s < p.splits; s += D) mx = fmaxf(mx, p.lse_part[base + s]);
+  mx = max_over_warp(mx);
+  if ((d & 31) == 0) red[d >> 5] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   if (mx == -INFINITY) mx = 0.f;
   float num = 0.f, den = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float lse = p.lse_part[base + s];
-    if (lse == -INFINITY) continue;
-    const float w = exp2f(lse - mx);
-    den += w;
-    num += p.o_part[(base + s) * D + d] * w;
+  for (int s0 = 0; s0 < p.splits; s0 += D) {
+    const int n = min(D, p.splits - s0);
+    if (d < n) wgt[d] = exp2f(p.lse_part[base + s0 + d] - mx);  // an empty share: 2^-inf = 0
+    __syncthreads();
+    const float* o = p.o_part + (base + s0) * D + d;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float w = wgt[s];
+      den += w;
+      num += w == 0.f ? 0.f : o[static_cast<size_t>(s) * D] * w;  // an empty share's output is not written
+    }
+    __syncthreads();
   }
   p.out[static_cast<size_t>(b) * p.ldo + h * D + d] = __float2bfloat16(den == 0.f ? 0.f : num / den);
 }
@@ -606,7 +652,8 @@ extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const 
   p.G = hq / hkv;
   p.splits = splits;
   p.tiles_per_split = tiles_per_split;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  p.q_sign = scale < 0.f ? -1.f : (scale == 0.f ? 0.f : 1.f);
   p.o_part = o_part;
   p.lse_part = lse_part;
   p.out = static_cast<__nv_bfloat16*>(out);

@@ -111,17 +111,27 @@ __device__ void append_kv(const Append& p) {
   int pages[WIN];
 #pragma unroll
   for (int w = 0; w < WIN; ++w) pages[w] = s_page[w];
-  for (int i = tid; i < p.T; i += THREADS) {
-    const int slot = __ldg(p.slots + i);
-    if (slot < 0) continue;
-    const int page = slot / PAGE;
+  // eight independent loads at a time: the look through a long step's slots
+  // waits for memory T / 2048 times
+  for (int i0 = tid; i0 < p.T; i0 += 8 * THREADS) {
+    int slot[8];
 #pragma unroll
-    for (int w = 0; w < WIN; ++w) {
-      if (page != pages[w]) continue;
-      if (i < w0 + w)
-        s_lead[w] = 0;  // an earlier row leads this page
-      else if (!bad_pos(p, i))
-        atomicMax(&s_row[w][slot % PAGE], i);
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * THREADS;
+      slot[u] = i < p.T ? __ldg(p.slots + i) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * THREADS;
+      const int page = slot[u] < 0 ? -2 : slot[u] / PAGE;
+#pragma unroll
+      for (int w = 0; w < WIN; ++w) {
+        if (page != pages[w]) continue;
+        if (i < w0 + w)
+          s_lead[w] = 0;  // an earlier row leads this page
+        else if (!bad_pos(p, i))
+          atomicMax(&s_row[w][slot[u] % PAGE], i);
+      }
     }
   }
   __syncthreads();
@@ -131,6 +141,10 @@ __device__ void append_kv(const Append& p) {
   for (int task = warp; task < WIN * n_heads; task += THREADS / 32) {
     const int w = task / n_heads;
     if (!s_lead[w]) continue;
+    // lane o (of 16) knows the batch row of the page's slot o
+    const int my_row = s_row[w][lane % PAGE];
+    const uint32_t live = __ballot_sync(0xffffffffu, my_row >= 0) & 0xffffu;
+    if (live == 0) continue;  // every row of the page has a bad position
     const int hh = y * p.group_heads + task % n_heads;
     const bool is_v = hh >= p.hkv;
     const int head = is_v ? hh - p.hkv : hh;
@@ -138,71 +152,102 @@ __device__ void append_kv(const Append& p) {
     uint8_t* sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
     uint8_t* codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
     const int e_old = *sf;
-    // this lane: dims 2 lane, 2 lane + 1 and their partners 64 further
-    float x[PAGE][4];
-    float amax = 0.f;
+    const int my_pos = my_row >= 0 && !is_v ? p.pos[my_row] : 0;
+    // this lane: dims 2 lane, 2 lane + 1 and their partners 64 further. All
+    // rows are loaded before any is used, without branches: slots that the
+    // batch does not write read its first row and count as zeros.
+    uint32_t raw[PAGE][2];
 #pragma unroll
     for (int o = 0; o < PAGE; ++o) {
-      const int r = s_row[w][o];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[o][i] = 0.f;
-      if (r < 0) continue;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qkv + static_cast<size_t>(r) * p.ldqkv +
+      const int row = max(__shfl_sync(0xffffffffu, my_row, o), 0);
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qkv + static_cast<size_t>(row) * p.ldqkv +
                                                               static_cast<size_t>(p.hq + hh) * D);
-      const uint32_t a = src[lane], b = src[lane + 32];
-      if (is_v) {
-        x[o][0] = bf16_lo(a);
-        x[o][1] = bf16_hi(a);
-        x[o][2] = bf16_lo(b);
-        x[o][3] = bf16_hi(b);
+      if (live >> o & 1) {
+        raw[o][0] = __ldg(src + lane);
+        raw[o][1] = __ldg(src + lane + 32);
       } else {
-        const float4 cs =
-            reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(p.pos[r]) * D)[lane];
-        x[o][0] = rot_a(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
-        x[o][1] = rot_a(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
-        x[o][2] = rot_b(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
-        x[o][3] = rot_b(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
+        raw[o][0] = raw[o][1] = 0u;
       }
     }
-#pragma unroll
-    for (int o = 0; o < PAGE; ++o)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float m = fabsf(x[o][i]);
-        if (m <= FLT_MAX)
-          amax = fmaxf(amax, m);
-        else
-          x[o][i] = NAN;  // e4m3 has no infinity
+    // the four values of slot o: made twice (for the maximum and for the
+    // codes) rather than held, which halves the registers
+    auto values = [&](int o, const float4& cs, float (&x)[4]) {
+      const uint32_t a = raw[o][0], b = raw[o][1];
+      if (is_v) {
+        x[0] = bf16_lo(a);
+        x[1] = bf16_hi(a);
+        x[2] = bf16_lo(b);
+        x[3] = bf16_hi(b);
+      } else {
+        x[0] = rot_a(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
+        x[1] = rot_a(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
+        x[2] = rot_b(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
+        x[3] = rot_b(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
       }
+    };
+    auto angles = [&](int o) -> float4 {
+      const int pos = __shfl_sync(0xffffffffu, my_pos, o);
+      return is_v ? make_float4(0.f, 0.f, 0.f, 0.f)
+                  : __ldg(reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos) * D) + lane);
+    };
+    float amax = 0.f;
+#pragma unroll
+    for (int o0 = 0; o0 < PAGE; o0 += 4) {
+      if ((live >> o0 & 0xfu) == 0) continue;
+      float4 cs[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) cs[u] = angles(o0 + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float x[4];
+        values(o0 + u, cs[u], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float m = fabsf(x[i]);
+          if (m <= FLT_MAX) amax = fmaxf(amax, m);  // finite values set the scale
+        }
+      }
+    }
     // non-negative floats are ordered like their bits
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-    const bool anew = s_row[w][0] >= 0;
-    bool any = false;
-#pragma unroll
-    for (int o = 0; o < PAGE; ++o) any = any || s_row[w][o] >= 0;
-    if (!any) continue;  // every row of the page has a bad position
+    const bool anew = live & 1;
     const int e = anew ? scale_exp(amax) : max(scale_exp(amax), e_old);
     const float inv = two_to(127 - e);
     if (!anew && e > e_old) {
       // one rounding more for codes that become subnormal, none for others
       const float f = two_to(max(e_old - e, -60));
+      uint32_t old[PAGE];
+#pragma unroll
+      for (int o = 0; o < PAGE; ++o)
+        if (!(live >> o & 1)) old[o] = reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(o) * p.hkv * D)[lane];
 #pragma unroll
       for (int o = 0; o < PAGE; ++o) {
-        if (s_row[w][o] >= 0) continue;
-        uint16_t* c = reinterpret_cast<uint16_t*>(codes + static_cast<size_t>(o) * p.hkv * D);
-        const float2 u = from_e4m3x2(c[lane]), v = from_e4m3x2(c[lane + 32]);
-        c[lane] = to_e4m3x2(u.x * f, u.y * f);
-        c[lane + 32] = to_e4m3x2(v.x * f, v.y * f);
+        if (live >> o & 1) continue;
+        const float2 u = from_e4m3x2(static_cast<uint16_t>(old[o])), v = from_e4m3x2(static_cast<uint16_t>(old[o] >> 16));
+        reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(o) * p.hkv * D)[lane] =
+            to_e4m3x2(u.x * f, u.y * f) | static_cast<uint32_t>(to_e4m3x2(v.x * f, v.y * f)) << 16;
       }
     }
 #pragma unroll
-    for (int o = 0; o < PAGE; ++o) {
-      if (s_row[w][o] < 0) continue;
-      uint16_t* c = reinterpret_cast<uint16_t*>(codes + static_cast<size_t>(o) * p.hkv * D);
-      c[lane] = to_e4m3x2(x[o][0] * inv, x[o][1] * inv);
-      c[lane + 32] = to_e4m3x2(x[o][2] * inv, x[o][3] * inv);
+    for (int o0 = 0; o0 < PAGE; o0 += 4) {
+      if ((live >> o0 & 0xfu) == 0) continue;
+      float4 cs[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) cs[u] = angles(o0 + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int o = o0 + u;
+        float x[4];
+        values(o, cs[u], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] * inv : NAN;  // e4m3 has no infinity
+        if (live >> o & 1) {
+          uint16_t* c = reinterpret_cast<uint16_t*>(codes + static_cast<size_t>(o) * p.hkv * D);
+          c[lane] = to_e4m3x2(x[0], x[1]);
+          c[lane + 32] = to_e4m3x2(x[2], x[3]);
+        }
+      }
     }
-    __syncwarp();
     if (lane == 0) *sf = static_cast<uint8_t>(e);
   }
 }
@@ -257,7 +302,7 @@ __device__ void rotate_q(const Append& p) {
     }
 }
 
-__global__ void __launch_bounds__(THREADS) append_kernel(const Append p) {
+__global__ void __launch_bounds__(THREADS, 3) append_kernel(const Append p) {
   pdl_trigger();
   pdl_wait();
   if (static_cast<int>(blockIdx.x) < p.kv_ctas)

@@ -165,11 +165,11 @@ def plain(q, kc, vc, pages, first, hq, hkv, scale):
     return [t.reshape(n, -1) for t in (out, size, unit)]
 
 
-# Single tokens. A weight is split into three e4m3 digits: off by at most 2^-14 of itself or 2^-20 where a weight at
-# the running maximum is 2^6, so 2^-26 of it, times the code at the largest V scale. That maximum may lag behind the
-# row's largest weight, never be above it, so p_max >= 2^6 / (sum of weights): the second part is at most 2^-26 of
-# ``unit``. Scores are 32-bit sums of exact products: 2^-20 of sum |q k| (at most 2^7 here) is 2^-13 of a weight, its
-# exponential and the sums some 2^-20 more: 2^-12 + 2^-14 + ... < 2^-11 of ``size``.
+# Single tokens. A weight is rounded to f16 and that split into three e4m3 digits: off by at most 2^-12 of itself or
+# 2^-20 where a weight at the running maximum is 2^6, so 2^-26 of it, times the code at the largest V scale. That
+# maximum may lag behind the row's largest weight, never be above it, so p_max >= 2^6 / (sum of weights): the second
+# part is at most 2^-26 of ``unit``. Scores are 32-bit sums of exact products: 2^-20 of sum |q k| (at most 2^7 here) is
+# 2^-13 of a weight, its exponential and the sums some 2^-20 more: 2^-12 + 2^-13 + 2^-20 < 2^-11 of ``size``.
 TOKEN = (2 ** -11, 2 ** -26)
 # Prompts. Weights are rounded to bf16: 2^-8 of each, so of ``size``, and the scores, exponentials and sums as above.
 PROMPT = (2 ** -8 + 2 ** -11, 0.0)
