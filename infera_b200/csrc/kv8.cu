@@ -14,6 +14,13 @@
 // the batch, wherever they stand in it, so one warp owns a (page, head) of a
 // channel: the first row of a page (its leader) looks its page's other rows
 // up among all slots of the batch. Nothing depends on the order of arrival.
+// Bound by HBM for prompts and by latency for single rows: 8192 rows of 32 + 2 x
+// 8 heads take 43 us (189 MB: 4.4 TB/s, 0.67 of the copy rate), 2048 rows 14.4
+// us, 64 decoding rows 5.0 us, one 3.4 us. What it took: a warp loads all 16
+// rows of a page before it uses any, 16 bytes a lane (100 us with a row at a
+// time), and makes the rotated values twice rather than hold them (80
+// registers, 3 CTAs per SM). Spreading the K/V CTAs among those that rotate q
+// gained nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -28,7 +35,7 @@ namespace kv8 {
 
 constexpr int D = 128;
 constexpr int PAGE = 16;
-constexpr int WIN = 4;        // batch rows per K/V CTA
+constexpr int WIN = 8;        // most batch rows per K/V CTA
 constexpr int THREADS = 256;
 
 __device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
@@ -65,7 +72,8 @@ struct Append {
   long long num_slots;
   int max_pos;
   int* status;
-  int kv_ctas;        // CTAs of the K/V part, the rest rotate q
+  int kv_ctas;        // CTAs of the K/V part, the others rotate q
+  int win;            // batch rows per K/V CTA
   int head_groups;    // K/V CTAs per window of rows
   int group_heads;    // K and V heads of one such CTA
 };
@@ -84,129 +92,140 @@ __device__ __forceinline__ bool bad_pos(const Append& p, int t) {
   return x < 0 || x >= p.max_pos;
 }
 
-__device__ void append_kv(const Append& p) {
-  __shared__ int s_page[WIN];
-  __shared__ int s_lead[WIN];
+__device__ void append_kv(const Append& p, int cta) {
+  __shared__ int s_page[WIN];       // pages that start in this window
+  __shared__ int s_first[WIN];      // and their first rows here
+  __shared__ int s_lead[WIN];       // 0: an earlier row, of another window, leads the page
   __shared__ int s_row[WIN][PAGE];  // the last valid batch row of each slot of the page
-  const int w0 = static_cast<int>(blockIdx.x) / p.head_groups * WIN;
-  const int y = static_cast<int>(blockIdx.x) % p.head_groups;
-  const int tid = threadIdx.x;
-  int lead = 0;
-  if (tid < WIN) {
-    const int t = w0 + tid;
-    const int slot = t < p.T ? p.slots[t] : -1;
-    int page = slot < 0 ? -1 : slot / PAGE;
-    if (slot >= p.num_slots) {
-      page = -1;
-      if (y == 0) record_status_detail(p.status, kStatusBadIndex, 2, t, slot);
-    }
+  __shared__ int s_n;
+  const int w0 = cta / p.head_groups * p.win;
+  const int y = cta % p.head_groups;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 0) {
+    const int t = w0 + lane;
+    const int slot = lane < p.win && t < p.T ? p.slots[t] : -1;
+    const int before = slot >= 0 && t > 0 ? p.slots[t - 1] : -1;
+    if (slot >= p.num_slots && y == 0) record_status_detail(p.status, kStatusBadIndex, 2, t, slot);
     // a row right behind one of the same page is not its first
-    if (page >= 0 && t > 0 && p.slots[t - 1] >= 0 && p.slots[t - 1] / PAGE == page) page = -1;
-    s_page[tid] = page;
-    lead = page >= 0;
-    s_lead[tid] = lead;
+    const bool lead = slot >= 0 && slot < p.num_slots && (before < 0 || before / PAGE != slot / PAGE);
+    const uint32_t leads = __ballot_sync(0xffffffffu, lead);
+    if (lead) {
+      const int n = __popc(leads & ((1u << lane) - 1u));
+      s_page[n] = slot / PAGE;
+      s_first[n] = t;
+      s_lead[n] = 1;
+    }
+    if (lane == 0) s_n = __popc(leads);
   }
   if (tid < WIN * PAGE) s_row[tid / PAGE][tid % PAGE] = -1;
-  if (!__syncthreads_or(lead)) return;
-  int pages[WIN];
-#pragma unroll
-  for (int w = 0; w < WIN; ++w) pages[w] = s_page[w];
-  // eight independent loads at a time: the look through a long step's slots
-  // waits for memory T / 2048 times
-  for (int i0 = tid; i0 < p.T; i0 += 8 * THREADS) {
-    int slot[8];
+  __syncthreads();
+  const int n_lead = s_n;
+  if (n_lead == 0) return;
+  auto found = [&](int w, int i, int off) {  // row i writes slot `off` of page w
+    if (i < s_first[w])
+      s_lead[w] = 0;  // an earlier row leads this page
+    else if (!bad_pos(p, i))
+      atomicMax(&s_row[w][off], i);
+  };
+  // all loads of 8192 slots in flight at once: a long step's slots are waited
+  // for once
+  const int n4 = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0 ? p.T / 4 : 0;
+  for (int i0 = tid; i0 < n4; i0 += 8 * THREADS) {
+    int4 v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = i0 + u * THREADS;
-      slot[u] = i < p.T ? __ldg(p.slots + i) : -1;
+      v[u] = i < n4 ? __ldg(reinterpret_cast<const int4*>(p.slots) + i) : make_int4(-1, -1, -1, -1);
     }
+    for (int w = 0; w < n_lead; ++w) {
+      const int base = s_page[w] * PAGE;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = i0 + u * THREADS;
-      const int page = slot[u] < 0 ? -2 : slot[u] / PAGE;
-#pragma unroll
-      for (int w = 0; w < WIN; ++w) {
-        if (page != pages[w]) continue;
-        if (i < w0 + w)
-          s_lead[w] = 0;  // an earlier row leads this page
-        else if (!bad_pos(p, i))
-          atomicMax(&s_row[w][slot[u] % PAGE], i);
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * THREADS;
+        if (i >= n4) break;
+        const unsigned o0 = v[u].x - base, o1 = v[u].y - base, o2 = v[u].z - base, o3 = v[u].w - base;
+        if (min(min(o0, o1), min(o2, o3)) < PAGE) {
+          if (o0 < PAGE) found(w, 4 * i, o0);
+          if (o1 < PAGE) found(w, 4 * i + 1, o1);
+          if (o2 < PAGE) found(w, 4 * i + 2, o2);
+          if (o3 < PAGE) found(w, 4 * i + 3, o3);
+        }
       }
+    }
+  }
+  for (int i = 4 * n4 + tid; i < p.T; i += THREADS) {
+    const int slot = __ldg(p.slots + i);
+    for (int w = 0; w < n_lead; ++w) {
+      const unsigned off = slot - s_page[w] * PAGE;
+      if (off < PAGE) found(w, i, off);
     }
   }
   __syncthreads();
-  const int warp = tid >> 5, lane = tid & 31;
   const int h_end = min(2 * p.hkv, (y + 1) * p.group_heads);
   const int n_heads = h_end - y * p.group_heads;
-  for (int task = warp; task < WIN * n_heads; task += THREADS / 32) {
+  for (int task = warp; task < n_lead * n_heads; task += THREADS / 32) {
     const int w = task / n_heads;
     if (!s_lead[w]) continue;
-    // lane o (of 16) knows the batch row of the page's slot o
-    const int my_row = s_row[w][lane % PAGE];
-    const uint32_t live = __ballot_sync(0xffffffffu, my_row >= 0) & 0xffffu;
-    if (live == 0) continue;  // every row of the page has a bad position
     const int hh = y * p.group_heads + task % n_heads;
     const bool is_v = hh >= p.hkv;
     const int head = is_v ? hh - p.hkv : hh;
-    const long long page = pages[w];
+    const long long page = s_page[w];
     uint8_t* sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
     uint8_t* codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
     const int e_old = *sf;
-    const int my_pos = my_row >= 0 && !is_v ? p.pos[my_row] : 0;
-    // this lane: dims 2 lane, 2 lane + 1 and their partners 64 further. All
-    // rows are loaded before any is used, without branches: slots that the
-    // batch does not write read its first row and count as zeros.
-    uint32_t raw[PAGE][2];
+    // Eight lanes per row, four slots of the page at a time (step s: slots
+    // 4 s .. 4 s + 3): a lane has dims 8 c .. 8 c + 7 and their partners 64
+    // further. All rows are loaded before any is used.
+    const int c = lane & 7, sub = lane >> 3;
+    int pos[4];
+    uint32_t live = 0;  // slots that the batch writes (bit 4 s + sub)
+    uint4 a[4], b[4];
 #pragma unroll
-    for (int o = 0; o < PAGE; ++o) {
-      const int row = max(__shfl_sync(0xffffffffu, my_row, o), 0);
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.qkv + static_cast<size_t>(row) * p.ldqkv +
-                                                              static_cast<size_t>(p.hq + hh) * D);
-      if (live >> o & 1) {
-        raw[o][0] = __ldg(src + lane);
-        raw[o][1] = __ldg(src + lane + 32);
-      } else {
-        raw[o][0] = raw[o][1] = 0u;
+    for (int s = 0; s < 4; ++s) {
+      const int row = s_row[w][4 * s + sub];
+      a[s] = b[s] = make_uint4(0u, 0u, 0u, 0u);
+      pos[s] = -1;
+      if (row >= 0) {
+        const __nv_bfloat16* src =
+            p.qkv + static_cast<size_t>(row) * p.ldqkv + static_cast<size_t>(p.hq + hh) * D + c * 8;
+        a[s] = __ldg(reinterpret_cast<const uint4*>(src));
+        b[s] = __ldg(reinterpret_cast<const uint4*>(src + D / 2));
+        pos[s] = __ldg(p.pos + row);
       }
+      const uint32_t on = __ballot_sync(0xffffffffu, row >= 0);  // a bit of each row's first lane
+      live |= ((on & 1u) | (on >> 7 & 2u) | (on >> 14 & 4u) | (on >> 21 & 8u)) << (4 * s);
     }
-    // the four values of slot o: made twice (for the maximum and for the
-    // codes) rather than held, which halves the registers
-    auto values = [&](int o, const float4& cs, float (&x)[4]) {
-      const uint32_t a = raw[o][0], b = raw[o][1];
-      if (is_v) {
-        x[0] = bf16_lo(a);
-        x[1] = bf16_hi(a);
-        x[2] = bf16_lo(b);
-        x[3] = bf16_hi(b);
-      } else {
-        x[0] = rot_a(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
-        x[1] = rot_a(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
-        x[2] = rot_b(bf16_lo(a), bf16_lo(b), cs.x, cs.y);
-        x[3] = rot_b(bf16_hi(a), bf16_hi(b), cs.z, cs.w);
+    if (live == 0) continue;  // every row of the page has a bad position
+    auto values = [&](int s, float (&x)[16]) {
+      const uint32_t av[4] = {a[s].x, a[s].y, a[s].z, a[s].w}, bv[4] = {b[s].x, b[s].y, b[s].z, b[s].w};
+      if (is_v || pos[s] < 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[2 * i] = bf16_lo(av[i]);
+          x[2 * i + 1] = bf16_hi(av[i]);
+          x[8 + 2 * i] = bf16_lo(bv[i]);
+          x[8 + 2 * i + 1] = bf16_hi(bv[i]);
+        }
+        return;
       }
-    };
-    auto angles = [&](int o) -> float4 {
-      const int pos = __shfl_sync(0xffffffffu, my_pos, o);
-      return is_v ? make_float4(0.f, 0.f, 0.f, 0.f)
-                  : __ldg(reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos) * D) + lane);
+      const float4* at = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos[s]) * D + c * 16);
+      const float4 cs[4] = {__ldg(at), __ldg(at + 1), __ldg(at + 2), __ldg(at + 3)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = rot_a(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
+        x[2 * i + 1] = rot_a(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
+        x[8 + 2 * i] = rot_b(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
+        x[8 + 2 * i + 1] = rot_b(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
+      }
     };
     float amax = 0.f;
 #pragma unroll
-    for (int o0 = 0; o0 < PAGE; o0 += 4) {
-      if ((live >> o0 & 0xfu) == 0) continue;
-      float4 cs[4];
+    for (int s = 0; s < 4; ++s) {
+      if ((live >> (4 * s) & 15u) == 0) continue;
+      float x[16];
+      values(s, x);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) cs[u] = angles(o0 + u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float x[4];
-        values(o0 + u, cs[u], x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float m = fabsf(x[i]);
-          if (m <= FLT_MAX) amax = fmaxf(amax, m);  // finite values set the scale
-        }
-      }
+      for (int i = 0; i < 16; ++i) amax = fabsf(x[i]) <= FLT_MAX ? fmaxf(amax, fabsf(x[i])) : amax;
     }
     // non-negative floats are ordered like their bits
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
@@ -216,36 +235,35 @@ __device__ void append_kv(const Append& p) {
     if (!anew && e > e_old) {
       // one rounding more for codes that become subnormal, none for others
       const float f = two_to(max(e_old - e, -60));
-      uint32_t old[PAGE];
 #pragma unroll
-      for (int o = 0; o < PAGE; ++o)
-        if (!(live >> o & 1)) old[o] = reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(o) * p.hkv * D)[lane];
+      for (int s = 0; s < 4; ++s) {
+        if (live >> (4 * s + sub) & 1) continue;
+        uint4* at = reinterpret_cast<uint4*>(codes + static_cast<size_t>(4 * s + sub) * p.hkv * D) + c;
+        const uint4 old = *at;
+        uint32_t v[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
-      for (int o = 0; o < PAGE; ++o) {
-        if (live >> o & 1) continue;
-        const float2 u = from_e4m3x2(static_cast<uint16_t>(old[o])), v = from_e4m3x2(static_cast<uint16_t>(old[o] >> 16));
-        reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(o) * p.hkv * D)[lane] =
-            to_e4m3x2(u.x * f, u.y * f) | static_cast<uint32_t>(to_e4m3x2(v.x * f, v.y * f)) << 16;
+        for (int i = 0; i < 4; ++i) {
+          const float2 u0 = from_e4m3x2(static_cast<uint16_t>(v[i])), u1 = from_e4m3x2(static_cast<uint16_t>(v[i] >> 16));
+          v[i] = to_e4m3x2(u0.x * f, u0.y * f) | static_cast<uint32_t>(to_e4m3x2(u1.x * f, u1.y * f)) << 16;
+        }
+        *at = make_uint4(v[0], v[1], v[2], v[3]);
       }
     }
 #pragma unroll
-    for (int o0 = 0; o0 < PAGE; o0 += 4) {
-      if ((live >> o0 & 0xfu) == 0) continue;
-      float4 cs[4];
+    for (int s = 0; s < 4; ++s) {
+      if ((live >> (4 * s) & 15u) == 0) continue;
+      float x[16];
+      values(s, x);  // made again (the angles come from the first-level cache) rather than held
+      uint32_t v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) cs[u] = angles(o0 + u);
+      for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] * inv : NAN;  // e4m3 has no infinity
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int o = o0 + u;
-        float x[4];
-        values(o, cs[u], x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] * inv : NAN;  // e4m3 has no infinity
-        if (live >> o & 1) {
-          uint16_t* c = reinterpret_cast<uint16_t*>(codes + static_cast<size_t>(o) * p.hkv * D);
-          c[lane] = to_e4m3x2(x[0], x[1]);
-          c[lane + 32] = to_e4m3x2(x[2], x[3]);
-        }
+      for (int i = 0; i < 4; ++i)
+        v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | static_cast<uint32_t>(to_e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16;
+      if (pos[s] >= 0) {
+        uint8_t* at = codes + static_cast<size_t>(4 * s + sub) * p.hkv * D + c * 8;
+        *reinterpret_cast<uint2*>(at) = make_uint2(v[0], v[1]);
+        *reinterpret_cast<uint2*>(at + D / 2) = make_uint2(v[2], v[3]);
       }
     }
     if (lane == 0) *sf = static_cast<uint8_t>(e);
@@ -268,9 +286,9 @@ __device__ __forceinline__ void rotate8(const uint4& a, const uint4& b, const fl
   *nb = make_uint4(rb[0], rb[1], rb[2], rb[3]);
 }
 
-__device__ void rotate_q(const Append& p) {
+__device__ void rotate_q(const Append& p, int cta) {
   const int ng = (p.hq + Q_HEADS - 1) / Q_HEADS;
-  const long long idx = static_cast<long long>(blockIdx.x - p.kv_ctas) * THREADS + threadIdx.x;
+  const long long idx = static_cast<long long>(cta) * THREADS + threadIdx.x;
   const int c = static_cast<int>(idx & 7);  // dims 8c .. 8c + 7 and their partners
   const long long rest = idx >> 3;
   const long long t = rest / ng;
@@ -305,10 +323,12 @@ __device__ void rotate_q(const Append& p) {
 __global__ void __launch_bounds__(THREADS, 3) append_kernel(const Append p) {
   pdl_trigger();
   pdl_wait();
-  if (static_cast<int>(blockIdx.x) < p.kv_ctas)
-    append_kv(p);
+  // the K/V CTAs, which take longest, first
+  const int cta = blockIdx.x;
+  if (cta < p.kv_ctas)
+    append_kv(p, cta);
   else
-    rotate_q(p);
+    rotate_q(p, cta - p.kv_ctas);
 }
 
 // ---------------------------------------------------------------- expansion
@@ -423,11 +443,14 @@ extern "C" int ib_kv8_append(const void* qkv, int T, int ldqkv, void* q_out, int
   p.num_slots = num_slots;
   p.max_pos = max_pos;
   p.status = status;
-  // few rows: two heads per CTA, so that every (row, head) has a warp of its
-  // own; many rows (prompts: one leader in 16 rows): a warp for each of 8 heads
-  p.group_heads = T <= 512 ? 2 : 8;
+  // Few rows: 4 of them and two heads per CTA, so that every (row, head) has a
+  // warp of its own. Many rows (prompts, one leading row in 16): fewer CTAs that
+  // lead nothing, and the look through the slots serves all heads.
+  const bool many = T > 512;
+  p.win = many ? 8 : 4;
+  p.group_heads = many ? 8 : 2;
   p.head_groups = (2 * hkv + p.group_heads - 1) / p.group_heads;
-  const long long kv_ctas = static_cast<long long>((T + WIN - 1) / WIN) * p.head_groups;
+  const long long kv_ctas = static_cast<long long>((T + p.win - 1) / p.win) * p.head_groups;
   const long long q_items = static_cast<long long>(T) * ((hq + Q_HEADS - 1) / Q_HEADS) * 8;
   const long long ctas = kv_ctas + (q_items + THREADS - 1) / THREADS;
   if (ctas > 0x7fffffffLL) return -1;
