@@ -46,18 +46,15 @@
 // merged by a combine kernel.
 //
 // Bound by HBM: two 8-bit codes per key, dim and KV head.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
-#include "sm100.cuh"
+#include "kv8.cuh"
 #include "tma_host.h"
 
 namespace ib200 {
 namespace dq8 {
 
-constexpr int D = 128;
+using namespace kv8;
+
 constexpr int BKV = 128;
-constexpr int PAGE = 16;
 constexpr int STAGES = 3;
 constexpr int BLK = 128 * 128;      // 128 rows x 128 codes
 constexpr int NS = 16;              // columns of S
@@ -97,33 +94,13 @@ struct Params {
   int* status;
 };
 
-__device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
-  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-}
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<uint16_t>(v), __NV_E4M3)));
-}
-// byte offset of (row, byte k) in a K-major block of 128-byte rows, 128-byte swizzle
-__device__ __forceinline__ uint32_t sw_offset(int row, int k) {
-  return static_cast<uint32_t>(row * 128 + (((k >> 4) ^ (row & 7)) << 4) + (k & 15));
-}
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // The leading e4m3 digits of two f16 values (|x| <= 256), and the rest of the
 // values after it, 32 times larger (exact in f16).
 __device__ __forceinline__ uint32_t digit2(__half2& x) {
   const __half2_raw raw = x;
   const uint32_t d = __nv_cvt_halfraw2_to_fp8x2(raw, __NV_SATFINITE, __NV_E4M3);
-  const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(d), __NV_E4M3));
-  x = __hmul2(__hsub2(x, back), __float2half2_rn(32.f));
+  x = __hmul2(__hsub2(x, from_e4m3x2_h(d)), __float2half2_rn(32.f));
   return d;
-}
-__device__ __forceinline__ float max_over_warp(float x) {  // a NaN counts as nothing
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-  return r;
 }
 // Barrier of the four softmax warps that ORs a predicate. Every one of them
 // passes the same number of these, whatever a bounded wait in between gave,
@@ -345,17 +322,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const int r = q4 * 32 + lane;     // key row of S, dim row of O
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     bool ok = true;
-    // Exponents of the pages of 16 tiles: one page per thread. A page id
-    // outside the cache (a bad table) loads zeros through the tensor map and
-    // takes the smallest exponents here, as do places behind the sequence.
+    // exponents of the pages of 16 tiles: one page per thread
     auto page_of = [&](int j) -> int {
       const int lp = (t0 + j) * (BKV / PAGE) + t;
       return lp < n_pages && j < nt ? __ldg(bt + lp) : -1;
     };
     auto load_sf = [&](int page) -> uint32_t {
-      if (page < 0 || page >= p.num_pages) return 0x0101u;
-      const size_t at = static_cast<size_t>(page) * p.hkv + kvh;
-      return max(static_cast<uint32_t>(p.ksf[at]), 1u) | max(static_cast<uint32_t>(p.vsf[at]), 1u) << 8;
+      int ke, ve;
+      page_exponents(p.ksf, p.vsf, p.num_pages, p.hkv, kvh, page, ke, ve);
+      return static_cast<uint32_t>(ke | ve << 8);
     };
     uint32_t sf_next = load_sf(page_of(0));  // this thread's page of the next batch
     int page_next = -1;
@@ -571,37 +546,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M); a NaN in a share stays
-// one. The weights are made once per block, a thread per share, and the loads
-// of the shares' outputs do not wait for one another.
-__global__ void __launch_bounds__(D) combine_kernel(const Params p) {
-  __shared__ float wgt[D], red[4];
+template <int W>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) combine_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
-  const size_t base = (static_cast<size_t>(b) * p.hq + h) * p.splits;
-  float mx = -INFINITY;
-  for (int s = d; s < p.splits; s += D) mx = fmaxf(mx, p.lse_part[base + s]);
-  mx = max_over_warp(mx);
-  if ((d & 31) == 0) red[d >> 5] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (mx == -INFINITY) mx = 0.f;
-  float num = 0.f, den = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += D) {
-    const int n = min(D, p.splits - s0);
-    if (d < n) wgt[d] = exp2f(p.lse_part[base + s0 + d] - mx);  // an empty share: 2^-inf = 0
-    __syncthreads();
-    const float* o = p.o_part + (base + s0) * D + d;
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float w = wgt[s];
-      den += w;
-      num += w == 0.f ? 0.f : o[static_cast<size_t>(s) * D] * w;  // an empty share's output is not written
-    }
-    __syncthreads();
-  }
-  p.out[static_cast<size_t>(b) * p.ldo + h * D + d] = __float2bfloat16(den == 0.f ? 0.f : num / den);
+  const int b = blockIdx.x, h = blockIdx.y * (MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
+  if (h >= p.hq) return;
+  const size_t part = (static_cast<size_t>(b) * p.hq + h) * p.splits;
+  merge_shares<W>(p.o_part + part * D, p.lse_part + part, p.splits, p.out + static_cast<size_t>(b) * p.ldo + h * D);
 }
 
 using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const Params);
@@ -626,9 +578,10 @@ extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const 
   if (B <= 0) return 0;
   if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 8 || splits < 1 || tiles_per_split < 1 || (ldq % 2) != 0 ||
       B > 65535 || splits > 65535 || num_slots < PAGE || num_slots % PAGE != 0 || max_pages < 0 ||
-      (reinterpret_cast<uintptr_t>(q) & 3) != 0)
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 3) != 0 || (ldo % 2) != 0)
     return -1;
-  if (splits > 1 && (o_part == nullptr || lse_part == nullptr)) return -1;
+  if (splits > 1 && (o_part == nullptr || lse_part == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0))
+    return -1;
   const int kvw = hkv * D;
   CUtensorMap tk, tv, tk8, tv8;
   const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -675,7 +628,10 @@ extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const 
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   if (splits > 1) {
-    launch_pdl(combine_kernel, dim3(B, hq), D, 0, stream, p);
+    if (merge_warps(static_cast<long long>(B) * hq, splits) > 1)
+      launch_pdl(combine_kernel<MERGE_WARPS>, dim3(B, hq), MERGE_WARPS * 32, 0, stream, p);
+    else
+      launch_pdl(combine_kernel<1>, dim3(B, (hq + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return static_cast<int>(e);
   }

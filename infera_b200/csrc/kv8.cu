@@ -1,5 +1,4 @@
-// The 8-bit paged KV cache: append (with the rotation of q and k) and the
-// expansion of pages to bf16 for prompt attention.
+// Append to the 8-bit paged KV cache, with the rotation of q and k.
 //
 // One layer's channel (K or V) holds e4m3 codes [num_slots, hkv * 128]
 // (slot = page * 16 + offset) and one power-of-two scale per page and head,
@@ -21,26 +20,15 @@
 // time), and makes the rotated values twice rather than hold them (80
 // registers, 3 CTAs per SM). Spreading the K/V CTAs among those that rotate q
 // gained nothing.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-#include <cuda_runtime.h>
 #include <float.h>
-#include <stdint.h>
 
-#include "sm100.cuh"
+#include "kv8.cuh"
 
 namespace ib200 {
 namespace kv8 {
 
-constexpr int D = 128;
-constexpr int PAGE = 16;
 constexpr int WIN = 8;        // most batch rows per K/V CTA
 constexpr int THREADS = 256;
-
-__device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
-  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-}
 
 // Smallest biased exponent e (1..254) with amax <= 448 * 2^(e - 127);
 // 448 = 1.75 * 2^8. amax >= 0 and finite; below 2^-126 it counts as 0.
@@ -48,15 +36,6 @@ __device__ __forceinline__ int scale_exp(float amax) {
   const uint32_t b = __float_as_uint(amax);
   const int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
   return max(1, min(254, e));
-}
-
-__device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-
-__device__ __forceinline__ float2 from_e4m3x2(uint16_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
-  return __half22float2(__half2(h));
 }
 
 struct Append {
@@ -243,8 +222,8 @@ __device__ void append_kv(const Append& p, int cta) {
         uint32_t v[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 u0 = from_e4m3x2(static_cast<uint16_t>(v[i])), u1 = from_e4m3x2(static_cast<uint16_t>(v[i] >> 16));
-          v[i] = to_e4m3x2(u0.x * f, u0.y * f) | static_cast<uint32_t>(to_e4m3x2(u1.x * f, u1.y * f)) << 16;
+          const float2 u0 = from_e4m3x2(v[i] & 0xffffu), u1 = from_e4m3x2(v[i] >> 16);
+          v[i] = to_e4m3x2(u0.x * f, u0.y * f) | to_e4m3x2(u1.x * f, u1.y * f) << 16;
         }
         *at = make_uint4(v[0], v[1], v[2], v[3]);
       }
@@ -259,7 +238,7 @@ __device__ void append_kv(const Append& p, int cta) {
       for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] * inv : NAN;  // e4m3 has no infinity
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | static_cast<uint32_t>(to_e4m3x2(x[4 * i + 2], x[4 * i + 3])) << 16;
+        v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | to_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16;
       if (pos[s] >= 0) {
         uint8_t* at = codes + static_cast<size_t>(4 * s + sub) * p.hkv * D + c * 8;
         *reinterpret_cast<uint2*>(at) = make_uint2(v[0], v[1]);
@@ -331,82 +310,6 @@ __global__ void __launch_bounds__(THREADS, 3) append_kernel(const Append p) {
     rotate_q(p, cta - p.kv_ctas);
 }
 
-// ---------------------------------------------------------------- expansion
-
-struct Expand {
-  const uint8_t *kq, *ksf, *vq, *vsf;
-  const int* block_table;
-  const int* bt_rows;
-  int ld_table;
-  const int* ctx_len;
-  int hkv, num_pages, most;      // most: pages of the longest sequence
-  long long out_pages;           // pages that k_out / v_out hold
-  __nv_bfloat16 *k_out, *v_out;  // [out_pages * 16, hkv * 128]
-  int* table_out;                // [sequences, most]
-  int* status;
-};
-
-__device__ __forceinline__ uint4 expand8(uint32_t lo, uint32_t hi, float f) {
-  const float2 a = from_e4m3x2(static_cast<uint16_t>(lo)), b = from_e4m3x2(static_cast<uint16_t>(lo >> 16));
-  const float2 c = from_e4m3x2(static_cast<uint16_t>(hi)), d = from_e4m3x2(static_cast<uint16_t>(hi >> 16));
-  return make_uint4(pack_bf16(a.x * f, a.y * f), pack_bf16(b.x * f, b.y * f), pack_bf16(c.x * f, c.y * f),
-                    pack_bf16(d.x * f, d.y * f));
-}
-
-// One CTA per page of a sequence: its K and V rows in bf16 at the sequence's
-// consecutive pages of the output (sequence after sequence), zeros behind the
-// sequence's last row, so that no stale code (a NaN) reaches the tensor core.
-__global__ void __launch_bounds__(256) expand_kernel(const Expand p) {
-  pdl_trigger();
-  pdl_wait();
-  const int pg = blockIdx.x, seq = blockIdx.y;
-  const int ctx = p.ctx_len[seq];
-  if (pg * PAGE >= ctx) return;
-  long long base = 0;
-  for (int j = 0; j < seq; ++j) base += (max(p.ctx_len[j], 0) + PAGE - 1) / PAGE;
-  const long long dst = base + pg;
-  if (dst >= p.out_pages) {  // lengths on the device disagree with the host's
-    if (threadIdx.x == 0) {
-      p.table_out[static_cast<size_t>(seq) * p.most + pg] = 0;
-      record_status(p.status, kStatusBadArgs);
-    }
-    return;
-  }
-  const int row = p.bt_rows != nullptr ? p.bt_rows[seq] : seq;
-  const int page = p.block_table[static_cast<size_t>(row) * p.ld_table + pg];
-  const bool ok = page >= 0 && page < p.num_pages;
-  if (threadIdx.x == 0) {
-    p.table_out[static_cast<size_t>(seq) * p.most + pg] = static_cast<int>(dst);
-    if (!ok) record_status_detail(p.status, kStatusBadIndex, 2, seq, page);
-  }
-  const int rows = min(PAGE, ctx - pg * PAGE);
-  const int per_row = p.hkv * (D / 16);  // 16-code pieces of a row
-  const int n = PAGE * per_row;
-  const size_t src = static_cast<size_t>(ok ? page : 0) * n;
-  const uint4* kin = reinterpret_cast<const uint4*>(p.kq) + src;
-  const uint4* vin = reinterpret_cast<const uint4*>(p.vq) + src;
-  uint4* kout = reinterpret_cast<uint4*>(p.k_out) + static_cast<size_t>(dst) * n * 2;
-  uint4* vout = reinterpret_cast<uint4*>(p.v_out) + static_cast<size_t>(dst) * n * 2;
-  const uint8_t* ksf = p.ksf + static_cast<size_t>(ok ? page : 0) * p.hkv;
-  const uint8_t* vsf = p.vsf + static_cast<size_t>(ok ? page : 0) * p.hkv;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const bool live = ok && i / per_row < rows;
-    const int head = (i % per_row) / (D / 16);
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (live) {
-      a = __ldg(kin + i);
-      b = __ldg(vin + i);
-    }
-    const float fk = two_to(max(static_cast<int>(ksf[head]), 1) - 127);
-    const float fv = two_to(max(static_cast<int>(vsf[head]), 1) - 127);
-    kout[2 * i] = expand8(a.x, a.y, fk);
-    kout[2 * i + 1] = expand8(a.z, a.w, fk);
-    vout[2 * i] = expand8(b.x, b.y, fv);
-    vout[2 * i + 1] = expand8(b.z, b.w, fv);
-  }
-}
-
 }  // namespace kv8
 }  // namespace ib200
 
@@ -456,39 +359,6 @@ extern "C" int ib_kv8_append(const void* qkv, int T, int ldqkv, void* q_out, int
   if (ctas > 0x7fffffffLL) return -1;
   p.kv_ctas = static_cast<int>(kv_ctas);
   launch_pdl(append_kernel, dim3(static_cast<unsigned>(ctas)), THREADS, 0, stream, p);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : static_cast<int>(e);
-}
-
-// The pages of n_seqs sequences (ctx_len keys each, block_table rows bt_rows
-// or 0, 1, ...) in bf16: k_out / v_out [out_pages * 16, hkv * 128], sequence
-// after sequence, and their page table table_out [n_seqs, most]; most: the
-// pages of the longest sequence. Rows behind a sequence's last are zero.
-extern "C" int ib_kv8_expand(const void* kq, const void* ksf, const void* vq, const void* vsf, int num_pages,
-                             int hkv, const int* block_table, const int* bt_rows, int ld_table, const int* ctx_len,
-                             int n_seqs, int most, long long out_pages, void* k_out, void* v_out, int* table_out,
-                             int* status, cudaStream_t stream) {
-  using namespace ib200::kv8;
-  if (n_seqs <= 0 || most <= 0) return 0;
-  if (hkv < 1 || n_seqs > 65535 || num_pages < 1) return -1;
-  Expand p;
-  p.kq = static_cast<const uint8_t*>(kq);
-  p.ksf = static_cast<const uint8_t*>(ksf);
-  p.vq = static_cast<const uint8_t*>(vq);
-  p.vsf = static_cast<const uint8_t*>(vsf);
-  p.block_table = block_table;
-  p.bt_rows = bt_rows;
-  p.ld_table = ld_table;
-  p.ctx_len = ctx_len;
-  p.hkv = hkv;
-  p.num_pages = num_pages;
-  p.most = most;
-  p.out_pages = out_pages;
-  p.k_out = static_cast<__nv_bfloat16*>(k_out);
-  p.v_out = static_cast<__nv_bfloat16*>(v_out);
-  p.table_out = table_out;
-  p.status = status;
-  launch_pdl(expand_kernel, dim3(most, n_seqs), 256, 0, stream, p);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }

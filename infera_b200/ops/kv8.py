@@ -296,7 +296,7 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
         out = torch.empty(B, hq * HEAD_DIM, dtype=_BF16, device=q.device)
         ldo = hq * HEAD_DIM
     else:
-        ldo = _check_rows("out", out, B, hq * HEAD_DIM, dev, 2)
+        ldo = _check_rows("out", out, B, hq * HEAD_DIM, dev, 4)
     if B == 0:
         return out
     if dev < 0:
@@ -340,24 +340,41 @@ def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale,
 # ---------------------------------------------------------------- prompt attention
 
 
+def prefill_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148
+                 ) -> tuple[int, int, int]:
+    """(items, rows, key shares) of :func:`attn_prefill`: an item is 256 rows
+    of (token, query head of one KV head). The share count minimises waves x
+    (key tiles per share + 2 to start), in units of the 1.6 us that a tile of
+    128 keys takes, plus the merge's launch and its bytes (each share's fp32
+    row written and read)."""
+    per = 256 // (hq // hkv)
+    rows = sum(q_lens)
+    items = sum(-(-n // per) for n in q_lens)
+    ctas = items * hkv
+    tiles = -(-max(ctx_lens, default=0) // 128)
+    best, best_cost = 1, -(-ctas // num_sms) * (tiles + 2)
+    for sp in range(2, min(32, tiles // 2) + 1):
+        cost = -(-ctas * sp // num_sms) * (-(-tiles // sp) + 2) + 2 + rows * hq * sp / 7800
+        if cost < best_cost:
+            best, best_cost = sp, cost
+    return items, rows, best
+
+
 def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_table: torch.Tensor,
-                 q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, tiles: torch.Tensor, hq: int,
-                 hkv: int, scale: float, out: torch.Tensor | None = None,
+                 q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, tiles: torch.Tensor | None,
+                 hq: int, hkv: int, scale: float, out: torch.Tensor | None = None,
                  host_meta: tuple[list[int], list[int]] | None = None, bt_rows: torch.Tensor | None = None,
                  kv_splits: int | None = None, tile_rows: int | None = None) -> torch.Tensor:
     """Causal attention for chunks of new tokens whose K/V already sit in the
     8-bit cache; arguments as of :func:`infera_b200.ops.kernels.attn_prefill`.
     ``host_meta`` (q lengths, context lengths on the host; read back from the
-    device without it) sizes the workspace.
-
-    Each sequence's pages are expanded to bf16 once (code times power of two is
-    exact there) and the flash-attention kernel reads those: its work is
-    bound by the softmax and the bf16 tensor core, so the expansion's bytes
-    cost less than conversions inside the kernel, which every query tile and
-    every query head of a group would repeat."""
-    _check_heads(hq, hkv, hq)
+    device without it) sizes the grid. The kernel makes its own work items of
+    256 / group tokens, so ``tiles`` and ``tile_rows`` are not used. Up to 8
+    query heads per KV head. A row that sees no key (a context shorter than
+    its chunk) is zero; rows of no sequence are left as they are."""
+    _check_heads(hq, hkv, 8)
     n, T, dev = q_len.shape[0], q.shape[0], q.get_device()
-    _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
+    ldq = _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
     _check_i32("q_start", q_start, n, dev)
     _check_i32("q_len", q_len, n, dev)
     _check_i32("ctx_len", ctx_len, n, dev)
@@ -367,31 +384,58 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
         if dev >= 0 and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attn_prefill over an 8-bit cache needs host_meta during capture")
         host_meta = (q_len.tolist(), ctx_len.tolist())
-    if len(host_meta[0]) != n or len(host_meta[1]) != n:
-        raise ValueError(f"host_meta is of {len(host_meta[0])} / {len(host_meta[1])} sequences, q_len of {n}")
-    if out is not None:
-        _check_rows("out", out, T, hq * HEAD_DIM, dev, 16)
+    q_lens, ctx_lens = host_meta
+    if len(q_lens) != n or len(ctx_lens) != n:
+        raise ValueError(f"host_meta is of {len(q_lens)} / {len(ctx_lens)} sequences, q_len of {n}")
+    if n and min(q_lens) < 0:
+        raise ValueError(f"a chunk of {min(q_lens)} tokens")
+    if out is None:
+        out = torch.empty(T, hq * HEAD_DIM, dtype=_BF16, device=q.device)
+        ldo = hq * HEAD_DIM
+    else:
+        ldo = _check_rows("out", out, T, hq * HEAD_DIM, dev, 16)
     if dev < 0:
-        return K.attn_prefill(q, k_cache.dequant(), v_cache.dequant(), block_table, q_start, q_len, ctx_len, tiles,
-                              hq, hkv, scale, out=out, host_meta=host_meta, bt_rows=bt_rows)
-    pages = [-(-max(c, 0) // PAGE) for c in host_meta[1]]
-    total, most = sum(pages), max(pages, default=0)
-    if most > block_table.shape[1]:
-        raise ValueError(f"a context of {max(host_meta[1])} keys needs {most} pages, block_table has room for "
-                         f"{block_table.shape[1]}")
-    if total == 0 or T == 0:
-        return out if out is not None else torch.empty(T, hq * HEAD_DIM, dtype=_BF16, device=q.device)
-    # this call's own workspace, as in attn_decode
-    width = hkv * HEAD_DIM
-    kv = torch.empty(2 * total * PAGE, width, dtype=_BF16, device=q.device)
-    kb, vb = kv.split(total * PAGE)
-    table = torch.empty(n, most, dtype=_I32, device=q.device)
-    rc = _native.kernels().ib_kv8_expand(k_cache.q.data_ptr(), k_cache.sf.data_ptr(), v_cache.q.data_ptr(),
-                                         v_cache.sf.data_ptr(), k_cache.slots // PAGE, hkv, block_table.data_ptr(),
-                                         K._ptr(bt_rows), block_table.stride(0), ctx_len.data_ptr(), n, most, total,
-                                         kb.data_ptr(), vb.data_ptr(), table.data_ptr(),
-                                         K.scratch(dev).status.data_ptr(), K._stream())
-    _native.check(rc, "ib_kv8_expand")
-    K._count()
-    return K.attn_prefill(q, kb, vb, table, q_start, q_len, ctx_len, tiles, hq, hkv, scale, out=out,
-                          host_meta=host_meta, kv_splits=kv_splits, tile_rows=tile_rows)
+        _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out, bt_rows)
+        return out
+    places = block_table.shape[1]
+    if n and max(ctx_lens) > places * PAGE:
+        raise ValueError(f"a context of {max(ctx_lens)} keys needs {-(-max(ctx_lens) // PAGE)} pages, block_table has "
+                         f"room for {places}")
+    items, rows, splits = prefill_plan(q_lens, ctx_lens, hq, hkv)
+    if kv_splits is not None:
+        splits = kv_splits
+        if splits < 1:
+            raise ValueError(f"kv_splits {splits}")
+    if rows > T:
+        raise ValueError(f"{rows} rows in the chunks, q has {T}")
+    if rows == 0:
+        return out
+    part = lse = None
+    if splits > 1:
+        # partials of this call, as in attn_decode
+        m = T * hq * splits
+        ws = torch.empty(m * (HEAD_DIM + 1), dtype=torch.float32, device=q.device)
+        part = ws.data_ptr()
+        lse = part + 4 * m * HEAD_DIM
+    rc = _native.kernels().ib_attn_prefill_kv8(q.data_ptr(), T, ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
+                                               v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
+                                               q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), n, items,
+                                               rows, block_table.data_ptr(), K._ptr(bt_rows), places,
+                                               block_table.stride(0), hq, hkv, scale, splits, part, lse,
+                                               out.data_ptr(), ldo, K.scratch(dev).status.data_ptr(), K._stream())
+    _native.check(rc, "ib_attn_prefill_kv8")
+    K._count(2 if splits > 1 else 1)
+    return out
+
+
+def _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out,
+                      bt_rows) -> None:
+    k, v = k_cache.dequant(), v_cache.dequant()
+    for i, (n, ctx, at) in enumerate(zip(q_lens, ctx_lens, q_start.tolist())):
+        row = block_table[i if bt_rows is None else int(bt_rows[i])][None]
+        blind = min(n, max(0, n - ctx))  # the first rows of a chunk longer than its context
+        out[at:at + blind, : hq * HEAD_DIM] = 0
+        if n > blind:
+            o, = K._ref_attention(q[at + blind:at + n, : hq * HEAD_DIM], k, v, row, [list(range(ctx - n + blind, ctx))],
+                                  [ctx], hq, hkv, scale)
+            out[at + blind:at + n, : hq * HEAD_DIM] = o.to(q.dtype)

@@ -291,6 +291,9 @@ PREFILL_REFUSALS = {
     "host lengths": dict(host_meta=([1, 1], [1, 1])),
     "q type": dict(q=torch.zeros(2, 4 * D)),
     "heads": dict(hq=5),
+    "group": dict(hq=18, q=torch.zeros(2, 18 * D, dtype=torch.bfloat16)),
+    "negative chunk": dict(host_meta=([-1], [1])),
+    "out rows": dict(out=torch.zeros(1, 4 * D, dtype=torch.bfloat16)),
     "bf16 caches": dict(v_cache=torch.zeros(32, 2 * D, dtype=torch.bfloat16)),
     "table rows": dict(block_table=torch.zeros(0, 2, dtype=torch.int32)),
 }
