@@ -446,6 +446,8 @@ def main(argv=None) -> None:
     p.add_argument("--kv-index-publisher", default="", help="publisher id in those events (the worker id)")
     p.add_argument("--kv-index-model", default="", help="served model name in those events")
     p.add_argument("--kv-index-compat", default="", help="compat key (tokenizer digest) in those events")
+    p.add_argument("--kv-cache-dtype", choices=("bf16", "fp8"), default="bf16",
+                   help="fp8: e4m3 KV cache with a scale per page and head (dense GQA models)")
     p.add_argument("--kv-tier", default=None)
     p.add_argument("--tp-size", type=int, default=1, help="tensor-parallel ranks (RANK / LOCAL_RANK / MASTER_* from env)")
     p.add_argument("--first-device", type=int, default=0, help="tensor-parallel rank r runs on cuda:(first + r)")
@@ -473,6 +475,7 @@ def main(argv=None) -> None:
                        max_batched_tokens=a.max_batched_tokens, gpu_memory_utilization=a.gpu_memory_utilization,
                        mixed_prefill_tokens=a.mixed_prefill_tokens,
                        num_pages=a.num_pages, use_cuda_graphs=not a.no_cuda_graphs, seed=a.seed, kv_tier=a.kv_tier,
+                       kv_cache_dtype=a.kv_cache_dtype,
                        disagg_mode=a.disagg_mode, kv_push_endpoint=a.kv_push_endpoint)
     eng = LLMEngine(cfg, device=device, event_sink=pub, tp=tp)
     feed = make_index_feed(a, cfg.page_size) if rank == 0 else None
@@ -537,7 +540,7 @@ def _main_dp(a) -> None:
     cfg = EngineConfig(model=a.model, page_size=a.page_size, max_num_seqs=a.max_num_seqs,
                        max_batched_tokens=a.max_batched_tokens, gpu_memory_utilization=a.gpu_memory_utilization,
                        mixed_prefill_tokens=a.mixed_prefill_tokens,
-                       num_pages=a.num_pages, use_cuda_graphs=False, seed=a.seed)
+                       num_pages=a.num_pages, use_cuda_graphs=False, seed=a.seed, kv_cache_dtype=a.kv_cache_dtype)
     dp = DPAttentionEngine(cfg, EPSpec(rank, world, group=None, gloo=gloo, fused=a.ep_fused and on_gpu),
                            device=device)
     if pub is not None:

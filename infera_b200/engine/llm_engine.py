@@ -72,6 +72,11 @@ class EngineConfig:
     mixed_prefill_tokens: int = 256
     max_model_len: int | None = None
     model_overrides: dict = field(default_factory=dict)
+    # KV cache: "bf16", or "fp8" (e4m3 with a scale per page and head, see
+    # ops/kv8.py: twice the tokens in the same memory). fp8 serves dense GQA
+    # models with 128-dim heads on one instance: without kv_tier and
+    # disagg_mode, whose chunk and push formats carry no scales
+    kv_cache_dtype: str = "bf16"
     # KV tiering: None (off), "pinned:<GiB>" (in-process page-locked arena of
     # page slots, DMA both ways), "host:<GiB>[:<nvme dir>]" (in-process host store,
     # optional NVMe tablespace), "host:<GiB>:files:<dir>" (NVMe tier of one
@@ -125,6 +130,8 @@ class LLMEngine:
             mcfg.max_model_len = cfg.max_model_len
         self.model_cfg = mcfg
         self.tp = tp
+        if cfg.kv_cache_dtype != "bf16":
+            self._check_kv8(cfg, mcfg)
         if getattr(mcfg, "kv_channels", 2) == 1:  # MLA: one latent cache row per token
             from infera_b200.models.mla import MLAModel
 
@@ -147,7 +154,8 @@ class LLMEngine:
                                    long_prefill_threshold=cfg.long_prefill_threshold,
                                    mixed_prefill_tokens=cfg.mixed_prefill_tokens)
         self.runner = ModelRunner(self.model, num_pages, cfg.page_size, cfg.max_num_seqs, cfg.max_batched_tokens,
-                                  use_graphs=cfg.use_cuda_graphs, exportable=cfg.disagg_mode == "decode")
+                                  use_graphs=cfg.use_cuda_graphs, exportable=cfg.disagg_mode == "decode",
+                                  kv8=cfg.kv_cache_dtype == "fp8")
         self.tier = None
         if cfg.kv_tier:
             from infera_b200.engine.tiering import TierManager
@@ -187,9 +195,28 @@ class LLMEngine:
         self.trace_phases = False
 
     # ------------------------------------------------------------------ sizing
+    @staticmethod
+    def _check_kv8(cfg: EngineConfig, mcfg) -> None:
+        from infera_b200.ops import kv8
+
+        if cfg.kv_cache_dtype != "fp8":
+            raise ValueError(f"kv_cache_dtype {cfg.kv_cache_dtype!r}: bf16 or fp8")
+        if getattr(mcfg, "kv_channels", 2) != 2 or mcfg.head_dim != kv8.HEAD_DIM \
+                or mcfg.num_heads // mcfg.num_kv_heads > 8:
+            raise ValueError(f"{mcfg.name}: an fp8 KV cache holds K and V heads of {kv8.HEAD_DIM}, with at most 8 query "
+                             "heads each")
+        if cfg.page_size != kv8.PAGE:
+            raise ValueError(f"page_size {cfg.page_size}: an fp8 KV cache has pages of {kv8.PAGE} tokens")
+        if cfg.kv_tier or cfg.disagg_mode != "mixed":
+            raise ValueError("an fp8 KV cache neither goes to a KV tier nor between prefill and decode instances: their "
+                             "formats carry no scales")
+
     def _derive_num_pages(self) -> int:
         mcfg = self.model.cfg  # this rank's shard of the model
-        per_page = getattr(mcfg, "kv_channels", 2) * mcfg.num_layers * self.cfg.page_size * mcfg.kv_size * 2
+        if self.cfg.kv_cache_dtype == "fp8":  # a byte each, and K's and V's scale of every head
+            per_page = 2 * mcfg.num_layers * (self.cfg.page_size * mcfg.kv_size + mcfg.num_kv_heads)
+        else:
+            per_page = getattr(mcfg, "kv_channels", 2) * mcfg.num_layers * self.cfg.page_size * mcfg.kv_size * 2
         if self.device.type != "cuda":
             return 512
         torch.cuda.synchronize()

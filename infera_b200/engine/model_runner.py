@@ -39,7 +39,8 @@ class StepResult:
 class ModelRunner:
     def __init__(self, model: DenseModel, num_pages: int, page_size: int, max_num_seqs: int,
                  max_batched_tokens: int, use_graphs: bool = True, graph_sizes: list[int] | None = None,
-                 exportable: bool = False):
+                 exportable: bool = False, kv8: bool = False):
+        """``kv8``: an 8-bit KV cache (:mod:`infera_b200.ops.kv8`)."""
         self.model = model
         cfg = model.cfg
         self.cfg = cfg
@@ -56,7 +57,14 @@ class ModelRunner:
         shape = (cfg.num_layers, slots, cfg.kv_size)
         # latent (MLA) caches have one channel: v_cache is a placeholder
         v_shape = shape if getattr(cfg, "kv_channels", 2) == 2 else (cfg.num_layers, 1, 1)
-        if exportable and self.on_gpu:
+        self.decode_plan = K.decode_plan
+        if kv8:
+            from infera_b200.ops import kv8 as kv8_ops
+
+            self.k_cache = kv8_ops.alloc(slots, cfg.num_kv_heads, layers=cfg.num_layers, device=self.dev)
+            self.v_cache = kv8_ops.alloc(slots, cfg.num_kv_heads, layers=cfg.num_layers, device=self.dev)
+            self.decode_plan = kv8_ops.decode_plan
+        elif exportable and self.on_gpu:
             # own cudaMalloc allocations: exportable whole with CUDA IPC
             # (the decode side of a PD pair maps them into prefill processes)
             from infera_b200.parallel.symmem import device_tensor
@@ -264,7 +272,7 @@ class ModelRunner:
             fb.d_bt_rows = v("drow")
             fb.num_decode = B
             if self.on_gpu:
-                fb.d_splits, fb.d_tps = K.decode_plan(B, self.cfg.num_kv_heads, max(d_lens))
+                fb.d_splits, fb.d_tps = self.decode_plan(B, self.cfg.num_kv_heads, max(d_lens))
         logits = self.model.forward(fb, self.k_cache, self.v_cache, self.bufs)
         self.last_logits = logits
         temp = v("temp").view(torch.float32)
@@ -331,7 +339,7 @@ class ModelRunner:
         v("drow").fill_(self.dummy_row)
         v("slots").fill_(-1)
         v("lidx").copy_(torch.arange(B, dtype=torch.int32, device=self.dev))
-        splits, tps = K.decode_plan(B, self.cfg.num_kv_heads, cls)
+        splits, tps = self.decode_plan(B, self.cfg.num_kv_heads, cls)
         fb = ForwardBatch(token_ids=v("ids"), positions=v("pos"), slots=v("slots"), logits_idx=v("lidx"),
                           num_prefill_tokens=0, d_block_table=self.block_table, d_seq_lens=v("dl"),
                           d_splits=splits, d_tps=tps, num_decode=B)

@@ -102,6 +102,8 @@ def parse_args(argv=None):
     p.add_argument("--drain-timeout", type=float, default=30.0)
     p.add_argument("--handback-after", type=float, default=None)
     p.add_argument("--tokenizer", default=None)
+    p.add_argument("--kv-cache-dtype", choices=("bf16", "fp8"), default="bf16",
+                   help="fp8: e4m3 KV cache with a scale per page and head (dense GQA models)")
     p.add_argument("--kv-tier", default=None, help="host:<GiB>[:<nvme dir>] or kvd:<socket>")
     p.add_argument("--in-process", action="store_true", help="run the engine on a thread of this process")
     p.add_argument("--attach-core", default=None, help="IN,OUT ipc addresses of a running engine core")
@@ -145,6 +147,8 @@ def _core_cmd(args, in_addr: str, out_addr: str) -> list[str]:
         cmd += ["--kv-index-endpoint", args.kv_index_endpoint, "--kv-index-publisher", worker_id(args),
                 "--kv-index-model", args.served_model_name or args.model,
                 "--kv-index-compat", getattr(args, "_compat", "")]
+    if getattr(args, "kv_cache_dtype", "bf16") != "bf16":
+        cmd += ["--kv-cache-dtype", args.kv_cache_dtype]
     if args.kv_tier:
         cmd += ["--kv-tier", args.kv_tier]
     cmd += ["--disagg-mode", args.disagg_mode]
@@ -165,7 +169,8 @@ async def start_engine(args):
                             max_batched_tokens=args.max_batched_tokens,
                             mixed_prefill_tokens=args.mixed_prefill_tokens,
                             gpu_memory_utilization=args.gpu_memory_utilization, num_pages=args.num_pages,
-                            use_cuda_graphs=not args.no_cuda_graphs, seed=args.seed, kv_tier=args.kv_tier,
+                            use_cuda_graphs=not args.no_cuda_graphs, seed=args.seed,
+                            kv_cache_dtype=getattr(args, "kv_cache_dtype", "bf16"), kv_tier=args.kv_tier,
                             disagg_mode=args.disagg_mode, kv_push_endpoint=args.kv_push_endpoint)
         eng = LLMEngine(ecfg, device=args.device, event_sink=pub)
         feed = None

@@ -179,7 +179,8 @@ class DenseModel:
                 bufs: dict | None = None) -> torch.Tensor:
         """Returns logits [S, vocab] for the rows in ``fb.logits_idx``.
 
-        ``k_caches`` / ``v_caches``: [num_layers, num_slots, kv_size] bf16.
+        ``k_caches`` / ``v_caches``: [num_layers, num_slots, kv_size] bf16, or
+        8-bit caches of all layers (:class:`infera_b200.ops.kv8.KV8Cache`).
         ``bufs``: optional preallocated activations (used by CUDA graphs).
         """
         cfg = self.cfg
@@ -201,8 +202,15 @@ class DenseModel:
         for li, lw in enumerate(self.w.layers):
             kc, vc = k_caches[li], v_caches[li]
             # a split qkv GEMM hands its fp32 workspace to rope_kvwrite (no
-            # finalize launch); with q / k norms the finalized rows are needed
-            ws = None if cfg.qk_norm else K.linear_deferred(x, lw["qkv"], qkv)
+            # finalize launch); with q / k norms, or an 8-bit cache, the
+            # finalized rows are needed
+            if cfg.qk_norm:
+                ws = None
+            elif isinstance(kc, torch.Tensor):
+                ws = K.linear_deferred(x, lw["qkv"], qkv)
+            else:
+                K.linear(x, lw["qkv"], out=qkv)
+                ws = None
             if ws is not None:
                 K.rope_kvwrite_ws(ws, qkv, fb.positions, fb.slots, self.cos_sin, cfg.num_heads, cfg.num_kv_heads,
                                   cfg.head_dim, kc, vc)
