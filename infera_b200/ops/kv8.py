@@ -52,21 +52,20 @@ class KV8Cache:
     def __init__(self, q: torch.Tensor, sf: torch.Tensor):
         self.q = q    # [(layers,) slots, hkv*128] float8_e4m3fn
         self.sf = sf  # [(layers,) slots/16, hkv] uint8
-        qs, ss = q.shape, sf.shape
+        qs, ss = tuple(q.shape), tuple(sf.shape)
         if q.dtype is not torch.float8_e4m3fn or sf.dtype is not torch.uint8:
             raise ValueError(f"a KV8Cache holds float8_e4m3fn codes and uint8 scales, not {q.dtype} and {sf.dtype}")
-        if not 2 <= len(qs) == len(ss) <= 3 or qs[-2] != ss[-2] * PAGE or qs[-1] != ss[-1] * HEAD_DIM \
-                or qs[:-2] != ss[:-2] or ss[-1] < 1 or ss[-2] < 1:
-            raise ValueError(f"codes {tuple(qs)} and scales {tuple(ss)} do not hold whole pages of {PAGE} slots with "
-                             f"heads of {HEAD_DIM}")
+        if len(ss) not in (2, 3) or 0 in ss or qs != (*ss[:-2], ss[-2] * PAGE, ss[-1] * HEAD_DIM):
+            raise ValueError(f"codes {qs} and scales {ss} do not hold whole pages of {PAGE} slots with heads of "
+                             f"{HEAD_DIM}")
         if not (q.is_contiguous() and sf.is_contiguous()):
             raise ValueError("a KV8Cache's tensors have to be contiguous")
         self.slots, self.hkv, self.dev = qs[-2], ss[-1], q.get_device()
         if sf.get_device() != self.dev:
             raise ValueError(f"codes on {q.device}, scales on {sf.device}")
-        if self.dev >= 0 and q.data_ptr() % 16:
+        if self.dev >= 0 and q.data_ptr() & 15:
             raise ValueError("a KV8Cache's codes have to start on a multiple of 16 bytes")
-        self._layers = [KV8Cache(q[i], sf[i]) for i in range(qs[0])] if len(qs) == 3 else None
+        self._layers = [KV8Cache(q[i], sf[i]) for i in range(ss[0])] if len(ss) == 3 else None
 
     @property
     def shape(self) -> torch.Size:
@@ -183,6 +182,14 @@ def _check_table(table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev:
         raise ValueError(f"block_table has {table.shape[0]} rows for {n} sequences")
 
 
+def _on(dev: int) -> tuple[int, int]:
+    """(status word, stream) of a launch on the current device, which ``dev`` has to be."""
+    sc = K._scratch.get(dev)
+    if sc is None or torch.cuda.current_device() != dev:
+        sc = K.scratch(dev)  # made now, or refused
+    return sc.status.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)
+
+
 # ---------------------------------------------------------------- append
 
 
@@ -218,10 +225,11 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
     if dev < 0:
         _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out)
         return q_out
+    status, stream = _on(dev)
     rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, ld, q_out.data_ptr(), ldq, pos.data_ptr(),
                                          slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, k_cache.q.data_ptr(),
                                          k_cache.sf.data_ptr(), v_cache.q.data_ptr(), v_cache.sf.data_ptr(),
-                                         k_cache.slots, max_pos, K.scratch(dev).status.data_ptr(), K._stream())
+                                         k_cache.slots, max_pos, status, stream)
     _native.check(rc, "ib_kv8_append")
     K._count()
     return q_out
@@ -313,12 +321,12 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
         ws = torch.empty(n * (HEAD_DIM + 1), dtype=torch.float32, device=q.device)
         part = ws.data_ptr()
         lse = part + 4 * n * HEAD_DIM
+    status, stream = _on(dev)
     rc = _native.kernels().ib_attn_decode_kv8(q.data_ptr(), ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
                                               v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
                                               block_table.data_ptr(), K._ptr(bt_rows), seq_lens.data_ptr(), places,
                                               block_table.stride(0), B, hq, hkv, splits, tiles_per_split, scale,
-                                              part, lse, out.data_ptr(), ldo, K.scratch(dev).status.data_ptr(),
-                                              K._stream())
+                                              part, lse, out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_decode_kv8")
     K._count(2 if splits > 1 else 1)
     return out
@@ -417,12 +425,13 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
         ws = torch.empty(m * (HEAD_DIM + 1), dtype=torch.float32, device=q.device)
         part = ws.data_ptr()
         lse = part + 4 * m * HEAD_DIM
+    status, stream = _on(dev)
     rc = _native.kernels().ib_attn_prefill_kv8(q.data_ptr(), T, ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
                                                v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
                                                q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), n, items,
                                                rows, block_table.data_ptr(), K._ptr(bt_rows), places,
                                                block_table.stride(0), hq, hkv, scale, splits, part, lse,
-                                               out.data_ptr(), ldo, K.scratch(dev).status.data_ptr(), K._stream())
+                                               out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_prefill_kv8")
     K._count(2 if splits > 1 else 1)
     return out
