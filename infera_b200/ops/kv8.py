@@ -352,19 +352,31 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_
                  ) -> tuple[int, int, int]:
     """(items, rows, key shares) of :func:`attn_prefill`: an item is 256 rows
     of (token, query head of one KV head). The share count minimises waves x
-    (key tiles per share + 2 to start), in units of the 1.6 us that a tile of
-    128 keys takes, plus the merge's launch and its bytes (each share's fp32
-    row written and read)."""
+    (key tiles per share + 2 to start), in units of a tile of 128 keys (2.1
+    us), plus the merge's launch and its bytes (each share's fp32 row written
+    and read; 1024 rows x 64 heads over 32768 keys at the power cap: 1152 us
+    in one share, 1172 in four). Of the counts with as many waves only the
+    largest is tried, and of those with as many tiles a share the smallest."""
     per = 256 // (hq // hkv)
-    rows = sum(q_lens)
-    items = sum(-(-n // per) for n in q_lens)
-    ctas = items * hkv
+    rows = items = 0
+    for n in q_lens:
+        rows += n
+        items += -(-n // per)
+    ctas = max(1, items * hkv)
     tiles = -(-max(ctx_lens, default=0) // 128)
     best, best_cost = 1, -(-ctas // num_sms) * (tiles + 2)
-    for sp in range(2, min(32, tiles // 2) + 1):
-        cost = -(-ctas * sp // num_sms) * (-(-tiles // sp) + 2) + 2 + rows * hq * sp / 7800
+    most = min(32, tiles // 2)
+    for waves in range(1, 5):
+        sp = min(most, num_sms * waves // ctas)
+        if sp < 2:
+            continue
+        share = -(-tiles // sp)
+        sp = -(-tiles // share)
+        cost = waves * (share + 2) + 2 + rows * hq * sp / 5000
         if cost < best_cost:
             best, best_cost = sp, cost
+        if sp >= most:
+            break
     return items, rows, best
 
 

@@ -309,3 +309,14 @@ def test_prefill_refuses(name):
     a.update(PREFILL_REFUSALS[name])
     with pytest.raises((ValueError, TypeError)):
         kv8.attn_prefill(**a)
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens", [([1], [1]), ([17], [4113]), ([224], [8416]), ([5, 0, 300], [5, 0, 9000]),
+                                             ([], []), ([2048] * 4, [2048] * 4), ([1], [131072])])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (6, 2), (64, 8)])
+def test_prefill_plan(q_lens, ctx_lens, hq, hkv):
+    items, rows, shares = kv8.prefill_plan(q_lens, ctx_lens, hq, hkv)
+    per = 256 // (hq // hkv)
+    assert rows == sum(q_lens) and items == sum(math.ceil(n / per) for n in q_lens)
+    tiles = math.ceil(max(ctx_lens, default=0) / 128)
+    assert 1 <= shares <= max(1, min(32, tiles // 2))
