@@ -81,7 +81,7 @@ struct Params {
   const int* block_table;
   const int* bt_rows;
   const int* seq_lens;
-  int max_pages, ld_table;  // places of a block-table row, and its pitch
+  int table_rows, max_pages, ld_table;  // rows of the block table, places of a row, and its pitch
   int hq, hkv, G;
   int splits;
   int tiles_per_split;  // split s covers tiles [s * this, (s + 1) * this) of every sequence
@@ -146,7 +146,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, b, len);
     len = p.max_pages * PAGE;
   }
+  const int* bt = table_row(p.block_table, p.bt_rows, p.table_rows, p.ld_table, b, p.status);
+  if (bt == nullptr) len = 0;
   const int n_tiles = (len + BKV - 1) / BKV;
+  if (split == p.splits - 1 && n_tiles > p.splits * static_cast<long long>(p.tiles_per_split) && threadIdx.x == 0)
+    record_status_detail(p.status, kStatusBadArgs, 5, b, len);  // keys that no split takes
   const int t0 = split * p.tiles_per_split;
   const int t1 = min(n_tiles, t0 + p.tiles_per_split);
   if (t0 >= t1) {  // nothing in this split
@@ -161,7 +165,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
   const int nt = t1 - t0;
   const int n_pages = (len + PAGE - 1) / PAGE;
-  const int* bt = p.block_table + static_cast<size_t>(p.bt_rows != nullptr ? p.bt_rows[b] : b) * p.ld_table;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -564,15 +567,15 @@ using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
 using namespace ib200;
 
 // q [B, ldq] bf16 (head h at columns h*128); kq / vq e4m3 [num_slots, hkv*128]
-// and ksf / vsf [num_slots/16, hkv]; block_table rows of max_pages places
-// (pitch ld_table), row bt_rows[b] (null: b); split s covers the 128-key tiles
+// and ksf / vsf [num_slots/16, hkv]; block_table [table_rows] rows of
+// max_pages places (pitch ld_table), row bt_rows[b] (null: b); split s covers the 128-key tiles
 // [s*tiles_per_split, (s+1)*tiles_per_split) of every sequence
 // (splits*tiles_per_split*128 must cover the longest one); o_part / lse_part:
 // fp32 [B*hq*splits*128] / [B*hq*splits], only touched when splits > 1.
 extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const void* ksf, const void* vq,
                                   const void* vsf, long long num_slots, const int* block_table, const int* bt_rows,
-                                  const int* seq_lens, int max_pages, int ld_table, int B, int hq, int hkv,
-                                  int splits, int tiles_per_split, float scale, float* o_part, float* lse_part, void* out,
+                                  const int* seq_lens, int table_rows, int max_pages, int ld_table, int B, int hq,
+                                  int hkv, int splits, int tiles_per_split, float scale, float* o_part, float* lse_part, void* out,
                                   int ldo, int* status, cudaStream_t stream) {
   using namespace ib200::dq8;
   if (B <= 0) return 0;
@@ -598,6 +601,7 @@ extern "C" int ib_attn_decode_kv8(const void* q, int ldq, const void* kq, const 
   p.block_table = block_table;
   p.bt_rows = bt_rows;
   p.seq_lens = seq_lens;
+  p.table_rows = table_rows;
   p.max_pages = max_pages;
   p.ld_table = ld_table;
   p.hq = hq;

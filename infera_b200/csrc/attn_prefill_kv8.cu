@@ -66,7 +66,7 @@ struct Params {
   int num_pages;
   const int* block_table;
   const int* bt_rows;
-  int max_pages, ld_table;
+  int table_rows, max_pages, ld_table;
   int hq, hkv, G, tokens;  // tokens: of an item, 256 / G
   int splits;
   float scale_log2;        // |scale| * log2(e)
@@ -176,6 +176,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int n_rows = min(p.tokens, qlen - first) * G;
   const int pos_first = ctx - qlen + first;
   const int row_first = p.q_start[seq] + first;
+  const int* bt = table_row(p.block_table, p.bt_rows, p.table_rows, p.ld_table, seq, p.status);
+  if (bt == nullptr) ctx = 0;
   if (ctx > p.max_pages * PAGE) {  // more keys than the page table has places for
     if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, seq, ctx);
     ctx = p.max_pages * PAGE;
@@ -206,7 +208,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
   for (int t = 0; t < 2; ++t) nu_t[t] = max(0, min(nuv_t[t] - 2 * j_lo, 2 * chunk));
   const int n_pages = (ctx + PAGE - 1) / PAGE;
-  const int* bt = p.block_table + static_cast<size_t>(p.bt_rows != nullptr ? p.bt_rows[seq] : seq) * p.ld_table;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -679,15 +680,15 @@ using namespace ib200;
 
 // q [T, ldq] bf16 (head h at columns h*128); kq / vq e4m3 [num_slots, hkv*128]
 // and ksf / vsf [num_slots/16, hkv]; q_start / q_len / ctx_len [n_seqs];
-// block_table rows of max_pages places (pitch ld_table), row bt_rows[s] (null:
-// s). n_items: sum of ceil(q_len / (256 / G)); n_rows: sum of q_len. splits
+// block_table [table_rows] rows of max_pages places (pitch ld_table), row
+// bt_rows[s] (null: s). n_items: sum of ceil(q_len / (256 / G)); n_rows: sum of q_len. splits
 // > 1: each item's key tiles in that many shares, o_part / lse_part fp32
 // [T*hq*splits*128] / [T*hq*splits].
 extern "C" int ib_attn_prefill_kv8(const void* q, int T, int ldq, const void* kq, const void* ksf, const void* vq,
                                    const void* vsf, long long num_slots, const int* q_start, const int* q_len,
                                    const int* ctx_len, int n_seqs, int n_items, int n_rows, const int* block_table,
-                                   const int* bt_rows, int max_pages, int ld_table, int hq, int hkv, float scale,
-                                   int splits, float* o_part, float* lse_part, void* out, int ldo, int* status,
+                                   const int* bt_rows, int table_rows, int max_pages, int ld_table, int hq, int hkv,
+                                   float scale, int splits, float* o_part, float* lse_part, void* out, int ldo, int* status,
                                    cudaStream_t stream) {
   using namespace ib200::pq8;
   if (T <= 0 || n_seqs <= 0 || n_items <= 0) return 0;
@@ -717,6 +718,7 @@ extern "C" int ib_attn_prefill_kv8(const void* q, int T, int ldq, const void* kq
   p.num_pages = static_cast<int>(num_slots / PAGE);
   p.block_table = block_table;
   p.bt_rows = bt_rows;
+  p.table_rows = table_rows;
   p.max_pages = max_pages;
   p.ld_table = ld_table;
   p.hq = hq;

@@ -151,7 +151,7 @@ __device__ void append_kv(const Append& p, int cta) {
     const long long page = s_page[w];
     uint8_t* sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
     uint8_t* codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
-    const int e_old = *sf;
+    const int e_old = max(static_cast<int>(*sf), 1);  // 0 counts as 1
     // Eight lanes per row, four slots of the page at a time (step s: slots
     // 4 s .. 4 s + 3): a lane has dims 8 c .. 8 c + 7 and their partners 64
     // further. All rows are loaded before any is used.

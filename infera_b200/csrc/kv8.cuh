@@ -87,6 +87,16 @@ __device__ __forceinline__ void umma_commit_if(uint32_t on, uint64_t* bar) {
 // a value that all lanes have, known to be uniform
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
+// The row of the page table that sequence s has, null (and a status) where
+// bt_rows names none of the table's rows.
+__device__ __forceinline__ const int* table_row(const int* table, const int* bt_rows, int table_rows, int ld_table,
+                                                int s, int* status) {
+  const int row = bt_rows != nullptr ? bt_rows[s] : s;
+  if (row >= 0 && row < table_rows) return table + static_cast<size_t>(row) * ld_table;
+  if (threadIdx.x == 0) record_status_detail(status, kStatusBadIndex, 4, s, row);
+  return nullptr;
+}
+
 // The exponents of K and V of a page and head (0 counts as 1). A page id
 // outside the cache (a bad table) loads zeros through the tensor map and takes
 // the smallest exponents, as does -1 (no page).

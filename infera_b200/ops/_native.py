@@ -126,10 +126,10 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
         "ib_kv8_append": [c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_vp,
                           c_ll, c_int, c_vp, c_vp],
         "ib_attn_prefill_kv8": [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int,
-                                c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_float, c_int, c_vp, c_vp, c_vp,
-                                c_int, c_vp, c_vp],
+                                c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_vp, c_vp,
+                                c_vp, c_int, c_vp, c_vp],
         "ib_attn_decode_kv8": [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int,
-                               c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
+                               c_int, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
         "ib_gemm_set_trace": [c_vp],
         "ib_gemm_set_tile_counters": [c_vp, c_int],
         "ib_gemm_fused_reduce": [],

@@ -168,7 +168,7 @@ def _check_rows(name: str, t: torch.Tensor, rows: int, width: int, dev: int, ali
         raise ValueError(f"{name} is on {t.device}, the queries on {_name(dev)}")
     if dev >= 0 and (t.data_ptr() | (2 * pitch if shape[0] > 1 else 0)) & (align - 1):
         raise ValueError(f"{name}: rows have to start on multiples of {align} bytes")
-    return pitch
+    return pitch if shape[0] > 1 else width  # (of a single row the pitch means nothing)
 
 
 def _check_table(table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev: int) -> None:
@@ -256,7 +256,7 @@ def _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out
             new = torch.where(new.isfinite(), new, float("nan"))
             e = _scale_exp(torch.nan_to_num(new, nan=0.0).abs().amax(dim=(0, 2)))
             if 0 not in at:
-                old = cache.sf[page].to(torch.int32)
+                old = cache.sf[page].to(torch.int32).clamp_min(1)
                 e = torch.maximum(e, old)
                 shift = _pow2((old - e).clamp_min(-60))
                 codes[page] = (codes[page].float() * shift[None, :, None]).to(torch.float8_e4m3fn)
@@ -291,15 +291,20 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
     ``splits`` and ``tiles_per_split`` come from :func:`decode_plan`: split s
     covers the 128-key tiles [s*T, (s+1)*T) of every sequence, so ``splits *
     tiles_per_split * 128`` must cover the longest one (``tiles_per_split=0``:
-    enough tiles for every key that the page table has room for)."""
+    enough tiles for every key that the page table has room for).
+
+    What the device finds wrong goes to the status word: keys that no split
+    covers (they are left out), a length beyond the page table's places (cut
+    there), a ``bt_rows`` entry that is no row of the table (the sequence gets
+    zeros). A page id outside the cache reads as zeros."""
     _check_heads(hq, hkv, 8)
     B, dev = seq_lens.shape[0], q.get_device()
     ldq = _check_rows("q", q, B, hq * HEAD_DIM, dev, 4)
     _check_i32("seq_lens", seq_lens, B, dev)
     _check_caches(k_cache, v_cache, hkv, dev)
     _check_table(block_table, bt_rows, B, dev)
-    if splits < 1 or tiles_per_split < 0:
-        raise ValueError(f"splits {splits}, tiles_per_split {tiles_per_split}")
+    if not 1 <= splits <= 65535 or tiles_per_split < 0 or B > 65535:
+        raise ValueError(f"splits {splits}, tiles_per_split {tiles_per_split}, {B} sequences")
     if out is None:
         out = torch.empty(B, hq * HEAD_DIM, dtype=_BF16, device=q.device)
         ldo = hq * HEAD_DIM
@@ -324,9 +329,10 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
     status, stream = _on(dev)
     rc = _native.kernels().ib_attn_decode_kv8(q.data_ptr(), ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
                                               v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
-                                              block_table.data_ptr(), K._ptr(bt_rows), seq_lens.data_ptr(), places,
-                                              block_table.stride(0), B, hq, hkv, splits, tiles_per_split, scale,
-                                              part, lse, out.data_ptr(), ldo, status, stream)
+                                              block_table.data_ptr(), K._ptr(bt_rows), seq_lens.data_ptr(),
+                                              block_table.shape[0], places, block_table.stride(0), B, hq, hkv,
+                                              splits, tiles_per_split, scale, part, lse, out.data_ptr(), ldo, status,
+                                              stream)
     _native.check(rc, "ib_attn_decode_kv8")
     K._count(2 if splits > 1 else 1)
     return out
@@ -391,7 +397,10 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     device without it) sizes the grid. The kernel makes its own work items of
     256 / group tokens, so ``tiles`` and ``tile_rows`` are not used. Up to 8
     query heads per KV head. A row that sees no key (a context shorter than
-    its chunk) is zero; rows of no sequence are left as they are."""
+    its chunk) is zero; rows of no sequence are left as they are. Bad lengths
+    and table rows are treated as in :func:`attn_decode`. A NaN among the values
+    of a key that a row does not see yet, but that shares the row's last tile
+    of 128 keys, reaches the row: a weight of zero does not cancel it."""
     _check_heads(hq, hkv, 8)
     n, T, dev = q_len.shape[0], q.shape[0], q.get_device()
     ldq = _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
@@ -441,8 +450,8 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     rc = _native.kernels().ib_attn_prefill_kv8(q.data_ptr(), T, ldq, k_cache.q.data_ptr(), k_cache.sf.data_ptr(),
                                                v_cache.q.data_ptr(), v_cache.sf.data_ptr(), k_cache.slots,
                                                q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), n, items,
-                                               rows, block_table.data_ptr(), K._ptr(bt_rows), places,
-                                               block_table.stride(0), hq, hkv, scale, splits, part, lse,
+                                               rows, block_table.data_ptr(), K._ptr(bt_rows), block_table.shape[0],
+                                               places, block_table.stride(0), hq, hkv, scale, splits, part, lse,
                                                out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_prefill_kv8")
     K._count(2 if splits > 1 else 1)

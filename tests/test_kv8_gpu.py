@@ -340,6 +340,87 @@ def test_decode_bad_table():
     assert bool(y.isfinite().all())
 
 
+def detail():
+    torch.cuda.synchronize()
+    d = K.scratch().read_status_detail()
+    K.scratch().clear_status()
+    return d
+
+
+def test_bad_table_rows_and_keys_that_no_split_takes():
+    """A row index outside the table gives zeros, keys behind the last split are left out; both are reported."""
+    lens = [300, 200]
+    q, kc, vc, bt, sl = decode_case(lens, 8, 2, seed=12)
+    good = kv8.attn_decode(q, kc, vc, bt, sl, 8, 2, 0.1, bt_rows=i32([0, 1]))
+    check_status()
+    for bad in (2, -1):
+        y = kv8.attn_decode(q, kc, vc, bt, sl, 8, 2, 0.1, splits=2, bt_rows=i32([0, bad]))
+        assert detail() == {"code": 7, "what": 4, "where": 1, "value": bad}
+        check_decode([300, 0], 8, 2, y, q, kc, vc, bt, 0.1)
+        y = kv8.attn_prefill(q, kc, vc, bt, i32([0, 1]), i32([1, 1]), sl, None, 8, 2, 0.1, bt_rows=i32([0, bad]),
+                             host_meta=([1, 1], lens), kv_splits=1)
+        assert detail() == {"code": 7, "what": 4, "where": 1, "value": bad}
+        assert not y[1].any() and bool(((y[0].float() - good[0].float()).abs() <= 2 ** -7 * good[0].abs() + 1e-2).all())
+    y = kv8.attn_decode(q, kc, vc, bt, sl, 8, 2, 0.1, splits=1, tiles_per_split=2)
+    assert detail() == {"code": 6, "what": 5, "where": 0, "value": 300}
+    check_decode([256, 200], 8, 2, y, q, kc, vc, bt, 0.1)
+
+
+def test_one_row_in_a_buffer_of_any_pitch():
+    q, kc, vc, bt, sl = decode_case([70], 8, 2, seed=13)
+    want = kv8.attn_decode(q, kc, vc, bt, sl, 8, 2, 0.1)
+    wide = torch.zeros(1, 8 * D + 5, dtype=torch.bfloat16, device=DEV)
+    wide[:, : 8 * D] = q
+    out = torch.zeros(1, 8 * D + 3, dtype=torch.bfloat16, device=DEV)
+    kv8.attn_decode(wide, kc, vc, bt, sl, 8, 2, 0.1, out=out)
+    check_status()
+    assert torch.equal(out[:, : 8 * D], want)
+    one = torch.ones(1, dtype=torch.int32, device=DEV)
+    a = kv8.attn_prefill(q, kc, vc, bt, one - 1, one, sl, None, 8, 2, 0.1, host_meta=([1], [70]))
+    b = kv8.attn_prefill(wide, kc, vc, bt, one - 1, one, sl, None, 8, 2, 0.1, host_meta=([1], [70]), out=out)
+    check_status()
+    assert torch.equal(a, b[:, : 8 * D])
+
+
+def test_scale_zero_counts_as_one():
+    """Codes under a scale exponent of 0 and of 1 are the same values, in attention and when the page's scale grows."""
+    q, kc, vc, bt, sl = decode_case([20], 4, 2, seed=14)
+    q = q * 2.0 ** 60
+    caches = []
+    for e in (0, 1):
+        k, v = kv8.KV8Cache(kc.q.clone(), torch.full_like(kc.sf, e)), kv8.KV8Cache(vc.q.clone(), torch.full_like(vc.sf, e))
+        caches.append((k, v))
+    a, b = [kv8.attn_decode(q, k, v, bt, sl, 4, 2, 2.0 ** 60) for k, v in caches]
+    assert torch.equal(a, b)
+    qkv = torch.full((1, 8 * D), 2.0 ** -115, dtype=torch.bfloat16, device=DEV)
+    slot = (bt[0, 1:2] * 16 + 9).contiguous()
+    for k, v in caches:
+        kv8.rope_kvwrite(qkv, i32([0]), slot, K.rope_cos_sin(2, D, 1e4, device=DEV), 4, 2, D, k, v)
+    check_status()
+    page = int(bt[0, 1])
+    for x, y in zip(*caches):
+        here = slice(page * 16, page * 16 + 16)
+        assert torch.equal(x.q[here].view(torch.uint8), y.q[here].view(torch.uint8))
+        assert torch.equal(x.sf[page], y.sf[page]) and int(x.sf[page, 0]) > 1
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_prefill_rows_that_see_nothing(splits):
+    """A context shorter than its chunk: the chunk's first rows see no key and are zero; a chunk over no context is."""
+    hq, hkv = 8, 2
+    q, kc, vc, bt, _ = decode_case([300, 300, 300], hq, hkv, seed=15)
+    ql, ctx = [40, 200, 5], [10, 129, 0]
+    g = torch.Generator().manual_seed(1)
+    q = (torch.randn(sum(ql) + 3, hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+    out = torch.full((sum(ql) + 3, hq * D), 3.0, dtype=torch.bfloat16, device=DEV)
+    kv8.attn_prefill(q, kc, vc, bt, i32([0, 40, 240]), i32(ql), i32(ctx), None, hq, hkv, 0.1, host_meta=(ql, ctx),
+                     out=out, kv_splits=splits)
+    check_status()
+    assert not out[:30].any() and not out[40:111].any() and not out[240:245].any() and bool((out[245:] == 3).all())
+    assert_close(out[30:40], plain(q[30:40], kc, vc, bt[0], 1, hq, hkv, 0.1), PROMPT)
+    assert_close(out[111:240], plain(q[111:240], kc, vc, bt[1], 1, hq, hkv, 0.1), PROMPT)
+
+
 def test_decode_and_append_in_a_far_page():
     """Codes more than 2^31 bytes into the cache."""
     hkv, hq, pages = 8, 16, (1 << 31) // (16 * 8 * D) + 40
