@@ -55,7 +55,6 @@ namespace dq8 {
 using namespace kv8;
 
 constexpr int BKV = 128;
-constexpr int STAGES = 3;
 constexpr int BLK = 128 * 128;      // 128 rows x 128 codes
 constexpr int NS = 16;              // columns of S
 constexpr int QBLK = NS * 128;
@@ -63,10 +62,16 @@ constexpr int NUM_THREADS = 192;
 constexpr float kLagLog2 = 2.0f;    // the running maximum may lag by this much
 constexpr int kTopLog2 = 6;         // weight of a key at the running maximum
 
+// Stages of K and V tiles, and CTAs per SM. Three CTAs of two stages hide a
+// tile's chain (S, softmax, W V) better than two of three where a tile has few
+// heads: 61 ragged sequences on scattered pages (4 heads) 125 us against 132,
+// 1 x 120001 43.5 against 45.5. Eight heads need the registers of two CTAs,
+// and the third stage: 32 x 8192 scattered 96 us against 112 with two.
+__host__ __device__ constexpr int stages(int gp) { return gp <= 4 ? 2 : 3; }
 // columns of O^T: three digits of GP heads
 __host__ __device__ constexpr int cols_o(int gp) { return 3 * gp <= 16 ? 16 : 32; }
 __host__ __device__ constexpr int smem_bytes(int gp) {
-  return 1024 + STAGES * 2 * BLK + QBLK + 2 * cols_o(gp) * 128 + 2048;
+  return 1024 + stages(gp) * 2 * BLK + QBLK + 2 * cols_o(gp) * 128 + 2048;
 }
 constexpr int SF_TILES = 16;        // tiles whose page exponents are staged at a time: a page per softmax thread
 constexpr uint32_t TMEM_COLS = 64;  // S0 [0,16) S1 [16,32) O [32,64)
@@ -129,10 +134,11 @@ __device__ __forceinline__ uint64_t make_mn_desc(uint32_t smem_addr, uint32_t mn
 }
 
 template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
-__global__ void __launch_bounds__(NUM_THREADS, 2)
+__global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
     decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ CUtensorMap tmK8, const __grid_constant__ CUtensorMap tmV8,
                   const Params p) {
+  constexpr int STAGES = stages(GP);
   constexpr int NO = cols_o(GP);
   constexpr int NC = NO / 16;           // 16-byte pieces of a key's digits
   constexpr int PBLK = NO * 128;

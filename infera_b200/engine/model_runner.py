@@ -63,7 +63,8 @@ class ModelRunner:
 
             self.k_cache = kv8_ops.alloc(slots, cfg.num_kv_heads, layers=cfg.num_layers, device=self.dev)
             self.v_cache = kv8_ops.alloc(slots, cfg.num_kv_heads, layers=cfg.num_layers, device=self.dev)
-            self.decode_plan = kv8_ops.decode_plan
+            group = cfg.num_heads // cfg.num_kv_heads
+            self.decode_plan = lambda b, hkv, n: kv8_ops.decode_plan(b, hkv, n, group=group)
         elif exportable and self.on_gpu:
             # own cudaMalloc allocations: exportable whole with CUDA IPC
             # (the decode side of a PD pair maps them into prefill processes)

@@ -40,6 +40,7 @@ from infera_b200.ops import kernels as K
 E4M3_MAX = 448.0
 PAGE = 16
 HEAD_DIM = 128
+_BF16, _I32, _U8, _E4M3 = torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
 
 
 class KV8Cache:
@@ -52,20 +53,27 @@ class KV8Cache:
     def __init__(self, q: torch.Tensor, sf: torch.Tensor):
         self.q = q    # [(layers,) slots, hkv*128] float8_e4m3fn
         self.sf = sf  # [(layers,) slots/16, hkv] uint8
-        qs, ss = tuple(q.shape), tuple(sf.shape)
-        if q.dtype is not torch.float8_e4m3fn or sf.dtype is not torch.uint8:
+        qs, ss = q.shape, sf.shape
+        if q.dtype is not _E4M3 or sf.dtype is not _U8:
             raise ValueError(f"a KV8Cache holds float8_e4m3fn codes and uint8 scales, not {q.dtype} and {sf.dtype}")
-        if len(ss) not in (2, 3) or 0 in ss or qs != (*ss[:-2], ss[-2] * PAGE, ss[-1] * HEAD_DIM):
-            raise ValueError(f"codes {qs} and scales {ss} do not hold whole pages of {PAGE} slots with heads of "
-                             f"{HEAD_DIM}")
+        if len(ss) == 2:
+            pages, heads = ss
+            whole = qs == (pages * PAGE, heads * HEAD_DIM)
+            self._layers = None
+        else:
+            layers, pages, heads = ss if len(ss) == 3 else (0, 0, 0)
+            whole = layers > 0 and qs == (layers, pages * PAGE, heads * HEAD_DIM)
+            self._layers = [KV8Cache(q[i], sf[i]) for i in range(layers)] if whole else None
+        if not whole or pages < 1 or heads < 1:
+            raise ValueError(f"codes {tuple(qs)} and scales {tuple(ss)} do not hold whole pages of {PAGE} slots with "
+                             f"heads of {HEAD_DIM}")
         if not (q.is_contiguous() and sf.is_contiguous()):
             raise ValueError("a KV8Cache's tensors have to be contiguous")
-        self.slots, self.hkv, self.dev = qs[-2], ss[-1], q.get_device()
+        self.slots, self.hkv, self.dev = pages * PAGE, heads, q.get_device()
         if sf.get_device() != self.dev:
             raise ValueError(f"codes on {q.device}, scales on {sf.device}")
         if self.dev >= 0 and q.data_ptr() & 15:
             raise ValueError("a KV8Cache's codes have to start on a multiple of 16 bytes")
-        self._layers = [KV8Cache(q[i], sf[i]) for i in range(ss[0])] if len(ss) == 3 else None
 
     @property
     def shape(self) -> torch.Size:
@@ -123,8 +131,6 @@ def _scale_exp(amax: torch.Tensor) -> torch.Tensor:
 # The calls take some 10 us of host time, a small batch's kernel less: each
 # check is one comparison of plain attributes, and words its error only after
 # it failed.
-
-_BF16, _I32 = torch.bfloat16, torch.int32
 
 
 def _check_caches(k: KV8Cache, v: KV8Cache, hkv: int, dev: int) -> None:
@@ -267,16 +273,20 @@ def _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out
 # ---------------------------------------------------------------- decode attention
 
 
-def decode_plan(batch: int, hkv: int, max_len: int, num_sms: int = 148) -> tuple[int, int]:
+def decode_plan(batch: int, hkv: int, max_len: int, num_sms: int = 148, group: int = 4) -> tuple[int, int]:
     """(splits, 128-key tiles per split) of :func:`attn_decode` for ``batch``
-    sequences whose longest has ``max_len`` keys: one wave of two CTAs on each
-    SM if all were that long, and at most 32 tiles. A CTA alone takes 0.75 us a
-    tile and some 3 us to start, so few sequences want short shares (1 x 8000
-    keys over 8 heads: 10.6 us in shares of 2 tiles, 47 us in one of 64), and
-    shares beyond 32 tiles gain no more (32 x 8192: 324 us at 1, 94 at 16, 87
-    at 32, 85 at 64) while ragged batches lose their balance."""
+    sequences whose longest has ``max_len`` keys, ``group`` query heads to a
+    KV head: one wave of the CTAs that fit (three on each SM, two for more
+    than 4 heads) if all were that long, and at most 32 tiles. A CTA alone
+    takes 0.75 to 1 us a tile and some 3 us to start, so few sequences want
+    short shares (1 x 8000 keys over 8 heads: 9.7 us in shares of 2 tiles, 47
+    us in one of 64), and shares beyond 32 tiles gain no more (32 x 8192 with
+    8 heads: 333 us at 1, 96 at 16, 89 at 32, 86 at 64) while ragged batches
+    lose their balance."""
     tiles = max(1, -(-max_len // 128))
-    tps = min(32, max(1, -(-batch * hkv * tiles // (2 * num_sms))))
+    ctas = max(1, batch * hkv)
+    shares = max(1, num_sms * (3 if group <= 4 else 2) // ctas)
+    tps = min(32, -(-tiles // shares))
     return -(-tiles // tps), tps
 
 

@@ -192,9 +192,10 @@ def test_alloc_layers_and_dequant():
 
 @pytest.mark.parametrize("batch", [1, 3, 64, 500])
 @pytest.mark.parametrize("hkv", [1, 8])
+@pytest.mark.parametrize("group", [1, 8])
 @pytest.mark.parametrize("longest", [0, 1, 128, 129, 5000, 131072])
-def test_decode_plan_covers(batch, hkv, longest):
-    splits, tps = kv8.decode_plan(batch, hkv, longest)
+def test_decode_plan_covers(batch, hkv, longest, group):
+    splits, tps = kv8.decode_plan(batch, hkv, longest, group=group)
     assert splits >= 1 and tps >= 1 and splits * tps * 128 >= longest
     assert (splits - 1) * tps * 128 < max(longest, 1)
 
