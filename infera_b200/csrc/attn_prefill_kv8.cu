@@ -29,9 +29,17 @@
 // in registers (one read of TMEM gives the maximum and the weights), and
 // publishes each unit's weights, so W V of the first overlaps the softmax of
 // the second.
+// Tiles of keys that some row does not see yet (the last ones) keep what is
+// masked apart: there R counts the pages that a row sees, row by row, and a
+// value that is NaN is multiplied as zero (a weight of zero would not cancel
+// it) and written at the end to the rows that see it. Both loops that do so
+// exist twice, for such tiles and for the others, which pay nothing for it
+// (6 % of a long prompt with one loop).
 // A CTA walks its item's key tiles or one share of them (few rows over a long
 // context); shares are merged by a combine kernel. Items are found from q_len
 // on the device, the ones with the most keys first.
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "tma_host.h"
 
@@ -63,6 +71,7 @@ struct Params {
   int n_seqs;
   const uint8_t* ksf;
   const uint8_t* vsf;
+  const uint8_t* vq;
   int num_pages;
   const int* block_table;
   const int* bt_rows;
@@ -102,6 +111,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// The top bits of the bytes of four codes that are NaN (seven ones below the sign).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t u) { return (u & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u; }
+
 // The item `at` when the sequences' items follow one another, those with the
 // most keys first (of the first 32 sequences; the others follow as they come),
 // and a sequence's from its last tokens to its first: the longest items start
@@ -134,6 +146,42 @@ __device__ __forceinline__ void locate_item(const int* q_len, const int* ctx_len
   }
 }
 
+// What a CTA works on: tokens of a sequence and the key tiles of its share.
+struct Item {
+  int row_first, n_tokens, pos_first, ctx, j_lo, nk;
+  const int* bt;
+};
+
+// Writes the NaN among the values of a CTA's last tiles, whose keys not every
+// row sees, to the rows that see them, a warp per token. Values that are NaN
+// are rare, so nothing here is tuned, and it stays out of the kernel's way: the
+// item comes from shared memory.
+__device__ __noinline__ void write_nan(const Params& p, const Item& it) {
+  const int lane = threadIdx.x & 31, kvh = blockIdx.x, z = blockIdx.z;
+  const int k_lo = max(it.j_lo, max(0, it.pos_first + 1) / BKV) * BKV, k_hi = (it.j_lo + it.nk) * BKV;
+  for (int token = threadIdx.x >> 5; token < it.n_tokens; token += NUM_THREADS / 32) {
+    const int row = it.row_first + token;
+    if (row < 0 || row >= p.T) continue;
+    const int end = min(min(it.pos_first + token + 1, it.ctx), k_hi);
+    uint32_t bad = 0;  // of dims 4 lane .. 4 lane + 3
+    for (int k = k_lo; k < end; ++k) {
+      const int page = it.bt[k / PAGE];
+      if (page < 0 || page >= p.num_pages) continue;
+      const size_t at = (static_cast<size_t>(page) * PAGE + k % PAGE) * p.hkv + kvh;
+      bad |= nan_codes(reinterpret_cast<const uint32_t*>(p.vq + at * D)[lane]);
+    }
+    if (bad == 0) continue;
+    for (int i = 0; i < 4 * p.G; ++i) {
+      if ((bad >> (8 * (i & 3)) & 0x80u) == 0) continue;
+      const int head = kvh * p.G + i / 4, d = 4 * lane + (i & 3);
+      if (p.splits > 1)
+        p.o_part[((static_cast<size_t>(row) * p.hq + head) * p.splits + z) * D + d] = NAN;
+      else
+        p.out[static_cast<size_t>(row) * p.ldo + head * D + d] = __float2bfloat16(NAN);
+    }
+  }
+}
+
 // The sequence of chunk row `at` and the row's place in it; seq -1 behind the
 // last. Called by whole warps.
 __device__ __forceinline__ void locate(const int* q_len, int n_seqs, int at, int& seq, int& place) {
@@ -163,9 +211,11 @@ __device__ __forceinline__ void locate(const int* q_len, int n_seqs, int at, int
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ CUtensorMap tmK8, const __grid_constant__ CUtensorMap tmV8,
-                   const Params p) {
+                   const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
+  __shared__ Item s_item;
+  __shared__ volatile int s_nan;  // a value was NaN in a tile that not every row sees whole
   const int kvh = blockIdx.x, z = blockIdx.z, S = p.splits, G = p.G;
   int seq, block;
   locate_item(p.q_len, p.ctx_len, p.n_seqs, p.tokens, blockIdx.y, seq, block);
@@ -215,7 +265,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint8_t* sK = sQ + 4 * BLK;            // [KST]
   uint8_t* sV8 = sK + KST * BLK;         // [VST] codes
   uint8_t* sV = sV8 + VST * BLK;         // [2] f16: dims 0..63, dims 64..127
-  float4* sSf = reinterpret_cast<float4*>(sV + 4 * BLK);  // [4 tiles][8 pages] 2^ke, weight exponent, its inverse
+  float4* sSf = reinterpret_cast<float4*>(sV + 4 * BLK);  // [4][8 pages] 2^ke, weight exponent, its inverse, ve
   int* sR = reinterpret_cast<int*>(sSf + 32);             // [4] R of the tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(sR + 4);
   uint64_t* q_ready = bars;
@@ -258,6 +308,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    s_nan = 0;
+    s_item = {row_first, n_rows / G, pos_first, ctx, j_lo, nk, bt};
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -389,9 +441,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // is done with it when the W V of tile j - 3 is (which the caller waited for).
     auto publish = [&](int j) {
       R = max(R, static_cast<int>(__reduce_max_sync(0xffu, max(ve, 1u))));
-      const int d = max(static_cast<int>(max(ve, 1u)) - R, kLeastLog2) + kTopLog2;
-      sSf[(j & 3) * 8 + ct] =
-          make_float4(two_to(static_cast<int>(max(ke, 1u)) - 127), static_cast<float>(d), two_to(-d), 0.f);
+      const int e = static_cast<int>(max(ve, 1u));
+      const int d = max(e - R, kLeastLog2) + kTopLog2;
+      sSf[(j & 3) * 8 + ct] = make_float4(two_to(static_cast<int>(max(ke, 1u)) - 127), static_cast<float>(d),
+                                          two_to(-d), static_cast<float>(e));
       if (ct == 0) sR[j & 3] = R;
       mbar_arrive(&sf_full[j & 3]);
     };
@@ -421,6 +474,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const uint8_t* src = sV8 + st * BLK;
       uint8_t* dst = sV + vb * 2 * BLK;
       const int live = ctx - (j_lo + j) * BKV;  // rows behind the sequence are zero: a stale code may be a NaN
+      auto convert = [&](auto edge) {
 #pragma unroll 4
       for (int i = 0; i < 1024 / CVT; ++i) {
         const int idx = ct + i * CVT;
@@ -428,8 +482,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int ch = (idx & 7) ^ (r & 7);     // dims 16 ch .. 16 ch + 15
         uint4 v = *reinterpret_cast<const uint4*>(src + idx * 16);
         if (r >= live) v = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        uint32_t u[4] = {v.x, v.y, v.z, v.w};
         uint32_t h[8];
+        if constexpr (decltype(edge)::value) {
+          const uint32_t x = nan_codes(u[0]), y = nan_codes(u[1]), z = nan_codes(u[2]), w = nan_codes(u[3]);
+          if ((x | y | z | w) != 0) {  // zero here, see write_nan
+            u[0] &= ~((x >> 7) * 255u);
+            u[1] &= ~((y >> 7) * 255u);
+            u[2] &= ~((z >> 7) * 255u);
+            u[3] &= ~((w >> 7) * 255u);
+            s_nan = 1;
+          }
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           h[2 * k] = h2_bits(from_e4m3x2_h(u[k] & 0xffffu));
@@ -444,6 +508,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         *reinterpret_cast<uint4*>(row + (((c + (up ? 1 : 0)) ^ (r & 7)) << 4)) = up ? b : a;
         *reinterpret_cast<uint4*>(row + (((c + (up ? 0 : 1)) ^ (r & 7)) << 4)) = up ? a : b;
       }
+      };
+      if ((j_lo + j) * BKV + BKV - 1 > pos_first)
+        convert(std::true_type{});
+      else
+        convert(std::false_type{});
       fence_proxy_async_smem();
       mbar_arrive(&v8_empty[st]);
       mbar_arrive(&v_full[vb]);
@@ -506,14 +575,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     float l_run = 0.f;
     int R_run = 0;
     bool ok = true;
-    for (int u = 0; u < nut && ok; ++u) {
+    // One unit; EDGE: of a tile that not every row sees whole.
+    auto unit = [&](auto edge, int u) -> bool {
+      constexpr bool EDGE = decltype(edge)::value;
       const int j = u >> 1, half = u & 1;
       if ((half == 0 && !mbar_wait_warp(&sf_full[j & 3], static_cast<uint32_t>((j >> 2) & 1), abort_flag, p.status,
                                         kStatusTimeoutFull)) ||
           (half == 0 && !mbar_wait_warp(&s_full[t], static_cast<uint32_t>(j & 1), abort_flag, p.status,
                                         kStatusTimeoutTmemFull))) {
-        ok = false;
-        break;
+        return false;
       }
       tc_fence_after();
       const uint32_t s_addr = lane_addr + t * 128 + half * UNIT;
@@ -522,12 +592,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint32_t v[UNIT];
       tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
       tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-      const int R = sR[j & 3];
+      int R = sR[j & 3];
       float4 f[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) f[g] = sf[g];
+      if constexpr (EDGE) {  // R of the pages that this row sees
+        R = R_run;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (kbase + 16 * g <= pos) R = max(R, static_cast<int>(f[g].w));
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = min(max(static_cast<int>(f[g].w) - R, kLeastLog2), 0) + kTopLog2;
+          f[g].y = static_cast<float>(d);
+          f[g].z = two_to(-d);
+        }
+      }
       tmem_ld_wait();
-      if (kbase + UNIT - 1 > pos0) {  // some row of the tile does not see all of the unit
+      if constexpr (EDGE) {
         const int lim = pos - kbase;  // key c of the unit is visible iff c <= lim
 #pragma unroll
         for (int i = 0; i < UNIT; ++i)
@@ -557,8 +639,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           // is issued until this unit's W is published
           if (half == 1 && !mbar_wait_warp(&o_done[t * 2], static_cast<uint32_t>(j & 1), abort_flag, p.status,
                                            kStatusTimeoutTmemFull)) {
-            ok = false;
-            break;
+            return false;
           }
           tc_fence_after();
           const float fo = alpha * two_to(max(R_run - R, -126));
@@ -603,7 +684,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[t * 2 + half]);
-    }
+      return true;
+    };
+    int u = 0;
+    const int whole = min(nut, 2 * ((pos0 + 1) / BKV - j_lo));
+    for (; u < whole && ok; ++u) ok = unit(std::false_type{}, u);
+    for (; u < nut && ok; ++u) ok = unit(std::true_type{}, u);
     ok = __all_sync(0xffffffffu, ok);
     const size_t part = (static_cast<size_t>(row) * p.hq + head) * S + z;
     if (nut <= 0) {
@@ -656,6 +742,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }
+  if (s_nan != 0) write_nan(p, s_item);
 }
 
 // Merge the key shares of a query row.
@@ -715,6 +802,7 @@ extern "C" int ib_attn_prefill_kv8(const void* q, int T, int ldq, const void* kq
   p.n_seqs = n_seqs;
   p.ksf = static_cast<const uint8_t*>(ksf);
   p.vsf = static_cast<const uint8_t*>(vsf);
+  p.vq = static_cast<const uint8_t*>(vq);
   p.num_pages = static_cast<int>(num_slots / PAGE);
   p.block_table = block_table;
   p.bt_rows = bt_rows;

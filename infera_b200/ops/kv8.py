@@ -408,9 +408,8 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     256 / group tokens, so ``tiles`` and ``tile_rows`` are not used. Up to 8
     query heads per KV head. A row that sees no key (a context shorter than
     its chunk) is zero; rows of no sequence are left as they are. Bad lengths
-    and table rows are treated as in :func:`attn_decode`. A NaN among the values
-    of a key that a row does not see yet, but that shares the row's last tile
-    of 128 keys, reaches the row: a weight of zero does not cancel it."""
+    and table rows are treated as in :func:`attn_decode`. Nothing of a key
+    that a row does not see reaches the row, a NaN neither."""
     _check_heads(hq, hkv, 8)
     n, T, dev = q_len.shape[0], q.shape[0], q.get_device()
     ldq = _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
@@ -471,6 +470,9 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
 def _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out,
                       bt_rows) -> None:
     k, v = k_cache.dequant(), v_cache.dequant()
+    # a value that is NaN reaches the rows that see it, and not by a weight of zero
+    nan = v.isnan()
+    v = v.masked_fill(nan, 0.0)
     for i, (n, ctx, at) in enumerate(zip(q_lens, ctx_lens, q_start.tolist())):
         row = block_table[i if bt_rows is None else int(bt_rows[i])][None]
         blind = min(n, max(0, n - ctx))  # the first rows of a chunk longer than its context
@@ -478,4 +480,7 @@ def _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_len
         if n > blind:
             o, = K._ref_attention(q[at + blind:at + n, : hq * HEAD_DIM], k, v, row, [list(range(ctx - n + blind, ctx))],
                                   [ctx], hq, hkv, scale)
-            out[at + blind:at + n, : hq * HEAD_DIM] = o.to(q.dtype)
+            slots = (row[0, : -(-ctx // PAGE)].long()[:, None] * PAGE + torch.arange(PAGE)).flatten()[:ctx]
+            seen = nan[slots].cumsum(0)[ctx - n + blind:] > 0
+            seen = seen.unflatten(-1, (hkv, 1, HEAD_DIM)).expand(-1, -1, hq // hkv, -1).flatten(1)
+            out[at + blind:at + n, : hq * HEAD_DIM] = o.masked_fill(seen, float("nan")).to(q.dtype)

@@ -300,6 +300,24 @@ PREFILL_REFUSALS = {
 }
 
 
+def test_prefill_nan_reaches_the_rows_that_see_it():
+    n, ctx, hq, hkv = 20, 40, 4, 2
+    kc, vc = random_cache(48, hkv, 1), random_cache(48, hkv, 2)
+    bt, one = torch.tensor([[2, 0, 1]], dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = (torch.randn(n, hq * D, generator=torch.Generator().manual_seed(1)) / 60).to(torch.bfloat16)
+
+    def run():
+        return kv8.attn_prefill(q, kc, vc, bt, one - 1, one * n, one * ctx, None, hq, hkv, 0.1)
+
+    clean = run()
+    vc.q.view(torch.uint8)[0 + 30 - 16, D + 5] = 0x7F  # key 30 stands in page 0: rows 10 .. see it
+    y = run()
+    want = torch.zeros(n, hq, D, dtype=torch.bool)
+    want[10:, 2:, 5] = True
+    want = want.view(n, -1)
+    assert torch.equal(y.isnan(), want) and torch.equal(y[~want], clean[~want])
+
+
 @pytest.mark.parametrize("name", PREFILL_REFUSALS)
 def test_prefill_refuses(name):
     a = attend_args()

@@ -421,6 +421,55 @@ def test_prefill_rows_that_see_nothing(splits):
     assert_close(out[111:240], plain(q[111:240], kc, vc, bt[1], 1, hq, hkv, 0.1), PROMPT)
 
 
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("G", [1, 4, 8])
+def test_prefill_nothing_unseen_reaches_a_row(G, splits):
+    """NaN values and keys, and values of 2^90, behind a row's last key: the row is what it is without them, and the rows
+    that do see them have them, dim by dim."""
+    hkv, n, ctx, scale = 2, 300, 811, 0.1  # rows see 512 .. 811 keys
+    hq = hkv * G
+    q, kc, vc, bt, _ = decode_case([ctx], hq, hkv, seed=16)
+    g = torch.Generator().manual_seed(2)
+    q = (torch.randn(n, hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+
+    def run():
+        return kv8.attn_prefill(q, kc, vc, bt, i32([0]), i32([n]), i32([ctx]), None, hq, hkv, scale,
+                                host_meta=([n], [ctx]), kv_splits=splits)
+
+    clean = run()
+    check_status()
+    assert_close(clean, plain(q, kc, vc, bt[0], ctx - n + 1, hq, hkv, scale), PROMPT)
+    slot = lambda k: int(bt[0, k // 16]) * 16 + k % 16  # noqa: E731
+    # (key, column of the values): seen by all, by the chunk's middle and last rows, the last key; both heads
+    holes = [(5, 7), (530, 3), (531, D + 64), (639, 127), (640, D + 127), (700, 0), (ctx - 1, D + 1)]
+    held = vc.q.clone()
+    for k, col in holes:
+        vc.q.view(torch.uint8)[slot(k), col] = 0x7F if col % 2 else 0xFF
+    y = run()
+    check_status()
+    want = torch.zeros(n, hkv, G, D, dtype=torch.bool, device=DEV)
+    for k, col in holes:
+        want[max(0, k - (ctx - n)):, col // D, :, col % D] = True
+    want = want.view(n, -1)
+    assert torch.equal(y.isnan(), want) and bool((y == clean)[~want].view(-1).all())
+    vc.q.copy_(held)
+    # a key that is NaN: whole rows, from the first that sees it
+    kc.q.view(torch.uint8)[slot(650), D + 9] = 0x7F
+    y = run()
+    check_status()
+    at = 650 - (ctx - n)
+    assert torch.equal(y[:at], clean[:at]) and bool(y[at:, G * D:].isnan().all())
+    assert torch.equal(y[at:, : G * D], clean[at:, : G * D])
+    kc.q.view(torch.uint8)[slot(650), D + 9] = 0
+    # pages of far larger values
+    kc.q.view(torch.uint8)[slot(650)] = 0
+    vc.sf[bt[0, 704 // 16:].long(), 0] += 90
+    y = run()
+    check_status()
+    for i in (0, 1, 100, 127, 128, 190, 191, 192, 200, 255, 256, n - 1):
+        assert_close(y[i:i + 1], plain(q[i:i + 1], kc, vc, bt[0], ctx - n + 1 + i, hq, hkv, scale), PROMPT)
+
+
 def test_decode_and_append_in_a_far_page():
     """Codes more than 2^31 bytes into the cache."""
     hkv, hq, pages = 8, 16, (1 << 31) // (16 * 8 * D) + 40
