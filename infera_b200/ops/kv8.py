@@ -371,8 +371,11 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_
     (key tiles per share + 2 to start), in units of a tile of 128 keys (2.1
     us), plus the merge's launch and its bytes (each share's fp32 row written
     and read; 1024 rows x 64 heads over 32768 keys at the power cap: 1152 us
-    in one share, 1172 in four). Of the counts with as many waves only the
-    largest is tried, and of those with as many tiles a share the smallest."""
+    in one share, 1172 in four). With few rows the shares are short (17 rows x
+    32 heads over 4113 keys: 70 us in one share, 19.1 in 11 of 3 tiles, 17.7
+    in 17; 5 rows over 1005 keys: 15 us in 4 shares, 12.8 in 8). Of the counts
+    with as many waves only the largest is tried, and of those with as many
+    tiles a share the smallest."""
     per = 256 // (hq // hkv)
     rows = items = 0
     for n in q_lens:
@@ -381,14 +384,14 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_
     ctas = max(1, items * hkv)
     tiles = -(-max(ctx_lens, default=0) // 128)
     best, best_cost = 1, -(-ctas // num_sms) * (tiles + 2)
-    most = min(32, tiles // 2)
+    most = min(64, tiles)
     for waves in range(1, 5):
         sp = min(most, num_sms * waves // ctas)
         if sp < 2:
             continue
         share = -(-tiles // sp)
         sp = -(-tiles // share)
-        cost = waves * (share + 2) + 2 + rows * hq * sp / 5000
+        cost = waves * (share + 2) + 2 + rows * hq * sp / 10000
         if cost < best_cost:
             best, best_cost = sp, cost
         if sp >= most:

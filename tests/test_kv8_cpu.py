@@ -338,4 +338,4 @@ def test_prefill_plan(q_lens, ctx_lens, hq, hkv):
     per = 256 // (hq // hkv)
     assert rows == sum(q_lens) and items == sum(math.ceil(n / per) for n in q_lens)
     tiles = math.ceil(max(ctx_lens, default=0) / 128)
-    assert 1 <= shares <= max(1, min(32, tiles // 2))
+    assert 1 <= shares <= max(1, min(64, tiles))

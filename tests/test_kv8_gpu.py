@@ -530,6 +530,7 @@ def test_decode_in_graphs_and_on_two_streams():
 CHUNKS = {
     "one row": ([1], [1]), "whole prompt": ([300], [300]), "chunk": ([130], [1000]), "one row of many": ([1], [2000]),
     "ragged": ([17, 256, 1, 300, 5], [17, 700, 90, 301, 1500]), "an empty one": ([20, 0, 40], [50, 0, 40]),
+    "shares of a tile": ([3], [8100]),
 }
 
 
