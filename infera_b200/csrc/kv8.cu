@@ -14,12 +14,14 @@
 // channel: the first row of a page (its leader) looks its page's other rows
 // up among all slots of the batch. Nothing depends on the order of arrival.
 // Bound by HBM for prompts and by latency for single rows: 8192 rows of 32 + 2 x
-// 8 heads take 43 us (189 MB: 4.4 TB/s, 0.67 of the copy rate), 2048 rows 14.4
-// us, 64 decoding rows 5.0 us, one 3.4 us. What it took: a warp loads all 16
-// rows of a page before it uses any, 16 bytes a lane (100 us with a row at a
-// time), and makes the rotated values twice rather than hold them (80
-// registers, 3 CTAs per SM). Spreading the K/V CTAs among those that rotate q
-// gained nothing.
+// 8 heads take 38 us (189 MB: 5.0 TB/s, 0.76 of the copy rate), 2048 rows 12.6
+// us, 64 decoding rows 5.0 us, one 3.4 us. What it took (8192 rows): a warp
+// loads all 16 rows of a page before it uses any, 16 bytes a lane (100 us with
+// a row at a time), and makes the rotated values twice rather than hold them
+// (80 registers, 3 CTAs per SM); infinities are looked for only where the
+// largest value is one (40.2 us, 41.2 with a test of each value); a page's
+// angles come from shared memory (38.1). Spreading the K/V CTAs among those
+// that rotate q gained nothing, nor did a prefetch of a leader's next rows.
 #include <float.h>
 
 #include "kv8.cuh"
@@ -77,6 +79,7 @@ __device__ void append_kv(const Append& p, int cta) {
   __shared__ int s_lead[WIN];       // 0: an earlier row, of another window, leads the page
   __shared__ int s_row[WIN][PAGE];  // the last valid batch row of each slot of the page
   __shared__ int s_n;
+  __shared__ float4 s_cs[PAGE][D / 4];  // (cos, sin) of a page's rows, see below
   const int w0 = cta / p.head_groups * p.win;
   const int y = cta % p.head_groups;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -142,6 +145,11 @@ __device__ void append_kv(const Append& p, int cta) {
   __syncthreads();
   const int h_end = min(2 * p.hkv, (y + 1) * p.group_heads);
   const int n_heads = h_end - y * p.group_heads;
+  // A CTA with one page and a head for every warp, K heads among them, loads the page's angles
+  // once for all of them, in the order in which the eight lanes of a row read
+  // them: lane c's float4 i at 8 i + c. (From global memory a lane's 64 bytes
+  // lie beside its neighbour's, so that each load of a warp touches 16 lines.)
+  const bool staged = n_lead == 1 && n_heads == THREADS / 32 && y * p.group_heads < p.hkv;
   for (int task = warp; task < n_lead * n_heads; task += THREADS / 32) {
     const int w = task / n_heads;
     if (!s_lead[w]) continue;
@@ -156,7 +164,14 @@ __device__ void append_kv(const Append& p, int cta) {
     // 4 s .. 4 s + 3): a lane has dims 8 c .. 8 c + 7 and their partners 64
     // further. All rows are loaded before any is used.
     const int c = lane & 7, sub = lane >> 3;
-    int pos[4];
+    int pos[4], at[2];
+    if (staged) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = s_row[0][(tid + i * THREADS) / (D / 4)];
+        at[i] = row >= 0 ? __ldg(p.pos + row) : 0;  // (a row that is not there has no bad position either)
+      }
+    }
     uint32_t live = 0;  // slots that the batch writes (bit 4 s + sub)
     uint4 a[4], b[4];
 #pragma unroll
@@ -175,6 +190,15 @@ __device__ void append_kv(const Append& p, int cta) {
       live |= ((on & 1u) | (on >> 7 & 2u) | (on >> 14 & 4u) | (on >> 21 & 8u)) << (4 * s);
     }
     if (live == 0) continue;  // every row of the page has a bad position
+    if (staged) {  // every warp comes here, once
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = tid + i * THREADS, j = k % (D / 4);
+        s_cs[k / (D / 4)][(j & 3) * 8 + j / 4] =
+            __ldg(reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(at[i]) * D) + j);
+      }
+      __syncthreads();
+    }
     auto values = [&](int s, float (&x)[16]) {
       const uint32_t av[4] = {a[s].x, a[s].y, a[s].z, a[s].w}, bv[4] = {b[s].x, b[s].y, b[s].z, b[s].w};
       if (is_v || pos[s] < 0) {
@@ -187,8 +211,15 @@ __device__ void append_kv(const Append& p, int cta) {
         }
         return;
       }
-      const float4* at = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos[s]) * D + c * 16);
-      const float4 cs[4] = {__ldg(at), __ldg(at + 1), __ldg(at + 2), __ldg(at + 3)};
+      float4 cs[4];
+      if (staged) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = s_cs[4 * s + sub][8 * i + c];
+      } else {
+        const float4* from = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos[s]) * D + c * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = __ldg(from + i);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[2 * i] = rot_a(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
@@ -204,10 +235,22 @@ __device__ void append_kv(const Append& p, int cta) {
       float x[16];
       values(s, x);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) amax = fabsf(x[i]) <= FLT_MAX ? fmaxf(amax, fabsf(x[i])) : amax;
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));  // (the larger of a NaN and a number is the number)
     }
     // non-negative floats are ordered like their bits
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    const bool inf = amax > FLT_MAX;
+    if (inf) {  // again, of the finite values
+      amax = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float x[16];
+        values(s, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = fabsf(x[i]) <= FLT_MAX ? fmaxf(amax, fabsf(x[i])) : amax;
+      }
+      amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    }
     const bool anew = live & 1;
     const int e = anew ? scale_exp(amax) : max(scale_exp(amax), e_old);
     const float inv = two_to(127 - e);
@@ -234,8 +277,11 @@ __device__ void append_kv(const Append& p, int cta) {
       float x[16];
       values(s, x);  // made again (the angles come from the first-level cache) rather than held
       uint32_t v[4];
+      if (inf)  // e4m3 has none
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] * inv : NAN;  // e4m3 has no infinity
+        for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] : NAN;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= inv;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | to_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16;
@@ -273,6 +319,15 @@ __device__ void rotate_q(const Append& p, int cta) {
   const long long t = rest / ng;
   if (t >= p.T) return;
   const int h0 = static_cast<int>(rest % ng) * Q_HEADS;
+  const __nv_bfloat16* in = p.qkv + t * p.ldqkv + c * 8;
+  __nv_bfloat16* out = p.q_out + t * p.ldq + c * 8;
+  uint4 a[Q_HEADS], b[Q_HEADS];
+#pragma unroll
+  for (int i = 0; i < Q_HEADS; ++i)
+    if (h0 + i < p.hq) {  // in flight while the position is
+      a[i] = *reinterpret_cast<const uint4*>(in + (h0 + i) * D);
+      b[i] = *reinterpret_cast<const uint4*>(in + (h0 + i) * D + D / 2);
+    }
   const int pos = p.pos[t];
   if (pos < 0 || pos >= p.max_pos) {
     if (c == 0 && h0 == 0) record_status_detail(p.status, kStatusBadIndex, 1, static_cast<int>(t), pos);
@@ -280,15 +335,6 @@ __device__ void rotate_q(const Append& p, int cta) {
   }
   const float4* src = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(pos) * D + c * 16);
   const float4 cs[4] = {__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3)};
-  const __nv_bfloat16* in = p.qkv + t * p.ldqkv + c * 8;
-  __nv_bfloat16* out = p.q_out + t * p.ldq + c * 8;
-  uint4 a[Q_HEADS], b[Q_HEADS];
-#pragma unroll
-  for (int i = 0; i < Q_HEADS; ++i)
-    if (h0 + i < p.hq) {
-      a[i] = *reinterpret_cast<const uint4*>(in + (h0 + i) * D);
-      b[i] = *reinterpret_cast<const uint4*>(in + (h0 + i) * D + D / 2);
-    }
 #pragma unroll
   for (int i = 0; i < Q_HEADS; ++i)
     if (h0 + i < p.hq) {
@@ -347,11 +393,15 @@ extern "C" int ib_kv8_append(const void* qkv, int T, int ldqkv, void* q_out, int
   p.max_pos = max_pos;
   p.status = status;
   // Few rows: 4 of them and two heads per CTA, so that every (row, head) has a
-  // warp of its own. Many rows (prompts, one leading row in 16): fewer CTAs that
-  // lead nothing, and the look through the slots serves all heads.
+  // warp of its own; more heads where these CTAs would not all run at once (3 per
+  // SM; 256 decoding rows 7.5 us, 8.8 with two heads). Many rows (prompts, one
+  // leading row in 16): fewer CTAs that lead nothing, and the look through the
+  // slots serves all heads (400 decoding rows would take 18 us so, not 8.4).
   const bool many = T > 512;
   p.win = many ? 8 : 4;
   p.group_heads = many ? 8 : 2;
+  while (p.group_heads < 8 && (T + p.win - 1) / p.win * ((2 * hkv + p.group_heads - 1) / p.group_heads) > 3 * 148)
+    p.group_heads *= 2;
   p.head_groups = (2 * hkv + p.group_heads - 1) / p.group_heads;
   const long long kv_ctas = static_cast<long long>((T + p.win - 1) / p.win) * p.head_groups;
   const long long q_items = static_cast<long long>(T) * ((hq + Q_HEADS - 1) / Q_HEADS) * 8;
