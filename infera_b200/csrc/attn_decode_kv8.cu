@@ -45,7 +45,11 @@
 // Split partials (output normalised by its own sum, LSE in log2 units) are
 // merged by a combine kernel.
 //
-// Bound by HBM: two 8-bit codes per key, dim and KV head.
+// Bound by HBM: two 8-bit codes per key, dim and KV head. 32 sequences of 8192
+// keys (64 heads over 8) take 89 us (6.0 TB/s, 0.92 of the copy rate), 61 ragged
+// ones on scattered pages (32 over 8) 126 us (0.89: boxes of 2 KB), one of
+// 120001 keys 44 us (0.84, with its start and the merge of 37 shares), one of
+// 100 keys 5.6 us.
 #include "kv8.cuh"
 #include "tma_host.h"
 

@@ -38,6 +38,13 @@
 // A CTA walks its item's key tiles or one share of them (few rows over a long
 // context); shares are merged by a combine kernel. Items are found from q_len
 // on the device, the ones with the most keys first.
+//
+// Bound by the chain S, softmax, W V of each query tile: 2.1 us for 256 rows x
+// 128 keys, where the tensor core needs 1.46 at the measured rate. 1024 rows of
+// 64 heads (over 8) and 32768 keys take 1130 us (958 TFLOP/s, 0.56 of the
+// library's bf16 rate), six ragged prompts of 64 heads 234 us (0.43), 224 rows
+// of 32 heads over 8416 keys 57 us, 17 rows over 4113 keys 18.2 us. Slower: sixteen softmax warps, an MMA warp for each query
+// tile, exponentials on the FMA pipe.
 #include <type_traits>
 
 #include "kv8.cuh"
