@@ -46,10 +46,10 @@
 // merged by a combine kernel.
 //
 // Bound by HBM: two 8-bit codes per key, dim and KV head. 32 sequences of 8192
-// keys (64 heads over 8) take 89 us (6.0 TB/s, 0.92 of the copy rate), 61 ragged
-// ones on scattered pages (32 over 8) 126 us (0.89: boxes of 2 KB), one of
-// 120001 keys 44 us (0.84, with its start and the merge of 37 shares), one of
-// 100 keys 5.6 us.
+// keys (64 heads over 8) take 88 us (6.1 TB/s, 0.93 of the copy rate), 61 ragged
+// ones on scattered pages (32 over 8) 125 us (0.90: boxes of 2 KB), one of
+// 120001 keys 44 us (0.85, with its start and the merge of 37 shares), one of
+// 100 keys 5.3 us.
 #include "kv8.cuh"
 #include "tma_host.h"
 
@@ -151,12 +151,13 @@ __global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
   pdl_wait();
   const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
   const int G = p.G;
+  const int table = p.bt_rows != nullptr ? p.bt_rows[b] : b;
   int len = max(p.seq_lens[b], 0);
   if (len > p.max_pages * PAGE) {  // more keys than the page table has places for
     if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, b, len);
     len = p.max_pages * PAGE;
   }
-  const int* bt = table_row(p.block_table, p.bt_rows, p.table_rows, p.ld_table, b, p.status);
+  const int* bt = table_row(p.block_table, table, p.table_rows, p.ld_table, b, p.status);
   if (bt == nullptr) len = 0;
   const int n_tiles = (len + BKV - 1) / BKV;
   if (split == p.splits - 1 && n_tiles > p.splits * static_cast<long long>(p.tiles_per_split) && threadIdx.x == 0)

@@ -42,9 +42,11 @@
 // Bound by the chain S, softmax, W V of each query tile: 2.1 us for 256 rows x
 // 128 keys, where the tensor core needs 1.46 at the measured rate. 1024 rows of
 // 64 heads (over 8) and 32768 keys take 1130 us (958 TFLOP/s, 0.56 of the
-// library's bf16 rate), six ragged prompts of 64 heads 234 us (0.43), 224 rows
-// of 32 heads over 8416 keys 57 us, 17 rows over 4113 keys 18.2 us. Slower: sixteen softmax warps, an MMA warp for each query
+// library's bf16 rate), six ragged prompts of 64 heads 231 us (0.43), 224 rows
+// of 32 heads over 8416 keys 56 us, 17 rows over 4113 keys 16.7 us. Slower: sixteen softmax warps, an MMA warp for each query
 // tile, exponentials on the FMA pipe.
+#include <limits.h>
+
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -125,32 +127,35 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t u) { return (u & 0x7f7f7f
 // most keys first (of the first 32 sequences; the others follow as they come),
 // and a sequence's from its last tokens to its first: the longest items start
 // first, so that none is left for the end. Called by whole warps.
-__device__ __forceinline__ void locate_item(const int* q_len, const int* ctx_len, int n_seqs, int per, int at,
-                                            int& seq, int& place) {
-  const int lane = threadIdx.x & 31;
-  seq = -1;
-  place = 0;
+struct Found {
+  int seq, block, q_len, ctx, q_start, table;  // block: the item's place in its sequence
+};
+__device__ __forceinline__ Found locate_item(const Params& p, int at) {
+  const int lane = threadIdx.x & 31, per = p.tokens;
   int before = 0;
-  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-    const bool in = s0 + lane < n_seqs;
-    const int n = in ? (max(q_len[s0 + lane], 0) + per - 1) / per : 0;
-    const int ctx = in && s0 == 0 ? ctx_len[s0 + lane] : 0;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const int s = s0 + lane, some = min(32, p.n_seqs - s0);
+    const bool in = lane < some;
+    const int len = in ? p.q_len[s] : 0, ctx = in ? p.ctx_len[s] : 0;
+    // what only the found sequence's lane needs, in flight with the lengths
+    const int start = in ? p.q_start[s] : 0, table = in && p.bt_rows != nullptr ? p.bt_rows[s] : s;
+    const int n = (max(len, 0) + per - 1) / per, key = s0 == 0 ? ctx : 0;
     int ahead = 0, total = 0;  // items of the sequences before this lane's
-#pragma unroll
-    for (int l = 0; l < 32; ++l) {
-      const int nl = __shfl_sync(0xffffffffu, n, l), cl = __shfl_sync(0xffffffffu, ctx, l);
-      if (cl > ctx || (cl == ctx && l < lane)) ahead += nl;
+    for (int l = 0; l < some; ++l) {
+      const int nl = __shfl_sync(0xffffffffu, n, l), kl = __shfl_sync(0xffffffffu, key, l);
+      if (kl > key || (kl == key && l < lane)) ahead += nl;
       total += nl;
     }
     const uint32_t has = __ballot_sync(0xffffffffu, at >= before + ahead && at < before + ahead + n);
     if (has != 0) {
       const int l = __ffs(has) - 1;
-      seq = s0 + l;
-      place = __shfl_sync(0xffffffffu, n - 1 - (at - before - ahead), l);
-      return;
+      return {s0 + l, __shfl_sync(0xffffffffu, n - 1 - (at - before - ahead), l), __shfl_sync(0xffffffffu, len, l),
+              __shfl_sync(0xffffffffu, ctx, l), __shfl_sync(0xffffffffu, start, l),
+              __shfl_sync(0xffffffffu, table, l)};
     }
     before += total;
   }
+  return {-1, 0, 0, 0, 0, 0};
 }
 
 // What a CTA works on: tokens of a sequence and the key tiles of its share.
@@ -189,15 +194,15 @@ __device__ __noinline__ void write_nan(const Params& p, const Item& it) {
   }
 }
 
-// The sequence of chunk row `at` and the row's place in it; seq -1 behind the
-// last. Called by whole warps.
-__device__ __forceinline__ void locate(const int* q_len, int n_seqs, int at, int& seq, int& place) {
+// The row of q and out of chunk row `at`, INT_MIN behind the last. Called by
+// whole warps.
+__device__ __forceinline__ int locate_row(const int* q_len, const int* q_start, int n_seqs, int at) {
   const int lane = threadIdx.x & 31;
-  seq = -1;
-  place = 0;
   int before = 0;
   for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-    const int n = s0 + lane < n_seqs ? max(q_len[s0 + lane], 0) : 0;
+    const bool in = s0 + lane < n_seqs;
+    const int n = in ? max(q_len[s0 + lane], 0) : 0;
+    const int start = in ? q_start[s0 + lane] : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -207,12 +212,11 @@ __device__ __forceinline__ void locate(const int* q_len, int n_seqs, int at, int
     const uint32_t has = __ballot_sync(0xffffffffu, at < before + sum);
     if (has != 0) {
       const int l = __ffs(has) - 1;
-      seq = s0 + l;
-      place = at - before - __shfl_sync(0xffffffffu, sum - n, l);
-      return;
+      return at - before + __shfl_sync(0xffffffffu, start - (sum - n), l);
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
+  return INT_MIN;
 }
 
 __global__ void __launch_bounds__(NUM_THREADS, 1)
@@ -224,16 +228,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __shared__ Item s_item;
   __shared__ volatile int s_nan;  // a value was NaN in a tile that not every row sees whole
   const int kvh = blockIdx.x, z = blockIdx.z, S = p.splits, G = p.G;
-  int seq, block;
-  locate_item(p.q_len, p.ctx_len, p.n_seqs, p.tokens, blockIdx.y, seq, block);
+  const Found it = locate_item(p, blockIdx.y);
+  const int seq = it.seq, qlen = it.q_len;
   if (seq < 0) return;
-  const int qlen = p.q_len[seq];
-  int ctx = max(p.ctx_len[seq], 0);
-  const int first = block * p.tokens;                 // the item's first token in the chunk
+  int ctx = max(it.ctx, 0);
+  const int first = it.block * p.tokens;              // the item's first token in the chunk
   const int n_rows = min(p.tokens, qlen - first) * G;
   const int pos_first = ctx - qlen + first;
-  const int row_first = p.q_start[seq] + first;
-  const int* bt = table_row(p.block_table, p.bt_rows, p.table_rows, p.ld_table, seq, p.status);
+  const int row_first = it.q_start + first;
+  const int* bt = table_row(p.block_table, it.table, p.table_rows, p.ld_table, seq, p.status);
   if (bt == nullptr) ctx = 0;
   if (ctx > p.max_pages * PAGE) {  // more keys than the page table has places for
     if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, seq, ctx);
@@ -757,10 +760,8 @@ template <int W>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) prefill_merge_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();
-  int seq, token;
-  locate(p.q_len, p.n_seqs, blockIdx.x, seq, token);
-  if (seq < 0) return;
-  const int row = p.q_start[seq] + token, head = blockIdx.y * (MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
+  const int row = locate_row(p.q_len, p.q_start, p.n_seqs, blockIdx.x);
+  const int head = blockIdx.y * (MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
   if (row < 0 || row >= p.T || head >= p.hq) return;
   const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits;
   merge_shares<W>(p.o_part + part * D, p.lse_part + part, p.splits,

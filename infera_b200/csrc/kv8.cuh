@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "sm100.cuh"
@@ -87,11 +88,10 @@ __device__ __forceinline__ void umma_commit_if(uint32_t on, uint64_t* bar) {
 // a value that all lanes have, known to be uniform
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-// The row of the page table that sequence s has, null (and a status) where
-// bt_rows names none of the table's rows.
-__device__ __forceinline__ const int* table_row(const int* table, const int* bt_rows, int table_rows, int ld_table,
-                                                int s, int* status) {
-  const int row = bt_rows != nullptr ? bt_rows[s] : s;
+// Row `row` of the page table, which sequence s has; null (and a status) where
+// the table has no such row.
+__device__ __forceinline__ const int* table_row(const int* table, int row, int table_rows, int ld_table, int s,
+                                                int* status) {
   if (row >= 0 && row < table_rows) return table + static_cast<size_t>(row) * ld_table;
   if (threadIdx.x == 0) record_status_detail(status, kStatusBadIndex, 4, s, row);
   return nullptr;
@@ -112,35 +112,49 @@ __device__ __forceinline__ void page_exponents(const uint8_t* ksf, const uint8_t
 // out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M) over the shares of one
 // row and head, by W warps of a block of MERGE_WARPS (warp w of them takes
 // shares w, w + W, ...; a lane has 4 dims and makes the weight of one share in
-// 32). A NaN in a share stays one; the output of a share whose lse is -inf is
-// not read. One warp a row is the least work; few rows with many shares wait
+// 32). A NaN in a share stays one, however small its weight; the output of a
+// share whose lse is -inf is not written, and not used. A warp's first four
+// shares are loaded before the weights are known. One warp a row is the least work; few rows with many shares wait
 // for one load after another then, and take all warps of the block (1 x 120001
 // keys, 37 shares: 47 us against 50).
 constexpr int MERGE_WARPS = 8;
 template <int W>
 __device__ __forceinline__ void merge_shares(const float* o_part, const float* lse_part, int splits,
                                              __nv_bfloat16* out) {
+  constexpr int AHEAD = 4;
   const int lane = threadIdx.x & 31, w0 = (threadIdx.x >> 5) % W;
+  const float4* o = reinterpret_cast<const float4*>(o_part) + w0 * (D / 4) + lane;
+  float4 first[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    first[i] = w0 + i * W < splits ? o[i * (W * D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
   float mx = -INFINITY;
   for (int s = lane; s < splits; s += 32) mx = fmaxf(mx, lse_part[s]);
   mx = max_over_warp(mx);
   if (mx == -INFINITY) mx = 0.f;
   float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int s0 = w0; s0 < splits; s0 += 32 * W) {
+  auto add = [&](float w, const float4& v) {
+    if (w == 0.f) return;
+    den += w;
+    num[0] += v.x * w;
+    num[1] += v.y * w;
+    num[2] += v.z * w;
+    num[3] += v.w * w;
+  };
+  for (int s0 = w0; s0 < splits; s0 += 32 * W, o += 32 * (W * D / 4)) {
     const int n = min(32, (splits - s0 + W - 1) / W);  // shares s0, s0 + W, ...
-    const float mine = lane < n ? exp2f(lse_part[s0 + lane * W] - mx) : 0.f;
-    const float4* o = reinterpret_cast<const float4*>(o_part + static_cast<size_t>(s0) * D) + lane;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float w = __shfl_sync(0xffffffffu, mine, s);
-      if (w == 0.f) continue;
-      const float4 v = o[s * (W * D / 4)];
-      den += w;
-      num[0] += v.x * w;
-      num[1] += v.y * w;
-      num[2] += v.z * w;
-      num[3] += v.w * w;
+    float mine = 0.f;
+    if (lane < n) {
+      const float lse = lse_part[s0 + lane * W];
+      mine = exp2f(lse - mx);
+      if (mine == 0.f && lse != -INFINITY) mine = FLT_MIN;
     }
+    if (s0 == w0) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) add(__shfl_sync(0xffffffffu, mine, i), first[i]);
+    }
+#pragma unroll 4
+    for (int s = s0 == w0 ? AHEAD : 0; s < n; ++s) add(__shfl_sync(0xffffffffu, mine, s), o[s * (W * D / 4)]);
   }
   if constexpr (W > 1) {
     __shared__ float4 s_num[W][32];

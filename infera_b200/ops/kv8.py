@@ -377,8 +377,8 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_
     us), plus the merge's launch and its bytes (each share's fp32 row written
     and read; 1024 rows x 64 heads over 32768 keys at the power cap: 1152 us
     in one share, 1172 in four). With few rows the shares are short (17 rows x
-    32 heads over 4113 keys: 70 us in one share, 19.1 in 11 of 3 tiles, 17.7
-    in 17; 5 rows over 1005 keys: 15 us in 4 shares, 12.8 in 8). Of the counts
+    32 heads over 4113 keys: 70 us in one share, 18.4 in 11 of 3 tiles, 16.7
+    in 17; 5 rows over 1005 keys: 14.2 us in 4 shares, 12.1 in 8). Of the counts
     with as many waves only the largest is tried, and of those with as many
     tiles a share the smallest."""
     per = 256 // (hq // hkv)
