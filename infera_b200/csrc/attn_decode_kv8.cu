@@ -48,7 +48,7 @@
 // Bound by HBM: two 8-bit codes per key, dim and KV head. 32 sequences of 8192
 // keys (64 heads over 8) take 88 us (6.1 TB/s, 0.93 of the copy rate), 61 ragged
 // ones on scattered pages (32 over 8) 125 us (0.90: boxes of 2 KB), one of
-// 120001 keys 44 us (0.85, with its start and the merge of 37 shares), one of
+// 120001 keys 44 us (0.85, with its start and the merge of 53 shares), one of
 // 100 keys 5.3 us.
 #include "kv8.cuh"
 #include "tma_host.h"

@@ -421,6 +421,78 @@ def test_prefill_rows_that_see_nothing(splits):
     assert_close(out[111:240], plain(q[111:240], kc, vc, bt[1], 1, hq, hkv, 0.1), PROMPT)
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (9, 3), (10, 2), (12, 2), (7, 1), (16, 2)])
+def test_prefill_heads(hq, hkv, splits):
+    """Items whose 256 rows end inside a token's heads, and query tiles that part them."""
+    ql, ctx = [100, 1, 37], [500, 129, 37]
+    g = torch.Generator().manual_seed(hq)
+    _, kc, vc, bt, sl = decode_case(ctx, hq, hkv, seed=hq)
+    poison(kc, vc, bt, ctx)
+    q = (torch.randn(sum(ql), hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+    y = kv8.attn_prefill(q, kc, vc, bt, i32([0, 100, 101]), i32(ql), sl, None, hq, hkv, 0.1, host_meta=(ql, ctx),
+                         kv_splits=splits)
+    check_status()
+    at = 0
+    for b, n in enumerate(ql):
+        assert_close(y[at:at + n], plain(q[at:at + n], kc, vc, bt[b], ctx[b] - n + 1, hq, hkv, 0.1), PROMPT)
+        at += n
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_prefill_many_sequences(splits):
+    """More sequences than a warp has lanes, some without a token in this step."""
+    n, hq, hkv = 70, 8, 2
+    ql, ctx = [(7 * i) % 11 for i in range(n)], [(7 * i) % 11 + (53 * i) % 300 for i in range(n)]
+    g = torch.Generator().manual_seed(4)
+    _, kc, vc, bt, sl = decode_case(ctx, hq, hkv, seed=17)
+    start = [sum(ql[:i]) + 3 for i in range(n)]
+    q = (torch.randn(sum(ql) + 5, hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+    out = torch.full_like(q, 3.0)
+    kv8.attn_prefill(q, kc, vc, bt, i32(start), i32(ql), sl, None, hq, hkv, 0.1, host_meta=(ql, ctx), out=out,
+                     kv_splits=splits)
+    check_status()
+    assert bool((out[:3] == 3).all()) and bool((out[-2:] == 3).all())
+    for b in range(n):
+        if ql[b]:
+            rows = slice(start[b], start[b] + ql[b])
+            assert_close(out[rows], plain(q[rows], kc, vc, bt[b], ctx[b] - ql[b] + 1, hq, hkv, 0.1), PROMPT)
+
+
+def test_append_and_prefill_in_a_graph():
+    """A step of an append and a prompt's attention, captured once and replayed with other rows, on another stream."""
+    n, ctx, hq, hkv = 60, 700, 8, 2
+    _, kc, vc, bt, sl = decode_case([ctx], hq, hkv, seed=18)
+    slots = i32([int(bt[0, p // 16]) * 16 + p % 16 for p in range(ctx - n, ctx)])
+    steps = [step(n, hq, hkv, seed=s, max_pos=900) for s in (1, 2)]
+    pos, cs = torch.arange(ctx - n, ctx, dtype=torch.int32, device=DEV), steps[0][2].to(DEV)
+    qkv = torch.empty_like(steps[0][0], device=DEV)
+    args = (i32([0]), i32([n]), sl, None, hq, hkv, 0.05)
+
+    def run(k, v):
+        q = torch.empty(n, hq * D, dtype=torch.bfloat16, device=DEV)
+        kv8.rope_kvwrite(qkv, pos, slots, cs, hq, hkv, D, k, v, q_out=q)
+        return kv8.attn_prefill(q, k, v, bt, *args, host_meta=([n], [ctx]), kv_splits=3)
+
+    caches = [kv8.KV8Cache(c.q.clone(), c.sf.clone()) for c in (kc, vc)]
+    want = []
+    for x in steps:
+        qkv.copy_(x[0])
+        want.append(run(*caches))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run(kc, vc)
+    side = torch.cuda.Stream()
+    for x, w in zip(steps, want):
+        with torch.cuda.stream(side):
+            qkv.copy_(x[0].to(DEV))
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, w)
+    check_status()
+    assert same(kc, caches[0].to("cpu")) and same(vc, caches[1].to("cpu"))
+
+
 @pytest.mark.parametrize("splits", [1, 3])
 @pytest.mark.parametrize("G", [1, 4, 8])
 def test_prefill_nothing_unseen_reaches_a_row(G, splits):
