@@ -123,6 +123,35 @@ def test_append_special_values():
     assert float(kc.dequant()[5, 0]) == 1.0 and float(vc.dequant()[5, 0]) == 1.0
 
 
+@pytest.mark.parametrize("hq,hkv", [(8, 4), (8, 8), (7, 7)])
+def test_append_long_step_with_everything(hq, hkv):
+    """Whole pages of a prompt with infinities, NaN, rows without a slot, slots named twice and bad positions among them."""
+    n, pages = 700, 50
+    qkv, pos, cs = step(n, hq, hkv, seed=5, max_pos=900)
+    g = torch.Generator().manual_seed(6)
+    slots = torch.tensor(chunk(0, n, pages, 3), dtype=torch.int32)
+    pick = torch.randperm(n, generator=g)
+    slots[pick[:20]], slots[pick[20:40]] = -1, slots[pick[40:60]]
+    pos[pick[60:70]], pos[pick[70:80]] = 900, -5
+    kv = qkv[:, hq * D:]
+    for i, x in enumerate((float("inf"), float("-inf"), float("nan"))):
+        rows = pick[100 + 30 * i:130 + 30 * i]
+        kv[rows, torch.randint(0, 2 * hkv * D, (30,), generator=g)] = x
+    kc, vc = random_cache(pages * 16, hkv, 1), random_cache(pages * 16, hkv, 2)
+    k_cpu, v_cpu = kc.to("cpu"), vc.to("cpu")
+    q_cpu = kv8.rope_kvwrite(qkv, pos, slots, cs, hq, hkv, D, k_cpu, v_cpu, q_out=torch.zeros(n, hq * D).bfloat16())
+    q = torch.zeros(n, hq * D, dtype=torch.bfloat16, device=DEV)
+    kv8.rope_kvwrite(*[t.to(DEV) for t in (qkv, pos, slots, cs)], hq, hkv, D, kc, vc, q_out=q)
+    torch.cuda.synchronize()
+    assert K.scratch().read_status_detail()["what"] == 1  # a position, whichever came first
+    K.scratch().clear_status()
+    assert torch.equal(q.cpu(), q_cpu)
+    for a, b in ((kc, k_cpu), (vc, v_cpu)):
+        x, y = a.q.cpu().float(), b.q.float()
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(), y.nan_to_num())
+        assert torch.equal(a.sf.cpu(), b.sf)
+
+
 @pytest.mark.parametrize("what,pos,slot,detail", [("position", 50, 3, 1), ("position", -1, 3, 1), ("slot", 5, 64, 2)])
 def test_append_bad_index_is_skipped(what, pos, slot, detail):
     qkv, _, cs = step(3, 4, 2, max_pos=50)
