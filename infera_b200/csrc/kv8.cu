@@ -11,16 +11,18 @@
 // starts anew with that scale, any other keeps at least the one it has and
 // its rows are brought to a grown one. The scale joins all rows of a page in
 // the batch, wherever they stand in it, so one warp owns a (page, head) of a
-// channel: the first row of a page (its leader) looks its page's other rows
-// up among all slots of the batch. Nothing depends on the order of arrival.
+// channel (of four heads, where the page has but one row): the first row of a
+// page (its leader) looks its page's other rows up among all slots of the batch. Nothing depends on the order of arrival.
 // Bound by HBM for prompts and by latency for single rows: 8192 rows of 32 + 2 x
-// 8 heads take 38 us (189 MB: 5.0 TB/s, 0.76 of the copy rate), 2048 rows 12.6
-// us, 64 decoding rows 5.0 us, one 3.4 us. What it took (8192 rows): a warp
+// 8 heads take 38 us (189 MB: 5.0 TB/s, 0.76 of the copy rate), 2048 rows 12.3
+// us, 256 decoding rows 5.5 us, one 3.1 us. What it took (8192 rows): a warp
 // loads all 16 rows of a page before it uses any, 16 bytes a lane (100 us with
 // a row at a time), and makes the rotated values twice rather than hold them
 // (80 registers, 3 CTAs per SM); infinities are looked for only where the
 // largest value is one (40.2 us, 41.2 with a test of each value); a page's
-// angles come from shared memory (38.1). Spreading the K/V CTAs among those
+// angles come from shared memory (38.1). Of a page with one new row a warp
+// takes four heads (256 decoding rows 5.5 us, 7.5 with a warp for each head; 128
+// beside a prompt's 1500 rows 12.7 us, 23.8). Spreading the K/V CTAs among those
 // that rotate q gained nothing, nor did a prefetch of a leader's next rows.
 #include <float.h>
 
@@ -66,6 +68,56 @@ __device__ __forceinline__ float rot_a(float a, float b, float c, float s) {
 }
 __device__ __forceinline__ float rot_b(float a, float b, float c, float s) {
   return __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+}
+
+// The codes of dims 8 c .. 8 c + 7 (v.x, v.y) and their partners (v.z, v.w);
+// e4m3 has no infinity, so where values may be one it becomes NaN.
+__device__ __forceinline__ uint4 codes_of(float (&x)[16], float inv, bool inf) {
+  if (inf)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] : NAN;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] *= inv;
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | to_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16;
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// A lane's values of a row: a and b as they are, or rotated.
+__device__ __forceinline__ void unpack16(const uint4& a, const uint4& b, float (&x)[16]) {
+  const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16_lo(av[i]);
+    x[2 * i + 1] = bf16_hi(av[i]);
+    x[8 + 2 * i] = bf16_lo(bv[i]);
+    x[8 + 2 * i + 1] = bf16_hi(bv[i]);
+  }
+}
+__device__ __forceinline__ void rotate16(const uint4& a, const uint4& b, const float4 (&cs)[4], float (&x)[16]) {
+  const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = rot_a(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
+    x[2 * i + 1] = rot_a(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
+    x[8 + 2 * i] = rot_b(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
+    x[8 + 2 * i + 1] = rot_b(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
+  }
+}
+
+// The page's codes at `at` (16 of them) under a scale that grew by 1 / f: one
+// rounding more for codes that become subnormal, none for others.
+__device__ __forceinline__ void shrink(uint4* at, float f) {
+  const uint4 old = *at;
+  uint32_t v[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u0 = from_e4m3x2(v[i] & 0xffffu), u1 = from_e4m3x2(v[i] >> 16);
+    v[i] = to_e4m3x2(u0.x * f, u0.y * f) | to_e4m3x2(u1.x * f, u1.y * f) << 16;
+  }
+  *at = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 __device__ __forceinline__ bool bad_pos(const Append& p, int t) {
@@ -150,9 +202,68 @@ __device__ void append_kv(const Append& p, int cta) {
   // them: lane c's float4 i at 8 i + c. (From global memory a lane's 64 bytes
   // lie beside its neighbour's, so that each load of a warp touches 16 lines.)
   const bool staged = n_lead == 1 && n_heads == THREADS / 32 && y * p.group_heads < p.hkv;
+  // the slots that the batch writes of page w
+  auto live_of = [&](int w) { return __ballot_sync(0xffffffffu, lane < PAGE && s_row[w][lane % PAGE] >= 0); };
+  // Eight lanes have a row: dims 8 c .. 8 c + 7 and their partners 64 further.
+  const int c = lane & 7, sub = lane >> 3;
+  // Pages with one new row (decoding): the four groups of lanes take a head each.
+  const int quads = (n_heads + 3) / 4;
+  for (int task = warp; task < n_lead * quads; task += THREADS / 32) {
+    const int w = task / quads;
+    const uint32_t live = live_of(w);
+    if (!s_lead[w] || __popc(live) != 1) continue;
+    const int off = __ffs(live) - 1, row = s_row[w][off];
+    const int hh = y * p.group_heads + task % quads * 4 + sub;
+    const bool on = hh < h_end;
+    const bool is_v = hh >= p.hkv;
+    const int head = is_v ? hh - p.hkv : hh;
+    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+    float4 cs[4];
+    uint8_t *sf = nullptr, *codes = nullptr;
+    int e_old = 1;
+    if (on) {
+      const __nv_bfloat16* src =
+          p.qkv + static_cast<size_t>(row) * p.ldqkv + static_cast<size_t>(p.hq + hh) * D + c * 8;
+      a = __ldg(reinterpret_cast<const uint4*>(src));
+      b = __ldg(reinterpret_cast<const uint4*>(src + D / 2));
+      const long long page = s_page[w];
+      sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
+      codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
+      e_old = max(static_cast<int>(*sf), 1);  // 0 counts as 1
+    }
+    const float4* from = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(p.pos[row]) * D + c * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = __ldg(from + i);
+    float x[16];
+    if (is_v)
+      unpack16(a, b, x);
+    else
+      rotate16(a, b, cs, x);
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = fabsf(x[i]) <= FLT_MAX ? fmaxf(amax, fabsf(x[i])) : amax;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (!on) continue;
+    const int e = off == 0 ? scale_exp(amax) : max(scale_exp(amax), e_old);
+    if (off != 0 && e > e_old) {
+      const float f = two_to(max(e_old - e, -60));
+#pragma unroll 4
+      for (int o = 0; o < PAGE; ++o)
+        if (o != off) shrink(reinterpret_cast<uint4*>(codes + static_cast<size_t>(o) * p.hkv * D) + c, f);
+    }
+    const uint4 v = codes_of(x, two_to(127 - e), true);
+    uint8_t* at = codes + static_cast<size_t>(off) * p.hkv * D + c * 8;
+    *reinterpret_cast<uint2*>(at) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(at + D / 2) = make_uint2(v.z, v.w);
+    if (c == 0) *sf = static_cast<uint8_t>(e);
+  }
+  // The others: a warp has a head, four slots at a time (step s: slots 4 s ..
+  // 4 s + 3). All rows are loaded before any is used.
   for (int task = warp; task < n_lead * n_heads; task += THREADS / 32) {
     const int w = task / n_heads;
-    if (!s_lead[w]) continue;
+    const uint32_t live = live_of(w);
+    if (!s_lead[w] || __popc(live) < 2) continue;  // (none: every row of the page has a bad position)
     const int hh = y * p.group_heads + task % n_heads;
     const bool is_v = hh >= p.hkv;
     const int head = is_v ? hh - p.hkv : hh;
@@ -160,10 +271,6 @@ __device__ void append_kv(const Append& p, int cta) {
     uint8_t* sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
     uint8_t* codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
     const int e_old = max(static_cast<int>(*sf), 1);  // 0 counts as 1
-    // Eight lanes per row, four slots of the page at a time (step s: slots
-    // 4 s .. 4 s + 3): a lane has dims 8 c .. 8 c + 7 and their partners 64
-    // further. All rows are loaded before any is used.
-    const int c = lane & 7, sub = lane >> 3;
     int pos[4], at[2];
     if (staged) {
 #pragma unroll
@@ -172,7 +279,6 @@ __device__ void append_kv(const Append& p, int cta) {
         at[i] = row >= 0 ? __ldg(p.pos + row) : 0;  // (a row that is not there has no bad position either)
       }
     }
-    uint32_t live = 0;  // slots that the batch writes (bit 4 s + sub)
     uint4 a[4], b[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -186,10 +292,7 @@ __device__ void append_kv(const Append& p, int cta) {
         b[s] = __ldg(reinterpret_cast<const uint4*>(src + D / 2));
         pos[s] = __ldg(p.pos + row);
       }
-      const uint32_t on = __ballot_sync(0xffffffffu, row >= 0);  // a bit of each row's first lane
-      live |= ((on & 1u) | (on >> 7 & 2u) | (on >> 14 & 4u) | (on >> 21 & 8u)) << (4 * s);
     }
-    if (live == 0) continue;  // every row of the page has a bad position
     if (staged) {  // every warp comes here, once
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -200,15 +303,8 @@ __device__ void append_kv(const Append& p, int cta) {
       __syncthreads();
     }
     auto values = [&](int s, float (&x)[16]) {
-      const uint32_t av[4] = {a[s].x, a[s].y, a[s].z, a[s].w}, bv[4] = {b[s].x, b[s].y, b[s].z, b[s].w};
       if (is_v || pos[s] < 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = bf16_lo(av[i]);
-          x[2 * i + 1] = bf16_hi(av[i]);
-          x[8 + 2 * i] = bf16_lo(bv[i]);
-          x[8 + 2 * i + 1] = bf16_hi(bv[i]);
-        }
+        unpack16(a[s], b[s], x);
         return;
       }
       float4 cs[4];
@@ -220,13 +316,7 @@ __device__ void append_kv(const Append& p, int cta) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) cs[i] = __ldg(from + i);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = rot_a(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
-        x[2 * i + 1] = rot_a(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
-        x[8 + 2 * i] = rot_b(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y);
-        x[8 + 2 * i + 1] = rot_b(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w);
-      }
+      rotate16(a[s], b[s], cs, x);
     };
     float amax = 0.f;
 #pragma unroll
@@ -255,40 +345,23 @@ __device__ void append_kv(const Append& p, int cta) {
     const int e = anew ? scale_exp(amax) : max(scale_exp(amax), e_old);
     const float inv = two_to(127 - e);
     if (!anew && e > e_old) {
-      // one rounding more for codes that become subnormal, none for others
       const float f = two_to(max(e_old - e, -60));
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         if (live >> (4 * s + sub) & 1) continue;
-        uint4* at = reinterpret_cast<uint4*>(codes + static_cast<size_t>(4 * s + sub) * p.hkv * D) + c;
-        const uint4 old = *at;
-        uint32_t v[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u0 = from_e4m3x2(v[i] & 0xffffu), u1 = from_e4m3x2(v[i] >> 16);
-          v[i] = to_e4m3x2(u0.x * f, u0.y * f) | to_e4m3x2(u1.x * f, u1.y * f) << 16;
-        }
-        *at = make_uint4(v[0], v[1], v[2], v[3]);
+        shrink(reinterpret_cast<uint4*>(codes + static_cast<size_t>(4 * s + sub) * p.hkv * D) + c, f);
       }
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if ((live >> (4 * s) & 15u) == 0) continue;
       float x[16];
-      values(s, x);  // made again (the angles come from the first-level cache) rather than held
-      uint32_t v[4];
-      if (inf)  // e4m3 has none
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = fabsf(x[i]) <= FLT_MAX ? x[i] : NAN;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= inv;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = to_e4m3x2(x[4 * i], x[4 * i + 1]) | to_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16;
+      values(s, x);  // made again rather than held
+      const uint4 v = codes_of(x, inv, inf);
       if (pos[s] >= 0) {
         uint8_t* at = codes + static_cast<size_t>(4 * s + sub) * p.hkv * D + c * 8;
-        *reinterpret_cast<uint2*>(at) = make_uint2(v[0], v[1]);
-        *reinterpret_cast<uint2*>(at + D / 2) = make_uint2(v[2], v[3]);
+        *reinterpret_cast<uint2*>(at) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(at + D / 2) = make_uint2(v.z, v.w);
       }
     }
     if (lane == 0) *sf = static_cast<uint8_t>(e);
@@ -298,17 +371,10 @@ __device__ void append_kv(const Append& p, int cta) {
 constexpr int Q_HEADS = 4;  // heads per thread: they share the loaded cos / sin
 
 __device__ __forceinline__ void rotate8(const uint4& a, const uint4& b, const float4 (&cs)[4], uint4* na, uint4* nb) {
-  const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-  uint32_t ra[4], rb[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ra[i] = pack_bf16(rot_a(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y),
-                      rot_a(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w));
-    rb[i] = pack_bf16(rot_b(bf16_lo(av[i]), bf16_lo(bv[i]), cs[i].x, cs[i].y),
-                      rot_b(bf16_hi(av[i]), bf16_hi(bv[i]), cs[i].z, cs[i].w));
-  }
-  *na = make_uint4(ra[0], ra[1], ra[2], ra[3]);
-  *nb = make_uint4(rb[0], rb[1], rb[2], rb[3]);
+  float x[16];
+  rotate16(a, b, cs, x);
+  *na = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  *nb = make_uint4(pack_bf16(x[8], x[9]), pack_bf16(x[10], x[11]), pack_bf16(x[12], x[13]), pack_bf16(x[14], x[15]));
 }
 
 __device__ void rotate_q(const Append& p, int cta) {
@@ -392,16 +458,15 @@ extern "C" int ib_kv8_append(const void* qkv, int T, int ldqkv, void* q_out, int
   p.num_slots = num_slots;
   p.max_pos = max_pos;
   p.status = status;
-  // Few rows: 4 of them and two heads per CTA, so that every (row, head) has a
-  // warp of its own; more heads where these CTAs would not all run at once (3 per
-  // SM; 256 decoding rows 7.5 us, 8.8 with two heads). Many rows (prompts, one
-  // leading row in 16): fewer CTAs that lead nothing, and the look through the
-  // slots serves all heads (400 decoding rows would take 18 us so, not 8.4).
+  // Few rows: 4 of them and two heads per CTA, so that they spread over the SMs
+  // (64 decoding rows 4.6 us, 5.2 with eight heads); eight heads where the CTAs
+  // would not all run at once, 3 per SM (a prompt of 300 rows 5.9 us, 6.4 with
+  // four heads, 7.4 with two). Many rows (prompts, one leading row in 16):
+  // windows of 8, fewer CTAs that lead nothing (for 512 rows and fewer a window
+  // of 4 is faster: 6.4 us against 8.3).
   const bool many = T > 512;
   p.win = many ? 8 : 4;
-  p.group_heads = many ? 8 : 2;
-  while (p.group_heads < 8 && (T + p.win - 1) / p.win * ((2 * hkv + p.group_heads - 1) / p.group_heads) > 3 * 148)
-    p.group_heads *= 2;
+  p.group_heads = many || static_cast<long long>((T + 3) / 4) * hkv > 3 * 148 ? 8 : 2;
   p.head_groups = (2 * hkv + p.group_heads - 1) / p.group_heads;
   const long long kv_ctas = static_cast<long long>((T + p.win - 1) / p.win) * p.head_groups;
   const long long q_items = static_cast<long long>(T) * ((hq + Q_HEADS - 1) / Q_HEADS) * 8;
