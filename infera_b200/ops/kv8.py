@@ -196,7 +196,7 @@ def _check_table(table: torch.Tensor, bt_rows: torch.Tensor | None, n: int, dev:
 def _on(dev: int) -> tuple[int, int]:
     """(status word, stream) of a launch on the current device, which ``dev`` has to be."""
     sc = K._scratch.get(dev)
-    if sc is None or torch.cuda.current_device() != dev:
+    if sc is None or torch._C._cuda_getDevice() != dev:
         sc = K.scratch(dev)  # made now, or refused
     return sc.status.data_ptr(), torch._C._cuda_getCurrentRawStream(dev)
 
