@@ -7,9 +7,11 @@
 //
 // Both operands of an f8f6f4 product are 8-bit, so the bf16 query and the
 // weights are split into e4m3 digits that stand in columns of their own:
-//   q * 2^s = hi + lo / 16            exact: bf16 has 8 significant bits, a
-//                                     digit 4; s brings the head's largest
-//                                     element to [2^7, 2^8)
+//   q * 2^s = hi + lo / 16            bf16 has 8 significant bits, a digit 4; s
+//                                     brings the head's largest element to
+//                                     [2^7, 2^8): exact for elements down to
+//                                     2^-13 of it, and off by at most 2^-21 of
+//                                     it below, where digits are subnormal
 //   w       = hi + mid / 32 + lo / 1024  a weight rounded to f16 (11 bits; bf16
 //                                     has 8): each digit is rounded to nearest,
 //                                     so what is left of it is at most half a

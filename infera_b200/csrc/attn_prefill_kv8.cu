@@ -2,11 +2,15 @@
 // cache, on tcgen05.
 //
 //   S = Q K^T     kind::f8f6f4: K's codes are an operand as they lie in memory.
-//                 q * 2^s = hi + lo in two e4m3 digits (s brings the row's
-//                 largest element to [2^7, 2^8); what is left of a rounded bf16
-//                 value fits the second digit, exact down to 2^-18 of that
-//                 element), so S is eight 32-wide products into one accumulator:
-//                 the tensor core's time of a bf16 product
+//                 q * 2^s = hi + lo, hi in e4m3 and lo in e5m2 (s brings the
+//                 row's largest element to [2^7, 2^8)). bf16 has 8 significant
+//                 bits; hi rounded to 4 leaves -8 .. 8 units of the last place,
+//                 which the 3 bits of e5m2 hold, and its exponents reach 2^-16:
+//                 exact for elements down to 2^-13 of the row's largest, and
+//                 off by at most 2^-21 of that one below (as a second e4m3
+//                 digit, whose steps end at 2^-9, 2^-9 and 2^-17). S is eight
+//                 32-wide products into one accumulator: the tensor core's time
+//                 of a bf16 product
 //   O += W V      kind::f16: V's codes converted to f16 (exact) once per tile
 //                 of keys, W rounded to f16 in TMEM (11 significant bits)
 //
@@ -380,7 +384,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
   } else if (warp == 1) {
     const uint32_t on = elect_one();
-    const uint32_t idesc_qk = make_idesc_e4m3(128, BKV);
+    const uint32_t idesc_hi = make_idesc_e4m3(128, BKV);
+    const uint32_t idesc_lo = idesc_hi | (1u << 7);  // A in e5m2
     // f16 operands (formats 0), B = V with adjacent dims (MN-major)
     const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
     const uint64_t q_desc = make_sw128_desc(smem_u32(sQ), 16, 1024);
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
           for (int s = 0; s < 8; ++s)
             umma_e4m3_if(on, tmem + t * 128, q_desc + (t * 2 * BLK + (s >> 2) * BLK + (s & 3) * 32) / 16,
-                         kd + (s & 3) * 32 / 16, idesc_qk, s > 0 ? 1u : 0u);
+                         kd + (s & 3) * 32 / 16, s < 4 ? idesc_hi : idesc_lo, s > 0 ? 1u : 0u);
           umma_commit_if(on, &s_full[t]);
         }
       }
@@ -571,7 +576,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const uint32_t a = to_e4m3x2(x[0], x[1]), b = to_e4m3x2(x[2], x[3]);
           const float2 fa = from_e4m3x2(a), fb = from_e4m3x2(b);
           dh[k] = a | b << 16;
-          dl[k] = to_e4m3x2(x[0] - fa.x, x[1] - fa.y) | to_e4m3x2(x[2] - fb.x, x[3] - fb.y) << 16;
+          dl[k] = to_e5m2x2(x[0] - fa.x, x[1] - fa.y) | to_e5m2x2(x[2] - fb.x, x[3] - fb.y) << 16;
         }
         *reinterpret_cast<uint4*>(hi + sw_offset(r, i * 8)) = make_uint4(dh[0], dh[1], dh[2], dh[3]);
         *reinterpret_cast<uint4*>(lo + sw_offset(r, i * 8)) = make_uint4(dl[0], dl[1], dl[2], dl[3]);

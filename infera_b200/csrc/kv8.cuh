@@ -24,6 +24,9 @@ __device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t to_e5m2x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
+}
 __device__ __forceinline__ __half2 from_e4m3x2_h(uint32_t v) {
   return __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3));
 }

@@ -23,9 +23,11 @@ subnormal round again), and code times scale is exact in bf16.
 * :func:`attn_prefill` attends causally with chunks of new tokens.
 
 Both give the result in bf16 as if from exact arithmetic over the codes, as
-long as a head's page scales of V are not worlds apart: a weight is rounded to
-2^-12 of itself, or to 2^-26 (prompts: 2^-31) of the row's largest weight
-counted at the largest scale that the row sees.
+long as neither a query's elements nor a head's page scales of V are worlds
+apart: a query element is exact down to 2^-13 of the head's largest element and
+off by at most 2^-21 of that one below it; a weight is rounded to 2^-12 of
+itself, or to 2^-26 (prompts: 2^-31) of the row's largest weight counted at the
+largest scale that the row sees.
 
 :mod:`infera_b200.ops.kernels`'s ``rope_kvwrite``, ``attn_decode`` and
 ``attn_prefill`` come here for :class:`KV8Cache` caches. On CPU every

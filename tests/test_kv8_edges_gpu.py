@@ -1,0 +1,61 @@
+"""The 8-bit paged KV cache on a GPU at the ends of its ranges: queries with
+one large dimension, the smallest and largest scales, page tables and split
+counts that no engine makes."""
+
+import pytest
+import torch
+
+from infera_b200.ops import kv8
+from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_status, decode_case, i32, plain
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("octaves", [7, 10, 13])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_one_large_query_dim(octaves, splits):
+    """A query element 2^octaves above the others, in a dimension that the keys are quiet in: the others count in full.
+    Each of them is 1 + (8 a + 1) / 128, so 4 significant bits of it leave 1 / 128 over; without it a score of 8 to 24
+    (all products are positive) is off by up to 2^-7 of itself, differently for each key, and weights by 2^-4. The
+    second digit holds it exactly down to 2^-13 of the largest element, so the bounds are those of any query."""
+    n, ctx, hq, hkv, scale = 40, 300, 8, 2, 0.16
+    g = torch.Generator(device=DEV).manual_seed(octaves)
+    _, kc, vc, bt, sl = decode_case([ctx], hq, hkv, seed=1)
+    slots = kc.q.shape[0]
+    k = torch.randn(slots, hkv, D, generator=g, device=DEV).abs() * 0.8 \
+        * (0.5 + torch.rand(slots, hkv, 1, generator=g, device=DEV))
+    k[..., 0] = 2.0 ** -9
+    kc = kv8.KV8Cache(k.view(slots, -1).to(torch.float8_e4m3fn), torch.full_like(kc.sf, 127))
+    vc = kv8.KV8Cache(vc.q.float().abs().to(torch.float8_e4m3fn), vc.sf)
+    a = torch.randint(0, 16, (n, hq, D), generator=g, device=DEV)
+    q = 1 + (8 * a + 1) / 128
+    q[..., 0] = 2.0 ** octaves
+    q = q.view(n, hq * D).to(torch.bfloat16)
+    y = kv8.attn_prefill(q, kc, vc, bt, i32([0]), i32([n]), sl, None, hq, hkv, scale, host_meta=([n], [ctx]),
+                         kv_splits=splits)
+    check_status()
+    assert_close(y, plain(q, kc, vc, bt[0], ctx - n + 1, hq, hkv, scale), PROMPT)
+    y = kv8.attn_decode(q[:1], kc, vc, bt, sl, hq, hkv, scale, splits=splits, tiles_per_split=3)
+    check_status()
+    assert_close(y, plain(q[:1], kc, vc, bt[0], ctx, hq, hkv, scale), TOKEN)
+
+
+def test_wide_range_of_query_elements():
+    """Queries whose elements spread over 2^20, over random keys. A digit pair is off by at most 2^-21 of the row's
+    largest element (2^-14 where that is 2^7 to 2^8), so a score by 2^-21 max|q| sum|k| scale, and a weight by twice
+    that of itself; the rest as for any query."""
+    n, ctx, hq, hkv, scale = 130, 700, 8, 2, 0.1
+    g = torch.Generator(device=DEV).manual_seed(4)
+    _, kc, vc, bt, sl = decode_case([ctx], hq, hkv, seed=2)
+    q = torch.randn(n, hq, D, generator=g, device=DEV) / 60
+    q = (q * torch.exp2(torch.randint(-20, 1, (n, hq, D), generator=g, device=DEV))).view(n, -1).to(torch.bfloat16)
+    k = kc.dequant().view(-1, hkv, D).abs().sum(-1).amax()
+    extra = 2 * float(2 ** -21 * q.abs().amax() * k * scale)
+    assert extra < 2 ** -9
+    y = kv8.attn_prefill(q, kc, vc, bt, i32([0]), i32([n]), sl, None, hq, hkv, scale, host_meta=([n], [ctx]))
+    check_status()
+    # weights in f16 2^-12, sums of the scores 2^-13, as in TOKEN; and the digits
+    assert_close(y, plain(q, kc, vc, bt[0], ctx - n + 1, hq, hkv, scale), (2 ** -11 + extra, 2 ** -26))
