@@ -164,8 +164,9 @@ __global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
   const int n_tiles = (len + BKV - 1) / BKV;
   if (split == p.splits - 1 && n_tiles > p.splits * static_cast<long long>(p.tiles_per_split) && threadIdx.x == 0)
     record_status_detail(p.status, kStatusBadArgs, 5, b, len);  // keys that no split takes
-  const int t0 = split * p.tiles_per_split;
-  const int t1 = min(n_tiles, t0 + p.tiles_per_split);
+  // (in 64 bits: the caller's product may pass 32)
+  const int t0 = static_cast<int>(min(static_cast<long long>(n_tiles), static_cast<long long>(split) * p.tiles_per_split));
+  const int t1 = static_cast<int>(min(static_cast<long long>(n_tiles), static_cast<long long>(t0) + p.tiles_per_split));
   if (t0 >= t1) {  // nothing in this split
     if (p.splits > 1) {
       if (threadIdx.x < G)

@@ -333,8 +333,8 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
         _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, out, bt_rows)
         return out
     places = block_table.shape[1]
-    if tiles_per_split == 0:
-        tiles_per_split = max(1, -(-(-(-places * PAGE // 128)) // splits))
+    room = max(1, -(-places * PAGE // 128))  # tiles of the longest sequence that the table can hold
+    tiles_per_split = min(tiles_per_split, room) if tiles_per_split else -(-room // splits)
     part = lse = None
     if splits > 1:
         # partials of this call: its own memory, so that calls on several

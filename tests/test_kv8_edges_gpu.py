@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from infera_b200.ops import kv8
-from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_status, decode_case, i32, plain
+from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,16 @@ def test_wide_range_of_query_elements():
     check_status()
     # weights in f16 2^-12, sums of the scores 2^-13, as in TOKEN; and the digits
     assert_close(y, plain(q, kc, vc, bt[0], ctx - n + 1, hq, hkv, scale), (2 ** -11 + extra, 2 ** -26))
+
+
+@pytest.mark.parametrize("splits", [1, 3, 70])
+@pytest.mark.parametrize("tps", [2 ** 28, 2 ** 30, 2 ** 31 - 1, 2 ** 33 + 1])
+def test_decode_shares_of_any_size(splits, tps):
+    """``splits * tiles_per_split`` has to cover the longest sequence and may be far above it, in more than 32 bits."""
+    lens, hq, hkv = [300, 0, 1500], 8, 2
+    q, kc, vc, bt, sl = decode_case(lens, hq, hkv, seed=24)
+    y = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, 0.1, splits=splits, tiles_per_split=tps)
+    check_status()
+    want = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, 0.1, splits=splits, tiles_per_split=12)
+    assert torch.equal(y, want)
+    check_decode(lens, hq, hkv, y, q, kc, vc, bt, 0.1)
