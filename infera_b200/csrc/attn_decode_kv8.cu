@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
         int cur[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) cur[i] = nxt[i];
+        known_pages(cur, p.num_pages);
         if (j + 1 < nt) load_tile_pages(bt, t0 + j + 1, n_pages, nxt);  // in flight while we wait
         if (!mbar_wait(&empty[st], static_cast<uint32_t>(((j / STAGES) & 1) ^ 1), abort_flag, p.status,
                        kStatusTimeoutEmpty))

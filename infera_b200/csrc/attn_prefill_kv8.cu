@@ -358,6 +358,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         int cur[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) cur[i] = nxt[i];
+        known_pages(cur, p.num_pages);
         if (j + 1 < nk) load_tile_pages(bt, j_lo + j + 1, n_pages, nxt);
         if (!mbar_wait(&empty[st], static_cast<uint32_t>(ph), abort_flag, p.status, kStatusTimeoutEmpty)) break;
         uint8_t* dst = dst0 + st * BLK;

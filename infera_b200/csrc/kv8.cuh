@@ -100,6 +100,14 @@ __device__ __forceinline__ const int* table_row(const int* table, int row, int t
   return nullptr;
 }
 
+// Page ids outside the cache become -1: rows -16 .. -1, which a tensor map
+// fills with zeros. (A far id times 16 would wrap to a row that exists.)
+__device__ __forceinline__ void known_pages(int (&pages)[8], int num_pages) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (static_cast<unsigned>(pages[i]) >= static_cast<unsigned>(num_pages)) pages[i] = -1;
+}
+
 // The exponents of K and V of a page and head (0 counts as 1). A page id
 // outside the cache (a bad table) loads zeros through the tensor map and takes
 // the smallest exponents, as does -1 (no page).

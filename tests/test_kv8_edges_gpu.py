@@ -72,3 +72,36 @@ def test_decode_shares_of_any_size(splits, tps):
     want = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, 0.1, splits=splits, tiles_per_split=12)
     assert torch.equal(y, want)
     check_decode(lens, hq, hkv, y, q, kc, vc, bt, 0.1)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_far_page_ids_read_as_zeros(runs):
+    """Page ids outside the cache, those among them whose first slot's number wraps to one of the cache (2^28 pages of 16
+    slots are 2^32): zeros, alone and in runs of eight that one box would load."""
+    ctx, n, hq, hkv = 700, 200, 8, 2
+    q, kc, vc, bt, sl = decode_case([ctx], hq, hkv, seed=25, runs=runs)
+    g = torch.Generator().manual_seed(1)
+    q = (torch.randn(n, hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+    pages = kc.sf.shape[0]
+    none = bt.clone()
+    swap = [slice(0, 8), slice(20, 23), slice(43, 44)] if runs else [slice(1, 4), slice(17, 18), slice(43, 44)]
+    blank = [kv8.KV8Cache(torch.cat([c.q, torch.zeros_like(c.q[:16])]), torch.cat([c.sf, torch.ones_like(c.sf[:1])]))
+             for c in (kc, vc)]
+    for s in swap:
+        none[0, s] = pages  # (the page of zeros of ``blank``)
+
+    def both(k, v, table):
+        y = kv8.attn_decode(q[:1], k, v, table, sl, hq, hkv, 0.1, splits=2, tiles_per_split=3)
+        yp = kv8.attn_prefill(q, k, v, table, i32([0]), i32([n]), sl, None, hq, hkv, 0.1, host_meta=([n], [ctx]))
+        check_status()
+        return y, yp
+
+    want = both(*blank, none)
+    assert_close(want[0], plain(q[:1], *blank, none[0], ctx, hq, hkv, 0.1), TOKEN)
+    assert_close(want[1], plain(q, *blank, none[0], ctx - n + 1, hq, hkv, 0.1), PROMPT)
+    for far in (pages, -pages - 5, 2 ** 28, -2 ** 28, 2 ** 27 + 3, 2 ** 31 - 1 - pages):
+        bad = bt.clone()
+        for s in swap:
+            bad[0, s] = (bt[0, s].long() + far).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+        for a, b in zip(both(kc, vc, bad), want):
+            assert torch.equal(a, b)
