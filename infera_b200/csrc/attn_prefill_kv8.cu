@@ -456,10 +456,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // The scales of tile j go to one of four places: the softmax of tile j - 4
     // is done with it when the W V of tile j - 3 is (which the caller waited for).
     auto publish = [&](int j) {
-      R = max(R, static_cast<int>(__reduce_max_sync(0xffu, max(ve, 1u))));
-      const int e = static_cast<int>(max(ve, 1u));
+      const int e = exponent_of(ve);
+      R = max(R, __reduce_max_sync(0xffu, e));
       const int d = max(e - R, kLeastLog2) + kTopLog2;
-      sSf[(j & 3) * 8 + ct] = make_float4(two_to(static_cast<int>(max(ke, 1u)) - 127), static_cast<float>(d),
+      sSf[(j & 3) * 8 + ct] = make_float4(two_to(exponent_of(ke) - 127), static_cast<float>(d),
                                           two_to(-d), static_cast<float>(e));
       if (ct == 0) sR[j & 3] = R;
       mbar_arrive(&sf_full[j & 3]);

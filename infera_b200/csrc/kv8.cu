@@ -34,12 +34,12 @@ namespace kv8 {
 constexpr int WIN = 8;        // most batch rows per K/V CTA
 constexpr int THREADS = 256;
 
-// Smallest biased exponent e (1..254) with amax <= 448 * 2^(e - 127);
+// Smallest biased exponent e (1..253) with amax <= 448 * 2^(e - 127);
 // 448 = 1.75 * 2^8. amax >= 0 and finite; below 2^-126 it counts as 0.
 __device__ __forceinline__ int scale_exp(float amax) {
   const uint32_t b = __float_as_uint(amax);
   const int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return max(1, min(254, e));
+  return max(1, min(MAX_EXP, e));
 }
 
 struct Append {
@@ -229,7 +229,7 @@ __device__ void append_kv(const Append& p, int cta) {
       const long long page = s_page[w];
       sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
       codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
-      e_old = max(static_cast<int>(*sf), 1);  // 0 counts as 1
+      e_old = exponent_of(*sf);
     }
     const float4* from = reinterpret_cast<const float4*>(p.cos_sin + static_cast<size_t>(p.pos[row]) * D + c * 16);
 #pragma unroll
@@ -270,7 +270,7 @@ __device__ void append_kv(const Append& p, int cta) {
     const long long page = s_page[w];
     uint8_t* sf = (is_v ? p.vsf : p.ksf) + page * p.hkv + head;
     uint8_t* codes = (is_v ? p.vq : p.kq) + page * PAGE * p.hkv * D + head * D;
-    const int e_old = max(static_cast<int>(*sf), 1);  // 0 counts as 1
+    const int e_old = exponent_of(*sf);
     int pos[4], at[2];
     if (staged) {
 #pragma unroll

@@ -16,6 +16,9 @@ namespace kv8 {
 
 constexpr int D = 128;    // head dim
 constexpr int PAGE = 16;  // tokens of a page
+// Largest biased exponent of a page's scale, so that its inverse is a normal
+// number too (bf16 rows need 247 at most).
+constexpr int MAX_EXP = 253;
 
 __device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
@@ -108,7 +111,10 @@ __device__ __forceinline__ void known_pages(int (&pages)[8], int num_pages) {
     if (static_cast<unsigned>(pages[i]) >= static_cast<unsigned>(num_pages)) pages[i] = -1;
 }
 
-// The exponents of K and V of a page and head (0 counts as 1). A page id
+// A stored exponent: 0 counts as 1, 254 and 255 as 253.
+__device__ __forceinline__ int exponent_of(uint32_t sf) { return min(max(static_cast<int>(sf), 1), MAX_EXP); }
+
+// The exponents of K and V of a page and head. A page id
 // outside the cache (a bad table) loads zeros through the tensor map and takes
 // the smallest exponents, as does -1 (no page).
 __device__ __forceinline__ void page_exponents(const uint8_t* ksf, const uint8_t* vsf, int num_pages, int hkv,
@@ -116,8 +122,8 @@ __device__ __forceinline__ void page_exponents(const uint8_t* ksf, const uint8_t
   ke = ve = 1;
   if (page < 0 || page >= num_pages) return;
   const size_t at = static_cast<size_t>(page) * hkv + kvh;
-  ke = max(static_cast<int>(ksf[at]), 1);
-  ve = max(static_cast<int>(vsf[at]), 1);
+  ke = exponent_of(ksf[at]);
+  ve = exponent_of(vsf[at]);
 }
 
 // out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M) over the shares of one

@@ -4,7 +4,9 @@ One channel (K or V) of a layer holds
 
 * ``q``  [slots, hkv*128] float8_e4m3fn, slot = page*16 + offset, and
 * ``sf`` [slots/16, hkv] uint8: one scale 2^(sf-127) for each page of 16
-  tokens and KV head (0 counts as 1, so a zeroed cache holds zeros).
+  tokens and KV head (0 counts as 1, so a zeroed cache holds zeros; 254 and
+  255 as 253, whose inverse is a normal number too: no append needs more than
+  247).
 
 A key or value element is ``q * 2^(sf-127)``: half the bytes of the bf16 cache
 plus 1/2048 for the scales. A power of two keeps both conversions exact: a
@@ -47,6 +49,7 @@ from infera_b200.ops import kernels as K
 E4M3_MAX = 448.0
 PAGE = 16
 HEAD_DIM = 128
+MAX_EXP = 253
 _BF16, _I32, _U8, _E4M3 = torch.bfloat16, torch.int32, torch.uint8, torch.float8_e4m3fn
 
 
@@ -108,7 +111,7 @@ class KV8Cache:
 
     def dequant(self) -> torch.Tensor:
         """fp32 [.., slots, hkv*128]."""
-        s = _pow2(self.sf.to(torch.int32).clamp_min(1) - 127)
+        s = _pow2(_exponents(self.sf) - 127)
         x = self.q.float().unflatten(-1, (self.hkv, -1)).unflatten(-3, (-1, PAGE))
         return (x * s[..., :, None, :, None]).flatten(-4, -3).flatten(-2)
 
@@ -127,11 +130,15 @@ def _pow2(e: torch.Tensor) -> torch.Tensor:
     return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
 
 
+def _exponents(sf: torch.Tensor) -> torch.Tensor:
+    return sf.to(torch.int32).clamp(1, MAX_EXP)
+
+
 def _scale_exp(amax: torch.Tensor) -> torch.Tensor:
-    """Smallest biased exponent e in [1, 254] with amax <= 448 * 2^(e-127)."""
+    """Smallest biased exponent e in [1, 253] with amax <= 448 * 2^(e-127)."""
     m, e = torch.frexp(amax.double() / E4M3_MAX)
     e = torch.where(m == 0.5, e - 1, e) + 127
-    return torch.where(amax > 0, e, torch.ones_like(e)).clamp(1, 254).to(torch.int32)
+    return torch.where(amax > 0, e, torch.ones_like(e)).clamp(1, MAX_EXP).to(torch.int32)
 
 
 # ---------------------------------------------------------------- checks
@@ -269,7 +276,7 @@ def _rope_kvwrite_cpu(qkv, pos, slots, cos_sin, hq, hkv, k_cache, v_cache, q_out
             new = torch.where(new.isfinite(), new, float("nan"))
             e = _scale_exp(torch.nan_to_num(new, nan=0.0).abs().amax(dim=(0, 2)))
             if 0 not in at:
-                old = cache.sf[page].to(torch.int32).clamp_min(1)
+                old = _exponents(cache.sf[page])
                 e = torch.maximum(e, old)
                 shift = _pow2((old - e).clamp_min(-60))
                 codes[page] = (codes[page].float() * shift[None, :, None]).to(torch.float8_e4m3fn)

@@ -5,8 +5,9 @@ counts that no engine makes."""
 import pytest
 import torch
 
+from infera_b200.ops import kernels as K
 from infera_b200.ops import kv8
-from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain
+from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,61 @@ def test_far_page_ids_read_as_zeros(runs):
             bad[0, s] = (bt[0, s].long() + far).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
         for a, b in zip(both(kc, vc, bad), want):
             assert torch.equal(a, b)
+
+
+def test_largest_scales():
+    """Exponents end at 253: 254 and 255 count as it, in attention and when rows join such a page."""
+    hq, hkv = 4, 2
+    q, kc, vc, bt, sl = decode_case([40], hq, hkv, seed=22)
+    q = torch.zeros_like(q)  # all keys alike
+    vq = torch.exp2(torch.randint(-9, -2, vc.q.shape, device=DEV).float()).to(torch.float8_e4m3fn)
+    qkv = torch.full((2, 8 * D), 2.0 ** 120, dtype=torch.bfloat16)
+    qkv[1] *= -3
+    cs = K.rope_cos_sin(2, D, 1e4)
+    slots = torch.tensor([int(bt[0, 0]) * 16 + 9, int(bt[0, 1]) * 16 + 3], dtype=torch.int32)
+    zero = torch.zeros(2, dtype=torch.int32)
+    outs, held = [], []
+    for e in (253, 254, 255):
+        k, v = kv8.KV8Cache(kc.q.clone(), torch.full_like(kc.sf, e)), kv8.KV8Cache(vq.clone(), torch.full_like(vc.sf, e))
+        y = kv8.attn_decode(q, k, v, bt, sl, hq, hkv, 0.1)
+        yp = kv8.attn_prefill(q, k, v, bt, i32([0]), i32([1]), sl, None, hq, hkv, 0.1, host_meta=([1], [40]))
+        check_status()
+        assert bool(y.isfinite().all()) and bool(y.any()) and bool(yp.isfinite().all()) and bool(yp.any())
+        outs.append((y, yp))
+        cpu = [c.to("cpu") for c in (k, v)]
+        assert torch.equal(cpu[1].dequant(), kv8.KV8Cache(vq.cpu(), torch.full_like(vc.sf, 253).cpu()).dequant())
+        kv8.rope_kvwrite(qkv.to(DEV), zero.to(DEV), slots.to(DEV), cs.to(DEV), hq, hkv, D, k, v)
+        check_status()
+        kv8.rope_kvwrite(qkv.clone(), zero, slots, cs, hq, hkv, D, *cpu)
+        for x, c in ((k, cpu[0]), (v, cpu[1])):
+            assert torch.equal(x.q.cpu().view(torch.uint8), c.q.view(torch.uint8))
+            assert torch.equal(x.sf.cpu(), c.sf)
+        rows = v.dequant().view(-1, hkv, D)[slots.long().to(DEV)]
+        assert bool((rows[0] == 2.0 ** 120).all()) and bool((rows[1] == -3 * 2.0 ** 120).all())
+        held.append((k, v))
+    for o, h in zip(outs[1:], held[1:]):
+        assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
+        for a, b in zip(h, held[0]):
+            page = bt[0, :2].long()
+            assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.sf[page], b.sf[page])
+
+
+def test_largest_scales_of_whole_pages():
+    """Several rows of a page at once, which another path of the append takes."""
+    hkv = 2
+    qkv = torch.randn(9, 8 * D, generator=torch.Generator().manual_seed(1)).mul(2.0 ** 119).to(torch.bfloat16)
+    slots, pos = torch.arange(3, 12, dtype=torch.int32), torch.arange(9, dtype=torch.int32)
+    cs = K.rope_cos_sin(16, D, 1e4)
+    for e in (253, 254, 255):
+        c = [kv8.KV8Cache(random_cache(16, hkv, 1).q, torch.full((1, hkv), e, dtype=torch.uint8, device=DEV))
+             for _ in range(2)]
+        cpu = [x.to("cpu") for x in c]
+        kv8.rope_kvwrite(qkv.to(DEV), pos.to(DEV), slots.to(DEV), cs.to(DEV), 4, hkv, D, *c)
+        check_status()
+        kv8.rope_kvwrite(qkv.clone(), pos, slots, cs, 4, hkv, D, *cpu)
+        for x, y in zip(c, cpu):
+            assert torch.equal(x.q.cpu().view(torch.uint8), y.q.view(torch.uint8)) and torch.equal(x.sf.cpu(), y.sf)
+        v = c[1].dequant()[3:12].double().cpu()
+        want = qkv[:, 6 * D:].double()
+        assert int(c[1].sf[0, 0]) == 253
+        assert bool(((v - want).abs() <= torch.maximum(want.abs() * 2 ** -4, torch.tensor(2.0 ** 116))).all())
