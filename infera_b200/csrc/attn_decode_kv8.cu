@@ -536,14 +536,14 @@ __global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
       if (lane == 0) red[q4 * GP + h] = v;
     }
     barrier_or(false);
-    const float back = two_to(R - 127) * (1.f / (1 << kTopLog2));
+    const float back = two_to(R - 127);  // (times 2^-kTopLog2 it may be too small for a normal number)
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
       if (h >= G || !ok) break;
       const float l = red[h] + red[GP + h] + red[2 * GP + h] + red[3 * GP + h];
       const float acc = fmaf(fmaf(__uint_as_float(ov[2 * GP + h]), 0.03125f, __uint_as_float(ov[GP + h])), 0.03125f,
                              __uint_as_float(ov[h]));
-      const float o = l == 0.f ? 0.f : acc / l * back;
+      const float o = l == 0.f ? 0.f : acc / l * (1.f / (1 << kTopLog2)) * back;
       const int head = kvh * G + h;
       if (p.splits == 1) {
         p.out[static_cast<size_t>(b) * p.ldo + head * D + r] = __float2bfloat16(o);

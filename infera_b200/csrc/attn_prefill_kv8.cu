@@ -720,8 +720,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                                     (nut & 1) ? static_cast<uint32_t>(((nut - 1) >> 1) & 1) : 0u, abort_flag, p.status,
                                     kStatusTimeoutTmemFull)) {
       tc_fence_after();
-      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // a NaN stays one
-      const float back = two_to(max(R_run, 1) - 127) * (1.f / (1 << kTopLog2));
+      const float inv = l_run == 0.f ? 0.f : 1.0f / l_run * (1.f / (1 << kTopLog2));   // a NaN stays one
+      const float back = two_to(max(R_run, 1) - 127);
       if (S > 1 && write) p.lse_part[part] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
 #pragma unroll 1
       for (int c0 = 0; c0 < 128; c0 += 32) {

@@ -164,3 +164,23 @@ def test_largest_scales_of_whole_pages():
         want = qkv[:, 6 * D:].double()
         assert int(c[1].sf[0, 0]) == 253
         assert bool(((v - want).abs() <= torch.maximum(want.abs() * 2 ** -4, torch.tensor(2.0 ** 116))).all())
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("e", [1, 4, 6, 7])
+def test_smallest_value_scales(e, splits):
+    """Values of 2^(e-127) times a code, 2^-126 times a code at the least, are normal bf16 numbers like others. (What
+    becomes smaller than 2^-126 on the way, in a share's output or in a product of the merge, may be lost: some 2^-126
+    for each share.)"""
+    lens, hq, hkv, scale = [300], 8, 2, 0.1
+    q, kc, vc, bt, sl = decode_case(lens, hq, hkv, seed=21)
+    vc = kv8.KV8Cache(vc.q, torch.full_like(vc.sf, e))
+    want = plain(q, kc, vc, bt[0], 300, hq, hkv, scale)
+    want[1] += 2.0 ** -126 * 4 / TOKEN[0]
+    y = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, scale, splits=splits, tiles_per_split=3)
+    check_status()
+    assert_close(y, want, TOKEN)
+    y = kv8.attn_prefill(q, kc, vc, bt, i32([0]), i32([1]), sl, None, hq, hkv, scale, host_meta=([1], lens),
+                         kv_splits=splits)
+    check_status()
+    assert_close(y, want, PROMPT)
