@@ -340,10 +340,11 @@ __global__ void __launch_bounds__(NUM_THREADS, GP <= 4 ? 3 : 2)
     const int r = q4 * 32 + lane;     // key row of S, dim row of O
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     bool ok = true;
-    // exponents of the pages of 16 tiles: one page per thread
+    // exponents of the split's pages, of 16 tiles at a time: one page per thread
+    const int end_page = min(n_pages, t1 * (BKV / PAGE));
     auto page_of = [&](int j) -> int {
       const int lp = (t0 + j) * (BKV / PAGE) + t;
-      return lp < n_pages && j < nt ? __ldg(bt + lp) : -1;
+      return lp < end_page ? __ldg(bt + lp) : -1;
     };
     auto load_sf = [&](int page) -> uint32_t {
       int ke, ve;

@@ -184,3 +184,22 @@ def test_smallest_value_scales(e, splits):
                          kv_splits=splits)
     check_status()
     assert_close(y, want, PROMPT)
+
+
+def test_decode_split_counts_its_own_pages():
+    """A split's weights are held against the largest V scale of its own pages: keys of the next split whose values are
+    2^30 times as large, and whose weights are nothing, cost the first split's output no digit."""
+    hq, hkv, mine, n = 8, 2, 256, 512
+    q, kc, vc, bt, sl = decode_case([n], hq, hkv, seed=23, spread=1)
+    q = torch.zeros_like(q).view(1, hq, D)
+    q[..., 0] = 1.0
+    q = q.view(1, -1)
+    far = bt[0, mine // 16:].long()
+    codes = kc.q.view(torch.uint8).view(-1, 16, hkv, D)
+    codes.zero_()
+    codes[far, :, :, 0] = 0xFE  # -448
+    vc.sf[far] += 30
+    y = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, 1.0, splits=2, tiles_per_split=2)
+    check_status()
+    # e^-448 of a value below 2^46 is nothing beside the first split's
+    assert_close(y, plain(q, kc, vc, bt[0], mine, hq, hkv, 1.0), TOKEN)
