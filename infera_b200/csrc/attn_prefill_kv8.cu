@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       uint4 v[16];
       uint32_t mb = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = write ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 16; ++i) v[i] = write ? src[i] : make_uint4(0u, 0u, 0u, 0u);  // (out may be q)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};

@@ -311,6 +311,7 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
     """Single-token attention per sequence over the 8-bit cache. q: [B,
     >=hq*128] bf16 (row stride free), seq_lens: int32 [B] (keys including the
     current token; 0 gives a row of zeros). Up to 8 query heads per KV head.
+    ``out`` may be ``q`` itself.
 
     ``splits`` and ``tiles_per_split`` come from :func:`decode_plan`: split s
     covers the 128-key tiles [s*T, (s+1)*T) of every sequence, so ``splits *
@@ -366,13 +367,13 @@ def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale,
     lens = [int(x) for x in seq_lens.tolist()]
     bt = block_table if bt_rows is None else block_table[bt_rows.long()]
     y = out[: len(lens), : hq * HEAD_DIM]
-    y.zero_()
     some = [b for b, n in enumerate(lens) if n > 0]
+    kept = [lens[b] for b in some]
+    rows = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
+                            [[n - 1] for n in kept], kept, hq, hkv, scale)
+    y.zero_()  # (may be q)
     if some:
-        kept = [lens[b] for b in some]
-        outs = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
-                                [[n - 1] for n in kept], kept, hq, hkv, scale)
-        y[some] = torch.cat(outs, 0).to(q.dtype)
+        y[some] = torch.cat(rows, 0).to(q.dtype)
 
 
 # ---------------------------------------------------------------- prompt attention
@@ -423,7 +424,7 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     ``host_meta`` (q lengths, context lengths on the host; read back from the
     device without it) sizes the grid. The kernel makes its own work items of
     256 / group tokens, so ``tiles`` and ``tile_rows`` are not used. Up to 8
-    query heads per KV head. A row that sees no key (a context shorter than
+    query heads per KV head. ``out`` may be ``q`` itself. A row that sees no key (a context shorter than
     its chunk) is zero; rows of no sequence are left as they are. Bad lengths
     and table rows are treated as in :func:`attn_decode`. Nothing of a key
     that a row does not see reaches the row, a NaN neither."""

@@ -25,3 +25,36 @@ def test_largest_scales(e):
         assert bool((c.dequant()[21] == 2.0 ** 120).all()) and bool((c.sf[1] == 253).all())
     rest = [16 + o for o in range(16) if o != 5]
     assert torch.equal(vc.q.float()[rest], old[rest]) and torch.equal(vc.q.float()[:16], old[:16])
+
+
+def attention_case(lens, hq, hkv, rows, seed=1):
+    """(q, K, V, page table) of sequences on pages of their own, two pages to spare."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // 16) for n in lens]
+    pool = sum(need) + 2
+    order = torch.randperm(pool, generator=g).to(torch.int32)
+    bt = torch.zeros(len(lens), max(need), dtype=torch.int32)
+    for i, n in enumerate(need):
+        bt[i, :n] = order[sum(need[:i]):sum(need[:i]) + n]
+    q = (torch.randn(rows, hq * D, generator=g) / 60).to(torch.bfloat16)
+    return q, random_cache(pool * 16, hkv, seed), random_cache(pool * 16, hkv, seed + 1), bt
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def test_attention_in_place():
+    """The output may be the queries' own memory."""
+    hq, hkv = 4, 2
+    q, kc, vc, bt = attention_case([40, 1, 70], hq, hkv, 3)
+    args = (kc, vc, bt, i32(40, 0, 70), hq, hkv, 0.1)
+    want = kv8.attn_decode(q, *args)
+    mine = q.clone()
+    assert kv8.attn_decode(mine, *args, out=mine) is mine and torch.equal(mine, want)
+    assert bool(want[0].any()) and not want[1].any()
+    q, kc, vc, bt = attention_case([40, 70], hq, hkv, 25)
+    args = (kc, vc, bt, i32(0, 20), i32(20, 5), i32(13, 70), None, hq, hkv, 0.1)
+    want = kv8.attn_prefill(q, *args)
+    kv8.attn_prefill(q, *args, out=q)
+    assert torch.equal(q, want)

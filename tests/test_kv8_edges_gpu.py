@@ -203,3 +203,22 @@ def test_decode_split_counts_its_own_pages():
     check_status()
     # e^-448 of a value below 2^46 is nothing beside the first split's
     assert_close(y, plain(q, kc, vc, bt[0], mine, hq, hkv, 1.0), TOKEN)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_attention_in_place(splits):
+    """The output may be the queries' own memory."""
+    hq, hkv, lens = 32, 8, [700, 0, 300]
+    q, kc, vc, bt, sl = decode_case(lens, hq, hkv, seed=26)
+    args = (kc, vc, bt, sl, hq, hkv, 0.1)
+    want = kv8.attn_decode(q, *args, splits=splits, tiles_per_split=6)
+    mine = q.clone()
+    kv8.attn_decode(mine, *args, splits=splits, tiles_per_split=6, out=mine)
+    assert torch.equal(mine, want)
+    n = [600, 0, 7]
+    q = (torch.randn(sum(n), hq * D, generator=torch.Generator().manual_seed(2)) / 60).to(torch.bfloat16).to(DEV)
+    args = (kc, vc, bt, i32([0, 600, 600]), i32(n), sl, None, hq, hkv, 0.1)
+    want = kv8.attn_prefill(q, *args, host_meta=(n, lens), kv_splits=splits)
+    kv8.attn_prefill(q, *args, host_meta=(n, lens), kv_splits=splits, out=q)
+    assert torch.equal(q, want)
+    check_status()
