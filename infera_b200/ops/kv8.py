@@ -363,14 +363,27 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
     return out
 
 
+def _cpu_view(k_cache, v_cache, block_table, bt_rows, lens) -> tuple:
+    """(K, V, page table, lengths) for the CPU forms, what the kernels find wrong treated alike: the values end with a
+    page of zeros, which page ids outside the cache name; lengths end where the table does, and are 0 where ``bt_rows``
+    names no row of it."""
+    pages, (table_rows, places) = k_cache.sf.shape[0], block_table.shape
+    k, v = (torch.cat([c.dequant(), torch.zeros(PAGE, c.hkv * HEAD_DIM)]) for c in (k_cache, v_cache))
+    rows = torch.arange(len(lens)) if bt_rows is None else bt_rows.long()
+    known = ((rows >= 0) & (rows < table_rows)).tolist()
+    if not table_rows:
+        return k, v, block_table.new_zeros(len(lens), places), [0] * len(lens)
+    bt = block_table[rows.clamp(0, table_rows - 1)].long()
+    return (k, v, torch.where((bt >= 0) & (bt < pages), bt, pages),
+            [min(max(n, 0), places * PAGE) if ok else 0 for n, ok in zip(lens, known)])
+
+
 def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, out, bt_rows) -> None:
-    lens = [int(x) for x in seq_lens.tolist()]
-    bt = block_table if bt_rows is None else block_table[bt_rows.long()]
+    k, v, bt, lens = _cpu_view(k_cache, v_cache, block_table, bt_rows, seq_lens.tolist())
     y = out[: len(lens), : hq * HEAD_DIM]
     some = [b for b, n in enumerate(lens) if n > 0]
     kept = [lens[b] for b in some]
-    rows = K._ref_attention(q[some, : hq * HEAD_DIM], k_cache.dequant(), v_cache.dequant(), bt[some],
-                            [[n - 1] for n in kept], kept, hq, hkv, scale)
+    rows = K._ref_attention(q[some, : hq * HEAD_DIM], k, v, bt[some], [[n - 1] for n in kept], kept, hq, hkv, scale)
     y.zero_()  # (may be q)
     if some:
         y[some] = torch.cat(rows, 0).to(q.dtype)
@@ -450,9 +463,6 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
         ldo = hq * HEAD_DIM
     else:
         ldo = _check_rows("out", out, T, hq * HEAD_DIM, dev, 16)
-    if dev < 0:
-        _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out, bt_rows)
-        return out
     places = block_table.shape[1]
     if n and max(ctx_lens) > places * PAGE:
         raise ValueError(f"a context of {max(ctx_lens)} keys needs {-(-max(ctx_lens) // PAGE)} pages, block_table has "
@@ -460,11 +470,14 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
     items, rows, splits = prefill_plan(q_lens, ctx_lens, hq, hkv)
     if kv_splits is not None:
         splits = kv_splits
-        if splits < 1:
+        if not 1 <= splits <= 65535:
             raise ValueError(f"kv_splits {splits}")
     if rows > T:
         raise ValueError(f"{rows} rows in the chunks, q has {T}")
     if rows == 0:
+        return out
+    if dev < 0:
+        _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out, bt_rows)
         return out
     part = lse = None
     if splits > 1:
@@ -487,18 +500,18 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
 
 def _attn_prefill_cpu(q, k_cache, v_cache, block_table, q_start, q_lens, ctx_lens, hq, hkv, scale, out,
                       bt_rows) -> None:
-    k, v = k_cache.dequant(), v_cache.dequant()
+    k, v, bt, ctx_lens = _cpu_view(k_cache, v_cache, block_table, bt_rows, ctx_lens)
     # a value that is NaN reaches the rows that see it, and not by a weight of zero
     nan = v.isnan()
     v = v.masked_fill(nan, 0.0)
     for i, (n, ctx, at) in enumerate(zip(q_lens, ctx_lens, q_start.tolist())):
-        row = block_table[i if bt_rows is None else int(bt_rows[i])][None]
+        row = bt[i:i + 1]
         blind = min(n, max(0, n - ctx))  # the first rows of a chunk longer than its context
         out[at:at + blind, : hq * HEAD_DIM] = 0
         if n > blind:
             o, = K._ref_attention(q[at + blind:at + n, : hq * HEAD_DIM], k, v, row, [list(range(ctx - n + blind, ctx))],
                                   [ctx], hq, hkv, scale)
-            slots = (row[0, : -(-ctx // PAGE)].long()[:, None] * PAGE + torch.arange(PAGE)).flatten()[:ctx]
+            slots = (row[0, : -(-ctx // PAGE), None] * PAGE + torch.arange(PAGE)).flatten()[:ctx]
             seen = nan[slots].cumsum(0)[ctx - n + blind:] > 0
             seen = seen.unflatten(-1, (hkv, 1, HEAD_DIM)).expand(-1, -1, hq // hkv, -1).flatten(1)
             out[at + blind:at + n, : hq * HEAD_DIM] = o.masked_fill(seen, float("nan")).to(q.dtype)

@@ -58,3 +58,38 @@ def test_attention_in_place():
     want = kv8.attn_prefill(q, *args)
     kv8.attn_prefill(q, *args, out=q)
     assert torch.equal(q, want)
+
+
+def test_bad_tables_and_lengths():
+    """What the kernels find wrong is treated alike on CPU: a row that the table has not gives zeros (a negative one is
+    not counted from the end), a page id outside the cache reads as zeros, a length ends where the table does."""
+    hq, hkv = 4, 2
+    q, kc, vc, bt = attention_case([70, 40], hq, hkv, 2)
+    decode = lambda table, lens, **kw: kv8.attn_decode(q, kc, vc, table, i32(*lens), hq, hkv, 0.1, **kw)  # noqa: E731
+    good = decode(bt, (70, 40))
+    for bad in (-1, 2, -3):
+        y = decode(bt, (70, 40), bt_rows=i32(0, bad))
+        assert torch.equal(y[0], good[0]) and not y[1].any()
+        yp = kv8.attn_prefill(q, kc, vc, bt, i32(0, 1), i32(1, 1), i32(70, 40), None, hq, hkv, 0.1, bt_rows=i32(bad, 0))
+        assert not yp[0].any() and bool(yp[1].any())
+    assert torch.equal(decode(bt, (1000, -7))[0], decode(bt, (16 * bt.shape[1], 0))[0])
+    assert not decode(bt, (1000, -7))[1].any()
+    pages = kc.sf.shape[0]
+    blank = [kv8.KV8Cache(torch.cat([c.q, torch.zeros_like(c.q[:16])]), torch.cat([c.sf, torch.ones_like(c.sf[:1])]))
+             for c in (kc, vc)]
+    none = bt.clone()
+    none[0, 1] = pages
+    want = kv8.attn_decode(q, *blank, none, i32(70, 40), hq, hkv, 0.1)
+    wantp = kv8.attn_prefill(q, *blank, none, i32(0), i32(2), i32(70), None, hq, hkv, 0.1)
+    for bad in (pages, -1, 2 ** 28 + 1, 2 ** 31 - 1):
+        none[0, 1] = bad
+        assert torch.equal(decode(none, (70, 40)), want)
+        assert torch.equal(kv8.attn_prefill(q, kc, vc, none, i32(0), i32(2), i32(70), None, hq, hkv, 0.1), wantp)
+
+
+def test_prefill_refuses_on_cpu_what_it_refuses_on_the_gpu():
+    hq, hkv = 4, 2
+    q, kc, vc, bt = attention_case([70], hq, hkv, 4)
+    for n, ctx, kw in ((4, 16 * bt.shape[1] + 1, {}), (5, 70, {}), (4, 70, dict(kv_splits=0)), (4, 70, dict(kv_splits=70000))):
+        with pytest.raises(ValueError):
+            kv8.attn_prefill(q, kc, vc, bt, i32(0), i32(n), i32(ctx), None, hq, hkv, 0.1, **kw)
