@@ -176,14 +176,16 @@ def _check_heads(hq: int, hkv: int, most: int) -> None:
         raise ValueError(f"{hq} query heads over {hkv} KV heads: a whole number of at most {most} to one")
 
 
-def _check_rows(name: str, t: torch.Tensor, rows: int, width: int, dev: int, align: int) -> int:
-    """Rows of ``width`` adjacent bf16 elements; returns their pitch."""
+def _check_rows(name: str, t: torch.Tensor, rows: int, width: int, dev: int, align: int, written: bool = False) -> int:
+    """Rows of ``width`` adjacent bf16 elements; returns their pitch. Rows that are written share no memory."""
     shape = t.shape
     if t.dtype is not _BF16 or len(shape) != 2 or shape[0] < rows or shape[1] < width:
         raise ValueError(f"{name}: bf16 [{rows} or more, {width} or more], not {tuple(shape)} {t.dtype}")
     pitch, one = t.stride()
     if one != 1:
         raise ValueError(f"{name}: a row's elements have to be adjacent, not {one} apart")
+    if written and pitch < width and shape[0] > 1:
+        raise ValueError(f"{name}: rows of {width} elements that start {pitch} apart share memory")
     if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, the queries on {_name(dev)}")
     if dev >= 0 and (t.data_ptr() | (2 * pitch if shape[0] > 1 else 0)) & (align - 1):
@@ -224,11 +226,11 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
         raise ValueError(f"head_dim {head_dim}: the 8-bit cache holds heads of {HEAD_DIM}")
     _check_heads(hq, hkv, hq)
     T, dev = qkv.shape[0], qkv.get_device()
-    ld = _check_rows("qkv", qkv, T, (hq + 2 * hkv) * HEAD_DIM, dev, 16)
+    ld = _check_rows("qkv", qkv, T, (hq + 2 * hkv) * HEAD_DIM, dev, 16, q_out is None)
     if q_out is None:
         q_out, ldq = qkv, ld
     else:
-        ldq = _check_rows("q_out", q_out, T, hq * HEAD_DIM, dev, 16)
+        ldq = _check_rows("q_out", q_out, T, hq * HEAD_DIM, dev, 16, True)
     _check_i32("pos", pos, T, dev)
     _check_i32("slots", slots, T, dev)
     _check_caches(k_cache, v_cache, hkv, dev)
@@ -334,7 +336,7 @@ def attn_decode(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_tab
         out = torch.empty(B, hq * HEAD_DIM, dtype=_BF16, device=q.device)
         ldo = hq * HEAD_DIM
     else:
-        ldo = _check_rows("out", out, B, hq * HEAD_DIM, dev, 4)
+        ldo = _check_rows("out", out, B, hq * HEAD_DIM, dev, 4, True)
     if B == 0:
         return out
     if dev < 0:
@@ -462,7 +464,7 @@ def attn_prefill(q: torch.Tensor, k_cache: KV8Cache, v_cache: KV8Cache, block_ta
         out = torch.empty(T, hq * HEAD_DIM, dtype=_BF16, device=q.device)
         ldo = hq * HEAD_DIM
     else:
-        ldo = _check_rows("out", out, T, hq * HEAD_DIM, dev, 16)
+        ldo = _check_rows("out", out, T, hq * HEAD_DIM, dev, 16, True)
     places = block_table.shape[1]
     if n and max(ctx_lens) > places * PAGE:
         raise ValueError(f"a context of {max(ctx_lens)} keys needs {-(-max(ctx_lens) // PAGE)} pages, block_table has "

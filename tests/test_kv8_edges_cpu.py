@@ -93,3 +93,25 @@ def test_prefill_refuses_on_cpu_what_it_refuses_on_the_gpu():
     for n, ctx, kw in ((4, 16 * bt.shape[1] + 1, {}), (5, 70, {}), (4, 70, dict(kv_splits=0)), (4, 70, dict(kv_splits=70000))):
         with pytest.raises(ValueError):
             kv8.attn_prefill(q, kc, vc, bt, i32(0), i32(n), i32(ctx), None, hq, hkv, 0.1, **kw)
+
+
+def test_rows_that_share_memory():
+    """Read, rows may start anywhere; written, they have to be apart."""
+    hq, hkv = 4, 2
+    q, kc, vc, bt = attention_case([30, 70], hq, hkv, 2)
+    one = torch.zeros(1, hq * D, dtype=torch.bfloat16)
+    shared = (one.expand(2, -1), torch.zeros(2 * hq * D, dtype=torch.bfloat16).as_strided((2, hq * D), (hq * D - 8, 1)))
+    want = kv8.attn_decode(q[:1].repeat(2, 1), kc, vc, bt, i32(30, 70), hq, hkv, 0.1)
+    assert torch.equal(kv8.attn_decode(q[:1].expand(2, -1), kc, vc, bt, i32(30, 70), hq, hkv, 0.1), want)
+    for out in shared:
+        with pytest.raises(ValueError, match="share memory"):
+            kv8.attn_decode(q, kc, vc, bt, i32(30, 70), hq, hkv, 0.1, out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            kv8.attn_prefill(q, kc, vc, bt, i32(0, 1), i32(1, 1), i32(30, 70), None, hq, hkv, 0.1, out=out)
+    qkv, cs = torch.ones(1, 8 * D, dtype=torch.bfloat16).expand(2, -1), K.rope_cos_sin(4, D, 1e4)
+    with pytest.raises(ValueError, match="share memory"):
+        kv8.rope_kvwrite(qkv, i32(0, 1), i32(3, 4), cs, hq, hkv, D, kc, vc)
+    for out in shared:
+        with pytest.raises(ValueError, match="share memory"):
+            kv8.rope_kvwrite(qkv, i32(0, 1), i32(3, 4), cs, hq, hkv, D, kc, vc, q_out=out)
+    kv8.rope_kvwrite(qkv, i32(0, 1), i32(3, 4), cs, hq, hkv, D, kc, vc, q_out=torch.empty_like(q))
