@@ -234,6 +234,9 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
     _check_i32("pos", pos, T, dev)
     _check_i32("slots", slots, T, dev)
     _check_caches(k_cache, v_cache, hkv, dev)
+    kq, vq = k_cache.q.data_ptr(), v_cache.q.data_ptr()
+    if abs(kq - vq) < k_cache.slots * hkv * HEAD_DIM or k_cache.sf.data_ptr() == v_cache.sf.data_ptr():
+        raise ValueError("K and V are appended to the same memory")
     max_pos = cos_sin.shape[0]
     if cos_sin.dtype is not torch.float32 or cos_sin.shape != (max_pos, HEAD_DIM // 2, 2) \
             or not cos_sin.is_contiguous():
@@ -249,8 +252,7 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
         return q_out
     status, stream = _on(dev)
     rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, ld, q_out.data_ptr(), ldq, pos.data_ptr(),
-                                         slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, k_cache.q.data_ptr(),
-                                         k_cache.sf.data_ptr(), v_cache.q.data_ptr(), v_cache.sf.data_ptr(),
+                                         slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, kq, k_cache.sf.data_ptr(), vq, v_cache.sf.data_ptr(),
                                          k_cache.slots, max_pos, status, stream)
     _native.check(rc, "ib_kv8_append")
     K._count()

@@ -115,3 +115,18 @@ def test_rows_that_share_memory():
         with pytest.raises(ValueError, match="share memory"):
             kv8.rope_kvwrite(qkv, i32(0, 1), i32(3, 4), cs, hq, hkv, D, kc, vc, q_out=out)
     kv8.rope_kvwrite(qkv, i32(0, 1), i32(3, 4), cs, hq, hkv, D, kc, vc, q_out=torch.empty_like(q))
+
+
+def test_one_cache_for_keys_and_values():
+    """K and V of an append need memory of their own; attention may read one cache as both."""
+    hq, hkv = 4, 2
+    q, kc, vc, bt = attention_case([30], hq, hkv, 1)
+    qkv, cs = torch.ones(1, 8 * D, dtype=torch.bfloat16), K.rope_cos_sin(4, D, 1e4)
+    long = random_cache(96, hkv)
+    for k, v in ((kc, kc), (kc, kv8.KV8Cache(kc.q, vc.sf)), (kc, kv8.KV8Cache(vc.q, kc.sf)),
+                 (kv8.KV8Cache(long.q[:64], long.sf[:4]), kv8.KV8Cache(long.q[32:], long.sf[2:]))):
+        with pytest.raises(ValueError, match="same memory"):
+            kv8.rope_kvwrite(qkv, i32(0), i32(3), cs, hq, hkv, D, k, v)
+    layers = kv8.alloc(32, hkv, layers=2, device="cpu")
+    kv8.rope_kvwrite(qkv, i32(0), i32(3), cs, hq, hkv, D, layers[0], layers[1])
+    assert bool(kv8.attn_decode(q, kc, kc, bt, i32(30), hq, hkv, 0.1).any())
