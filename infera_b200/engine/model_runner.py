@@ -93,9 +93,10 @@ class ModelRunner:
         if self.on_gpu:
             sc = K.scratch(self.dev)
             sc.ensure_gemm(8 * 1024 * 1024)
-            max_splits = max(4, K.decode_plan(max_num_seqs, cfg.num_kv_heads, cfg.max_model_len)[0])
-            sc.ensure_decode(max_num_seqs * cfg.num_heads * max_splits * 128 + 64 * cfg.num_heads * 64 * 128,
-                             max_num_seqs * cfg.num_heads * max_splits + 64 * cfg.num_heads * 64)
+            if not kv8:  # (8-bit attention's partials are each call's own)
+                max_splits = max(4, K.decode_plan(max_num_seqs, cfg.num_kv_heads, cfg.max_model_len)[0])
+                sc.ensure_decode(max_num_seqs * cfg.num_heads * max_splits * 128 + 64 * cfg.num_heads * 64 * 128,
+                                 max_num_seqs * cfg.num_heads * max_splits + 64 * cfg.num_heads * 64)
         self.graph_sizes = [g for g in (graph_sizes or DEFAULT_GRAPH_SIZES) if g <= max_num_seqs]
         # decode graphs are captured per length class (the longest sequence
         # of the step): the split count of the decode attention is fixed in a

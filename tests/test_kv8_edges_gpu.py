@@ -222,3 +222,19 @@ def test_attention_in_place(splits):
     kv8.attn_prefill(q, *args, host_meta=(n, lens), kv_splits=splits, out=q)
     assert torch.equal(q, want)
     check_status()
+
+
+def test_engine_holds_no_decode_workspace(monkeypatch):
+    """8-bit attention's partials are each call's own: an engine with this cache sizes no bf16 decode workspace."""
+    from infera_b200.engine.llm_engine import EngineConfig, LLMEngine
+    from infera_b200.engine.request import SamplingParams
+
+    def never(self, o_numel, lse_numel):
+        raise AssertionError(f"a decode workspace of {o_numel} + {lse_numel} elements")
+
+    monkeypatch.setattr(K.DeviceScratch, "ensure_decode", never)
+    eng = LLMEngine(EngineConfig(model="tiny-dense-gpu", kv_cache_dtype="fp8", num_pages=64, max_num_seqs=4,
+                                 max_batched_tokens=96), device="cuda:0")
+    outs = eng.generate([[5, 6, 7], list(range(2, 150))], SamplingParams(max_tokens=5, ignore_eos=True))
+    check_status()
+    assert [len(o) for o in outs] == [5, 5]
