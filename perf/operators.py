@@ -292,7 +292,7 @@ def _own(st):
         kv8.rope_kvwrite(st["qkv"], st["pos"], st["slots"], st["cos_sin"], hq, hkv, D, kc, vc, q_out=q)
         return q
     if op == "decode":
-        splits, tps = kv8.decode_plan(len(st["keys"]), hkv, max(st["keys"]))
+        splits, tps = kv8.decode_plan(len(st["keys"]), hkv, max(st["keys"]), group=hq // hkv)
         return K.attn_decode(st["qkv"], kc, vc, st["table"], st["len"], hq, hkv, st["scale"], splits=splits, tiles_per_split=tps)
     return K.attn_prefill(st["qkv"], kc, vc, st["table"], st["start"], st["n"], st["len"], st["tiles"], hq, hkv, st["scale"],
                           host_meta=(st["rows"], st["keys"]), tile_rows=256)
