@@ -2,12 +2,14 @@
 one large dimension, the smallest and largest scales, page tables and split
 counts that no engine makes."""
 
+import math
+
 import pytest
 import torch
 
 from infera_b200.ops import kernels as K
 from infera_b200.ops import kv8
-from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain, random_cache
+from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain, poison, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +240,68 @@ def test_engine_holds_no_decode_workspace(monkeypatch):
     outs = eng.generate([[5, 6, 7], list(range(2, 150))], SamplingParams(max_tokens=5, ignore_eos=True))
     check_status()
     assert [len(o) for o in outs] == [5, 5]
+
+
+@pytest.mark.parametrize("ql,ctx", [([17], [4113]), ([300], [300]), ([1], [2000]), ([3], [8100]),
+                                    ([17, 256, 1, 300, 5], [17, 700, 90, 301, 1500]), ([20, 0, 40], [50, 0, 40])])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (8, 8), (32, 8)])
+def test_prefill_reads_its_lengths_back(ql, ctx, hq, hkv):
+    """Without host lengths the call reads them from the device and makes the same plan: the same bits, in a wider buffer
+    too, whose other columns and rows stay as they are."""
+    g = torch.Generator().manual_seed(hq)
+    _, kc, vc, bt, sl = decode_case(ctx, hq, hkv, seed=hq)
+    poison(kc, vc, bt, ctx)
+    T = sum(ql)
+    q = (torch.randn(T, hq * D, generator=g) / 60).to(torch.bfloat16).to(DEV)
+    start = [sum(ql[:i]) for i in range(len(ql))]
+    args = (q, kc, vc, bt, i32(start), i32(ql), sl, None, hq, hkv, 0.1)
+    y = kv8.attn_prefill(*args, host_meta=(ql, ctx))
+    out = torch.full((T + 2, hq * D + 8), 3.0, dtype=torch.bfloat16, device=DEV)
+    kv8.attn_prefill(*args, out=out)
+    check_status()
+    assert torch.equal(out[:T, : hq * D], y) and bool((out[T:] == 3).all()) and bool((out[:, hq * D:] == 3).all())
+
+
+@pytest.mark.parametrize("lens", [[8192, 8192], [8192, 100, 4097, 1], [1000] * 8])
+@pytest.mark.parametrize("hq,hkv", [(64, 8), (10, 2), (8, 1)])
+def test_decode_as_planned_for_more_than_four_heads(lens, hq, hkv):
+    """The splits that an engine takes for five to eight query heads to a KV head: one wave of two CTAs per SM."""
+    q, kc, vc, bt, sl = decode_case(lens, hq, hkv, seed=hq + len(lens))
+    splits, tps = kv8.decode_plan(len(lens), hkv, max(lens), group=hq // hkv)
+    assert splits == 1 or splits * len(lens) * hkv <= 2 * 148
+    y = kv8.attn_decode(q, kc, vc, bt, sl, hq, hkv, 1 / math.sqrt(D), splits=splits, tiles_per_split=tps)
+    check_status()
+    for b, n in enumerate(lens):
+        assert_close(y[b:b + 1], plain(q[b:b + 1], kc, vc, bt[b], n, hq, hkv, 1 / math.sqrt(D)), TOKEN)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("model,over", [("tiny-dense-gpu", {"qk_norm": True}), ("tiny-moe-gqa-gpu", {})])
+def test_models(model, over, graphs):
+    """Models with q / k norms and with routed experts over an 8-bit cache: the first layer's K and V depend on tokens
+    and positions alone. An element is off by half a step of e4m3 (2^-4 of it; 2^-10 of the scale below the normals,
+    and the scale is at most 2^-7 of its page's largest element; once more where a page's scale grew), and by a step of
+    bf16 where the two engines' products round differently."""
+    from infera_b200.engine.llm_engine import EngineConfig, LLMEngine
+    from infera_b200.engine.request import SamplingParams
+
+    g = torch.Generator().manual_seed(3)
+    ask = [torch.randint(2, 4096, (n,), generator=g).tolist() for n in (40, 300, 33)]
+    got = []
+    for kv in ("fp8", "bf16"):
+        e = LLMEngine(EngineConfig(model=model, kv_cache_dtype=kv, num_pages=64, max_batched_tokens=96, max_num_seqs=4,
+                                   use_cuda_graphs=graphs, model_overrides=dict(over)), device="cuda:0")
+        e.generate(ask, SamplingParams(max_tokens=1, ignore_eos=True))
+        check_status()
+        k, v = e.runner.k_cache, e.runner.v_cache
+        got.append((k[0].dequant(), v[0].dequant()) if kv == "fp8" else (k[0].float(), v[0].float()))
+        if kv == "fp8":
+            got[0] = tuple(t.clone() for t in got[0])
+            outs = e.generate([p + [5, 6] for p in ask], SamplingParams(max_tokens=12, ignore_eos=True))
+            check_status()
+            assert [len(o) for o in outs] == [12, 12, 12]
+    for x, y in zip(*got):
+        used = y.abs().sum(-1) > 0
+        assert int(used.sum()) >= 320 and torch.equal(used, x.abs().sum(-1) > 0)
+        page = y.view(-1, 16, 2, D).abs().amax(dim=(1, 3))[:, None, :, None].expand(-1, 16, 2, D).reshape(y.shape)
+        assert bool(((x - y).abs() <= y.abs() * (2 ** -4 + 2 ** -7) + (2 * 2 ** -10 * 2 ** -7 + 2 ** -20) * page).all())
