@@ -47,11 +47,13 @@
 // Split partials (output normalised by its own sum, LSE in log2 units) are
 // merged by a combine kernel.
 //
-// Bound by HBM: two 8-bit codes per key, dim and KV head. 32 sequences of 8192
-// keys (64 heads over 8) take 88 us (6.1 TB/s, 0.93 of the copy rate), 61 ragged
-// ones on scattered pages (32 over 8) 125 us (0.90: boxes of 2 KB), one of
-// 120001 keys 44 us (0.85, with its start and the merge of 53 shares), one of
-// 100 keys 5.3 us.
+// Bound by HBM: two 8-bit codes per key, dim and KV head. Captured calls of 32
+// sequences of 8192 keys (64 heads over 8) take 87 to 89 us (6.1 TB/s, 0.93 of
+// the copy rate), of 61 ragged ones on scattered pages (32 over 8) 124 to 126 us
+// (0.90: boxes of 2 KB), of one of 120001 keys 44 us (0.85, with its start and
+// the merge of 53 shares), of one of 100 keys 5.5 us. Eager calls on changing
+// inputs take 89 to 94 (0.87), 127 to 135 (0.83), 43 to 45 and, bound by the
+// host, 16 us.
 #include "kv8.cuh"
 #include "tma_host.h"
 

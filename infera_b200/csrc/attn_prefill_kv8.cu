@@ -43,12 +43,17 @@
 // context); shares are merged by a combine kernel. Items are found from q_len
 // on the device, the ones with the most keys first.
 //
-// Bound by the chain S, softmax, W V of each query tile: 2.1 us for 256 rows x
-// 128 keys, where the tensor core needs 1.46 at the measured rate. 1024 rows of
-// 64 heads (over 8) and 32768 keys take 1130 us (958 TFLOP/s, 0.56 of the
-// library's bf16 rate), six ragged prompts of 64 heads 231 us (0.43), 224 rows
-// of 32 heads over 8416 keys 56 us, 17 rows over 4113 keys 16.7 us. Slower: sixteen softmax warps, an MMA warp for each query
-// tile, exponentials on the FMA pipe.
+// Bound by two things. A tile of 256 rows x 128 keys takes 2.1 us, the chain S,
+// softmax, W V of each query tile, where the tensor core needs 1.46 at the
+// measured rate. And a CTA takes one item or share, one CTA to an SM, so each
+// exposes its start (Q staged, first tiles loaded) and its end, and the last
+// round of CTAs leaves SMs idle. Captured calls of 1024 rows of 64 heads (over 8)
+// and 32768 keys take 1113 to 1150 us (942 to 973 TFLOP/s, 0.55 to 0.57 of the
+// library's bf16 rate; 917 us at 2.1 us a tile on all SMs), of six ragged prompts
+// of 64 heads 230 us (0.43; 156), of 224 rows of 32 heads over 8416 keys 56 us
+// (30), of 17 rows over 4113 keys 16.2 to 16.7 us. Eager calls on changing inputs
+// take 1165 to 1191, 234 to 240, 59 and 24 us. Slower: sixteen softmax warps, an
+// MMA warp for each query tile, exponentials on the FMA pipe.
 #include <limits.h>
 
 #include <type_traits>

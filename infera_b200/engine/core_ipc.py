@@ -447,7 +447,7 @@ def main(argv=None) -> None:
     p.add_argument("--kv-index-model", default="", help="served model name in those events")
     p.add_argument("--kv-index-compat", default="", help="compat key (tokenizer digest) in those events")
     p.add_argument("--kv-cache-dtype", choices=("bf16", "fp8"), default="bf16",
-                   help="fp8: e4m3 KV cache with a scale per page and head (dense GQA models)")
+                   help="fp8: e4m3 KV cache with a scale per page and head (GQA models, dense or with experts)")
     p.add_argument("--kv-tier", default=None)
     p.add_argument("--tp-size", type=int, default=1, help="tensor-parallel ranks (RANK / LOCAL_RANK / MASTER_* from env)")
     p.add_argument("--first-device", type=int, default=0, help="tensor-parallel rank r runs on cuda:(first + r)")

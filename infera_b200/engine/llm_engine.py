@@ -73,9 +73,10 @@ class EngineConfig:
     max_model_len: int | None = None
     model_overrides: dict = field(default_factory=dict)
     # KV cache: "bf16", or "fp8" (e4m3 with a scale per page and head, see
-    # ops/kv8.py: twice the tokens in the same memory). fp8 serves dense GQA
-    # models with 128-dim heads on one instance: without kv_tier and
-    # disagg_mode, whose chunk and push formats carry no scales
+    # ops/kv8.py: twice the tokens in the same memory). fp8 serves GQA models
+    # (dense or with routed experts) with 128-dim heads and at most 8 query
+    # heads to a KV head on one instance: without kv_tier and disagg_mode,
+    # whose chunk and push formats carry no scales
     kv_cache_dtype: str = "bf16"
     # KV tiering: None (off), "pinned:<GiB>" (in-process page-locked arena of
     # page slots, DMA both ways), "host:<GiB>[:<nvme dir>]" (in-process host store,

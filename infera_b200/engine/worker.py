@@ -103,7 +103,7 @@ def parse_args(argv=None):
     p.add_argument("--handback-after", type=float, default=None)
     p.add_argument("--tokenizer", default=None)
     p.add_argument("--kv-cache-dtype", choices=("bf16", "fp8"), default="bf16",
-                   help="fp8: e4m3 KV cache with a scale per page and head (dense GQA models)")
+                   help="fp8: e4m3 KV cache with a scale per page and head (GQA models, dense or with experts)")
     p.add_argument("--kv-tier", default=None, help="host:<GiB>[:<nvme dir>] or kvd:<socket>")
     p.add_argument("--in-process", action="store_true", help="run the engine on a thread of this process")
     p.add_argument("--attach-core", default=None, help="IN,OUT ipc addresses of a running engine core")
