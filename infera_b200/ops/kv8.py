@@ -252,8 +252,8 @@ def rope_kvwrite(qkv: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor, cos_
         return q_out
     status, stream = _on(dev)
     rc = _native.kernels().ib_kv8_append(qkv.data_ptr(), T, ld, q_out.data_ptr(), ldq, pos.data_ptr(),
-                                         slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, kq, k_cache.sf.data_ptr(), vq, v_cache.sf.data_ptr(),
-                                         k_cache.slots, max_pos, status, stream)
+                                         slots.data_ptr(), cos_sin.data_ptr(), hq, hkv, kq, k_cache.sf.data_ptr(),
+                                         vq, v_cache.sf.data_ptr(), k_cache.slots, max_pos, status, stream)
     _native.check(rc, "ib_kv8_append")
     K._count()
     return q_out

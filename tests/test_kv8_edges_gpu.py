@@ -9,7 +9,8 @@ import torch
 
 from infera_b200.ops import kernels as K
 from infera_b200.ops import kv8
-from test_kv8_gpu import PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain, poison, random_cache
+from test_kv8_gpu import (PROMPT, TOKEN, assert_close, check_decode, check_status, decode_case, i32, plain, poison,
+                          random_cache)
 
 pytestmark = pytest.mark.gpu
 
