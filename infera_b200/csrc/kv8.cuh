@@ -1,5 +1,7 @@
 // What the kernels of the 8-bit KV cache share: e4m3 conversions, powers of
-// two, the exponents of pages, and the merge of key shares.
+// two, the exponents of pages, and the merge of key shares. The attention
+// kernels of the bf16 cache that came after them use the tcgen05 issue, the
+// page checks and the merge too.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -69,6 +71,16 @@ __device__ __forceinline__ void umma_e4m3_if(uint32_t on, uint32_t d_tmem, uint6
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.ne.b32 q, %5, 0;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void umma_bf16_if(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
       : "memory");
 }

@@ -1,0 +1,409 @@
+// Which keys of a cache stay, and moving them together.
+//
+// select_kernel: for each (sequence, KV head), of L keys with accumulated
+// weights x: the first `sink`, the last `recent`, and of the others those with
+// the largest x (equal ones: the lowest place first), `keep` in all, as places
+// in ascending order. The threshold is found digit by digit (11, 11 and 10 bits
+// of the weight as an unsigned number of the same order) in histograms; a last
+// pass counts and one writes the places, each behind what lies before it. A
+// cluster of CTAs shares a list: each takes a run of places and adds up the
+// others' histograms through distributed shared memory.
+//
+// compact_kernel: rows src[i] -> i of a sequence's places, in place. src[i] >=
+// i, so a row is never written before a row that is read later lies there:
+// places are taken in ascending order, and a group's rows are all read (into
+// registers) before the first of them is written. A CTA owns its columns, so
+// no other one touches them.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "kv8.cuh"
+
+namespace ib200 {
+namespace sel {
+
+namespace cg = cooperative_groups;
+using kv8::table_row;
+
+constexpr int THREADS = 1024;
+constexpr int WARPS = THREADS / 32;
+constexpr int BINS = 2048;
+
+struct SelectParams {
+  float* mass;            // [mass_rows, hkv, cap]
+  int mass_rows, hkv;
+  long long cap;
+  const int* seq_lens;
+  const int* bt_rows;
+  int keep, sink, recent;
+  int update;             // write the kept weights back, zero behind them
+  int* kept;              // [n, hkv, keep]
+  float* kept_mass;       // [n, hkv, keep]
+  int* count;             // [n]
+  int* status;
+};
+
+// An unsigned number in the order of the weights: a NaN below all, -0 as 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  uint32_t u = __float_as_uint(x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
+  if ((u << 1) == 0u) u = 0u;
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
+  pdl_trigger();
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int list = blockIdx.x / C, s = list / p.hkv, h = list % p.hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ uint32_t hist[BINS];
+  __shared__ uint32_t wsum[WARPS], wgt[WARPS], weq[WARPS];
+  __shared__ uint32_t s_bin, s_want, totals[2];
+
+  const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
+  long long n_keys = max(p.seq_lens[s], 0);
+  bool bad = row < 0 || row >= p.mass_rows;
+  if (bad && tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, row);
+  if (!bad && n_keys > p.cap) {
+    if (tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, static_cast<int>(n_keys));
+    n_keys = p.cap;
+  }
+  if (!bad && p.update && p.bt_rows != nullptr) {  // a row that an earlier sequence has is that one's to change
+    bool twice = false;
+    for (int i = tid; i < s; i += THREADS) twice = twice || p.bt_rows[i] == row;
+    if (__syncthreads_or(twice)) {
+      if (tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 7, s, row);
+      bad = true;
+    }
+  }
+  const int L = bad ? 0 : static_cast<int>(n_keys);
+  float* x = p.mass + (static_cast<size_t>(bad ? 0 : row) * p.hkv + h) * static_cast<size_t>(p.cap);
+  int* kept = p.kept + static_cast<size_t>(list) * p.keep;
+  float* kept_mass = p.kept_mass + static_cast<size_t>(list) * p.keep;
+  if (h == 0 && rank == 0 && tid == 0) p.count[s] = min(L, p.keep);
+  const int all = C * THREADS, at = rank * THREADS + tid;
+  if (L <= p.keep) {  // all stay (the whole cluster is here)
+    for (int i = at; i < p.keep; i += all) {
+      kept[i] = i < L ? i : -1;
+      kept_mass[i] = i < L ? x[i] : 0.f;
+    }
+    return;
+  }
+  const int lo = p.sink, hi = L - p.recent;
+  for (int i = at; i < p.sink; i += all) {
+    kept[i] = i;
+    kept_mass[i] = x[i];
+  }
+  for (int i = at; i < p.recent; i += all) {
+    kept[p.keep - p.recent + i] = hi + i;
+    kept_mass[p.keep - p.recent + i] = x[hi + i];
+  }
+  // this CTA's run of places, and within it one for each warp
+  const int run = (((hi - lo + C - 1) / C + THREADS - 1) / THREADS) * THREADS;
+  const int first = min(hi, lo + min(rank, (hi - lo) / run + 1) * run), last = min(hi, first + run);
+  uint32_t want = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // of those that match the digits so far
+  uint32_t prefix = 0, known = 0;
+  if (want > 0) {
+#pragma unroll 1
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bits = digit == 2 ? 10 : 11;
+      for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = first + tid; i < last; i += THREADS) {
+        const uint32_t k = order_of(x[i]);
+        if (((k ^ prefix) & known) == 0) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+      }
+      cluster.sync();
+      // the bin in which the want-th largest lies: thread t has the bins 2 t and 2 t + 1 from the top
+      uint32_t c[2] = {0u, 0u};
+      const int top = BINS - 1 - 2 * tid;
+      for (int r = 0; r < C; ++r) {
+        const uint32_t* other = cluster.map_shared_rank(hist, r);
+        c[0] += other[top];
+        c[1] += other[top - 1];
+      }
+      uint32_t sum = c[0] + c[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (lane == 31) wsum[warp] = sum;
+      __syncthreads();
+      uint32_t before = sum - c[0] - c[1];
+      for (int w = 0; w < warp; ++w) before += wsum[w];
+      if (before < want && before + c[0] + c[1] >= want) {
+        const bool second = before + c[0] < want;
+        s_bin = static_cast<uint32_t>(second ? top - 1 : top);
+        s_want = want - before - (second ? c[0] : 0u);
+      }
+      cluster.sync();  // s_bin; and the histograms are read
+      want = s_want;
+      prefix |= s_bin << shift;
+      known |= ((1u << bits) - 1) << shift;
+    }
+  } else {
+    prefix = 0xffffffffu;  // above every weight's number but that of a NaN that none has
+  }
+  // places above the threshold and at it, of which the first `want` stay
+  const int seg = run / WARPS;
+  const int w0 = min(last, first + warp * seg), w1 = min(last, w0 + seg);
+  uint32_t gt = 0, eq = 0;
+#pragma unroll 4
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t k = order_of(x[i]);
+    gt += k > prefix;
+    eq += k == prefix;
+  }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
+    wgt[warp] = gt;
+    weq[warp] = eq;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, wgt[lane]), b = __reduce_add_sync(0xffffffffu, weq[lane]);
+    if (lane == 0) {
+      totals[0] = a;
+      totals[1] = b;
+    }
+  }
+  cluster.sync();
+  gt = eq = 0;
+  for (int r = 0; r < rank; ++r) {
+    const uint32_t* other = cluster.map_shared_rank(totals, r);
+    gt += other[0];
+    eq += other[1];
+  }
+  for (int w = 0; w < warp; ++w) {
+    gt += wgt[w];
+    eq += weq[w];
+  }
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const float v = i < w1 ? x[i] : 0.f;
+    const uint32_t k = order_of(v);
+    const uint32_t above = __ballot_sync(0xffffffffu, i < w1 && k > prefix);
+    const uint32_t same = __ballot_sync(0xffffffffu, i < w1 && k == prefix);
+    const uint32_t lower = (1u << lane) - 1;
+    const uint32_t g = gt + __popc(above & lower), e = eq + __popc(same & lower);
+    if ((above >> lane & 1) || ((same >> lane & 1) && e < want)) {
+      const int to = p.sink + static_cast<int>(g + min(e, want));
+      kept[to] = i;
+      kept_mass[to] = v;
+    }
+    gt += __popc(above);
+    eq += __popc(same);
+  }
+  cluster.sync();  // (no CTA leaves while another reads its totals)
+  if (p.update) {
+    for (int i = at; i < L; i += all) x[i] = i < p.keep ? __ldcg(kept_mass + i) : 0.f;
+  }
+}
+
+constexpr int MOVE_THREADS = 512;
+constexpr int ENTRIES = 2 * MOVE_THREADS;  // places resolved at a time
+constexpr int UNITS = 8;                   // 16-byte pieces that a thread holds
+
+struct MoveParams {
+  uint8_t* k;
+  uint8_t* v;
+  int layers, group;         // layers of a CTA
+  long long layer_bytes;
+  int pitch;                 // bytes of a slot
+  int width, lanes;          // bytes of a list's columns, 16-byte pieces of a CTA's
+  int parts;
+  int num_pages;
+  const int* block_table;
+  const int* bt_rows;
+  int table_rows, max_pages, ld_table;
+  const int* src;            // [n, heads, m]
+  int heads, m;
+  const int* count;          // [n]
+  const int* start;          // [n] or null
+  int* status;
+};
+
+__global__ void __launch_bounds__(MOVE_THREADS) compact_kernel(const MoveParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int s = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int from[ENTRIES], to[ENTRIES];
+  __shared__ int wsum[MOVE_THREADS / 32];
+  const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
+  const int* bt = table_row(p.block_table, row, p.table_rows, p.ld_table, s, p.status);
+  if (p.bt_rows != nullptr) {  // a sequence whose places an earlier one has too stays as that one leaves it
+    bool twice = false;
+    for (int i = tid; i < s; i += MOVE_THREADS) twice = twice || p.bt_rows[i] == row;
+    if (__syncthreads_or(twice)) {
+      if (tid == 0) record_status_detail(p.status, kStatusBadIndex, 7, s, row);
+      return;
+    }
+  }
+  const int count = min(max(p.count[s], 0), p.m);
+  const long long start = p.start != nullptr ? p.start[s] : 0;
+  if (bt == nullptr || count == 0) return;
+  if (start < 0) {
+    if (tid == 0) record_status_detail(p.status, kStatusBadIndex, 1, s, static_cast<int>(start));
+    return;
+  }
+  const int* src = p.src + (static_cast<size_t>(s) * p.heads + h) * p.m;
+  const int l0 = blockIdx.z * p.group, layers = min(p.group, p.layers - l0);
+  uint8_t* cache = (static_cast<int>(blockIdx.y) < p.parts ? p.k : p.v) + l0 * p.layer_bytes + static_cast<size_t>(h) * p.width +
+                   static_cast<size_t>(blockIdx.y % p.parts) * p.lanes * 16;
+  const long long places = static_cast<long long>(p.max_pages) * kv8::PAGE;
+  for (int e0 = 0; e0 < count; e0 += ENTRIES) {
+    // slots of the next places that move, in order
+    int a[2], b[2];
+    bool moves[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = e0 + 2 * tid + i;
+      const int v = e < count ? src[e] : -1;
+      const long long pa = start + v, pb = start + e;
+      moves[i] = v > e;
+      if ((v < e && v != -1 && e < count) || (moves[i] && pa >= places)) {
+        record_status_detail(p.status, kStatusBadIndex, 8, s, v);
+        moves[i] = false;
+      }
+      a[i] = b[i] = 0;
+      if (moves[i]) {
+        const int ga = bt[pa / kv8::PAGE], gb = bt[pb / kv8::PAGE];
+        if (static_cast<unsigned>(ga) >= static_cast<unsigned>(p.num_pages) ||
+            static_cast<unsigned>(gb) >= static_cast<unsigned>(p.num_pages)) {
+          record_status_detail(p.status, kStatusBadIndex, 2, s, static_cast<unsigned>(ga) >= static_cast<unsigned>(p.num_pages) ? ga : gb);
+          moves[i] = false;
+        }
+        a[i] = ga * kv8::PAGE + static_cast<int>(pa % kv8::PAGE);
+        b[i] = gb * kv8::PAGE + static_cast<int>(pb % kv8::PAGE);
+      }
+    }
+    const int mine = moves[0] + moves[1];
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) wsum[warp] = sum;
+    __syncthreads();
+    int total = 0, at = sum - mine;
+#pragma unroll
+    for (int w = 0; w < MOVE_THREADS / 32; ++w) {
+      at += w < warp ? wsum[w] : 0;
+      total += wsum[w];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (moves[i]) {
+        from[at] = a[i];
+        to[at++] = b[i];
+      }
+    __syncthreads();
+    const unsigned per_layer = static_cast<unsigned>(total) * p.lanes, units = per_layer * layers;
+    for (unsigned u0 = 0; u0 < units; u0 += MOVE_THREADS * UNITS) {
+      uint4 v[UNITS];
+      auto place = [&](unsigned u, const int* slot) {
+        const unsigned l = u / per_layer, w = u - l * per_layer, e = w / p.lanes, c = w - e * p.lanes;
+        return reinterpret_cast<uint4*>(cache + l * p.layer_bytes + static_cast<size_t>(slot[e]) * p.pitch + c * 16);
+      };
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const unsigned u = u0 + i * MOVE_THREADS + tid;
+        if (u < units) v[i] = __ldcg(place(u, from));
+      }
+      __syncthreads();  // all are read
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const unsigned u = u0 + i * MOVE_THREADS + tid;
+        if (u < units) *place(u, to) = v[i];
+      }
+    }
+    __syncthreads();  // the list is used
+  }
+}
+
+}  // namespace sel
+}  // namespace ib200
+
+using namespace ib200;
+
+// mass fp32 [mass_rows, hkv, cap], row bt_rows[s] (null: s); kept / kept_mass
+// [n, hkv, keep], count [n]. sink + recent <= keep. cluster: CTAs of a list, 1 to 8.
+extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, const int* seq_lens,
+                            const int* bt_rows, int n, int keep, int sink, int recent, int update, int cluster,
+                            int* kept, float* kept_mass, int* count, int* status, cudaStream_t stream) {
+  using namespace ib200::sel;
+  if (n <= 0) return 0;
+  if (hkv <= 0 || keep < 1 || sink < 0 || recent < 0 || sink > keep - recent || cap < 0 ||
+      (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) ||
+      static_cast<long long>(n) * hkv * cluster > INT32_MAX)
+    return -1;
+  SelectParams p{mass, mass_rows, hkv, cap, seq_lens, bt_rows, keep, sink, recent, update, kept, kept_mass, count, status};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(n) * hkv * cluster);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, select_kernel, p));
+}
+
+// Caches [layers, num_slots, row_bytes] (v null: one channel). src [n, heads, m]:
+// list (s, h) moves the columns h * row_bytes / heads .. of places start[s] +
+// src[s, h, i] to start[s] + i, i < count[s].
+extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, int row_bytes, const int* block_table,
+                             const int* bt_rows, int table_rows, int max_pages, int ld_table, const int* src, int n,
+                             int heads, int m, const int* count, const int* start, int num_sms, int* status,
+                             cudaStream_t stream) {
+  using namespace ib200::sel;
+  if (n <= 0 || m <= 0 || layers <= 0) return 0;
+  if (heads <= 0 || row_bytes <= 0 || row_bytes % heads != 0 || (row_bytes / heads) % 16 != 0 || num_slots < kv8::PAGE ||
+      num_slots % kv8::PAGE != 0 || num_slots > INT32_MAX || max_pages < 0 || k == nullptr || num_sms <= 0 ||
+      static_cast<long long>(n) * heads > INT32_MAX ||
+      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0)
+    return -1;
+  MoveParams p;
+  p.k = static_cast<uint8_t*>(k);
+  p.v = static_cast<uint8_t*>(v);
+  const int channels = v != nullptr ? 2 : 1;
+  p.layers = layers;
+  p.layer_bytes = num_slots * row_bytes;
+  p.pitch = row_bytes;
+  p.width = row_bytes / heads;
+  p.num_pages = static_cast<int>(num_slots / kv8::PAGE);
+  p.block_table = block_table;
+  p.bt_rows = bt_rows;
+  p.table_rows = table_rows;
+  p.max_pages = max_pages;
+  p.ld_table = ld_table;
+  p.src = src;
+  p.heads = heads;
+  p.m = m;
+  p.count = count;
+  p.start = start;
+  p.status = status;
+  const long long lists = static_cast<long long>(n) * heads * channels;
+  // one CTA moves about 20 GB/s a row group at a time, so few lists are cut
+  // into columns of 64 bytes or more, and few sequences into groups of layers
+  p.parts = 1;
+  while (p.parts < 4 && lists * p.parts < 2 * num_sms && p.width % (2 * p.parts * 64) == 0) p.parts *= 2;
+  p.lanes = p.width / 16 / p.parts;
+  const long long groups = std::min<long long>(layers, std::max<long long>(1, 4LL * num_sms / (lists * p.parts)));
+  p.group = static_cast<int>((layers + groups - 1) / groups);
+  if (static_cast<long long>(p.group) * ENTRIES * p.lanes > INT32_MAX) return -1;
+  const dim3 grid(static_cast<unsigned>(n) * heads, channels * p.parts, (layers + p.group - 1) / p.group);
+  if (grid.z > 65535) return -1;
+  return static_cast<int>(launch_pdl(compact_kernel, grid, MOVE_THREADS, 0, stream, p));
+}

@@ -130,6 +130,17 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
                                 c_vp, c_int, c_vp, c_vp],
         "ib_attn_decode_kv8": [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                                c_int, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
+        "ib_attn_decode_mass": [c_vp, c_int, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
+                                c_int, c_int, c_int, c_float, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_ll, c_vp, c_int,
+                                c_vp, c_vp],
+        "ib_kv_select": [c_vp, c_int, c_int, c_ll, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp,
+                         c_vp, c_vp, c_vp],
+        "ib_kv_compact": [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_int, c_int,
+                          c_vp, c_vp, c_int, c_vp, c_vp],
+        "ib_attn_tree": [c_vp, c_int, c_int, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp,
+                         c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
+        "ib_tree_mask": [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp],
+        "ib_tree_accept": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp],
         "ib_gemm_set_trace": [c_vp],
         "ib_gemm_set_tile_counters": [c_vp, c_int],
         "ib_gemm_fused_reduce": [],

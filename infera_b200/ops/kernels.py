@@ -526,7 +526,8 @@ def decode_splits(batch: int, hkv: int, max_len: int, num_sms: int = 148) -> int
 def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                 seq_lens: torch.Tensor, hq: int, hkv: int, scale: float, splits: int = 1,
                 out: torch.Tensor | None = None, bt_rows: torch.Tensor | None = None,
-                impl: str = "tc", tiles_per_split: int = 0, l2_policy: int = 0) -> torch.Tensor:
+                impl: str = "tc", tiles_per_split: int = 0, l2_policy: int = 0,
+                mass: torch.Tensor | None = None) -> torch.Tensor:
     """Single-token attention per sequence. q: [B, >=hq*D] (row stride
     free), seq_lens: int32 [B] (keys including the current token).
 
@@ -536,7 +537,14 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     every sequence (``splits * T * 128`` must cover the longest), so CTAs
     reading a shared prefix run together; ``l2_policy`` 0/1/2: K/V loads
     evict_first / evict_normal / evict_last. 8-bit caches go to
-    :func:`infera_b200.ops.kv8.attn_decode`."""
+    :func:`infera_b200.ops.kv8.attn_decode`; with ``mass`` the call goes to
+    :func:`infera_b200.ops.evict.attn_decode`, which also adds what each key
+    received (``impl`` and ``l2_policy`` have no meaning there)."""
+    if mass is not None:
+        from infera_b200.ops import evict
+
+        return evict.attn_decode(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale, mass, splits=splits,
+                                 out=out, bt_rows=bt_rows, tiles_per_split=tiles_per_split)
     if not isinstance(k_cache, torch.Tensor):
         from infera_b200.ops import kv8
 
@@ -755,6 +763,27 @@ def kv_push_pages(src_k: torch.Tensor, src_v: torch.Tensor, dst_k, dst_v, src_pa
                                             src_k.element_size(), C, _stream())
     _native.check(rc, "ib_kv_push_pages")
     _count()
+
+
+def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, src: torch.Tensor,
+               count: torch.Tensor, start: torch.Tensor | None = None, bt_rows: torch.Tensor | None = None) -> None:
+    """Move rows within sequences' pages, in place: place ``start[s] +
+    src[s, (h,) i]`` to ``start[s] + i``, for i < ``count[s]``. Caches bf16
+    [slots, width] of one layer or [L, slots, width]; a latent (MLA) cache
+    moves its one channel (:func:`kv_channels`). ``src`` int32 [n, hkv, m]:
+    each KV head's columns by a list of their own (the places that
+    :func:`infera_b200.ops.evict.select_keys` keeps); [n, m]: whole rows (the
+    path of :func:`infera_b200.ops.tree.tree_accept`). ``start`` None: 0.
+
+    An entry is at least its index; -1 moves nothing. Rows move as if all were
+    read before the first is written. A sequence's pages have to be its own:
+    what else reads them (a shared prefix) sees the moved rows. To the status
+    word, and not moved: another entry below its index, one beyond the page
+    table's places, a page id outside the cache; a ``bt_rows`` entry that is no
+    row of the table or that an earlier sequence has."""
+    from infera_b200.ops import paged
+
+    paged.kv_compact(k_cache, v_cache, block_table, src, count, start, bt_rows)
 
 
 # ---------------------------------------------------------------- mixture of experts
