@@ -111,15 +111,14 @@ def tree_accept(tokens: torch.Tensor, target: torch.Tensor, parents: torch.Tenso
 
 @lru_cache(maxsize=256)
 def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: int, num_sms: int) -> tuple[int, int]:
-    most = max(q_lens)
-    per = (128 if most * group <= 128 else 256) // group
-    tiles = [-(-c // 128) for c in ctx_lens]
+    per = 128 // group
+    tiles = [-(-c // 64) for c in ctx_lens]
     top = max(1, max(tiles))
     items = [-(-n // per) for n in q_lens]
     best = best_cost = None
-    for tps in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 1 << 30):
+    for tps in (2, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 1 << 30):
         ctas = hkv * sum(i * -(-t // tps) for i, t in zip(items, tiles))
-        cost = -(-ctas // num_sms) * (min(tps, top) + 3) + (2 if tps < top else 0)
+        cost = -(-ctas // (2 * num_sms)) * (min(tps, top) + 3) + (2 if tps < top else 0)
         if best is None or cost < best_cost:
             best, best_cost = min(tps, top), cost
         if tps >= top:
@@ -128,7 +127,7 @@ def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: i
 
 
 def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, int]:
-    """(key shares, 128-key tiles of a share) of :func:`attn_tree`: the share that minimises rounds of CTAs (one to an
+    """(key shares, 64-key tiles of a share) of :func:`attn_tree`: the share that minimises rounds of CTAs (two to an
     SM) x (its tiles + 3 to start and end), and a merge's worth more where a sequence is cut."""
     if not q_lens:
         return 1, 1
