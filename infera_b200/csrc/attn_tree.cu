@@ -22,9 +22,10 @@
 // not cancel them) and written at the end to the rows that see them, and V rows
 // behind the sequence, which a recycled page may have left as NaN, are zeroed.
 //
-// An item's key tiles are cut into shares, the same number of tiles for every
-// sequence, so ragged batches stay balanced; rows with more than one share are
-// merged by a second kernel.
+// The tiles of all items, laid end to end, are cut into equal runs, one for each
+// CTA of a single wave: batches of any raggedness are balanced, and the loads of
+// a run's next item are under way while the one before ends. An item that a cut
+// falls in is merged from its pieces by a second kernel.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -34,7 +35,6 @@ namespace ib200 {
 namespace atree {
 
 using kv8::elect_one;
-using kv8::table_row;
 using kv8::umma_bf16_if;
 using kv8::umma_commit_if;
 using kv8::umma_f16_ts_if;
@@ -54,6 +54,7 @@ constexpr int SMEM_BYTES = 1024 + 2 * QBLK + SLOTS * TILE;  // barriers in the f
 constexpr uint32_t TMEM_COLS = 256;   // S0 [0,64) S1 [64,128), W over them; O [128,256)
 constexpr uint32_t O_COL = 128;
 constexpr float kLagLog2 = 8.0f;      // the running maximum may lag by this much
+constexpr int kStart = 3;             // what an item's start and end cost, in key tiles
 
 struct Params {
   const __nv_bfloat16* q;
@@ -69,46 +70,146 @@ struct Params {
   const int* block_table;
   const int* bt_rows;
   int table_rows, max_pages, ld_table;
+  int n_seqs;
   int hq, hkv, G, nodes;   // nodes: of an item, 128 / G
-  int blocks;              // items of the longest tree
-  int splits, tiles_per_split;
+  int blocks;              // items of the longest tree and KV head
+  int splits;              // pieces of an item at most; 1: no item is cut
   float c;                 // |scale| * log2(e)
   uint32_t q_flip, q_keep;
   float* o_part;           // [T, hq, splits, 128]
   float* lse_part;         // [T, hq, splits]
+  int* pieces;             // [n_seqs, hkv, blocks]
   __nv_bfloat16* out;
   int ldo;
   int* status;
 };
 
-// What both kernels know of a sequence. `tps` tiles are a share's, so that the
-// shares cover it; `shares` of them have keys.
+// A sequence: its rows, its keys and how many of them come before the nodes,
+// and its items (each KV head's `blocks`, of `tiles` tiles; one where there are no keys).
 struct Seq {
-  int start, n, ctx, base, tps, shares;  // base: its keys before the nodes
+  int start, n, ctx, base, blocks, tiles;
   const int* bt;
 };
 __device__ __forceinline__ Seq sequence(const Params& p, int s, int* status) {
   Seq q;
+  const int want = max(p.q_len[s], 0), row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
   q.start = p.q_start[s];
-  const int want = max(p.q_len[s], 0);
-  const int cover = min(p.blocks * p.nodes, 32 * p.words);
-  q.n = min(want, cover);
+  q.ctx = max(p.ctx_len[s], 0);
+  q.n = min(want, min(p.blocks * p.nodes, 32 * p.words));
   if (q.start < 0 || q.start > p.T) q.n = 0;
   q.n = min(q.n, p.T - q.start);
-  q.ctx = max(p.ctx_len[s], 0);
   q.base = q.ctx - want;  // (may be negative: nodes without a key)
-  q.bt = table_row(p.block_table, p.bt_rows != nullptr ? p.bt_rows[s] : s, p.table_rows, p.ld_table, s, status);
-  if (q.bt == nullptr) q.ctx = 0;
-  if (threadIdx.x == 0) {
-    if (q.n < want) record_status_detail(status, kStatusBadIndex, 9, s, want);
-    if (q.ctx > p.max_pages * PAGE) record_status_detail(status, kStatusBadIndex, 1, s, q.ctx);
-  }
+  if (q.n < want) record_status_detail(status, kStatusBadIndex, 9, s, want);
+  if (q.ctx > p.max_pages * PAGE) record_status_detail(status, kStatusBadIndex, 1, s, q.ctx);
   q.ctx = min(q.ctx, p.max_pages * PAGE);
-  const int tiles = (q.ctx + BKV - 1) / BKV;
-  q.tps = max(p.tiles_per_split, (tiles + p.splits - 1) / p.splits);
-  q.shares = (tiles + q.tps - 1) / q.tps;
+  q.bt = p.block_table + static_cast<size_t>(row) * p.ld_table;
+  if (row < 0 || row >= p.table_rows) {
+    record_status_detail(status, kStatusBadIndex, 4, s, row);
+    q.ctx = 0;
+    q.bt = p.block_table;
+  }
+  q.blocks = (q.n + p.nodes - 1) / p.nodes;
+  q.tiles = max(1, (q.ctx + BKV - 1) / BKV);
   return q;
 }
+
+// A CTA's run, segment by segment. All items lie end to end on a line, an item
+// of `tiles` tiles taking kStart + tiles units (its start costs as much as some
+// tiles); first each sequence's first 128 rows, then the second ones of those
+// that have more, and so on, so that with equal trees the runs that read the
+// same keys read them at the same time. Run w of C goes from total * w / C to
+// total * (w + 1) / C. Called by whole warps, which all walk alike.
+struct Walk {
+  long long at, end, first, total;  // this segment's first unit, the run's end, the item's first unit
+  int ctas;
+  int s, kvh, block;
+  Seq sq;
+
+  // units of a sequence's items of one block
+  __device__ __forceinline__ static long long units(const Params& p, const Seq& q, int block) {
+    return q.blocks > block ? static_cast<long long>(p.hkv) * (kStart + q.tiles) : 0;
+  }
+  __device__ __forceinline__ Walk(const Params& p, int* status) {
+    const int lane = threadIdx.x & 31;
+    total = 0;
+    int most = 1;
+    for (int i = lane; i < p.n_seqs; i += 32) {
+      const Seq q = sequence(p, i, status);
+      total += units(p, q, 0) * q.blocks;
+      if (q.n > 0) most = max(most, kStart + q.tiles);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    most = __reduce_max_sync(0xffffffffu, most);
+    // every run has a unit, and is long enough that no item has more than `splits` pieces
+    long long runs = min(static_cast<long long>(gridDim.x), total);
+    if (p.splits > 1) runs = min(runs, total * (p.splits - 1) / most);
+    ctas = static_cast<int>(max(1ll, runs));
+    at = end = 0;
+    if (static_cast<int>(blockIdx.x) >= ctas) return;
+    at = total * blockIdx.x / ctas;
+    end = total * (blockIdx.x + 1) / ctas;
+    if (at >= end) return;
+    long long before = 0;
+    for (block = 0;; ++block) {
+      for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+        const int i = s0 + lane;
+        const long long mine = i < p.n_seqs ? units(p, sequence(p, i, nullptr), block) : 0;
+        long long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        const uint32_t has = __ballot_sync(0xffffffffu, at < before + sum);
+        if (has != 0) {
+          const int l = __ffs(has) - 1;
+          s = s0 + l;
+          first = before + __shfl_sync(0xffffffffu, sum - mine, l);
+          sq = sequence(p, s, nullptr);
+          kvh = static_cast<int>((at - first) / (kStart + sq.tiles));
+          first += static_cast<long long>(kvh) * (kStart + sq.tiles);
+          if (p.splits == 1 && at > first) {  // the item is the run's in which it begins
+            at = first + kStart + sq.tiles;
+            enter(p);
+          }
+          return;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+  }
+  __device__ __forceinline__ bool more() const { return at < end; }
+  __device__ __forceinline__ long long last(const Params& p) const {  // one past the segment
+    const long long stop = first + kStart + sq.tiles;
+    return p.splits == 1 ? stop : min(stop, end);
+  }
+  // the segment's key tiles: first one and count
+  __device__ __forceinline__ int tile() const { return static_cast<int>(max(0ll, at - first - kStart)); }
+  __device__ __forceinline__ int count(const Params& p) const {
+    return sq.ctx > 0 ? max(0, static_cast<int>(last(p) - first) - kStart - tile()) : 0;
+  }
+  // the run that unit u lies in
+  __device__ __forceinline__ int run_of(long long u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
+  __device__ __forceinline__ void advance(const Params& p) {
+    at = last(p);
+    enter(p);
+  }
+  // to the item that begins at `at`, if the one before ended there
+  __device__ __forceinline__ void enter(const Params& p) {
+    if (at < first + kStart + sq.tiles) return;
+    first = at;
+    if (at >= end || ++kvh < p.hkv) return;
+    kvh = 0;
+    do {  // (units are left, so there is such a sequence)
+      if (++s == p.n_seqs) {
+        s = 0;
+        ++block;
+      }
+      sq = sequence(p, s, nullptr);
+    } while (sq.blocks <= block);
+  }
+};
 
 __device__ __forceinline__ uint64_t f2pack(float a, float b) {
   uint64_t d;
@@ -153,35 +254,24 @@ __device__ __forceinline__ uint64_t seen_of(const int* mask, int words, int k, i
   return bits & there;
 }
 
-// Writes what is not finite among the values of a CTA's nodes to the rows that
-// see it, a warp per node. Rare, so nothing here is tuned.
-__device__ __noinline__ void write_not_finite(const Params& p, const Seq& sq, int first, int n, int kvh, int z, int k_lo,
-                                              int k_hi) {
-  const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += NUM_THREADS / 32) {
-    const int row = sq.start + first + i;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of dims 4 lane .. 4 lane + 3: an infinity, a NaN, or 0
-    for (int k = max(k_lo, max(sq.base, 0)); k < min(k_hi, sq.ctx); ++k) {
-      const int j = k - sq.base, page = sq.bt[k / PAGE];
-      if (j >= 32 * p.words || (p.mask[static_cast<size_t>(row) * p.words + (j >> 5)] >> (j & 31) & 1) == 0) continue;
-      if (page < 0 || page >= p.num_pages) continue;
-      const uint2 u = *reinterpret_cast<const uint2*>(
-          p.v + ((static_cast<size_t>(page) * PAGE + k % PAGE) * p.hkv + kvh) * D + 4 * lane);
-      const float x[4] = {bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y)};
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-        if (!(fabsf(x[d]) <= 3.4e38f)) sum[d] += x[d];
+// Writes what is not finite among the values of a segment's nodes to the row's
+// output (dst) where the row sees it. Rare, so nothing here is tuned.
+template <typename T>
+__device__ __noinline__ void write_not_finite(const Params& p, const int* bt, const int* mask, int kvh, int base, int k_lo,
+                                              int k_hi, T* dst) {
+  for (int d = 0; d < D; d += 2) {
+    float lo = 0.f, hi = 0.f;  // an infinity, a NaN, or 0
+    for (int k = max(k_lo, max(base, 0)); k < k_hi; ++k) {
+      const int j = k - base, page = bt[k / PAGE];
+      if (j >= 32 * p.words || (mask[j >> 5] >> (j & 31) & 1) == 0) continue;
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) continue;
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(
+          p.v + ((static_cast<size_t>(page) * PAGE + k % PAGE) * p.hkv + kvh) * D + d);
+      if ((u & 0x7f80u) == 0x7f80u) lo += bf16_lo(u);
+      if ((u & 0x7f800000u) == 0x7f800000u) hi += bf16_hi(u);
     }
-    for (int g = 0; g < p.G; ++g)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        if (sum[d] == 0.f) continue;
-        const int head = kvh * p.G + g;
-        if (sq.shares > 1)
-          p.o_part[((static_cast<size_t>(row) * p.hq + head) * p.splits + z) * D + 4 * lane + d] = sum[d];
-        else
-          p.out[static_cast<size_t>(row) * p.ldo + head * D + 4 * lane + d] = __float2bfloat16(sum[d]);
-      }
+    if (lo != 0.f) dst[d] = static_cast<T>(lo);
+    if (hi != 0.f) dst[d + 1] = static_cast<T>(hi);
   }
 }
 
@@ -191,23 +281,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
                 const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  const int block = blockIdx.x % p.blocks, kvh = blockIdx.x / p.blocks, seq = blockIdx.y, z = blockIdx.z, G = p.G;
-  const Seq sq = sequence(p, seq, p.status);
-  const int first = block * p.nodes;                  // the item's first node
-  const int n_nodes = min(p.nodes, sq.n - first);
-  if (n_nodes <= 0) return;
-  const int n_rows = n_nodes * G;
-  const int j_lo = z * sq.tps;
-  const int nk = min((sq.ctx + BKV - 1) / BKV - j_lo, sq.tps);  // key tiles of this share
-  if (nk <= 0) {
-    if (z == 0)  // no keys at all
-      for (int i = threadIdx.x; i < n_rows * (D / 8); i += NUM_THREADS) {
-        const int row = sq.start + first + i / (D / 8) / G, head = kvh * G + i / (D / 8) % G;
-        reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * p.ldo + head * D)[i % (D / 8)] = make_uint4(0u, 0u, 0u, 0u);
-      }
-    return;
-  }
-  const int n_pages = (sq.ctx + PAGE - 1) / PAGE;
+  Walk walk(p, blockIdx.x == 0 && threadIdx.x < 32 ? p.status : nullptr);
+  if (!walk.more()) return;
 
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // (the 128-byte swizzle counts from multiples of 1024)
@@ -267,6 +342,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       // another item of the sequence reads these keys too, or none
       const uint64_t pol = p.blocks > 1 ? policy_evict_last() : policy_evict_first();
       int issued = 0, st = 0, ph = 1;
+      bool ok = true;
+      for (; walk.more() && ok; walk.advance(p)) {
+      const Seq& sq = walk.sq;
+      const int kvh = walk.kvh, j_lo = walk.tile(), nk = walk.count(p);
+      const int n_pages = (sq.ctx + PAGE - 1) / PAGE;
       int nxt[TILE_PAGES];
       auto load_pages = [&](int j) {
 #pragma unroll
@@ -275,8 +355,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           nxt[i] = __ldg(sq.bt + (lp < n_pages ? lp : 0));
         }
       };
-      load_pages(0);
-      bool ok = true;
+      if (nk > 0) load_pages(0);
       for (int j = 0; j < nk && ok; ++j) {
         int cur[TILE_PAGES];
 #pragma unroll
@@ -315,6 +394,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           }
         }
       }
+      }
       for (int i = max(0, issued - SLOTS); i < issued; ++i)
         mbar_wait(&full[i % SLOTS], static_cast<uint32_t>((i / SLOTS) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
     }
@@ -325,10 +405,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const uint64_t q_desc = make_sw128_desc(smem_u32(sQ), 16, 1024);
     const uint64_t k_desc = make_sw128_desc(smem_u32(sKV), 16, 1024);
     const uint64_t v_desc = make_sw128_desc(smem_u32(sKV), BLK, 1024);
-    bool ok = mbar_wait_warp(q_ready, 0, abort_flag, p.status, kStatusTimeoutFull);
+    bool ok = true;
+    int done = 0;        // tiles of the segments before
+    uint32_t seg = 0;
     // (descriptor addresses are in units of 16 bytes)
-    for (int j = 0; j <= nk && ok; ++j) {
-      if (j < nk) {
+    for (; walk.more() && ok; walk.advance(p)) {
+    const int nk = walk.count(p);
+    if (nk == 0) continue;
+    ok = mbar_wait_warp(q_ready, seg++ & 1, abort_flag, p.status, kStatusTimeoutFull);
+    for (int j = done; j <= done + nk && ok; ++j) {
+      if (j < done + nk) {
         const int i = 2 * j, st = i % SLOTS;
         ok = mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull);
         if (!ok) break;
@@ -340,7 +426,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         umma_commit_if(on, &s_full[j & 1]);
         umma_commit_if(on, &empty[st]);
       }
-      if (j > 0) {
+      if (j > done) {
         const int jj = j - 1, i = 2 * jj + 1, st = i % SLOTS;
         ok = mbar_wait_warp(&p_full[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
                             kStatusTimeoutTmemEmpty) &&
@@ -351,20 +437,52 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         for (int s = 0; s < BKV / 16; ++s)
           // W packs keys 16s .. 16s + 15 of the tile into columns 8s .. 8s + 7 of its S
           umma_f16_ts_if(on, tmem + O_COL, tmem + (jj & 1) * BKV + s * 8, v_desc + (st * TILE + s * 2048) / 16, idesc_o,
-                         (jj > 0 || s > 0) ? 1u : 0u);
+                         (jj > done || s > 0) ? 1u : 0u);
         umma_commit_if(on, &pv_done[jj & 1]);
         umma_commit_if(on, &empty[st]);
       }
+    }
+    done += nk;
     }
     umma_commit_if(on, drain);
     mbar_wait_warp(drain, 0, nullptr, p.status, kStatusTimeoutFull);
   } else {
     const int q4 = warp & 3;
     const int r = q4 * 32 + lane;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    bool ok = true;
+    int done = 0;        // tiles of the segments before
+    // the W V of tile jj has completed: its commit is completion (jj >> 1) + 1
+    // of pv_done[jj & 1], and no later one on that barrier can have been issued
+    auto wait_pv = [&](int jj) {
+      if (ok) ok = mbar_wait_warp(&pv_done[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
+                                  kStatusTimeoutTmemFull);
+      tc_fence_after();
+    };
+    for (; walk.more() && ok; walk.advance(p)) {
+    const Seq& sq = walk.sq;
+    const int G = p.G, kvh = walk.kvh, block = walk.block;
+    const int j_lo = walk.tile(), nk = walk.count(p);
+    const int first = block * p.nodes;                  // the item's first node
+    const int n_rows = min(p.nodes, sq.n - first) * G;
     const bool live = r < n_rows;
     const int node = first + (live ? r / G : 0), head = kvh * G + (live ? r % G : 0);
     const int row = sq.start + node;
-    {  // stage this row (rows that do not exist are zero)
+    // the item's pieces are those of the runs that it lies in
+    const int run = walk.run_of(walk.first), piece = static_cast<int>(blockIdx.x) - run;
+    const int pieces = p.splits == 1 ? 1 : walk.run_of(walk.first + kStart + sq.tiles - 1) - run + 1;
+    if (p.splits > 1 && piece == 0 && threadIdx.x == 64) p.pieces[(walk.s * p.hkv + kvh) * p.blocks + block] = pieces;
+    if (nk == 0) {  // no key tile in this piece, or none at all
+      if (live) {
+        if (pieces > 1)
+          p.lse_part[(static_cast<size_t>(row) * p.hq + head) * p.splits + piece] = -INFINITY;
+        else
+          for (int i = 0; i < D / 8; ++i)
+            reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * p.ldo + head * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      continue;
+    }
+    {  // stage this row (rows that do not exist are zero); the scores of the segment before are made
       const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<size_t>(row) * p.ldq + head * D);
       uint4 v[16];
 #pragma unroll
@@ -376,23 +494,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         *reinterpret_cast<uint4*>(sQ + (i >> 3) * QBLK + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = v[i];
       }
       fence_proxy_async_smem();
+      tc_fence_before();
       mbar_arrive(q_ready);
     }
-    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const int* mask = p.mask + static_cast<size_t>(row) * p.words;
     const bool awake = __any_sync(0xffffffffu, live);    // a warp without rows only keeps step
     float m_run = -INFINITY;
     float l_run = 0.f;
-    bool ok = true;
-    // the W V of tile jj has completed: its commit is completion (jj >> 1) + 1
-    // of pv_done[jj & 1], and no later one on that barrier can have been issued
-    auto wait_pv = [&](int jj) {
-      if (ok) ok = mbar_wait_warp(&pv_done[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
-                                  kStatusTimeoutTmemFull);
-      tc_fence_after();
-    };
-    for (int j = 0; j < nk && ok; ++j) {
-      const int k0 = (j_lo + j) * BKV;
+    for (int j = done; j < done + nk && ok; ++j) {
+      const int k0 = (j_lo + j - done) * BKV;
       const bool edge = k0 + BKV > sq.base;              // the tile has nodes, or ends behind the sequence
       if (!mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
                           kStatusTimeoutTmemFull)) {
@@ -460,7 +570,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           const float m_use = grow ? top : m_run;
           const float alpha = m_run == -INFINITY ? 0.f : exp2f(m_run - m_use);  // nothing before it: zeros
           l_run *= alpha;
-          if (j > 0) {
+          if (j > done) {
             // O *= alpha once the W V of the tile before has landed; none is issued until this tile's W is published
             wait_pv(j - 1);
             if (!ok) break;
@@ -499,11 +609,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       mbar_arrive(&p_full[j & 1]);
     }
     ok = __all_sync(0xffffffffu, ok);
-    wait_pv(nk - 1);
+    done += nk;
+    wait_pv(done - 1);
     if (ok) {
-      const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits + z;
+      const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits + piece;
       const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // a NaN stays one
-      const bool merge = sq.shares > 1;
+      const bool merge = pieces > 1;
       if (merge && live) p.lse_part[part] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
 #pragma unroll 1
       for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -530,6 +641,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           }
         }
       }
+      if (*not_finite != 0 && live) {
+        const int k_lo = j_lo * BKV, k_hi = min(sq.ctx, (j_lo + nk) * BKV);
+        if (merge)
+          write_not_finite(p, sq.bt, mask, kvh, sq.base, k_lo, k_hi, p.o_part + part * D);
+        else
+          write_not_finite(p, sq.bt, mask, kvh, sq.base, k_lo, k_hi, p.out + static_cast<size_t>(row) * p.ldo + head * D);
+      }
+      __syncwarp();
+    }
     }
   }
 
@@ -540,7 +660,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     __syncwarp();
     tmem_dealloc(tmem, TMEM_COLS);
   }
-  if (*not_finite != 0) write_not_finite(p, sq, first, n_nodes, kvh, z, j_lo * BKV, (j_lo + nk) * BKV);
 }
 
 // Merge the key shares of a (node, head) row.
@@ -551,10 +670,12 @@ __global__ void __launch_bounds__(kv8::MERGE_WARPS * 32) tree_merge_kernel(const
   const Seq sq = sequence(p, blockIdx.y, nullptr);
   const int at = blockIdx.x * (kv8::MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
   const int node = at / p.hq, head = at % p.hq;
-  if (sq.shares <= 1 || node >= sq.n) return;  // (W > 1: the same for the whole block)
+  if (node >= sq.n) return;  // (W > 1: the same for the whole block)
+  const int pieces = p.pieces[(blockIdx.y * p.hkv + head / p.G) * p.blocks + node / p.nodes];
+  if (pieces <= 1) return;
   const int row = sq.start + node;
   const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits;
-  kv8::merge_shares<W>(p.o_part + part * D, p.lse_part + part, sq.shares,
+  kv8::merge_shares<W>(p.o_part + part * D, p.lse_part + part, pieces,
                        p.out + static_cast<size_t>(row) * p.ldo + head * D);
 }
 
@@ -565,23 +686,24 @@ using namespace ib200;
 
 // q [T, ldq] bf16 (head h at columns h*128); caches bf16 [num_slots, hkv*128];
 // q_start / q_len / ctx_len [n_seqs], ctx_len with the nodes; mask int32 [T,
-// words]; max_nodes: the most nodes of a sequence. Each sequence's 64-key tiles
-// in shares of tiles_per_split, or of what `splits` shares need. o_part /
-// lse_part: fp32 [T*hq*splits*128] / [T*hq*splits], used where a sequence has
-// more than one share.
+// words]; max_nodes: the most nodes of a sequence. ctas: equal runs that the
+// 64-key tiles of all items are cut into (fewer where an item would have more
+// than `splits` pieces; splits 1: an item goes to the run in which it begins).
+// With splits > 1: o_part / lse_part fp32 [T*hq*splits*128] / [T*hq*splits], pieces
+// [n_seqs * hkv * ceil(max_nodes / (128 / G))].
 extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, const void* v_cache, long long num_slots,
                             const int* q_start, const int* q_len, const int* ctx_len, const int* mask, int words,
                             int n_seqs, int max_nodes, const int* block_table, const int* bt_rows, int table_rows,
-                            int max_pages, int ld_table, int hq, int hkv, float scale, int splits, int tiles_per_split,
-                            float* o_part, float* lse_part, void* out, int ldo, int* status, cudaStream_t stream) {
+                            int max_pages, int ld_table, int hq, int hkv, float scale, int ctas, int splits,
+                            float* o_part, float* lse_part, int* pieces, void* out, int ldo, int* status, cudaStream_t stream) {
   using namespace ib200::atree;
   if (T <= 0 || n_seqs <= 0 || max_nodes <= 0) return 0;
-  if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 16 || splits < 1 || tiles_per_split < 1 || words < 1 || words > 8 ||
+  if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 16 || splits < 1 || ctas < 1 || words < 1 || words > 8 ||
       max_nodes > 32 * words || n_seqs > 65535 || (ldq % 8) != 0 || (ldo % 8) != 0 || num_slots < PAGE ||
       num_slots % PAGE != 0 || max_pages < 0 || max_pages > (1 << 27) - 1 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return -1;
-  if (splits > 1 && (o_part == nullptr || lse_part == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0))
+  if (splits > 1 && (o_part == nullptr || lse_part == nullptr || pieces == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0))
     return -1;
   try {
     const int kvw = hkv * D;
@@ -613,8 +735,9 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     p.G = hq / hkv;
     p.nodes = BQ / p.G;
     p.blocks = (max_nodes + p.nodes - 1) / p.nodes;
+    p.n_seqs = n_seqs;
     p.splits = splits;
-    p.tiles_per_split = tiles_per_split;
+    p.pieces = pieces;
     p.c = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);  // positive: masked scores are -inf times it
     p.q_flip = scale < 0.f ? 0x80008000u : 0u;
     p.q_keep = scale == 0.f ? 0u : ~0u;
@@ -623,7 +746,6 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     p.out = static_cast<__nv_bfloat16*>(out);
     p.ldo = ldo;
     p.status = status;
-    if (splits > 65535) return -1;
     static bool attr_set[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -633,7 +755,7 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
       if (e != cudaSuccess) return static_cast<int>(e);
       if (dev >= 0 && dev < 64) attr_set[dev] = true;
     }
-    e = launch_pdl(tree_kernel, dim3(p.blocks * hkv, n_seqs, splits), NUM_THREADS, SMEM_BYTES, stream, tk, tv, tk4, tv4, p);
+    e = launch_pdl(tree_kernel, dim3(ctas), NUM_THREADS, SMEM_BYTES, stream, tk, tv, tk4, tv4, p);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (splits > 1) {
       const long long rows = static_cast<long long>(max_nodes) * hq;

@@ -111,26 +111,18 @@ def tree_accept(tokens: torch.Tensor, target: torch.Tensor, parents: torch.Tenso
 
 @lru_cache(maxsize=256)
 def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: int, num_sms: int) -> tuple[int, int]:
-    per = 128 // group
-    tiles = [-(-c // 64) for c in ctx_lens]
-    top = max(1, max(tiles))
-    items = [-(-n // per) for n in q_lens]
-    best = best_cost = None
-    for tps in (2, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 1 << 30):
-        ctas = hkv * sum(i * -(-t // tps) for i, t in zip(items, tiles))
-        cost = -(-ctas // (2 * num_sms)) * (min(tps, top) + 3) + (2 if tps < top else 0)
-        if best is None or cost < best_cost:
-            best, best_cost = min(tps, top), cost
-        if tps >= top:
-            break
-    return -(-top // best), best
+    per_item = 128 // group
+    units = [3 + (-(-c // 64) or 1) for c in ctx_lens]  # an item's start and end cost some three tiles
+    items = [-(-n // per_item) for n in q_lens]
+    total = hkv * sum(i * u for i, u in zip(items, units))
+    top, levels = max((u for i, u in zip(items, units) if i), default=4), max(1, max(items))
+    ctas = max(1, min(2 * num_sms // levels * levels or levels, -(-total // 5)))
+    return ctas, 1 if top <= 7 else -(-top * ctas // total) + 1
 
 
 def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, int]:
-    """(key shares, 64-key tiles of a share) of :func:`attn_tree`: the share that minimises rounds of CTAs (two to an
-    SM) x (its tiles + 3 to start and end), and a merge's worth more where a sequence is cut."""
-    if not q_lens:
-        return 1, 1
+    """(CTAs, most pieces of an item) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each 128 rows of
+    the longest tree, at least two tiles of 64 keys each; contexts of up to four tiles are not cut."""
     return _plan(tuple(q_lens), tuple(ctx_lens), hq // hkv, hkv, num_sms)
 
 
@@ -144,7 +136,7 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     [T, words] names (:func:`tree_mask`, or any other mask: its own node need not be among them). Up to 32*words nodes
     (words 1 to 8), up to 16 query heads per KV head. ``out`` may be ``q`` itself.
 
-    ``host_meta`` (q_len, ctx_len on the host; read back from the device without it) sizes the grid and the key shares
+    ``host_meta`` (q_len, ctx_len on the host; read back from the device without it) sizes the grid and the workspace
     (``plan``: :func:`tree_plan`). In a captured graph the lengths on the device may change from replay to replay: up
     to the most nodes of ``host_meta``, and any context that the page table holds.
 
@@ -197,22 +189,24 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         _attn_tree_cpu(q, k_cache, v_cache, block_table, q_start.tolist(), q_lens, ctx_lens, mask, hq, hkv, scale, out,
                        bt_rows)
         return out
-    splits, tps = plan or tree_plan(q_lens, ctx_lens, hq, hkv, K._num_sms())
-    if splits < 1 or tps < 1:
-        raise ValueError(f"plan {splits}, {tps}")
-    part = lse = None
+    ctas, splits = plan or tree_plan(q_lens, ctx_lens, hq, hkv, K._num_sms())
+    if splits < 1 or ctas < 1:
+        raise ValueError(f"plan {ctas}, {splits}")
+    part = lse = pieces = None
     if splits > 1:
         # partials of this call: its own memory, so that calls on several streams and captured graphs share none
         m = T * hq * splits
-        ws = torch.empty(m * (HEAD_DIM + 1), dtype=torch.float32, device=q.device)
+        ws = torch.empty(m * (HEAD_DIM + 1) + n * hkv * -(-most // (128 // (hq // hkv))), dtype=torch.float32,
+                         device=q.device)
         part = ws.data_ptr()
         lse = part + 4 * m * HEAD_DIM
+        pieces = lse + 4 * m
     status, stream = _on(dev)
     rc = _native.kernels().ib_attn_tree(q.data_ptr(), T, ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
                                         q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), mask.data_ptr(),
                                         words, n, most, block_table.data_ptr(), K._ptr(bt_rows), block_table.shape[0],
-                                        places, block_table.stride(0), hq, hkv, scale, splits, tps, part, lse,
-                                        out.data_ptr(), ldo, status, stream)
+                                        places, block_table.stride(0), hq, hkv, scale, ctas, splits, part, lse,
+                                        pieces, out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_tree")
     K._count(2 if splits > 1 else 1)
     return out

@@ -120,7 +120,7 @@ CASES = {
 }
 
 
-@pytest.mark.parametrize("plan", [None, (1, 100), (3, 1), (9, 2)])
+@pytest.mark.parametrize("plan", [None, (300, 1), (1, 3), (2, 9), (31, 5), (300, 40)])
 @pytest.mark.parametrize("name", CASES)
 def test_attention(name, plan):
     n, ctx, hq, hkv, words = CASES[name]
@@ -147,7 +147,7 @@ def test_any_mask_scale_and_stride(runs, scale):
 
 
 @pytest.mark.parametrize("n,hq", [(20, 4), (40, 4)])
-@pytest.mark.parametrize("plan", [(1, 100), (4, 1)])
+@pytest.mark.parametrize("plan", [(7, 1), (3, 9)])
 def test_what_is_masked_may_be_anything(n, hq, plan):
     ctx = 250
     q, k, v, table, mask, masks = batch([n], [ctx], hq, 1, 2, 4)
@@ -179,7 +179,7 @@ def test_scores_of_very_different_size():
     size = torch.linspace(0.1, 40, ctx[0])
     for p in range(ctx[0]):
         k[int(table[0, p // 16]) * 16 + p % 16] *= size[p if p % 2 else ctx[0] - 1 - p]
-    for plan in ((1, 100), (4, 2)):
+    for plan in ((2, 1), (9, 9)):
         out = tree.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32([0]), i32(n), i32(ctx), mask.cuda(), hq, 1,
                              SCALE, plan=plan)
         check(out.cpu(), q, k, v, table, masks, n, ctx, hq, 1)
