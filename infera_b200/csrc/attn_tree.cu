@@ -9,7 +9,7 @@
 // takes 128 rows and walks its keys in tiles of 64 (4 pages), 16 KB of K and 16
 // KB of V in a ring of five slots that both take in turn:
 //   warp 0      TMA producer
-//   warp 1      MMA issuer: S(j), then W V of tile j - 1
+//   warp 1      MMA issuer: W V of tile j, then S(j + 2)
 //   warps 2..5  softmax, a thread per row; they also stage Q
 // S is double-buffered in TMEM, so the scores of a tile are made while the
 // softmax of the one before runs; a tile's weights lie over its scores. Two
@@ -35,6 +35,8 @@ namespace ib200 {
 namespace atree {
 
 using kv8::elect_one;
+using kv8::mbar_expect_tx_if;
+using kv8::tma_load_2d_if;
 using kv8::umma_bf16_if;
 using kv8::umma_commit_if;
 using kv8::umma_f16_ts_if;
@@ -113,6 +115,11 @@ __device__ __forceinline__ Seq sequence(const Params& p, int s, int* status) {
   return q;
 }
 
+__device__ __forceinline__ long long divide(long long a, long long b) {  // a, b >= 0; in 32 bits where that does
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 // A CTA's run, segment by segment. All items lie end to end on a line, an item
 // of `tiles` tiles taking kStart + tiles units (its start costs as much as some
 // tiles); first each sequence's first 128 rows, then the second ones of those
@@ -133,8 +140,10 @@ struct Walk {
     const int lane = threadIdx.x & 31;
     total = 0;
     int most = 1;
+    Seq mine0{};  // the lane's first sequence
     for (int i = lane; i < p.n_seqs; i += 32) {
       const Seq q = sequence(p, i, status);
+      if (i == lane) mine0 = q;
       total += units(p, q, 0) * q.blocks;
       if (q.n > 0) most = max(most, kStart + q.tiles);
     }
@@ -143,18 +152,18 @@ struct Walk {
     most = __reduce_max_sync(0xffffffffu, most);
     // every run has a unit, and is long enough that no item has more than `splits` pieces
     long long runs = min(static_cast<long long>(gridDim.x), total);
-    if (p.splits > 1) runs = min(runs, total * (p.splits - 1) / most);
+    if (p.splits > 1) runs = min(runs, divide(total * (p.splits - 1), most));
     ctas = static_cast<int>(max(1ll, runs));
     at = end = 0;
     if (static_cast<int>(blockIdx.x) >= ctas) return;
-    at = total * blockIdx.x / ctas;
-    end = total * (blockIdx.x + 1) / ctas;
+    at = divide(total * blockIdx.x, ctas);
+    end = divide(total * (blockIdx.x + 1), ctas);
     if (at >= end) return;
     long long before = 0;
     for (block = 0;; ++block) {
       for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int i = s0 + lane;
-        const long long mine = i < p.n_seqs ? units(p, sequence(p, i, nullptr), block) : 0;
+        const long long mine = i < p.n_seqs ? units(p, s0 == 0 ? mine0 : sequence(p, i, nullptr), block) : 0;
         long long sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -167,7 +176,7 @@ struct Walk {
           s = s0 + l;
           first = before + __shfl_sync(0xffffffffu, sum - mine, l);
           sq = sequence(p, s, nullptr);
-          kvh = static_cast<int>((at - first) / (kStart + sq.tiles));
+          kvh = static_cast<int>(divide(at - first, kStart + sq.tiles));
           first += static_cast<long long>(kvh) * (kStart + sq.tiles);
           if (p.splits == 1 && at > first) {  // the item is the run's in which it begins
             at = first + kStart + sq.tiles;
@@ -190,7 +199,7 @@ struct Walk {
     return sq.ctx > 0 ? max(0, static_cast<int>(last(p) - first) - kStart - tile()) : 0;
   }
   // the run that unit u lies in
-  __device__ __forceinline__ int run_of(long long u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
+  __device__ __forceinline__ int run_of(long long u) const { return static_cast<int>(divide((u + 1) * ctas - 1, total)); }
   __device__ __forceinline__ void advance(const Params& p) {
     at = last(p);
     enter(p);
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     return;
   }
   uint8_t* sQ = smem + 1024;             // dims 0..63, dims 64..127
-  uint8_t* sKV = sQ + 2 * QBLK;          // slot i % SLOTS: load i = K (even) or V (odd) of tile i / 2
+  uint8_t* sKV = sQ + 2 * QBLK;          // load i in slot i % SLOTS
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   uint64_t* q_ready = bars;
   uint64_t* full = bars + 1;             // [SLOTS]
@@ -338,66 +347,69 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   const uint32_t tmem = uniform(*tmem_slot);
 
   if (warp == 0) {
-    if (lane == 0) {
-      // another item of the sequence reads these keys too, or none
-      const uint64_t pol = p.blocks > 1 ? policy_evict_last() : policy_evict_first();
-      int issued = 0, st = 0, ph = 1;
-      bool ok = true;
-      for (; walk.more() && ok; walk.advance(p)) {
+    // The whole warp runs along and the elected lane issues, so that the operands stay in uniform registers: a lane
+    // of its own took some 80 cycles a box, 16 of them a tile of scattered pages.
+    const uint32_t on = elect_one();
+    // another item of the sequence reads these keys too, or none
+    const uint64_t pol = p.blocks > 1 ? policy_evict_last() : policy_evict_first();
+    int issued = 0, st = 0, ph = 1;
+    bool ok = true;
+    for (; walk.more() && ok; walk.advance(p)) {
       const Seq& sq = walk.sq;
       const int kvh = walk.kvh, j_lo = walk.tile(), nk = walk.count(p);
+      if (nk == 0) continue;
       const int n_pages = (sq.ctx + PAGE - 1) / PAGE;
-      int nxt[TILE_PAGES];
+      int next[TILE_PAGES], pages[TILE_PAGES], before[TILE_PAGES];  // of K's next tile, K's, V's
       auto load_pages = [&](int j) {
 #pragma unroll
         for (int i = 0; i < TILE_PAGES; ++i) {
           const int lp = (j_lo + j) * TILE_PAGES + i;
-          nxt[i] = __ldg(sq.bt + (lp < n_pages ? lp : 0));
+          next[i] = __ldg(sq.bt + (lp < n_pages ? lp : 0));
         }
       };
-      if (nk > 0) load_pages(0);
-      for (int j = 0; j < nk && ok; ++j) {
-        int cur[TILE_PAGES];
-#pragma unroll
-        for (int i = 0; i < TILE_PAGES; ++i)  // (page ids outside the cache load zeros)
-          cur[i] = static_cast<unsigned>(nxt[i]) < static_cast<unsigned>(p.num_pages) ? nxt[i] : -1;
-        if (j + 1 < nk) load_pages(j + 1);  // in flight while we wait
+      auto load_tile = [&](int j, const int (&at)[TILE_PAGES], const CUtensorMap* tm1, const CUtensorMap* tm4) {
+        ok = mbar_wait_warp(&empty[st], static_cast<uint32_t>(ph), abort_flag, p.status, kStatusTimeoutEmpty);
+        if (!ok) return;
         // consecutive pages are one box per half (the swizzle repeats every 8 rows)
         bool run = true;
 #pragma unroll
-        for (int pg = 1; pg < TILE_PAGES; ++pg) run = run && cur[pg] == cur[0] + pg;
+        for (int pg = 1; pg < TILE_PAGES; ++pg) run = run && at[pg] == at[0] + pg;
         const int n = min(TILE_PAGES, n_pages - (j_lo + j) * TILE_PAGES);  // pages that the sequence has here
+        uint8_t* dst = sKV + st * TILE;
+        mbar_expect_tx_if(on, &full[st], 2 * n * PAGE * 128);
+        if (run && n == TILE_PAGES) {
+          tma_load_2d_if(on, dst, tm4, &full[st], kvh * D, at[0] * PAGE, pol);
+          tma_load_2d_if(on, dst + BLK, tm4, &full[st], kvh * D + 64, at[0] * PAGE, pol);
+        } else {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          if (!ok) break;
-          ok = mbar_wait(&empty[st], static_cast<uint32_t>(ph), abort_flag, p.status, kStatusTimeoutEmpty);
-          if (!ok) break;
-          uint8_t* dst = sKV + st * TILE;
-          mbar_expect_tx(&full[st], 2 * n * PAGE * 128);
-          if (run && n == TILE_PAGES) {
-            const CUtensorMap* tm4 = v ? &tmV4 : &tmK4;
-            tma_load_2d(dst, tm4, &full[st], kvh * D, cur[0] * PAGE, pol);
-            tma_load_2d(dst + BLK, tm4, &full[st], kvh * D + 64, cur[0] * PAGE, pol);
-          } else {
-            const CUtensorMap* tm1 = v ? &tmV : &tmK;
-#pragma unroll
-            for (int pg = 0; pg < TILE_PAGES; ++pg)
-              if (pg < n) {
-                tma_load_2d(dst + pg * PAGE * 128, tm1, &full[st], kvh * D, cur[pg] * PAGE, pol);
-                tma_load_2d(dst + BLK + pg * PAGE * 128, tm1, &full[st], kvh * D + 64, cur[pg] * PAGE, pol);
-              }
-          }
-          ++issued;
-          if (++st == SLOTS) {
-            st = 0;
-            ph ^= 1;
-          }
+          for (int pg = 0; pg < TILE_PAGES; ++pg)
+            if (pg < n) {
+              tma_load_2d_if(on, dst + pg * PAGE * 128, tm1, &full[st], kvh * D, at[pg] * PAGE, pol);
+              tma_load_2d_if(on, dst + BLK + pg * PAGE * 128, tm1, &full[st], kvh * D + 64, at[pg] * PAGE, pol);
+            }
         }
+        ++issued;
+        if (++st == SLOTS) {
+          st = 0;
+          ph ^= 1;
+        }
+      };
+      load_pages(0);
+      // in the order in which the MMA warp takes them: K(j), then V(j - 1)
+      for (int j = 0; j <= nk && ok; ++j) {
+#pragma unroll
+        for (int i = 0; i < TILE_PAGES; ++i) {
+          before[i] = pages[i];
+          const int pg = static_cast<int>(uniform(next[i]));  // (page ids outside the cache load zeros)
+          pages[i] = static_cast<unsigned>(pg) < static_cast<unsigned>(p.num_pages) ? pg : -1;
+        }
+        if (j + 1 < nk) load_pages(j + 1);  // in flight while we wait
+        if (j < nk) load_tile(j, pages, &tmK, &tmK4);
+        if (j > 0 && ok) load_tile(j - 1, before, &tmV, &tmV4);
       }
-      }
-      for (int i = max(0, issued - SLOTS); i < issued; ++i)
-        mbar_wait(&full[i % SLOTS], static_cast<uint32_t>((i / SLOTS) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
     }
+    for (int i = max(0, issued - SLOTS); i < issued; ++i)
+      mbar_wait_warp(&full[i % SLOTS], static_cast<uint32_t>((i / SLOTS) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
   } else if (warp == 1) {
     const uint32_t on = elect_one();
     const uint32_t idesc_s = make_idesc_bf16(128, BKV);
@@ -407,42 +419,53 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const uint64_t v_desc = make_sw128_desc(smem_u32(sKV), BLK, 1024);
     bool ok = true;
     int done = 0;        // tiles of the segments before
+    int load = 0;        // loads taken
     uint32_t seg = 0;
+    // the next load, K0 K1 V0 K2 V1 ..; its slot
+    auto take = [&]() -> int {
+      const int st = load % SLOTS;
+      ok = ok && mbar_wait_warp(&full[st], static_cast<uint32_t>((load / SLOTS) & 1), abort_flag, p.status,
+                                kStatusTimeoutFull);
+      ++load;
+      return st;
+    };
     // (descriptor addresses are in units of 16 bytes)
+    auto scores = [&](int j, int st) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        umma_bf16_if(on, tmem + (j & 1) * BKV, q_desc + ((s >> 2) * QBLK + (s & 3) * 32) / 16,
+                     k_desc + (st * TILE + (s >> 2) * BLK + (s & 3) * 32) / 16, idesc_s, s > 0 ? 1u : 0u);
+      umma_commit_if(on, &s_full[j & 1]);
+      umma_commit_if(on, &empty[st]);
+    };
     for (; walk.more() && ok; walk.advance(p)) {
-    const int nk = walk.count(p);
-    if (nk == 0) continue;
-    ok = mbar_wait_warp(q_ready, seg++ & 1, abort_flag, p.status, kStatusTimeoutFull);
-    for (int j = done; j <= done + nk && ok; ++j) {
-      if (j < done + nk) {
-        const int i = 2 * j, st = i % SLOTS;
-        ok = mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull);
+      const int nk = walk.count(p);
+      if (nk == 0) continue;
+      ok = mbar_wait_warp(q_ready, seg++ & 1, abort_flag, p.status, kStatusTimeoutFull);
+      for (int j = done; j < done + min(nk, 2) && ok; ++j) {
+        const int st = take();
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          umma_bf16_if(on, tmem + (j & 1) * BKV, q_desc + ((s >> 2) * QBLK + (s & 3) * 32) / 16,
-                       k_desc + (st * TILE + (s >> 2) * BLK + (s & 3) * 32) / 16, idesc_s, s > 0 ? 1u : 0u);
-        umma_commit_if(on, &s_full[j & 1]);
-        umma_commit_if(on, &empty[st]);
+        scores(j, st);
       }
-      if (j > done) {
-        const int jj = j - 1, i = 2 * jj + 1, st = i % SLOTS;
-        ok = mbar_wait_warp(&p_full[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
-                            kStatusTimeoutTmemEmpty) &&
-             mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull);
+      for (int j = done; j < done + nk && ok; ++j) {
+        // what the weights do not depend on is waited for before them: W V and the next scores then follow at once
+        const bool more = j + 2 < done + nk;
+        const int sv = take(), sk = more ? take() : 0;
+        ok = ok && mbar_wait_warp(&p_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
+                                  kStatusTimeoutTmemEmpty);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int s = 0; s < BKV / 16; ++s)
           // W packs keys 16s .. 16s + 15 of the tile into columns 8s .. 8s + 7 of its S
-          umma_f16_ts_if(on, tmem + O_COL, tmem + (jj & 1) * BKV + s * 8, v_desc + (st * TILE + s * 2048) / 16, idesc_o,
-                         (jj > done || s > 0) ? 1u : 0u);
-        umma_commit_if(on, &pv_done[jj & 1]);
-        umma_commit_if(on, &empty[st]);
+          umma_f16_ts_if(on, tmem + O_COL, tmem + (j & 1) * BKV + s * 8, v_desc + (sv * TILE + s * 2048) / 16, idesc_o,
+                         (j > done || s > 0) ? 1u : 0u);
+        umma_commit_if(on, &pv_done[j & 1]);
+        umma_commit_if(on, &empty[sv]);
+        if (more) scores(j + 2, sk);
       }
-    }
-    done += nk;
+      done += nk;
     }
     umma_commit_if(on, drain);
     mbar_wait_warp(drain, 0, nullptr, p.status, kStatusTimeoutFull);
@@ -513,7 +536,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       if (edge) {
         // V rows of the tile, half a row a thread: zeroed behind the sequence, and where a node's is not finite. (S of
         // this tile was issued after the product that freed the slot: the barrier is in this load's phase or past it.)
-        const int i = 2 * j + 1, st = i % SLOTS, vr = r & (BKV - 1), key = k0 + vr;
+        const int at = j - done, i = 2 * done + (at + 1 < nk ? 2 * at + 2 : 2 * nk - 1);  // loads: K0, K1, V0, K2, V1, ..
+        const int st = i % SLOTS, vr = r & (BKV - 1), key = k0 + vr;
         if (!mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull)) {
           ok = false;
           break;
@@ -662,21 +686,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// Merge the key shares of a (node, head) row.
-template <int W>
-__global__ void __launch_bounds__(kv8::MERGE_WARPS * 32) tree_merge_kernel(const __grid_constant__ Params p) {
+// Merge the pieces of cut items: a warp a row.
+constexpr int MERGE_ROWS = 8;
+__global__ void __launch_bounds__(MERGE_ROWS * 32) merge_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  const Seq sq = sequence(p, blockIdx.y, nullptr);
-  const int at = blockIdx.x * (kv8::MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
-  const int node = at / p.hq, head = at % p.hq;
-  if (node >= sq.n) return;  // (W > 1: the same for the whole block)
-  const int pieces = p.pieces[(blockIdx.y * p.hkv + head / p.G) * p.blocks + node / p.nodes];
-  if (pieces <= 1) return;
-  const int row = sq.start + node;
+  const int item = blockIdx.x, s = item / (p.hkv * p.blocks), kvh = item / p.blocks % p.hkv, block = item % p.blocks;
+  const int pieces = p.pieces[item];  // (of an item that there is)
+  const int r = blockIdx.y * MERGE_ROWS + (threadIdx.x >> 5), node = block * p.nodes + r / p.G;
+  const Seq sq = sequence(p, s, nullptr);
+  if (r >= p.nodes * p.G || node >= sq.n || pieces <= 1) return;
+  const int row = sq.start + node, head = kvh * p.G + r % p.G;
   const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits;
-  kv8::merge_shares<W>(p.o_part + part * D, p.lse_part + part, pieces,
-                       p.out + static_cast<size_t>(row) * p.ldo + head * D);
+  kv8::merge_shares<1>(p.o_part + part * D, p.lse_part + part, pieces, p.out + static_cast<size_t>(row) * p.ldo + head * D);
 }
 
 }  // namespace atree
@@ -757,17 +779,9 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     }
     e = launch_pdl(tree_kernel, dim3(ctas), NUM_THREADS, SMEM_BYTES, stream, tk, tv, tk4, tv4, p);
     if (e != cudaSuccess) return static_cast<int>(e);
-    if (splits > 1) {
-      const long long rows = static_cast<long long>(max_nodes) * hq;
-      // a block a row where there are many shares: one warp would wait for four of them after another (61 nodes of 32
-      // heads, 17 shares)
-      if (splits >= 8 && rows * n_seqs <= 16384)
-        e = launch_pdl(tree_merge_kernel<kv8::MERGE_WARPS>, dim3(static_cast<unsigned>(rows), n_seqs),
-                       kv8::MERGE_WARPS * 32, 0, stream, p);
-      else
-        e = launch_pdl(tree_merge_kernel<1>, dim3(static_cast<unsigned>((rows + kv8::MERGE_WARPS - 1) / kv8::MERGE_WARPS), n_seqs),
-                       kv8::MERGE_WARPS * 32, 0, stream, p);
-    }
+    if (splits > 1)
+      e = launch_pdl(merge_kernel, dim3(static_cast<unsigned>(n_seqs) * hkv * p.blocks, BQ / MERGE_ROWS),
+                     MERGE_ROWS * 32, 0, stream, p);
     return static_cast<int>(e);
   } catch (...) {  // (no memory for a tensor map's entry)
     return -3;

@@ -103,6 +103,25 @@ __device__ __forceinline__ void umma_commit_if(uint32_t on, uint64_t* bar) {
       "r"(on)
       : "memory");
 }
+// TMA loads by a whole warp in the same way
+__device__ __forceinline__ void mbar_expect_tx_if(uint32_t on, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(bytes), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_if(uint32_t on, void* dst, const CUtensorMap* tm, uint64_t* bar, int c0,
+                                               int c1, uint64_t cache_hint) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;\n\t}\n" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "l"(cache_hint), "r"(on)
+      : "memory");
+}
 // a value that all lanes have, known to be uniform
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
