@@ -9,7 +9,7 @@
 // takes 128 rows and walks its keys in tiles of 64 (4 pages), 16 KB of K and 16
 // KB of V in a ring of five slots that both take in turn:
 //   warp 0      TMA producer
-//   warp 1      MMA issuer: W V of tile j, then S(j + 2)
+//   warp 1      MMA issuer: S(j), then W V of tile j - 1
 //   warps 2..5  softmax, a thread per row; they also stage Q
 // S is double-buffered in TMEM, so the scores of a tile are made while the
 // softmax of the one before runs; a tile's weights lie over its scores. Two
@@ -421,51 +421,41 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     int done = 0;        // tiles of the segments before
     int load = 0;        // loads taken
     uint32_t seg = 0;
-    // the next load, K0 K1 V0 K2 V1 ..; its slot
-    auto take = [&]() -> int {
-      const int st = load % SLOTS;
-      ok = ok && mbar_wait_warp(&full[st], static_cast<uint32_t>((load / SLOTS) & 1), abort_flag, p.status,
-                                kStatusTimeoutFull);
-      ++load;
-      return st;
-    };
     // (descriptor addresses are in units of 16 bytes)
-    auto scores = [&](int j, int st) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-        umma_bf16_if(on, tmem + (j & 1) * BKV, q_desc + ((s >> 2) * QBLK + (s & 3) * 32) / 16,
-                     k_desc + (st * TILE + (s >> 2) * BLK + (s & 3) * 32) / 16, idesc_s, s > 0 ? 1u : 0u);
-      umma_commit_if(on, &s_full[j & 1]);
-      umma_commit_if(on, &empty[st]);
-    };
     for (; walk.more() && ok; walk.advance(p)) {
-      const int nk = walk.count(p);
-      if (nk == 0) continue;
-      ok = mbar_wait_warp(q_ready, seg++ & 1, abort_flag, p.status, kStatusTimeoutFull);
-      for (int j = done; j < done + min(nk, 2) && ok; ++j) {
-        const int st = take();
+    const int nk = walk.count(p);
+    if (nk == 0) continue;
+    ok = mbar_wait_warp(q_ready, seg++ & 1, abort_flag, p.status, kStatusTimeoutFull);
+    for (int j = done; j <= done + nk && ok; ++j) {
+      if (j < done + nk) {
+        const int i = load++, st = i % SLOTS;
+        ok = mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull);
         if (!ok) break;
         tc_fence_after();
-        scores(j, st);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          umma_bf16_if(on, tmem + (j & 1) * BKV, q_desc + ((s >> 2) * QBLK + (s & 3) * 32) / 16,
+                       k_desc + (st * TILE + (s >> 2) * BLK + (s & 3) * 32) / 16, idesc_s, s > 0 ? 1u : 0u);
+        umma_commit_if(on, &s_full[j & 1]);
+        umma_commit_if(on, &empty[st]);
       }
-      for (int j = done; j < done + nk && ok; ++j) {
-        // what the weights do not depend on is waited for before them: W V and the next scores then follow at once
-        const bool more = j + 2 < done + nk;
-        const int sv = take(), sk = more ? take() : 0;
-        ok = ok && mbar_wait_warp(&p_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
-                                  kStatusTimeoutTmemEmpty);
+      if (j > done) {
+        const int jj = j - 1, i = load++, st = i % SLOTS;
+        ok = mbar_wait_warp(&p_full[jj & 1], static_cast<uint32_t>((jj >> 1) & 1), abort_flag, p.status,
+                            kStatusTimeoutTmemEmpty) &&
+             mbar_wait_warp(&full[st], static_cast<uint32_t>((i / SLOTS) & 1), abort_flag, p.status, kStatusTimeoutFull);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int s = 0; s < BKV / 16; ++s)
           // W packs keys 16s .. 16s + 15 of the tile into columns 8s .. 8s + 7 of its S
-          umma_f16_ts_if(on, tmem + O_COL, tmem + (j & 1) * BKV + s * 8, v_desc + (sv * TILE + s * 2048) / 16, idesc_o,
-                         (j > done || s > 0) ? 1u : 0u);
-        umma_commit_if(on, &pv_done[j & 1]);
-        umma_commit_if(on, &empty[sv]);
-        if (more) scores(j + 2, sk);
+          umma_f16_ts_if(on, tmem + O_COL, tmem + (jj & 1) * BKV + s * 8, v_desc + (st * TILE + s * 2048) / 16, idesc_o,
+                         (jj > done || s > 0) ? 1u : 0u);
+        umma_commit_if(on, &pv_done[jj & 1]);
+        umma_commit_if(on, &empty[st]);
       }
-      done += nk;
+    }
+    done += nk;
     }
     umma_commit_if(on, drain);
     mbar_wait_warp(drain, 0, nullptr, p.status, kStatusTimeoutFull);
