@@ -290,9 +290,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
                 const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  Walk walk(p, blockIdx.x == 0 && threadIdx.x < 32 ? p.status : nullptr);
-  if (!walk.more()) return;
-
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // (the 128-byte swizzle counts from multiples of 1024)
     if (threadIdx.x == 0) record_status(p.status, kStatusBadArgs);
@@ -341,6 +338,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
+  Walk walk(p, blockIdx.x == 0 && threadIdx.x < 32 ? p.status : nullptr);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -676,19 +674,71 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// Merge the pieces of cut items: a warp a row.
-constexpr int MERGE_ROWS = 8;
-__global__ void __launch_bounds__(MERGE_ROWS * 32) merge_kernel(const __grid_constant__ Params p) {
+// Merge the pieces of cut items. An item's rows are (node, head) pairs.
+struct Row {
+  int pieces;              // 1: nothing to merge
+  size_t part;             // of its first piece
+  __nv_bfloat16* out;
+};
+__device__ __forceinline__ Row merge_row(const Params& p, const Seq& sq, int item, int r) {
+  const int kvh = item / p.blocks % p.hkv, block = item % p.blocks, node = block * p.nodes + r / p.G;
+  if (r >= p.nodes * p.G || node >= sq.n) return {1, 0, nullptr};
+  const int row = sq.start + node, head = kvh * p.G + r % p.G;
+  return {p.pieces[item], (static_cast<size_t>(row) * p.hq + head) * p.splits, p.out + static_cast<size_t>(row) * p.ldo + head * D};
+}
+// W warps a row.
+constexpr int MERGE_WARPS = kv8::MERGE_WARPS;
+template <int W>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  const int item = blockIdx.x, s = item / (p.hkv * p.blocks), kvh = item / p.blocks % p.hkv, block = item % p.blocks;
-  const int pieces = p.pieces[item];  // (of an item that there is)
-  const int r = blockIdx.y * MERGE_ROWS + (threadIdx.x >> 5), node = block * p.nodes + r / p.G;
-  const Seq sq = sequence(p, s, nullptr);
-  if (r >= p.nodes * p.G || node >= sq.n || pieces <= 1) return;
-  const int row = sq.start + node, head = kvh * p.G + r % p.G;
-  const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits;
-  kv8::merge_shares<1>(p.o_part + part * D, p.lse_part + part, pieces, p.out + static_cast<size_t>(row) * p.ldo + head * D);
+  const int item = blockIdx.x, r = blockIdx.y * (MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
+  const Row row = merge_row(p, sequence(p, item / (p.hkv * p.blocks), nullptr), item, r);
+  if (row.pieces <= 1) return;  // (W > 1: the same for the whole block)
+  kv8::merge_shares<W>(p.o_part + row.part * D, p.lse_part + row.part, row.pieces, row.out);
+}
+// Up to MERGE_FEW pieces: MERGE_ROWS rows a warp, all of whose loads are under way at once.
+constexpr int MERGE_FEW = 4, MERGE_ROWS = 4;
+__global__ void __launch_bounds__(128) merge_few_kernel(const __grid_constant__ Params p) {
+  pdl_trigger();
+  pdl_wait();
+  const int item = blockIdx.x, lane = threadIdx.x & 31, r0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * MERGE_ROWS;
+  const Seq sq = sequence(p, item / (p.hkv * p.blocks), nullptr);
+  Row row[MERGE_ROWS];
+  float lse[MERGE_ROWS][MERGE_FEW];
+  float4 o[MERGE_ROWS][MERGE_FEW];
+#pragma unroll
+  for (int i = 0; i < MERGE_ROWS; ++i) {
+    row[i] = merge_row(p, sq, item, r0 + i);
+#pragma unroll
+    for (int k = 0; k < MERGE_FEW; ++k) {
+      const bool in = row[i].pieces > 1 && k < row[i].pieces;
+      lse[i][k] = in ? p.lse_part[row[i].part + k] : -INFINITY;
+      o[i][k] = in ? reinterpret_cast<const float4*>(p.o_part + (row[i].part + k) * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MERGE_ROWS; ++i) {
+    if (row[i].pieces <= 1) continue;
+    float mx = fmaxf(fmaxf(lse[i][0], lse[i][1]), fmaxf(lse[i][2], lse[i][3]));
+    if (mx == -INFINITY) mx = 0.f;
+    float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+    for (int k = 0; k < MERGE_FEW; ++k) {
+      if (lse[i][k] == -INFINITY) continue;  // (a piece without keys wrote no more)
+      const float w = fmaxf(exp2f(lse[i][k] - mx), FLT_MIN);  // (a NaN in a piece stays one)
+      den += w;
+      num[0] += o[i][k].x * w;
+      num[1] += o[i][k].y * w;
+      num[2] += o[i][k].z * w;
+      num[3] += o[i][k].w * w;
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    uint2 w;
+    w.x = pack_bf16(num[0] * inv, num[1] * inv);
+    w.y = pack_bf16(num[2] * inv, num[3] * inv);
+    reinterpret_cast<uint2*>(row[i].out)[lane] = w;
+  }
 }
 
 }  // namespace atree
@@ -769,9 +819,14 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     }
     e = launch_pdl(tree_kernel, dim3(ctas), NUM_THREADS, SMEM_BYTES, stream, tk, tv, tk4, tv4, p);
     if (e != cudaSuccess) return static_cast<int>(e);
-    if (splits > 1)
-      e = launch_pdl(merge_kernel, dim3(static_cast<unsigned>(n_seqs) * hkv * p.blocks, BQ / MERGE_ROWS),
-                     MERGE_ROWS * 32, 0, stream, p);
+    const unsigned items = static_cast<unsigned>(n_seqs) * hkv * p.blocks;
+    // many pieces of few rows: a block a row (61 nodes of 32 heads in 20 pieces: 12 us with a warp each)
+    if (splits > MERGE_FEW && static_cast<long long>(T) * hq <= 16384)
+      e = launch_pdl(merge_kernel<MERGE_WARPS>, dim3(items, BQ), MERGE_WARPS * 32, 0, stream, p);
+    else if (splits > MERGE_FEW)
+      e = launch_pdl(merge_kernel<1>, dim3(items, BQ / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, p);
+    else if (splits > 1)
+      e = launch_pdl(merge_few_kernel, dim3(items, BQ / (4 * MERGE_ROWS)), 128, 0, stream, p);
     return static_cast<int>(e);
   } catch (...) {  // (no memory for a tensor map's entry)
     return -3;
