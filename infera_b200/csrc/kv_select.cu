@@ -3,17 +3,24 @@
 // select_kernel: for each (sequence, KV head), of L keys with accumulated
 // weights x: the first `sink`, the last `recent`, and of the others those with
 // the largest x (equal ones: the lowest place first), `keep` in all, as places
-// in ascending order. The threshold is found digit by digit (11, 11 and 10 bits
-// of the weight as an unsigned number of the same order) in histograms; a last
-// pass counts and one writes the places, each behind what lies before it. A
-// cluster of CTAs shares a list: each takes a run of places and adds up the
-// others' histograms through distributed shared memory.
+// in ascending order. The weights are read once, into shared memory; the
+// threshold is found digit by digit (11, 11 and 10 bits of the weight as an
+// unsigned number of the same order) in histograms; a last pass counts and one
+// writes the places, each behind what lies before it. A cluster of CTAs shares a
+// list: each takes a run of places and adds up the others' histograms through
+// distributed shared memory.
 //
-// compact_kernel: rows src[i] -> i of a sequence's places, in place. src[i] >=
-// i, so a row is never written before a row that is read later lies there:
-// places are taken in ascending order, and a group's rows are all read (into
-// registers) before the first of them is written. A CTA owns its columns, so
-// no other one touches them.
+// The moves: rows src[i] -> i of a sequence's places, in place. src[i] >= i, so
+// a row is never written before a row that is read later lies there: places are
+// taken in ascending order, and a group's rows are all read before the first of
+// them is written. A CTA owns its columns, so no other one touches them.
+//   stream_kernel  long lists: groups of rows pass through a ring in shared
+//                  memory (asynchronous loads run groups ahead of the stores,
+//                  which is no harm: what is written lies before all that is
+//                  read later), the places' slots looked up one group further
+//   batch_kernel   short lists over many layers (the accepted path of a tree):
+//                  the moves are listed once, and rows of several layers are
+//                  held in registers at a time
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -29,6 +36,7 @@ using kv8::table_row;
 constexpr int THREADS = 1024;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
+constexpr int MAX_CACHED = 48 * 1024;  // places that a CTA holds in shared memory, 192 KB
 
 struct SelectParams {
   float* mass;            // [mass_rows, hkv, cap]
@@ -52,6 +60,9 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// CACHED: a CTA's run of places fits into its shared memory; else they are read
+// in each pass.
+template <bool CACHED>
 __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   pdl_trigger();
   pdl_wait();
@@ -59,12 +70,20 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int list = blockIdx.x / C, s = list / p.hkv, h = list % p.hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  __shared__ uint32_t hist[BINS];
+  extern __shared__ float cached[];
+  __shared__ uint32_t hist[3][BINS];  // a digit's each, so that one is not cleared while another CTA reads it
   __shared__ uint32_t wsum[WARPS], wgt[WARPS], weq[WARPS];
   __shared__ uint32_t s_bin, s_want, totals[2];
+  auto sync_all = [&]() {  // of the CTAs that share the list
+    if (C > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
 
   const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
   long long n_keys = max(p.seq_lens[s], 0);
+  for (int i = tid; i < 3 * BINS / 4; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
   bool bad = row < 0 || row >= p.mass_rows;
   if (bad && tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, row);
   if (!bad && n_keys > p.cap) {
@@ -93,69 +112,86 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     return;
   }
   const int lo = p.sink, hi = L - p.recent;
-  for (int i = at; i < p.sink; i += all) {
-    kept[i] = i;
-    kept_mass[i] = x[i];
-  }
-  for (int i = at; i < p.recent; i += all) {
-    kept[p.keep - p.recent + i] = hi + i;
-    kept_mass[p.keep - p.recent + i] = x[hi + i];
-  }
   // this CTA's run of places, and within it one for each warp
   const int run = (((hi - lo + C - 1) / C + THREADS - 1) / THREADS) * THREADS;
   const int first = min(hi, lo + min(rank, (hi - lo) / run + 1) * run), last = min(hi, first + run);
+  const float* mine = CACHED ? cached - first : x;
   uint32_t want = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // of those that match the digits so far
   uint32_t prefix = 0, known = 0;
-  if (want > 0) {
+  __syncthreads();  // (the histograms are clear)
 #pragma unroll 1
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bits = digit == 2 ? 10 : 11;
-      for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
-      __syncthreads();
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bits = digit == 2 ? 10 : 11;
+    if (digit == 0) {
+      // groups of loads, then what they are for
+      constexpr int AHEAD = 8;
+      for (int i0 = first + tid; i0 < last; i0 += AHEAD * THREADS) {
+        float v[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) v[a] = i0 + a * THREADS < last ? x[i0 + a * THREADS] : 0.f;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          const int i = i0 + a * THREADS;
+          if (i >= last) break;
+          if (CACHED) cached[i - first] = v[a];
+          atomicAdd(&hist[0][order_of(v[a]) >> 21], 1u);
+        }
+      }
+      if (rank == 0) {
+        for (int i = tid; i < p.sink; i += THREADS) {
+          kept[i] = i;
+          kept_mass[i] = x[i];
+        }
+        for (int i = tid; i < p.recent; i += THREADS) {
+          kept[p.keep - p.recent + i] = hi + i;
+          kept_mass[p.keep - p.recent + i] = x[hi + i];
+        }
+      }
+    } else {
 #pragma unroll 4
       for (int i = first + tid; i < last; i += THREADS) {
-        const uint32_t k = order_of(x[i]);
-        if (((k ^ prefix) & known) == 0) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        const uint32_t k = order_of(mine[i]);
+        if (((k ^ prefix) & known) == 0) atomicAdd(&hist[digit][(k >> shift) & ((1u << bits) - 1)], 1u);
       }
-      cluster.sync();
-      // the bin in which the want-th largest lies: thread t has the bins 2 t and 2 t + 1 from the top
-      uint32_t c[2] = {0u, 0u};
-      const int top = BINS - 1 - 2 * tid;
-      for (int r = 0; r < C; ++r) {
-        const uint32_t* other = cluster.map_shared_rank(hist, r);
-        c[0] += other[top];
-        c[1] += other[top - 1];
-      }
-      uint32_t sum = c[0] + c[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      if (lane == 31) wsum[warp] = sum;
-      __syncthreads();
-      uint32_t before = sum - c[0] - c[1];
-      for (int w = 0; w < warp; ++w) before += wsum[w];
-      if (before < want && before + c[0] + c[1] >= want) {
-        const bool second = before + c[0] < want;
-        s_bin = static_cast<uint32_t>(second ? top - 1 : top);
-        s_want = want - before - (second ? c[0] : 0u);
-      }
-      cluster.sync();  // s_bin; and the histograms are read
-      want = s_want;
-      prefix |= s_bin << shift;
-      known |= ((1u << bits) - 1) << shift;
     }
-  } else {
-    prefix = 0xffffffffu;  // above every weight's number but that of a NaN that none has
+    sync_all();
+    // the bin in which the want-th largest lies: thread t has the bins 2 t and 2 t + 1 from the top
+    uint32_t c[2] = {0u, 0u};
+    const int top = BINS - 2 - 2 * tid;
+    for (int r = 0; r < C; ++r) {
+      const uint32_t* other = C > 1 ? cluster.map_shared_rank(hist[digit], r) : hist[digit];
+      const uint2 two = *reinterpret_cast<const uint2*>(other + top);
+      c[0] += two.y;
+      c[1] += two.x;
+    }
+    uint32_t sum = c[0] + c[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) wsum[warp] = sum;
+    __syncthreads();
+    uint32_t before = sum - c[0] - c[1] + __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
+    if (before < want && before + c[0] + c[1] >= want) {
+      const bool second = before + c[0] < want;
+      s_bin = static_cast<uint32_t>(second ? top : top + 1);
+      s_want = want - before - (second ? c[0] : 0u);
+    }
+    __syncthreads();  // s_bin
+    if (want == 0) break;  // (of the middle nothing stays)
+    want = s_want;
+    prefix |= s_bin << shift;
+    known |= ((1u << bits) - 1) << shift;
   }
+  if (known == 0) prefix = 0xffffffffu;  // above the number of every weight
   // places above the threshold and at it, of which the first `want` stay
   const int seg = run / WARPS;
   const int w0 = min(last, first + warp * seg), w1 = min(last, w0 + seg);
   uint32_t gt = 0, eq = 0;
 #pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t k = order_of(x[i]);
+    const uint32_t k = order_of(mine[i]);
     gt += k > prefix;
     eq += k == prefix;
   }
@@ -166,27 +202,26 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     weq[warp] = eq;
   }
   __syncthreads();
-  if (warp == 0) {
-    const uint32_t a = __reduce_add_sync(0xffffffffu, wgt[lane]), b = __reduce_add_sync(0xffffffffu, weq[lane]);
-    if (lane == 0) {
-      totals[0] = a;
-      totals[1] = b;
+  gt = __reduce_add_sync(0xffffffffu, lane < warp ? wgt[lane] : 0u);
+  eq = __reduce_add_sync(0xffffffffu, lane < warp ? weq[lane] : 0u);
+  if (C > 1) {
+    if (warp == WARPS - 1 && lane == 0) {
+      totals[0] = gt + wgt[WARPS - 1];
+      totals[1] = eq + weq[WARPS - 1];
     }
-  }
-  cluster.sync();
-  gt = eq = 0;
-  for (int r = 0; r < rank; ++r) {
-    const uint32_t* other = cluster.map_shared_rank(totals, r);
-    gt += other[0];
-    eq += other[1];
-  }
-  for (int w = 0; w < warp; ++w) {
-    gt += wgt[w];
-    eq += weq[w];
+    cluster.sync();
+    uint32_t a = 0, b = 0;
+    if (lane < rank) {
+      const uint32_t* other = cluster.map_shared_rank(totals, lane);
+      a = other[0];
+      b = other[1];
+    }
+    gt += __reduce_add_sync(0xffffffffu, a);
+    eq += __reduce_add_sync(0xffffffffu, b);
   }
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int i = i0 + lane;
-    const float v = i < w1 ? x[i] : 0.f;
+    const float v = i < w1 ? mine[i] : 0.f;
     const uint32_t k = order_of(v);
     const uint32_t above = __ballot_sync(0xffffffffu, i < w1 && k > prefix);
     const uint32_t same = __ballot_sync(0xffffffffu, i < w1 && k == prefix);
@@ -200,15 +235,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     gt += __popc(above);
     eq += __popc(same);
   }
-  cluster.sync();  // (no CTA leaves while another reads its totals)
+  if (C > 1 || p.update) sync_all();  // (no CTA leaves while another reads its totals)
   if (p.update) {
     for (int i = at; i < L; i += all) x[i] = i < p.keep ? __ldcg(kept_mass + i) : 0.f;
   }
 }
-
-constexpr int MOVE_THREADS = 512;
-constexpr int ENTRIES = 2 * MOVE_THREADS;  // places resolved at a time
-constexpr int UNITS = 8;                   // 16-byte pieces that a thread holds
 
 struct MoveParams {
   uint8_t* k;
@@ -222,42 +253,167 @@ struct MoveParams {
   const int* block_table;
   const int* bt_rows;
   int table_rows, max_pages, ld_table;
-  const int* src;            // [n, heads, m]
+  const int* src;            // [n, heads, m], or [n, m] where `shared`
   int heads, m;
+  bool shared;               // all heads' columns move by the sequence's list
   const int* count;          // [n]
   const int* start;          // [n] or null
   int* status;
 };
 
-__global__ void __launch_bounds__(MOVE_THREADS) compact_kernel(const MoveParams p) {
+// What the CTAs of a sequence know; count 0: nothing moves.
+struct MoveSeq {
+  const int* bt;
+  int count;
+  long long start;
+};
+__device__ __forceinline__ MoveSeq move_seq(const MoveParams& p, int s) {
+  const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
+  MoveSeq q{table_row(p.block_table, row, p.table_rows, p.ld_table, s, p.status), min(max(p.count[s], 0), p.m),
+            p.start != nullptr ? p.start[s] : 0};
+  if (q.bt == nullptr) q.count = 0;
+  if (q.start < 0) {
+    if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, s, static_cast<int>(q.start));
+    q.count = 0;
+  }
+  if (p.bt_rows != nullptr) {  // a sequence whose places an earlier one has too stays as that one leaves it
+    bool twice = false;
+    for (int i = threadIdx.x; i < s; i += blockDim.x) twice = twice || p.bt_rows[i] == row;
+    if (__syncthreads_or(twice)) {
+      if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 7, s, row);
+      q.count = 0;
+    }
+  }
+  return q;
+}
+// Whether entry e of value v moves: what does not and should goes to the status word.
+__device__ __forceinline__ bool moves_at(const MoveParams& p, const MoveSeq& q, int s, int e, int v) {
+  if (v == e || v == -1) return false;
+  if (v > e && q.start + v < static_cast<long long>(p.max_pages) * kv8::PAGE) return true;
+  record_status_detail(p.status, kStatusBadIndex, 8, s, v);
+  return false;
+}
+// The slots of a move between pages ga and gb; false (and a status) where there is no such page.
+__device__ __forceinline__ bool known(const MoveParams& p, int s, int ga, int gb) {
+  const bool a = static_cast<unsigned>(ga) < static_cast<unsigned>(p.num_pages);
+  const bool b = static_cast<unsigned>(gb) < static_cast<unsigned>(p.num_pages);
+  if (!a || !b) record_status_detail(p.status, kStatusBadIndex, 2, s, a ? gb : ga);
+  return a && b;
+}
+
+constexpr int STREAM_WARPS = 8;
+constexpr int STAGE = 4096;  // bytes of a warp and stage
+constexpr int STAGES = 3;
+
+template <int RB>  // bytes of a row that a CTA moves
+__global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const MoveParams p) {
+  constexpr int RW = STAGE / RB;                  // rows of a warp and stage
+  constexpr int RL = (RW + 31) / 32;              // rows that a lane looks up
+  constexpr int LANES = RB / 16;                  // lanes of a row
+  constexpr int PIECES = STAGE / 16 / 32;
+  extern __shared__ __align__(16) uint8_t ring[];  // [STAGES][STREAM_WARPS][STAGE]
+  __shared__ int2 slots[STAGES][STREAM_WARPS][RW];
+  pdl_trigger();
+  pdl_wait();
+  const int s = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const MoveSeq q = move_seq(p, s);
+  if (q.count == 0) return;
+  const int* src = p.src + static_cast<size_t>(p.shared ? s : blockIdx.x) * p.m;
+  uint8_t* cache = (static_cast<int>(blockIdx.y) < p.parts ? p.k : p.v) + blockIdx.z * p.layer_bytes +
+                   static_cast<size_t>(h) * p.width + static_cast<size_t>(blockIdx.y % p.parts) * RB;
+  const int n = (q.count + STREAM_WARPS * RW - 1) / (STREAM_WARPS * RW);
+  auto entry = [&](int k, int i) { return (k * STREAM_WARPS + warp) * RW + lane + 32 * i; };
+  int v[RL], at[RL], ga[RL], gb[RL];  // entries of the stage after next to load; of the next one: entries (or -1), pages
+  auto load_src = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+      const int e = entry(k, i);
+      v[i] = e < q.count && lane + 32 * i < RW ? __ldg(src + e) : -1;
+    }
+  };
+  auto load_pages = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+      const int e = entry(k, i);
+      at[i] = moves_at(p, q, s, e, v[i]) ? v[i] : -1;
+      ga[i] = gb[i] = 0;
+      if (at[i] >= 0) {
+        ga[i] = __ldg(q.bt + (q.start + at[i]) / kv8::PAGE);
+        gb[i] = __ldg(q.bt + (q.start + e) / kv8::PAGE);
+      }
+    }
+  };
+  auto load_rows = [&](int k) {
+    if (k < n) {
+      int2* list = slots[k % STAGES][warp];
+#pragma unroll
+      for (int i = 0; i < RL; ++i) {
+        if (lane + 32 * i >= RW) break;
+        const bool on = at[i] >= 0 && known(p, s, ga[i], gb[i]);
+        list[lane + 32 * i] = on ? make_int2(ga[i] * kv8::PAGE + static_cast<int>((q.start + at[i]) % kv8::PAGE),
+                                             gb[i] * kv8::PAGE + static_cast<int>((q.start + entry(k, i)) % kv8::PAGE))
+                                 : make_int2(-1, -1);
+      }
+      __syncwarp();
+      const uint32_t dst = smem_u32(ring) + ((k % STAGES) * STREAM_WARPS + warp) * STAGE + lane * 16;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int from = list[i * (32 / LANES) + lane / LANES].x;
+        if (from >= 0)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * 512),
+                       "l"(cache + static_cast<size_t>(from) * p.pitch + (lane % LANES) * 16)
+                       : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  load_src(0);
+  load_pages(0);
+  load_src(1);
+  for (int k = 0; k < STAGES - 1; ++k) {
+    load_rows(k);
+    load_pages(k + 1);
+    load_src(k + 2);
+  }
+  for (int k = 0; k < n; ++k) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();  // the stage's rows are read, of all warps
+    const int2* list = slots[k % STAGES][warp];
+    const uint8_t* from = ring + ((k % STAGES) * STREAM_WARPS + warp) * STAGE + lane * 16;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int to = list[i * (32 / LANES) + lane / LANES].y;
+      if (to >= 0)
+        *reinterpret_cast<uint4*>(cache + static_cast<size_t>(to) * p.pitch + (lane % LANES) * 16) =
+            *reinterpret_cast<const uint4*>(from + i * 512);
+    }
+    __syncwarp();  // the list of stage k + STAGES - 1 is not that of stage k, but k + STAGES' is
+    load_rows(k + STAGES - 1);
+    load_pages(k + STAGES);
+    load_src(k + STAGES + 1);
+  }
+}
+
+constexpr int MOVE_THREADS = 512;
+constexpr int ENTRIES = 2 * MOVE_THREADS;  // places resolved at a time
+constexpr int UNITS = 8;                   // 16-byte pieces that a thread holds
+
+__global__ void __launch_bounds__(MOVE_THREADS) batch_kernel(const MoveParams p) {
   pdl_trigger();
   pdl_wait();
   const int s = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int from[ENTRIES], to[ENTRIES];
   __shared__ int wsum[MOVE_THREADS / 32];
-  const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
-  const int* bt = table_row(p.block_table, row, p.table_rows, p.ld_table, s, p.status);
-  if (p.bt_rows != nullptr) {  // a sequence whose places an earlier one has too stays as that one leaves it
-    bool twice = false;
-    for (int i = tid; i < s; i += MOVE_THREADS) twice = twice || p.bt_rows[i] == row;
-    if (__syncthreads_or(twice)) {
-      if (tid == 0) record_status_detail(p.status, kStatusBadIndex, 7, s, row);
-      return;
-    }
-  }
-  const int count = min(max(p.count[s], 0), p.m);
-  const long long start = p.start != nullptr ? p.start[s] : 0;
-  if (bt == nullptr || count == 0) return;
-  if (start < 0) {
-    if (tid == 0) record_status_detail(p.status, kStatusBadIndex, 1, s, static_cast<int>(start));
-    return;
-  }
+  const MoveSeq q = move_seq(p, s);
+  const int count = q.count;
+  const long long start = q.start;
+  if (count == 0) return;
   const int* src = p.src + (static_cast<size_t>(s) * p.heads + h) * p.m;
   const int l0 = blockIdx.z * p.group, layers = min(p.group, p.layers - l0);
   uint8_t* cache = (static_cast<int>(blockIdx.y) < p.parts ? p.k : p.v) + l0 * p.layer_bytes + static_cast<size_t>(h) * p.width +
                    static_cast<size_t>(blockIdx.y % p.parts) * p.lanes * 16;
-  const long long places = static_cast<long long>(p.max_pages) * kv8::PAGE;
   for (int e0 = 0; e0 < count; e0 += ENTRIES) {
     // slots of the next places that move, in order
     int a[2], b[2];
@@ -266,22 +422,13 @@ __global__ void __launch_bounds__(MOVE_THREADS) compact_kernel(const MoveParams 
     for (int i = 0; i < 2; ++i) {
       const int e = e0 + 2 * tid + i;
       const int v = e < count ? src[e] : -1;
-      const long long pa = start + v, pb = start + e;
-      moves[i] = v > e;
-      if ((v < e && v != -1 && e < count) || (moves[i] && pa >= places)) {
-        record_status_detail(p.status, kStatusBadIndex, 8, s, v);
-        moves[i] = false;
-      }
+      moves[i] = moves_at(p, q, s, e, v);
       a[i] = b[i] = 0;
       if (moves[i]) {
-        const int ga = bt[pa / kv8::PAGE], gb = bt[pb / kv8::PAGE];
-        if (static_cast<unsigned>(ga) >= static_cast<unsigned>(p.num_pages) ||
-            static_cast<unsigned>(gb) >= static_cast<unsigned>(p.num_pages)) {
-          record_status_detail(p.status, kStatusBadIndex, 2, s, static_cast<unsigned>(ga) >= static_cast<unsigned>(p.num_pages) ? ga : gb);
-          moves[i] = false;
-        }
-        a[i] = ga * kv8::PAGE + static_cast<int>(pa % kv8::PAGE);
-        b[i] = gb * kv8::PAGE + static_cast<int>(pb % kv8::PAGE);
+        const int ga = q.bt[(start + v) / kv8::PAGE], gb = q.bt[(start + e) / kv8::PAGE];
+        moves[i] = known(p, s, ga, gb);
+        a[i] = ga * kv8::PAGE + static_cast<int>((start + v) % kv8::PAGE);
+        b[i] = gb * kv8::PAGE + static_cast<int>((start + e) % kv8::PAGE);
       }
     }
     const int mine = moves[0] + moves[1];
@@ -341,14 +488,26 @@ extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, 
                             int* kept, float* kept_mass, int* count, int* status, cudaStream_t stream) {
   using namespace ib200::sel;
   if (n <= 0) return 0;
-  if (hkv <= 0 || keep < 1 || sink < 0 || recent < 0 || sink > keep - recent || cap < 0 ||
+  if (hkv <= 0 || keep < 1 || sink < 0 || recent < 0 || sink > keep - recent || cap < 0 || cap > INT32_MAX / 2 ||
       (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) ||
       static_cast<long long>(n) * hkv * cluster > INT32_MAX)
     return -1;
   SelectParams p{mass, mass_rows, hkv, cap, seq_lens, bt_rows, keep, sink, recent, update, kept, kept_mass, count, status};
+  // the longest run of places of a CTA
+  const long long run = ((cap + cluster - 1) / cluster + THREADS - 1) / THREADS * THREADS;
+  const bool cached = run <= MAX_CACHED;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CACHED * 4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(n) * hkv * cluster);
   cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = cached ? static_cast<size_t>(run) * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -357,7 +516,7 @@ extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, select_kernel, p));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, cached ? select_kernel<true> : select_kernel<false>, p));
 }
 
 // Caches [layers, num_slots, row_bytes] (v null: one channel). src [n, heads, m]:
@@ -377,7 +536,6 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
   MoveParams p;
   p.k = static_cast<uint8_t*>(k);
   p.v = static_cast<uint8_t*>(v);
-  const int channels = v != nullptr ? 2 : 1;
   p.layers = layers;
   p.layer_bytes = num_slots * row_bytes;
   p.pitch = row_bytes;
@@ -389,14 +547,38 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
   p.max_pages = max_pages;
   p.ld_table = ld_table;
   p.src = src;
-  p.heads = heads;
   p.m = m;
   p.count = count;
   p.start = start;
   p.status = status;
+  const int channels = v != nullptr ? 2 : 1;
+  // long lists, and those of single heads, in columns of up to 256 bytes; whole rows of other widths in batches
+  if (layers <= 65535 && (heads > 1 ? p.width == 256 : m > 64 && row_bytes % 256 == 0)) {
+    p.shared = heads == 1;
+    p.width = 256;
+    p.heads = row_bytes / 256;
+    const long long lists = static_cast<long long>(n) * p.heads * channels * layers;
+    // a CTA moves some 50 GB/s: where the lists are few, two or four share their columns
+    p.parts = lists >= 2 * num_sms ? 1 : (2 * lists >= 2 * num_sms ? 2 : 4);
+    const auto kernel = p.parts == 1 ? stream_kernel<256> : (p.parts == 2 ? stream_kernel<128> : stream_kernel<64>);
+    constexpr int smem = STAGES * STREAM_WARPS * STAGE;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+      for (auto k : {stream_kernel<256>, stream_kernel<128>, stream_kernel<64>}) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return static_cast<int>(e);
+      }
+      if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+    return static_cast<int>(launch_pdl(kernel, dim3(static_cast<unsigned>(n) * p.heads, channels * p.parts, layers),
+                                       STREAM_WARPS * 32, smem, stream, p));
+  }
+  p.shared = false;
+  p.heads = heads;
   const long long lists = static_cast<long long>(n) * heads * channels;
-  // one CTA moves about 20 GB/s a row group at a time, so few lists are cut
-  // into columns of 64 bytes or more, and few sequences into groups of layers
+  // few lists are cut into columns of 64 bytes or more, and few sequences into groups of layers
   p.parts = 1;
   while (p.parts < 4 && lists * p.parts < 2 * num_sms && p.width % (2 * p.parts * 64) == 0) p.parts *= 2;
   p.lanes = p.width / 16 / p.parts;
@@ -405,5 +587,5 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
   if (static_cast<long long>(p.group) * ENTRIES * p.lanes > INT32_MAX) return -1;
   const dim3 grid(static_cast<unsigned>(n) * heads, channels * p.parts, (layers + p.group - 1) / p.group);
   if (grid.z > 65535) return -1;
-  return static_cast<int>(launch_pdl(compact_kernel, grid, MOVE_THREADS, 0, stream, p));
+  return static_cast<int>(launch_pdl(batch_kernel, grid, MOVE_THREADS, 0, stream, p));
 }
