@@ -36,7 +36,13 @@ using kv8::table_row;
 constexpr int THREADS = 1024;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int MAX_CACHED = 48 * 1024;  // places that a CTA holds in shared memory, 192 KB
+constexpr int CANDIDATES = 2048;
+constexpr int MAX_CACHED = 44 * 1024;  // places that a CTA holds in shared memory, 176 KB
+
+// places of a run when `of` ones are shared by `among`, in whole groups of a warp
+__host__ __device__ constexpr int run_of(long long of, int among) {
+  return static_cast<int>(((of + among - 1) / among + 127) / 128 * 128);
+}
 
 struct SelectParams {
   float* mass;            // [mass_rows, hkv, cap]
@@ -52,12 +58,15 @@ struct SelectParams {
   int* status;
 };
 
-// An unsigned number in the order of the weights: a NaN below all, -0 as 0.
+// An unsigned number in the order of the weights: a NaN below all, -0 as 0; and back.
 __device__ __forceinline__ uint32_t order_of(float x) {
   uint32_t u = __float_as_uint(x);
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
   if ((u << 1) == 0u) u = 0u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float weight_of(uint32_t k) {
+  return k == 0u ? NAN : __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
 // CACHED: a CTA's run of places fits into its shared memory; else they are read
@@ -70,10 +79,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int list = blockIdx.x / C, s = list / p.hkv, h = list % p.hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  extern __shared__ float cached[];
-  __shared__ uint32_t hist[3][BINS];  // a digit's each, so that one is not cleared while another CTA reads it
-  __shared__ uint32_t wsum[WARPS], wgt[WARPS], weq[WARPS];
-  __shared__ uint32_t s_bin, s_want, totals[2];
+  extern __shared__ __align__(16) uint32_t cached[];  // the run's weights as order_of gives them
+  // a histogram a digit, so that none is cleared while another CTA reads it
+  __shared__ __align__(16) uint32_t hist0[BINS], hist1[BINS], hist2[BINS / 2];
+  __shared__ uint32_t candidates[CANDIDATES];  // those whose first digit is the threshold's
+  __shared__ uint32_t n_candidates, wsum[WARPS], wgt[WARPS], weq[WARPS], s_bin, s_want, totals[2];
   auto sync_all = [&]() {  // of the CTAs that share the list
     if (C > 1)
       cluster.sync();
@@ -83,7 +93,12 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
 
   const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
   long long n_keys = max(p.seq_lens[s], 0);
-  for (int i = tid; i < 3 * BINS / 4; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid < BINS / 4) {
+    reinterpret_cast<uint4*>(hist0)[tid] = make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(hist1)[tid] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (tid < BINS / 8) reinterpret_cast<uint4*>(hist2)[tid] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid == 0) n_candidates = 0;
   bool bad = row < 0 || row >= p.mass_rows;
   if (bad && tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, row);
   if (!bad && n_keys > p.cap) {
@@ -111,11 +126,33 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     }
     return;
   }
-  const int lo = p.sink, hi = L - p.recent;
-  // this CTA's run of places, and within it one for each warp
-  const int run = (((hi - lo + C - 1) / C + THREADS - 1) / THREADS) * THREADS;
-  const int first = min(hi, lo + min(rank, (hi - lo) / run + 1) * run), last = min(hi, first + run);
-  const float* mine = CACHED ? cached - first : x;
+  const int lo = p.sink, hi = L - p.recent;  // what lies before and behind stays
+  // this CTA's run of places, in groups of four; and within it one for each warp
+  const int run = run_of(L, C), first = min(L, rank * run), last = min(L, first + run);
+  const int seg = run_of(run, WARPS), w0 = min(last, first + warp * seg), w1 = min(last, w0 + seg);
+  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  auto read4 = [&](int i) -> float4 {  // weights i .. i + 3, those behind the run as 0
+    if (wide && i + 4 <= last) return *reinterpret_cast<const float4*>(x + i);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < last) v.x = x[i];
+    if (i + 1 < last) v.y = x[i + 1];
+    if (i + 2 < last) v.z = x[i + 2];
+    if (i + 3 < last) v.w = x[i + 3];
+    return v;
+  };
+  struct Keys {
+    uint32_t k[4];
+  };
+  auto keys_of = [&](const float4& v) -> Keys { return {{order_of(v.x), order_of(v.y), order_of(v.z), order_of(v.w)}}; };
+  auto keys = [&](int i) -> Keys {
+    if constexpr (CACHED) {
+      const uint4 k = *reinterpret_cast<const uint4*>(cached + (i - first));
+      return {{k.x, k.y, k.z, k.w}};
+    } else {
+      return keys_of(read4(i));
+    }
+  };
+  const int mid0 = max(first, lo), mid1 = min(last, hi);  // the run's places that compete
   uint32_t want = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // of those that match the digits so far
   uint32_t prefix = 0, known = 0;
   __syncthreads();  // (the histograms are clear)
@@ -123,43 +160,51 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bits = digit == 2 ? 10 : 11;
     if (digit == 0) {
-      // groups of loads, then what they are for
-      constexpr int AHEAD = 8;
-      for (int i0 = first + tid; i0 < last; i0 += AHEAD * THREADS) {
-        float v[AHEAD];
+      constexpr int AHEAD = 4;  // loads, then what they are for
+      for (int i0 = first + 4 * tid; i0 < last; i0 += AHEAD * 4 * THREADS) {
+        float4 v[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) v[a] = i0 + a * THREADS < last ? x[i0 + a * THREADS] : 0.f;
+        for (int a = 0; a < AHEAD; ++a) v[a] = read4(i0 + a * 4 * THREADS);
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-          const int i = i0 + a * THREADS;
+          const int i = i0 + a * 4 * THREADS;
           if (i >= last) break;
-          if (CACHED) cached[i - first] = v[a];
-          atomicAdd(&hist[0][order_of(v[a]) >> 21], 1u);
+          const Keys k = keys_of(v[a]);
+          if constexpr (CACHED) *reinterpret_cast<uint4*>(cached + (i - first)) = make_uint4(k.k[0], k.k[1], k.k[2], k.k[3]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (i + c >= mid0 && i + c < mid1) atomicAdd(&hist0[k.k[c] >> 21], 1u);
         }
       }
-      if (rank == 0) {
-        for (int i = tid; i < p.sink; i += THREADS) {
-          kept[i] = i;
-          kept_mass[i] = x[i];
-        }
-        for (int i = tid; i < p.recent; i += THREADS) {
-          kept[p.keep - p.recent + i] = hi + i;
-          kept_mass[p.keep - p.recent + i] = x[hi + i];
-        }
+    } else if (digit == 1) {
+      for (int i = first + 4 * tid; i < last; i += 4 * THREADS) {
+        const Keys k = keys(i);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if ((k.k[c] ^ prefix) >> 21 == 0 && i + c >= mid0 && i + c < mid1) {
+            atomicAdd(&hist1[k.k[c] >> 10 & (BINS - 1)], 1u);
+            const uint32_t n = atomicAdd(&n_candidates, 1u);
+            if (n < CANDIDATES) candidates[n] = k.k[c];
+          }
       }
+    } else if (n_candidates <= CANDIDATES) {
+      for (int i = tid; i < static_cast<int>(n_candidates); i += THREADS)
+        if ((candidates[i] ^ prefix) >> 10 == 0) atomicAdd(&hist2[candidates[i] & (BINS / 2 - 1)], 1u);
     } else {
-#pragma unroll 4
-      for (int i = first + tid; i < last; i += THREADS) {
-        const uint32_t k = order_of(mine[i]);
-        if (((k ^ prefix) & known) == 0) atomicAdd(&hist[digit][(k >> shift) & ((1u << bits) - 1)], 1u);
+      for (int i = first + 4 * tid; i < last; i += 4 * THREADS) {
+        const Keys k = keys(i);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if ((k.k[c] ^ prefix) >> 10 == 0 && i + c >= mid0 && i + c < mid1) atomicAdd(&hist2[k.k[c] & (BINS / 2 - 1)], 1u);
       }
     }
     sync_all();
     // the bin in which the want-th largest lies: thread t has the bins 2 t and 2 t + 1 from the top
     uint32_t c[2] = {0u, 0u};
-    const int top = BINS - 2 - 2 * tid;
-    for (int r = 0; r < C; ++r) {
-      const uint32_t* other = C > 1 ? cluster.map_shared_rank(hist[digit], r) : hist[digit];
+    const int top = (1 << bits) - 2 - 2 * tid;
+    uint32_t* hist = digit == 0 ? hist0 : (digit == 1 ? hist1 : hist2);
+    for (int r = 0; r < C && top >= 0; ++r) {
+      const uint32_t* other = C > 1 ? cluster.map_shared_rank(hist, r) : hist;
       const uint2 two = *reinterpret_cast<const uint2*>(other + top);
       c[0] += two.y;
       c[1] += two.x;
@@ -172,7 +217,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     }
     if (lane == 31) wsum[warp] = sum;
     __syncthreads();
-    uint32_t before = sum - c[0] - c[1] + __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
+    const uint32_t before = sum - c[0] - c[1] + __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
     if (before < want && before + c[0] + c[1] >= want) {
       const bool second = before + c[0] < want;
       s_bin = static_cast<uint32_t>(second ? top : top + 1);
@@ -185,15 +230,17 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     known |= ((1u << bits) - 1) << shift;
   }
   if (known == 0) prefix = 0xffffffffu;  // above the number of every weight
-  // places above the threshold and at it, of which the first `want` stay
-  const int seg = run / WARPS;
-  const int w0 = min(last, first + warp * seg), w1 = min(last, w0 + seg);
+  // places above the threshold and at it, of which the first `want` stay: a count of each in 16 bits of a word would not
+  // do for long runs, so the warp's run is counted in two words
   uint32_t gt = 0, eq = 0;
-#pragma unroll 4
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t k = order_of(mine[i]);
-    gt += k > prefix;
-    eq += k == prefix;
+  for (int i = w0 + 4 * lane; i < w1; i += 128) {
+    const Keys k = keys(i);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool in = i + c >= lo && i + c < min(w1, hi);
+      gt += in && k.k[c] > prefix;
+      eq += in && k.k[c] == prefix;
+    }
   }
   gt = __reduce_add_sync(0xffffffffu, gt);
   eq = __reduce_add_sync(0xffffffffu, eq);
@@ -219,21 +266,39 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     gt += __reduce_add_sync(0xffffffffu, a);
     eq += __reduce_add_sync(0xffffffffu, b);
   }
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const float v = i < w1 ? mine[i] : 0.f;
-    const uint32_t k = order_of(v);
-    const uint32_t above = __ballot_sync(0xffffffffu, i < w1 && k > prefix);
-    const uint32_t same = __ballot_sync(0xffffffffu, i < w1 && k == prefix);
-    const uint32_t lower = (1u << lane) - 1;
-    const uint32_t g = gt + __popc(above & lower), e = eq + __popc(same & lower);
-    if ((above >> lane & 1) || ((same >> lane & 1) && e < want)) {
-      const int to = p.sink + static_cast<int>(g + min(e, want));
-      kept[to] = i;
-      kept_mass[to] = v;
+  // a place goes behind all that stay before it
+  for (int i0 = w0; i0 < w1; i0 += 128) {
+    const int i = i0 + 4 * lane;
+    const Keys k = i < w1 ? keys(i) : Keys{};
+    uint32_t mine = 0;  // above the threshold in the low half, at it in the high one
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool in = i + c >= lo && i + c < min(w1, hi);
+      mine += (in && k.k[c] > prefix ? 1u : 0u) + (in && k.k[c] == prefix ? 0x10000u : 0u);
     }
-    gt += __popc(above);
-    eq += __popc(same);
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    uint32_t g = gt + ((sum - mine) & 0xffffu), e = eq + ((sum - mine) >> 16);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int place = i + c;
+      if (place >= w1) break;
+      const bool in = place >= lo && place < hi, above = in && k.k[c] > prefix, same = in && k.k[c] == prefix;
+      if (!in || above || (same && e < want)) {
+        const int to = min(place, lo) + max(0, place - hi) + static_cast<int>(g + min(e, want));
+        kept[to] = place;
+        kept_mass[to] = weight_of(k.k[c]);
+      }
+      g += above;
+      e += same;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31);
+    gt += total & 0xffffu;
+    eq += total >> 16;
   }
   if (C > 1 || p.update) sync_all();  // (no CTA leaves while another reads its totals)
   if (p.update) {
@@ -395,7 +460,7 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Move
   }
 }
 
-constexpr int MOVE_THREADS = 512;
+constexpr int MOVE_THREADS = 256;
 constexpr int ENTRIES = 2 * MOVE_THREADS;  // places resolved at a time
 constexpr int UNITS = 8;                   // 16-byte pieces that a thread holds
 
@@ -407,28 +472,29 @@ __global__ void __launch_bounds__(MOVE_THREADS) batch_kernel(const MoveParams p)
   __shared__ int from[ENTRIES], to[ENTRIES];
   __shared__ int wsum[MOVE_THREADS / 32];
   const MoveSeq q = move_seq(p, s);
-  const int count = q.count;
-  const long long start = q.start;
-  if (count == 0) return;
+  if (q.count == 0) return;
   const int* src = p.src + (static_cast<size_t>(s) * p.heads + h) * p.m;
   const int l0 = blockIdx.z * p.group, layers = min(p.group, p.layers - l0);
+  // this thread's 16 bytes of a row, and its first row in a round of `rows`
+  const int part = blockIdx.y % p.parts, lanes = min(p.lanes, p.width / 16 - part * p.lanes);
+  const int rows = MOVE_THREADS / lanes, mine_row = tid / lanes;
   uint8_t* cache = (static_cast<int>(blockIdx.y) < p.parts ? p.k : p.v) + l0 * p.layer_bytes + static_cast<size_t>(h) * p.width +
-                   static_cast<size_t>(blockIdx.y % p.parts) * p.lanes * 16;
-  for (int e0 = 0; e0 < count; e0 += ENTRIES) {
+                   static_cast<size_t>(part * p.lanes + tid % lanes) * 16;
+  for (int e0 = 0; e0 < q.count; e0 += ENTRIES) {
     // slots of the next places that move, in order
     int a[2], b[2];
     bool moves[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int e = e0 + 2 * tid + i;
-      const int v = e < count ? src[e] : -1;
+      const int v = e < q.count ? src[e] : -1;
       moves[i] = moves_at(p, q, s, e, v);
       a[i] = b[i] = 0;
       if (moves[i]) {
-        const int ga = q.bt[(start + v) / kv8::PAGE], gb = q.bt[(start + e) / kv8::PAGE];
+        const int ga = q.bt[(q.start + v) / kv8::PAGE], gb = q.bt[(q.start + e) / kv8::PAGE];
         moves[i] = known(p, s, ga, gb);
-        a[i] = ga * kv8::PAGE + static_cast<int>((start + v) % kv8::PAGE);
-        b[i] = gb * kv8::PAGE + static_cast<int>((start + e) % kv8::PAGE);
+        a[i] = ga * kv8::PAGE + static_cast<int>((q.start + v) % kv8::PAGE);
+        b[i] = gb * kv8::PAGE + static_cast<int>((q.start + e) % kv8::PAGE);
       }
     }
     const int mine = moves[0] + moves[1];
@@ -453,23 +519,24 @@ __global__ void __launch_bounds__(MOVE_THREADS) batch_kernel(const MoveParams p)
         to[at++] = b[i];
       }
     __syncthreads();
-    const unsigned per_layer = static_cast<unsigned>(total) * p.lanes, units = per_layer * layers;
-    for (unsigned u0 = 0; u0 < units; u0 += MOVE_THREADS * UNITS) {
+    // rounds of rows, layer by layer: UNITS rounds are read before the first is written
+    int l = 0, e = mine_row;  // this thread's row of the next round: its layer and move
+    const int more = total > 0 && mine_row < rows ? layers : 0;
+    for (int done = 0; done < layers * total; done += rows * UNITS) {
       uint4 v[UNITS];
-      auto place = [&](unsigned u, const int* slot) {
-        const unsigned l = u / per_layer, w = u - l * per_layer, e = w / p.lanes, c = w - e * p.lanes;
-        return reinterpret_cast<uint4*>(cache + l * p.layer_bytes + static_cast<size_t>(slot[e]) * p.pitch + c * 16);
-      };
+      int ll = l, ee = e;
 #pragma unroll
       for (int i = 0; i < UNITS; ++i) {
-        const unsigned u = u0 + i * MOVE_THREADS + tid;
-        if (u < units) v[i] = __ldcg(place(u, from));
+        while (ee >= total && ll < more) ee -= total, ++ll;
+        if (ll < more) v[i] = __ldcg(reinterpret_cast<const uint4*>(cache + ll * p.layer_bytes + static_cast<size_t>(from[ee]) * p.pitch));
+        ee += rows;
       }
       __syncthreads();  // all are read
 #pragma unroll
       for (int i = 0; i < UNITS; ++i) {
-        const unsigned u = u0 + i * MOVE_THREADS + tid;
-        if (u < units) *place(u, to) = v[i];
+        while (e >= total && l < more) e -= total, ++l;
+        if (l < more) *reinterpret_cast<uint4*>(cache + l * p.layer_bytes + static_cast<size_t>(to[e]) * p.pitch) = v[i];
+        e += rows;
       }
     }
     __syncthreads();  // the list is used
@@ -493,8 +560,7 @@ extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, 
       static_cast<long long>(n) * hkv * cluster > INT32_MAX)
     return -1;
   SelectParams p{mass, mass_rows, hkv, cap, seq_lens, bt_rows, keep, sink, recent, update, kept, kept_mass, count, status};
-  // the longest run of places of a CTA
-  const long long run = ((cap + cluster - 1) / cluster + THREADS - 1) / THREADS * THREADS;
+  const int run = run_of(cap, cluster);  // the longest of a CTA
   const bool cached = run <= MAX_CACHED;
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -578,13 +644,13 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
   p.shared = false;
   p.heads = heads;
   const long long lists = static_cast<long long>(n) * heads * channels;
-  // few lists are cut into columns of 64 bytes or more, and few sequences into groups of layers
-  p.parts = 1;
-  while (p.parts < 4 && lists * p.parts < 2 * num_sms && p.width % (2 * p.parts * 64) == 0) p.parts *= 2;
-  p.lanes = p.width / 16 / p.parts;
-  const long long groups = std::min<long long>(layers, std::max<long long>(1, 4LL * num_sms / (lists * p.parts)));
+  // rows of more than 4 KB in parts; layers in as many groups as give the SMs eight CTAs each
+  const int pieces = p.width / 16;
+  p.parts = (pieces + MOVE_THREADS - 1) / MOVE_THREADS;
+  p.lanes = (pieces + p.parts - 1) / p.parts;
+  const long long groups = std::min<long long>(layers, std::max<long long>(1, 8LL * num_sms / (lists * p.parts)));
   p.group = static_cast<int>((layers + groups - 1) / groups);
-  if (static_cast<long long>(p.group) * ENTRIES * p.lanes > INT32_MAX) return -1;
+  if (static_cast<long long>(p.group) * ENTRIES > INT32_MAX) return -1;
   const dim3 grid(static_cast<unsigned>(n) * heads, channels * p.parts, (layers + p.group - 1) / p.group);
   if (grid.z > 65535) return -1;
   return static_cast<int>(launch_pdl(batch_kernel, grid, MOVE_THREADS, 0, stream, p));
