@@ -37,6 +37,7 @@ constexpr int THREADS = 1024;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
 constexpr int CANDIDATES = 2048;
+constexpr uint32_t STAYS = 0xffffffffu;  // (the largest weight, infinity, has 0xff800000)
 constexpr int MAX_CACHED = 44 * 1024;  // places that a CTA holds in shared memory, 176 KB
 
 // places of a run when `of` ones are shared by `among`, in whole groups of a warp
@@ -143,16 +144,23 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
   struct Keys {
     uint32_t k[4];
   };
-  auto keys_of = [&](const float4& v) -> Keys { return {{order_of(v.x), order_of(v.y), order_of(v.z), order_of(v.w)}}; };
+  // What lies before and behind the middle stays: above every weight's number.
+  auto keys_of = [&](int i, const float4& v) -> Keys {
+    Keys q{{order_of(v.x), order_of(v.y), order_of(v.z), order_of(v.w)}};
+    if (i < lo || i + 4 > hi)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (i + c < lo || i + c >= hi) q.k[c] = STAYS;
+    return q;
+  };
   auto keys = [&](int i) -> Keys {
     if constexpr (CACHED) {
       const uint4 k = *reinterpret_cast<const uint4*>(cached + (i - first));
       return {{k.x, k.y, k.z, k.w}};
     } else {
-      return keys_of(read4(i));
+      return keys_of(i, read4(i));
     }
   };
-  const int mid0 = max(first, lo), mid1 = min(last, hi);  // the run's places that compete
   uint32_t want = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // of those that match the digits so far
   uint32_t prefix = 0, known = 0;
   __syncthreads();  // (the histograms are clear)
@@ -169,11 +177,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
         for (int a = 0; a < AHEAD; ++a) {
           const int i = i0 + a * 4 * THREADS;
           if (i >= last) break;
-          const Keys k = keys_of(v[a]);
+          const Keys k = keys_of(i, v[a]);
           if constexpr (CACHED) *reinterpret_cast<uint4*>(cached + (i - first)) = make_uint4(k.k[0], k.k[1], k.k[2], k.k[3]);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            if (i + c >= mid0 && i + c < mid1) atomicAdd(&hist0[k.k[c] >> 21], 1u);
+            if (k.k[c] != STAYS) atomicAdd(&hist0[k.k[c] >> 21], 1u);
         }
       }
     } else if (digit == 1) {
@@ -181,7 +189,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
         const Keys k = keys(i);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if ((k.k[c] ^ prefix) >> 21 == 0 && i + c >= mid0 && i + c < mid1) {
+          if ((k.k[c] ^ prefix) >> 21 == 0 && k.k[c] != STAYS) {
             atomicAdd(&hist1[k.k[c] >> 10 & (BINS - 1)], 1u);
             const uint32_t n = atomicAdd(&n_candidates, 1u);
             if (n < CANDIDATES) candidates[n] = k.k[c];
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
         const Keys k = keys(i);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if ((k.k[c] ^ prefix) >> 10 == 0 && i + c >= mid0 && i + c < mid1) atomicAdd(&hist2[k.k[c] & (BINS / 2 - 1)], 1u);
+          if ((k.k[c] ^ prefix) >> 10 == 0 && k.k[c] != STAYS) atomicAdd(&hist2[k.k[c] & (BINS / 2 - 1)], 1u);
       }
     }
     sync_all();
@@ -229,17 +237,15 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     prefix |= s_bin << shift;
     known |= ((1u << bits) - 1) << shift;
   }
-  if (known == 0) prefix = 0xffffffffu;  // above the number of every weight
-  // places above the threshold and at it, of which the first `want` stay: a count of each in 16 bits of a word would not
-  // do for long runs, so the warp's run is counted in two words
+  if (known == 0) prefix = STAYS - 1;  // above the number of every weight
+  // places above the threshold, and at it, of which the first `want` stay
   uint32_t gt = 0, eq = 0;
   for (int i = w0 + 4 * lane; i < w1; i += 128) {
     const Keys k = keys(i);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const bool in = i + c >= lo && i + c < min(w1, hi);
-      gt += in && k.k[c] > prefix;
-      eq += in && k.k[c] == prefix;
+      gt += k.k[c] > prefix && i + c < w1;
+      eq += k.k[c] == prefix && i + c < w1;
     }
   }
   gt = __reduce_add_sync(0xffffffffu, gt);
@@ -272,29 +278,28 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     const Keys k = i < w1 ? keys(i) : Keys{};
     uint32_t mine = 0;  // above the threshold in the low half, at it in the high one
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool in = i + c >= lo && i + c < min(w1, hi);
-      mine += (in && k.k[c] > prefix ? 1u : 0u) + (in && k.k[c] == prefix ? 0x10000u : 0u);
-    }
+    for (int c = 0; c < 4; ++c)
+      if (i + c < w1) mine += (k.k[c] > prefix ? 1u : 0u) + (k.k[c] == prefix ? 0x10000u : 0u);
     uint32_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += v;
     }
-    uint32_t g = gt + ((sum - mine) & 0xffffu), e = eq + ((sum - mine) >> 16);
+    if (mine != 0) {
+      uint32_t g = gt + ((sum - mine) & 0xffffu), e = eq + ((sum - mine) >> 16);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int place = i + c;
-      if (place >= w1) break;
-      const bool in = place >= lo && place < hi, above = in && k.k[c] > prefix, same = in && k.k[c] == prefix;
-      if (!in || above || (same && e < want)) {
-        const int to = min(place, lo) + max(0, place - hi) + static_cast<int>(g + min(e, want));
-        kept[to] = place;
-        kept_mass[to] = weight_of(k.k[c]);
+      for (int c = 0; c < 4; ++c) {
+        if (i + c >= w1) break;
+        const bool above = k.k[c] > prefix, same = k.k[c] == prefix;
+        if (above || (same && e < want)) {
+          const uint32_t to = g + min(e, want);
+          kept[to] = i + c;
+          kept_mass[to] = k.k[c] == STAYS ? x[i + c] : weight_of(k.k[c]);
+        }
+        g += above;
+        e += same;
       }
-      g += above;
-      e += same;
     }
     const uint32_t total = __shfl_sync(0xffffffffu, sum, 31);
     gt += total & 0xffffu;
