@@ -129,6 +129,23 @@ __device__ __forceinline__ uint64_t make_mn_desc(uint32_t smem_addr, uint32_t mn
   return d;
 }
 
+// The scores stay in L2 for the second kernel (67 MB for 32 sequences of 8192 keys and 64 heads).
+template <int N>
+__device__ __forceinline__ void store_scores(float* dst, const float (&x)[N], uint64_t policy) {
+  if constexpr (N == 1) {
+    asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(dst), "f"(x[0]), "l"(policy) : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(dst), "f"(x[0]), "f"(x[1]), "l"(policy)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int h = 0; h < N; h += 4)
+      asm volatile("st.global.L2::cache_hint.v4.f32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(dst + h), "f"(x[h]), "f"(x[h + 1]),
+                   "f"(x[h + 2]), "f"(x[h + 3]), "l"(policy)
+                   : "memory");
+  }
+}
+
 template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
 __global__ void __launch_bounds__(NUM_THREADS, 2)
     decode_mass_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -208,55 +225,55 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   const uint32_t tmem = kv8::uniform(*tmem_slot);
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol = policy_evict_first();
-      int issued = 0, st = 0, ph = 1;
-      int nxt[8];
-      load_tile_pages(sq.bt, t0, n_pages, nxt);
-      for (int j = 0; j < nt; ++j) {
-        int cur[8];
+    // The whole warp runs along and the elected lane issues, so that the operands stay in uniform registers: a lane of
+    // its own issued the 32 boxes of a tile of scattered pages too slowly (61 ragged sequences 268 us against 260).
+    const uint32_t on = elect_one();
+    const uint64_t pol = policy_evict_first();
+    int issued = 0, st = 0, ph = 1;
+    bool ok = true;
+    int nxt[8];
+    load_tile_pages(sq.bt, t0, n_pages, nxt);
+    for (int j = 0; j < nt && ok; ++j) {
+      int cur[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cur[i] = nxt[i];
-        known_pages(cur, p.num_pages);
-        if (j + 1 < nt) load_tile_pages(sq.bt, t0 + j + 1, n_pages, nxt);  // in flight while we wait
-        // eight consecutive pages are one 128-row box per half (the swizzle
-        // repeats every 8 rows: the same image as eight page boxes)
-        bool run = true;
+      for (int i = 0; i < 8; ++i) cur[i] = static_cast<int>(kv8::uniform(nxt[i]));
+      known_pages(cur, p.num_pages);
+      if (j + 1 < nt) load_tile_pages(sq.bt, t0 + j + 1, n_pages, nxt);  // in flight while we wait
+      // eight consecutive pages are one 128-row box per half (the swizzle
+      // repeats every 8 rows: the same image as eight page boxes)
+      bool run = true;
 #pragma unroll
-        for (int pg = 1; pg < BKV / PAGE; ++pg) run = run && cur[pg] == cur[0] + pg;
-        const int n = min(BKV / PAGE, n_pages - (t0 + j) * (BKV / PAGE));  // pages that the sequence has here
-        bool ok = true;
+      for (int pg = 1; pg < BKV / PAGE; ++pg) run = run && cur[pg] == cur[0] + pg;
+      const int n = min(BKV / PAGE, n_pages - (t0 + j) * (BKV / PAGE));  // pages that the sequence has here
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          if (!ok) break;
-          ok = mbar_wait(&empty[st], static_cast<uint32_t>(ph), abort_flag, p.status, kStatusTimeoutEmpty);
-          if (!ok) break;
-          const CUtensorMap* tm1 = v ? &tmV : &tmK;
-          uint8_t* dst = sKV + st * TILE;
-          mbar_expect_tx(&full[st], 2 * n * PAGE * 128);
-          if (run && n == BKV / PAGE) {
-            const CUtensorMap* tm8 = v ? &tmV8 : &tmK8;
-            tma_load_2d(dst, tm8, &full[st], kvh * D, cur[0] * PAGE, pol);
-            tma_load_2d(dst + BLK, tm8, &full[st], kvh * D + 64, cur[0] * PAGE, pol);
-          } else {
-#pragma unroll
-            for (int pg = 0; pg < BKV / PAGE; ++pg)
-              if (pg < n) {
-                tma_load_2d(dst + pg * PAGE * 128, tm1, &full[st], kvh * D, cur[pg] * PAGE, pol);
-                tma_load_2d(dst + BLK + pg * PAGE * 128, tm1, &full[st], kvh * D + 64, cur[pg] * PAGE, pol);
-              }
-          }
-          ++issued;
-          if (++st == SLOTS) {
-            st = 0;
-            ph ^= 1;
-          }
-        }
+      for (int v = 0; v < 2; ++v) {
         if (!ok) break;
+        ok = mbar_wait_warp(&empty[st], static_cast<uint32_t>(ph), abort_flag, p.status, kStatusTimeoutEmpty);
+        if (!ok) break;
+        const CUtensorMap* tm1 = v ? &tmV : &tmK;
+        uint8_t* dst = sKV + st * TILE;
+        kv8::mbar_expect_tx_if(on, &full[st], 2 * n * PAGE * 128);
+        if (run && n == BKV / PAGE) {
+          const CUtensorMap* tm8 = v ? &tmV8 : &tmK8;
+          kv8::tma_load_2d_if(on, dst, tm8, &full[st], kvh * D, cur[0] * PAGE, pol);
+          kv8::tma_load_2d_if(on, dst + BLK, tm8, &full[st], kvh * D + 64, cur[0] * PAGE, pol);
+        } else {
+#pragma unroll
+          for (int pg = 0; pg < BKV / PAGE; ++pg)
+            if (pg < n) {
+              kv8::tma_load_2d_if(on, dst + pg * PAGE * 128, tm1, &full[st], kvh * D, cur[pg] * PAGE, pol);
+              kv8::tma_load_2d_if(on, dst + BLK + pg * PAGE * 128, tm1, &full[st], kvh * D + 64, cur[pg] * PAGE, pol);
+            }
+        }
+        ++issued;
+        if (++st == SLOTS) {
+          st = 0;
+          ph ^= 1;
+        }
       }
-      for (int i = max(0, issued - SLOTS); i < issued; ++i)
-        mbar_wait(&full[i % SLOTS], static_cast<uint32_t>((i / SLOTS) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
     }
+    for (int i = max(0, issued - SLOTS); i < issued; ++i)
+      mbar_wait_warp(&full[i % SLOTS], static_cast<uint32_t>((i / SLOTS) & 1), nullptr, nullptr, 0, kWaitLimitNs / 4);
   } else if (warp == 1) {
     const uint32_t on = elect_one();
     const uint32_t idesc_s = make_idesc_bf16(128, NQ);
@@ -331,6 +348,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
                                   kStatusTimeoutTmemFull);
       tc_fence_after();
     };
+    const uint64_t keep = policy_evict_last();
     float* scores = p.scores + (static_cast<size_t>(b) * p.hkv + kvh) * static_cast<size_t>(p.keys) * GP;
     for (int j = 0; j < nt; ++j) {
       if (ok) ok = mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
@@ -349,17 +367,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
         x[h] = valid ? __uint_as_float(sv[h]) : -INFINITY;
         above = above || x[h] > limit[h];
       }
-      if (valid) {
-        float* dst = scores + static_cast<size_t>(key) * GP;
-        if constexpr (GP == 1)
-          dst[0] = x[0];
-        else if constexpr (GP == 2)
-          *reinterpret_cast<float2*>(dst) = make_float2(x[0], x[1]);
-        else
-#pragma unroll
-          for (int h = 0; h < GP; h += 4)
-            *reinterpret_cast<float4*>(dst + h) = make_float4(x[h], x[(h + 1) % GP], x[(h + 2) % GP], x[(h + 3) % GP]);
-      }
+      if (valid) store_scores(scores + static_cast<size_t>(key) * GP, x, keep);
       if (barrier_or(above)) {
         // uniform over the CTA: every thread derives the same maxima
 #pragma unroll
@@ -535,6 +543,12 @@ __global__ void __launch_bounds__(FIN_THREADS) finish_kernel(const Params p) {
       return;
     }
   }
+  float m[GP], inv[GP];
+#pragma unroll
+  for (int h = 0; h < GP; ++h) {
+    m[h] = h < G ? s_m[h] : 0.f;
+    inv[h] = h < G ? s_inv[h] : 0.f;
+  }
   const float* scores = p.scores + (static_cast<size_t>(b) * p.hkv + kvh) * static_cast<size_t>(p.keys) * GP;
   float* mass = p.mass + (static_cast<size_t>(sq.row) * p.hkv + kvh) * static_cast<size_t>(p.cap);
   const long long end = min(min(static_cast<long long>(len), p.cap), k0 + FIN_KEYS);
@@ -557,7 +571,7 @@ __global__ void __launch_bounds__(FIN_THREADS) finish_kernel(const Params p) {
     float w = 0.f;
 #pragma unroll
     for (int h = 0; h < GP; ++h)
-      if (h < G) w += exp2f(fmaf(s[h], p.c, -s_m[h])) * s_inv[h];
+      if (h < G) w = fmaf(exp2f(fmaf(s[h], p.c, -m[h])), inv[h], w);
     mass[k] += w;
   }
 }
