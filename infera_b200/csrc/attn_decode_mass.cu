@@ -6,8 +6,9 @@
 //
 // A weight is known only when the last key has been seen, so the pass over K
 // and V keeps the raw scores (4 bytes a key and query head, against 512 of K
-// and V a key and KV head) and a second kernel, which merges the shares too,
-// turns them into weights.
+// and V a key and KV head). A second kernel merges the shares and turns the
+// scores into weights; where a sequence is one share and short, its CTA does
+// that itself at its end.
 //
 //   S^T[128 keys, 16]  = K_tile . Q^T     (A = K, K-major)
 //   O^T[128 dims, 16]  = V_tile^T . W     (A = V, MN-major)
@@ -79,6 +80,7 @@ struct Params {
   long long cap;
   __nv_bfloat16* out;
   int ldo;
+  bool fused;                   // one share, whose CTA finishes
   int* status;
 };
 
@@ -144,6 +146,129 @@ __device__ __forceinline__ void store_scores(float* dst, const float (&x)[N], ui
                    "f"(x[h + 2]), "f"(x[h + 3]), "l"(policy)
                    : "memory");
   }
+}
+
+// ---- from parts and scores to the output and the mass, by CTAs of N threads
+//   o = sum_s O_s 2^(m_s - M) / L,  L = sum_s l_s 2^(m_s - M)
+//   mass[j] += sum_h 2^(c s[h, j] - M[h]) / L[h]
+
+// Keys of a sequence that the splits cover.
+__device__ __forceinline__ int covered(const Params& p, const Seq& sq) {
+  return static_cast<int>(
+      min(static_cast<long long>(sq.len), static_cast<long long>(p.splits) * p.tiles_per_split * BKV));
+}
+// M and 1 / L of the group's heads.
+template <int N>
+__device__ __forceinline__ void make_sums(const Params& p, int b, int kvh, float* s_m, float* s_inv) {
+  const int lane = threadIdx.x & 31;
+  for (int h = threadIdx.x >> 5; h < p.G; h += N / 32) {
+    const float2* ml = p.ml + (static_cast<size_t>(b) * p.hq + kvh * p.G + h) * p.splits;
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, __ldcg(ml + s).x);
+    m = max_over_warp(m);
+    if (m == -INFINITY) m = 0.f;
+    for (int s = lane; s < p.splits; s += 32) {
+      const float2 v = __ldcg(ml + s);
+      if (v.x != -INFINITY) l += v.y * exp2f(v.x - m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {
+      s_m[h] = m;
+      s_inv[h] = l == 0.f ? 0.f : 1.f / l;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void merge_parts(const Params& p, int b, int kvh, const float* s_m, const float* s_inv) {
+  for (int i = threadIdx.x; i < p.G * (D / 4); i += N) {
+    const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+    const size_t base = (static_cast<size_t>(b) * p.hq + kvh * p.G + h) * p.splits;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float m = __ldcg(p.ml + base + s).x;
+      if (m == -INFINITY) continue;  // a share without keys wrote nothing
+      const float w = exp2f(m - s_m[h]);
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(p.o_part + (base + s) * D + d));
+      a[0] += o.x * w;
+      a[1] += o.y * w;
+      a[2] += o.z * w;
+      a[3] += o.w * w;
+    }
+    const float inv = s_inv[h];
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(b) * p.ldo + (kvh * p.G + h) * D + d);
+    dst[0] = pack_bf16(a[0] * inv, a[1] * inv);
+    dst[1] = pack_bf16(a[2] * inv, a[3] * inv);
+  }
+}
+// The weights of keys k0 .. k0 + n, four a thread at a time. Called by all threads.
+template <int GP, int N>
+__device__ __forceinline__ void add_mass(const Params& p, const Seq& sq, int b, int kvh, int k0, int n, const float* s_m,
+                                         const float* s_inv) {
+  const int G = p.G, len = covered(p, sq), stop = min(len - k0, n) + k0;
+  if (sq.row >= p.mass_rows || stop > p.cap) {
+    if (threadIdx.x == 0)
+      record_status_detail(p.status, kStatusBadIndex, 6, b, sq.row >= p.mass_rows ? sq.row : len);
+    if (sq.row >= p.mass_rows) return;
+  }
+  if (p.bt_rows != nullptr) {  // a row that an earlier sequence of the batch has: that one's weights alone are added
+    bool twice = false;
+    for (int i = threadIdx.x; i < b; i += N) twice = twice || p.bt_rows[i] == sq.row;
+    if (__syncthreads_or(twice)) {
+      if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 7, b, sq.row);
+      return;
+    }
+  }
+  float m[GP], inv[GP];
+#pragma unroll
+  for (int h = 0; h < GP; ++h) {
+    m[h] = h < G ? s_m[h] : 0.f;
+    inv[h] = h < G ? s_inv[h] : 0.f;
+  }
+  const float* scores = p.scores + (static_cast<size_t>(b) * p.hkv + kvh) * static_cast<size_t>(p.keys) * GP;
+  float* mass = p.mass + (static_cast<size_t>(sq.row) * p.hkv + kvh) * static_cast<size_t>(p.cap);
+  const int end = static_cast<int>(min(static_cast<long long>(stop), p.cap));
+  constexpr int KEYS = 4;
+  for (int at = k0 + static_cast<int>(threadIdx.x); at < end; at += KEYS * N) {
+    float x[KEYS][GP], was[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {  // all loads under way at once
+      const int k = at + i * N;
+      if (k >= end) break;
+      const float* src = scores + static_cast<size_t>(k) * GP;
+      if constexpr (GP == 1) {
+        x[i][0] = __ldcg(src);
+      } else if constexpr (GP == 2) {
+        *reinterpret_cast<float2*>(&x[i][0]) = __ldcg(reinterpret_cast<const float2*>(src));
+      } else {
+#pragma unroll
+        for (int h = 0; h < GP; h += 4)
+          *reinterpret_cast<float4*>(&x[i][h]) = __ldcg(reinterpret_cast<const float4*>(src + h));
+      }
+      was[i] = mass[k];
+    }
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int k = at + i * N;
+      if (k >= end) break;
+      float w = 0.f;
+#pragma unroll
+      for (int h = 0; h < GP; ++h)
+        if (h < G) w = fmaf(exp2f(fmaf(x[i][h], p.c, -m[h])), inv[h], w);
+      mass[k] = was[i] + w;
+    }
+  }
+}
+// The end of a sequence of one share. All threads, after the scores were written.
+template <int GP>
+__device__ __forceinline__ void end_share(const Params& p, const Seq& sq, int b, int kvh) {
+  __shared__ float s_m[8], s_inv[8];
+  __threadfence_block();
+  __syncthreads();
+  make_sums<NUM_THREADS>(p, b, kvh, s_m, s_inv);
+  __syncthreads();
+  add_mass<GP, NUM_THREADS>(p, sq, b, kvh, 0, sq.len, s_m, s_inv);
 }
 
 template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
@@ -471,109 +596,27 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     __syncwarp();
     tmem_dealloc(tmem, TMEM_COLS);
   }
+  if (p.fused) end_share<GP>(p, sq, b, kvh);
 }
 
-// Block 0 of a (sequence, KV head) merges the shares,
-//   o = sum_s O_s 2^(m_s - M) / L,  L = sum_s l_s 2^(m_s - M);
-// the others turn the scores of FIN_KEYS keys into weights 2^(c s - M) / L and
-// add them, summed over the group's heads, to the mass.
+// Block 0 of a (sequence, KV head) merges the shares, the others take FIN_KEYS
+// keys each.
 template <int GP>
 __global__ void __launch_bounds__(FIN_THREADS) finish_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();
-  const int kvh = blockIdx.y, b = blockIdx.z, G = p.G;
+  const int kvh = blockIdx.y, b = blockIdx.z;
   const Seq sq = sequence(p, b, nullptr);
-  const long long covered = static_cast<long long>(p.splits) * p.tiles_per_split * BKV;
-  const int len = static_cast<int>(min(static_cast<long long>(sq.len), covered));
   const bool merge = blockIdx.x == 0;
-  const long long k0 = static_cast<long long>(blockIdx.x - 1) * FIN_KEYS;
-  if (merge ? p.splits == 1 : k0 >= len) return;
+  const int k0 = (static_cast<int>(blockIdx.x) - 1) * FIN_KEYS;
+  if (merge ? p.splits == 1 : k0 >= covered(p, sq)) return;
   __shared__ float s_m[8], s_inv[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < G) {
-    const float2* ml = p.ml + (static_cast<size_t>(b) * p.hq + kvh * G + warp) * p.splits;
-    float m = -INFINITY, l = 0.f;
-    for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, ml[s].x);
-    m = max_over_warp(m);
-    if (m == -INFINITY) m = 0.f;
-    for (int s = lane; s < p.splits; s += 32) {
-      const float2 v = ml[s];
-      if (v.x != -INFINITY) l += v.y * exp2f(v.x - m);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_inv[warp] = l == 0.f ? 0.f : 1.f / l;
-    }
-  }
+  make_sums<FIN_THREADS>(p, b, kvh, s_m, s_inv);
   __syncthreads();
-  if (merge) {
-    for (int i = threadIdx.x; i < G * (D / 4); i += FIN_THREADS) {
-      const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-      const size_t base = (static_cast<size_t>(b) * p.hq + kvh * G + h) * p.splits;
-      float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int s = 0; s < p.splits; ++s) {
-        const float m = p.ml[base + s].x;
-        if (m == -INFINITY) continue;  // a share without keys wrote nothing
-        const float w = exp2f(m - s_m[h]);
-        const float4 o = *reinterpret_cast<const float4*>(p.o_part + (base + s) * D + d);
-        a[0] += o.x * w;
-        a[1] += o.y * w;
-        a[2] += o.z * w;
-        a[3] += o.w * w;
-      }
-      const float inv = s_inv[h];
-      uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(b) * p.ldo + (kvh * G + h) * D + d);
-      dst[0] = pack_bf16(a[0] * inv, a[1] * inv);
-      dst[1] = pack_bf16(a[2] * inv, a[3] * inv);
-    }
-    return;
-  }
-  if (sq.row >= p.mass_rows || (k0 + FIN_KEYS > p.cap && len > p.cap)) {
-    if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 6, b, sq.row >= p.mass_rows ? sq.row : len);
-    if (sq.row >= p.mass_rows) return;
-  }
-  if (p.bt_rows != nullptr) {  // a row that an earlier sequence of the batch has: that one's weights alone are added
-    bool twice = false;
-    for (int i = threadIdx.x; i < b; i += FIN_THREADS) twice = twice || p.bt_rows[i] == sq.row;
-    if (__syncthreads_or(twice)) {
-      if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 7, b, sq.row);
-      return;
-    }
-  }
-  float m[GP], inv[GP];
-#pragma unroll
-  for (int h = 0; h < GP; ++h) {
-    m[h] = h < G ? s_m[h] : 0.f;
-    inv[h] = h < G ? s_inv[h] : 0.f;
-  }
-  const float* scores = p.scores + (static_cast<size_t>(b) * p.hkv + kvh) * static_cast<size_t>(p.keys) * GP;
-  float* mass = p.mass + (static_cast<size_t>(sq.row) * p.hkv + kvh) * static_cast<size_t>(p.cap);
-  const long long end = min(min(static_cast<long long>(len), p.cap), k0 + FIN_KEYS);
-#pragma unroll
-  for (int i = 0; i < FIN_KEYS / FIN_THREADS; ++i) {
-    const long long k = k0 + i * FIN_THREADS + threadIdx.x;
-    if (k >= end) continue;
-    float s[GP];
-    const float* src = scores + static_cast<size_t>(k) * GP;
-    if constexpr (GP == 1) {
-      s[0] = src[0];
-    } else if constexpr (GP == 2) {
-      const float2 v = *reinterpret_cast<const float2*>(src);
-      s[0] = v.x;
-      s[GP - 1] = v.y;
-    } else {
-#pragma unroll
-      for (int h = 0; h < GP; h += 4) *reinterpret_cast<float4*>(&s[h]) = *reinterpret_cast<const float4*>(src + h);
-    }
-    float w = 0.f;
-#pragma unroll
-    for (int h = 0; h < GP; ++h)
-      if (h < G) w = fmaf(exp2f(fmaf(s[h], p.c, -m[h])), inv[h], w);
-    mass[k] += w;
-  }
+  if (merge)
+    merge_parts<FIN_THREADS>(p, b, kvh, s_m, s_inv);
+  else
+    add_mass<GP, FIN_THREADS>(p, sq, b, kvh, k0, FIN_KEYS, s_m, s_inv);
 }
 
 template <int GP>
@@ -589,7 +632,7 @@ int launch(const CUtensorMap (&tm)[4], const Params& p, int B, cudaStream_t stre
   }
   cudaError_t e = launch_pdl(decode_mass_kernel<GP>, dim3(p.hkv, B, p.splits), NUM_THREADS, SMEM_BYTES, stream, tm[0],
                              tm[1], tm[2], tm[3], p);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  if (e != cudaSuccess || p.fused) return static_cast<int>(e);
   const unsigned blocks = static_cast<unsigned>(1 + (p.keys + FIN_KEYS - 1) / FIN_KEYS);
   return static_cast<int>(launch_pdl(finish_kernel<GP>, dim3(blocks, p.hkv, B), FIN_THREADS, 0, stream, p));
 }
@@ -606,22 +649,23 @@ using namespace ib200;
 // (s+1)*tiles_per_split) of every sequence; scores: fp32 scratch of B*hkv*keys*GP
 // (GP = hq/hkv rounded up to 1, 2, 4 or 8; keys: at least what the splits cover or the
 // table holds, the lesser), ml of 2*B*hq*splits, o_part of B*hq*splits*128 (only
-// touched when splits > 1).
+// touched when splits > 1). fused (splits 1): the first kernel's CTAs finish, else a
+// second kernel.
 extern "C" int ib_attn_decode_mass(const void* q, int ldq, const void* k_cache, const void* v_cache,
                                    long long num_slots, const int* block_table, const int* bt_rows,
                                    const int* seq_lens, int table_rows, int max_pages, int ld_table, int B, int hq,
                                    int hkv, int splits, int tiles_per_split, float scale, float* scores,
                                    long long keys, float* ml, float* o_part, float* mass, int mass_rows,
-                                   long long cap, void* out, int ldo, int* status, cudaStream_t stream) {
+                                   long long cap, int fused, void* out, int ldo, int* status, cudaStream_t stream) {
   using namespace ib200::dmass;
   if (B <= 0) return 0;
   if (hkv <= 0 || hkv > 65535 || hq % hkv != 0 || hq / hkv > 8 || splits < 1 || tiles_per_split < 1 || (ldq % 2) != 0 ||
-      B > 65535 || splits > 65535 || num_slots < PAGE || num_slots % PAGE != 0 || max_pages < 0 || max_pages > (1 << 27) - 1 ||
+      B > 65535 || splits > 65535 || num_slots < PAGE || num_slots % PAGE != 0 || max_pages < 0 || max_pages > (1 << 26) ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 3) != 0 || (ldo % 2) != 0 || cap < 0 ||
       keys < 1 || (reinterpret_cast<uintptr_t>(scores) & 15) != 0 || scores == nullptr || ml == nullptr ||
       (reinterpret_cast<uintptr_t>(ml) & 7) != 0)
     return -1;
-  if (splits > 1 && (o_part == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0)) return -1;
+  if (splits > 1 && (o_part == nullptr || fused != 0 || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0)) return -1;
   if (keys < std::min(static_cast<long long>(splits) * tiles_per_split * BKV, static_cast<long long>(max_pages) * PAGE))
     return -1;
   try {
@@ -657,6 +701,7 @@ extern "C" int ib_attn_decode_mass(const void* q, int ldq, const void* k_cache, 
     p.ml = reinterpret_cast<float2*>(ml);
     p.mass = mass;
     p.mass_rows = mass_rows;
+    p.fused = fused != 0;
     p.cap = cap;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.ldo = ldo;

@@ -131,8 +131,8 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
         "ib_attn_decode_kv8": [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int,
                                c_int, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
         "ib_attn_decode_mass": [c_vp, c_int, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
-                                c_int, c_int, c_int, c_float, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_ll, c_vp, c_int,
-                                c_vp, c_vp],
+                                c_int, c_int, c_int, c_float, c_vp, c_ll, c_vp, c_vp, c_vp, c_int, c_ll, c_int, c_vp,
+                                c_int, c_vp, c_vp],
         "ib_kv_select": [c_vp, c_int, c_int, c_ll, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp,
                          c_vp, c_vp, c_vp],
         "ib_kv_compact": [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_int, c_int,

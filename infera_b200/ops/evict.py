@@ -25,6 +25,10 @@ from infera_b200.ops import paged
 from infera_b200.ops.kv8 import HEAD_DIM, PAGE, _check_heads, _check_i32, _check_rows, _check_table, _name, _on
 
 _BF16, _F32 = torch.bfloat16, torch.float32
+# Scores of a KV head that the CTA of an uncut sequence turns into weights itself; more are spread over the GPU by a
+# second kernel. (1 x 100 keys of 32 heads: 8.3 us in one kernel, 8.75 in two; a CTA takes some 1.2 us for 3000 scores,
+# and 61 ragged sequences up to 12000 keys took 287 us that way, 256 in two kernels.)
+FUSED_SCORES = 8192
 
 
 def alloc_mass(rows: int, hkv: int, places: int, layers: int | None = None,
@@ -98,15 +102,16 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     scores = ws.data_ptr()
     part = scores + 4 * n_s
     ml = part + 4 * n * HEAD_DIM if splits > 1 else part
+    fused = splits == 1 and keys * gp <= FUSED_SCORES
     status, stream = _on(dev)
     rc = _native.kernels().ib_attn_decode_mass(q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
                                                k_cache.shape[0], block_table.data_ptr(), K._ptr(bt_rows),
                                                seq_lens.data_ptr(), block_table.shape[0], places,
                                                block_table.stride(0), B, hq, hkv, splits, tiles_per_split, scale,
                                                scores, keys, ml, part if splits > 1 else None, mass.data_ptr(),
-                                               mass.shape[0], mass.shape[2], out.data_ptr(), ldo, status, stream)
+                                               mass.shape[0], mass.shape[2], fused, out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_decode_mass")
-    K._count(2)
+    K._count(1 if fused else 2)
     return out
 
 
