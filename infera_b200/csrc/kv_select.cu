@@ -33,11 +33,10 @@ namespace sel {
 namespace cg = cooperative_groups;
 using kv8::table_row;
 
-constexpr int THREADS = 1024;
-constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
 constexpr int CANDIDATES = 2048;
 constexpr uint32_t STAYS = 0xffffffffu;  // (the largest weight, infinity, has 0xff800000)
+constexpr int FEW = 4096;              // places of a CTA of 512 threads, at most
 constexpr int MAX_CACHED = 44 * 1024;  // places that a CTA holds in shared memory, 176 KB
 
 // places of a run when `of` ones are shared by `among`, in whole groups of a warp
@@ -72,10 +71,11 @@ __device__ __forceinline__ float weight_of(uint32_t k) {
 
 // CACHED: a CTA's run of places fits into its shared memory; else they are read
 // in each pass.
-template <bool CACHED>
-__global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
+template <bool CACHED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_kernel(const SelectParams p) {
   pdl_trigger();
   pdl_wait();
+  constexpr int WARPS = THREADS / 32, MINE = BINS / THREADS;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int list = blockIdx.x / C, s = list / p.hkv, h = list % p.hkv;
@@ -94,11 +94,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
 
   const int row = p.bt_rows != nullptr ? p.bt_rows[s] : s;
   long long n_keys = max(p.seq_lens[s], 0);
-  if (tid < BINS / 4) {
-    reinterpret_cast<uint4*>(hist0)[tid] = make_uint4(0u, 0u, 0u, 0u);
-    reinterpret_cast<uint4*>(hist1)[tid] = make_uint4(0u, 0u, 0u, 0u);
+  for (int i = tid; i < BINS / 4; i += THREADS) {
+    reinterpret_cast<uint4*>(hist0)[i] = make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(hist1)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (i < BINS / 8) reinterpret_cast<uint4*>(hist2)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  if (tid < BINS / 8) reinterpret_cast<uint4*>(hist2)[tid] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) n_candidates = 0;
   bool bad = row < 0 || row >= p.mass_rows;
   if (bad && tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, row);
@@ -207,17 +207,23 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
       }
     }
     sync_all();
-    // the bin in which the want-th largest lies: thread t has the bins 2 t and 2 t + 1 from the top
-    uint32_t c[2] = {0u, 0u};
-    const int top = (1 << bits) - 2 - 2 * tid;
+    // the bin in which the want-th largest lies: thread t has MINE bins, from MINE t on from the top
+    uint32_t c[MINE] = {};
+    const int top = (1 << bits) - MINE - MINE * tid;
     uint32_t* hist = digit == 0 ? hist0 : (digit == 1 ? hist1 : hist2);
     for (int r = 0; r < C && top >= 0; ++r) {
-      const uint32_t* other = C > 1 ? cluster.map_shared_rank(hist, r) : hist;
-      const uint2 two = *reinterpret_cast<const uint2*>(other + top);
-      c[0] += two.y;
-      c[1] += two.x;
+      const uint32_t* other = (C > 1 ? cluster.map_shared_rank(hist, r) : hist) + top;
+#pragma unroll
+      for (int i = 0; i < MINE; i += 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(other + i);
+        c[MINE - 1 - i] += v.x;
+        c[MINE - 2 - i] += v.y;
+      }
     }
-    uint32_t sum = c[0] + c[1];
+    uint32_t own = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) own += c[i];
+    uint32_t sum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -225,11 +231,14 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectParams p) {
     }
     if (lane == 31) wsum[warp] = sum;
     __syncthreads();
-    const uint32_t before = sum - c[0] - c[1] + __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
-    if (before < want && before + c[0] + c[1] >= want) {
-      const bool second = before + c[0] < want;
-      s_bin = static_cast<uint32_t>(second ? top : top + 1);
-      s_want = want - before - (second ? c[0] : 0u);
+    uint32_t before = sum - own + __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0u);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      if (before < want && before + c[i] >= want) {
+        s_bin = static_cast<uint32_t>(top + MINE - 1 - i);
+        s_want = want - before;
+      }
+      before += c[i];
     }
     __syncthreads();  // s_bin
     if (want == 0) break;  // (of the middle nothing stays)
@@ -567,17 +576,21 @@ extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, 
   SelectParams p{mass, mass_rows, hkv, cap, seq_lens, bt_rows, keep, sink, recent, update, kept, kept_mass, count, status};
   const int run = run_of(cap, cluster);  // the longest of a CTA
   const bool cached = run <= MAX_CACHED;
+  // few weights a thread: the barriers of half as many warps are quicker (1025 keys 8.2 us against 9.2)
+  const int threads = run <= FEW ? 512 : 1024;
+  const auto kernel = threads == 512 ? select_kernel<true, 512> : (cached ? select_kernel<true, 1024> : select_kernel<false, 1024>);
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CACHED * 4);
+    const cudaError_t e =
+        cudaFuncSetAttribute(select_kernel<true, 1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CACHED * 4);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(n) * hkv * cluster);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = cached ? static_cast<size_t>(run) * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -587,7 +600,7 @@ extern "C" int ib_kv_select(float* mass, int mass_rows, int hkv, long long cap, 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, cached ? select_kernel<true> : select_kernel<false>, p));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
 // Caches [layers, num_slots, row_bytes] (v null: one channel). src [n, heads, m]:

@@ -137,7 +137,7 @@ def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale,
 def _select_ctas(lists: int, places: int, num_sms: int = 148) -> int:
     """CTAs that share a list of :func:`select_keys`."""
     ctas = 1
-    while ctas < 8 and 2 * lists * ctas <= num_sms and places > 2048 * ctas:
+    while ctas < 8 and 2 * lists * ctas <= num_sms and places > 4096 * ctas:
         ctas *= 2
     return ctas
 

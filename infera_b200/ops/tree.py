@@ -26,6 +26,9 @@ from infera_b200.ops.kv8 import HEAD_DIM, PAGE, _check_heads, _check_i32, _check
 
 _BF16, _I32 = torch.bfloat16, torch.int32
 MAX_NODES = 256
+# Contexts of up to so many tiles of 64 keys are not cut: 8 nodes of 32 heads over 508 keys take 12 us either way on the
+# GPU, and one launch instead of two.
+UNCUT = 10
 
 
 def _rows_of(q_start: list[int], q_len: list[int], T: int, most: int) -> list[tuple[int, int]]:
@@ -117,12 +120,12 @@ def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: i
     total = hkv * sum(i * u for i, u in zip(items, units))
     top, levels = max((u for i, u in zip(items, units) if i), default=4), max(1, max(items))
     ctas = max(1, min(2 * num_sms // levels * levels or levels, -(-total // 5)))
-    return ctas, 1 if top <= 7 else -(-top * ctas // total) + 1
+    return ctas, 1 if top <= UNCUT + 3 else -(-top * ctas // total) + 1
 
 
 def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, int]:
     """(CTAs, most pieces of an item) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each 128 rows of
-    the longest tree, at least two tiles of 64 keys each; contexts of up to four tiles are not cut."""
+    the longest tree, at least two tiles of 64 keys each; contexts of up to :data:`UNCUT` tiles are not cut."""
     return _plan(tuple(q_lens), tuple(ctx_lens), hq // hkv, hkv, num_sms)
 
 
