@@ -14,8 +14,8 @@
 //   O^T[128 dims, 16]  = V_tile^T . W     (A = V, MN-major)
 //
 // The 16 columns of O^T hold two bf16 digits of the weights of up to 8 heads,
-// w = hi + lo: a weight is off by at most 2^-17 of itself instead of bf16's
-// 2^-9, and the digits cost no matrix instruction.
+// w = hi + lo: a weight is off by at most 2^-16 of itself instead of bf16's
+// 2^-8, and the digits cost no matrix instruction.
 //
 // One CTA handles (sequence, KV head, share) and walks its keys in tiles of 128
 // (8 pages), 32 KB of K and 32 KB of V in a ring of three slots that both take

@@ -2,8 +2,8 @@
 // bf16 paged KV cache, on tcgen05. A sequence's last q_len keys are its nodes;
 // node i sees the keys before them and node j where bit j of its mask is set.
 //
-//   S = Q K^T, O += W V,  w = 2^(c s - m) in bf16 (rounded, 2^-9 of itself, as
-//   the prompt kernel's), the sum of the softmax over the fp32 weights
+//   S = Q K^T, O += W V,  w = 2^(c s - m) in bf16 (rounded, by up to 2^-8 of
+//   itself, as in the prompt kernel), the sum of the softmax over the fp32 weights
 //
 // The query heads of a KV head are packed: rows are (node, head) pairs. A CTA
 // takes 128 rows and walks its keys in tiles of 64 (4 pages), 16 KB of K and 16
@@ -25,7 +25,9 @@
 // The tiles of all items, laid end to end, are cut into equal runs, one for each
 // CTA of a single wave: batches of any raggedness are balanced, and the loads of
 // a run's next item are under way while the one before ends. An item that a cut
-// falls in is merged from its pieces by a second kernel.
+// falls in is merged from its pieces by a second kernel; a run has at most two
+// such pieces, the end of an item and the beginning of one, so the workspace does
+// not depend on the batch.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -75,12 +77,12 @@ struct Params {
   int n_seqs;
   int hq, hkv, G, nodes;   // nodes: of an item, 128 / G
   int blocks;              // items of the longest tree and KV head
-  int splits;              // pieces of an item at most; 1: no item is cut
+  bool cut;                // items may be cut; else one goes to the run in which it begins
   float c;                 // |scale| * log2(e)
   uint32_t q_flip, q_keep;
-  float* o_part;           // [T, hq, splits, 128]
-  float* lse_part;         // [T, hq, splits]
-  int* pieces;             // [n_seqs, hkv, blocks]
+  float* o_part;           // [2 * runs, 128 rows, 128]: of run w the piece that an item begins with in 2 w + 1, another in 2 w
+  float* lse_part;         // [2 * runs, 128]
+  int2* pieces;            // [n_seqs, hkv, blocks] first run and number of runs of an item
   __nv_bfloat16* out;
   int ldo;
   int* status;
@@ -98,8 +100,7 @@ __device__ __forceinline__ Seq sequence(const Params& p, int s, int* status) {
   q.start = p.q_start[s];
   q.ctx = max(p.ctx_len[s], 0);
   q.n = min(want, min(p.blocks * p.nodes, 32 * p.words));
-  if (q.start < 0 || q.start > p.T) q.n = 0;
-  q.n = min(q.n, p.T - q.start);
+  q.n = q.start < 0 || q.start > p.T ? 0 : min(q.n, p.T - q.start);
   q.base = q.ctx - want;  // (may be negative: nodes without a key)
   if (q.n < want) record_status_detail(status, kStatusBadIndex, 9, s, want);
   if (q.ctx > p.max_pages * PAGE) record_status_detail(status, kStatusBadIndex, 1, s, q.ctx);
@@ -139,28 +140,22 @@ struct Walk {
   __device__ __forceinline__ Walk(const Params& p, int* status) {
     const int lane = threadIdx.x & 31;
     total = 0;
-    int most = 1;
     Seq mine0{};  // the lane's first sequence
     for (int i = lane; i < p.n_seqs; i += 32) {
       const Seq q = sequence(p, i, status);
       if (i == lane) mine0 = q;
       total += units(p, q, 0) * q.blocks;
-      if (q.n > 0) most = max(most, kStart + q.tiles);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    most = __reduce_max_sync(0xffffffffu, most);
-    // every run has a unit, and is long enough that no item has more than `splits` pieces
-    long long runs = min(static_cast<long long>(gridDim.x), total);
-    if (p.splits > 1) runs = min(runs, divide(total * (p.splits - 1), most));
-    ctas = static_cast<int>(max(1ll, runs));
+    ctas = static_cast<int>(max(1ll, min(static_cast<long long>(gridDim.x), total)));  // every run has a unit
     at = end = 0;
     if (static_cast<int>(blockIdx.x) >= ctas) return;
     at = divide(total * blockIdx.x, ctas);
     end = divide(total * (blockIdx.x + 1), ctas);
     if (at >= end) return;
     long long before = 0;
-    for (block = 0;; ++block) {
+    for (block = 0; block < p.blocks; ++block) {
       for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int i = s0 + lane;
         const long long mine = i < p.n_seqs ? units(p, s0 == 0 ? mine0 : sequence(p, i, nullptr), block) : 0;
@@ -178,7 +173,7 @@ struct Walk {
           sq = sequence(p, s, nullptr);
           kvh = static_cast<int>(divide(at - first, kStart + sq.tiles));
           first += static_cast<long long>(kvh) * (kStart + sq.tiles);
-          if (p.splits == 1 && at > first) {  // the item is the run's in which it begins
+          if (!p.cut && at > first) {  // the item is the run's in which it begins
             at = first + kStart + sq.tiles;
             enter(p);
           }
@@ -187,11 +182,12 @@ struct Walk {
         before += __shfl_sync(0xffffffffu, sum, 31);
       }
     }
+    end = at;  // (the lengths changed under the kernel)
   }
   __device__ __forceinline__ bool more() const { return at < end; }
   __device__ __forceinline__ long long last(const Params& p) const {  // one past the segment
     const long long stop = first + kStart + sq.tiles;
-    return p.splits == 1 ? stop : min(stop, end);
+    return p.cut ? min(stop, end) : stop;
   }
   // the segment's key tiles: first one and count
   __device__ __forceinline__ int tile() const { return static_cast<int>(max(0ll, at - first - kStart)); }
@@ -213,7 +209,10 @@ struct Walk {
     do {  // (units are left, so there is such a sequence)
       if (++s == p.n_seqs) {
         s = 0;
-        ++block;
+        if (++block >= p.blocks) {  // (the lengths changed under the kernel)
+          end = at;
+          return;
+        }
       }
       sq = sequence(p, s, nullptr);
     } while (sq.blocks <= block);
@@ -480,13 +479,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     const int node = first + (live ? r / G : 0), head = kvh * G + (live ? r % G : 0);
     const int row = sq.start + node;
     // the item's pieces are those of the runs that it lies in
-    const int run = walk.run_of(walk.first), piece = static_cast<int>(blockIdx.x) - run;
-    const int pieces = p.splits == 1 ? 1 : walk.run_of(walk.first + kStart + sq.tiles - 1) - run + 1;
-    if (p.splits > 1 && piece == 0 && threadIdx.x == 64) p.pieces[(walk.s * p.hkv + kvh) * p.blocks + block] = pieces;
+    const int run = walk.run_of(walk.first);
+    const int pieces = p.cut ? walk.run_of(walk.first + kStart + sq.tiles - 1) - run + 1 : 1;
+    const bool begins = walk.at == walk.first;
+    const size_t part = (2 * static_cast<size_t>(blockIdx.x) + begins) * BQ + r;
+    if (p.cut && begins && threadIdx.x == 64) p.pieces[(walk.s * p.hkv + kvh) * p.blocks + block] = make_int2(run, pieces);
     if (nk == 0) {  // no key tile in this piece, or none at all
       if (live) {
         if (pieces > 1)
-          p.lse_part[(static_cast<size_t>(row) * p.hq + head) * p.splits + piece] = -INFINITY;
+          p.lse_part[part] = -INFINITY;
         else
           for (int i = 0; i < D / 8; ++i)
             reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * p.ldo + head * D)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -624,7 +625,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     done += nk;
     wait_pv(done - 1);
     if (ok) {
-      const size_t part = (static_cast<size_t>(row) * p.hq + head) * p.splits + piece;
       const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // a NaN stays one
       const bool merge = pieces > 1;
       if (merge && live) p.lse_part[part] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
@@ -674,71 +674,79 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// Merge the pieces of cut items. An item's rows are (node, head) pairs.
-struct Row {
-  int pieces;              // 1: nothing to merge
-  size_t part;             // of its first piece
-  __nv_bfloat16* out;
-};
-__device__ __forceinline__ Row merge_row(const Params& p, const Seq& sq, int item, int r) {
-  const int kvh = item / p.blocks % p.hkv, block = item % p.blocks, node = block * p.nodes + r / p.G;
-  if (r >= p.nodes * p.G || node >= sq.n) return {1, 0, nullptr};
-  const int row = sq.start + node, head = kvh * p.G + r % p.G;
-  return {p.pieces[item], (static_cast<size_t>(row) * p.hq + head) * p.splits, p.out + static_cast<size_t>(row) * p.ldo + head * D};
-}
-// W warps a row.
-constexpr int MERGE_WARPS = kv8::MERGE_WARPS;
-template <int W>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const __grid_constant__ Params p) {
+// Merge the pieces of cut items, W warps a row (a lane has 4 dims),
+//   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M)
+// a warp's first AHEAD pieces at a time under way.
+template <int W, int ROWS>  // rows of a block, W warps each
+__global__ void __launch_bounds__(W * ROWS * 32) merge_kernel(const __grid_constant__ Params p) {
+  constexpr int AHEAD = 4;
   pdl_trigger();
   pdl_wait();
-  const int item = blockIdx.x, r = blockIdx.y * (MERGE_WARPS / W) + (threadIdx.x >> 5) / W;
-  const Row row = merge_row(p, sequence(p, item / (p.hkv * p.blocks), nullptr), item, r);
-  if (row.pieces <= 1) return;  // (W > 1: the same for the whole block)
-  kv8::merge_shares<W>(p.o_part + row.part * D, p.lse_part + row.part, row.pieces, row.out);
-}
-// Up to MERGE_FEW pieces: MERGE_ROWS rows a warp, all of whose loads are under way at once.
-constexpr int MERGE_FEW = 4, MERGE_ROWS = 4;
-__global__ void __launch_bounds__(128) merge_few_kernel(const __grid_constant__ Params p) {
-  pdl_trigger();
-  pdl_wait();
-  const int item = blockIdx.x, lane = threadIdx.x & 31, r0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * MERGE_ROWS;
-  const Seq sq = sequence(p, item / (p.hkv * p.blocks), nullptr);
-  Row row[MERGE_ROWS];
-  float lse[MERGE_ROWS][MERGE_FEW];
-  float4 o[MERGE_ROWS][MERGE_FEW];
+  const int item = blockIdx.x, s = item / (p.hkv * p.blocks), kvh = item / p.blocks % p.hkv, block = item % p.blocks;
+  const int2 pc = p.pieces[item];  // (of an item that there is)
+  const Seq sq = sequence(p, s, nullptr);
+  const int lane = threadIdx.x & 31, w0 = (threadIdx.x >> 5) % W, r = blockIdx.y * ROWS + (threadIdx.x >> 5) / W;
+  const int node = block * p.nodes + r / p.G;
+  if (r >= p.nodes * p.G || node >= sq.n || pc.y <= 1) return;  // (the same for a row's warps)
+  auto part = [&](int k) { return (2 * static_cast<size_t>(pc.x + k) + (k == 0)) * BQ + r; };
+  float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f, top = -INFINITY;
+  for (int k0 = w0; k0 < pc.y; k0 += AHEAD * W) {
+    float lse[AHEAD];
+    float4 o[AHEAD];
 #pragma unroll
-  for (int i = 0; i < MERGE_ROWS; ++i) {
-    row[i] = merge_row(p, sq, item, r0 + i);
-#pragma unroll
-    for (int k = 0; k < MERGE_FEW; ++k) {
-      const bool in = row[i].pieces > 1 && k < row[i].pieces;
-      lse[i][k] = in ? p.lse_part[row[i].part + k] : -INFINITY;
-      o[i][k] = in ? reinterpret_cast<const float4*>(p.o_part + (row[i].part + k) * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < AHEAD; ++i) {
+      const int k = k0 + i * W;
+      lse[i] = k < pc.y ? p.lse_part[part(k)] : -INFINITY;
+      o[i] = k < pc.y ? reinterpret_cast<const float4*>(p.o_part + part(k) * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-  }
+    const float mx = fmaxf(fmaxf(fmaxf(lse[0], lse[1]), fmaxf(lse[2], lse[3])), top);
+    const float f = top == -INFINITY ? 0.f : exp2f(top - mx);
+    den *= f;
 #pragma unroll
-  for (int i = 0; i < MERGE_ROWS; ++i) {
-    if (row[i].pieces <= 1) continue;
-    float mx = fmaxf(fmaxf(lse[i][0], lse[i][1]), fmaxf(lse[i][2], lse[i][3]));
-    if (mx == -INFINITY) mx = 0.f;
-    float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+    for (int d = 0; d < 4; ++d) num[d] *= f;
+    top = mx;
+    const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int k = 0; k < MERGE_FEW; ++k) {
-      if (lse[i][k] == -INFINITY) continue;  // (a piece without keys wrote no more)
-      const float w = fmaxf(exp2f(lse[i][k] - mx), FLT_MIN);  // (a NaN in a piece stays one)
+    for (int i = 0; i < AHEAD; ++i) {
+      if (lse[i] == -INFINITY) continue;  // (a piece without keys wrote no more)
+      const float w = fmaxf(exp2f(lse[i] - ref), FLT_MIN);  // (a NaN in a piece stays one)
       den += w;
-      num[0] += o[i][k].x * w;
-      num[1] += o[i][k].y * w;
-      num[2] += o[i][k].z * w;
-      num[3] += o[i][k].w * w;
+      num[0] += o[i].x * w;
+      num[1] += o[i].y * w;
+      num[2] += o[i].z * w;
+      num[3] += o[i].w * w;
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    uint2 w;
-    w.x = pack_bf16(num[0] * inv, num[1] * inv);
-    w.y = pack_bf16(num[2] * inv, num[3] * inv);
-    reinterpret_cast<uint2*>(row[i].out)[lane] = w;
   }
+  if constexpr (W > 1) {
+    __shared__ float4 s_num[ROWS][W][32];
+    __shared__ float2 s_den[ROWS][W];
+    const int i = (threadIdx.x >> 5) / W;
+    s_num[i][w0][lane] = make_float4(num[0], num[1], num[2], num[3]);
+    if (lane == 0) s_den[i][w0] = make_float2(top, den);
+    static_assert(ROWS == 1, "the barrier below is the row's");
+    __syncthreads();
+    if (w0 != 0) return;
+    float mx = -INFINITY;
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_den[i][w].x);
+    den = num[0] = num[1] = num[2] = num[3] = 0.f;
+    for (int w = 0; w < W; ++w) {
+      const float2 td = s_den[i][w];
+      if (td.x == -INFINITY && td.y == 0.f) continue;
+      const float f = fmaxf(exp2f(td.x - mx), FLT_MIN);
+      const float4 v = s_num[i][w][lane];
+      den += td.y * f;
+      num[0] += v.x * f;
+      num[1] += v.y * f;
+      num[2] += v.z * f;
+      num[3] += v.w * f;
+    }
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const int head = kvh * p.G + r % p.G;
+  uint2 w;
+  w.x = pack_bf16(num[0] * inv, num[1] * inv);
+  w.y = pack_bf16(num[2] * inv, num[3] * inv);
+  reinterpret_cast<uint2*>(p.out + static_cast<size_t>(sq.start + node) * p.ldo + head * D)[lane] = w;
 }
 
 }  // namespace atree
@@ -748,24 +756,24 @@ using namespace ib200;
 
 // q [T, ldq] bf16 (head h at columns h*128); caches bf16 [num_slots, hkv*128];
 // q_start / q_len / ctx_len [n_seqs], ctx_len with the nodes; mask int32 [T,
-// words]; max_nodes: the most nodes of a sequence. ctas: equal runs that the
-// 64-key tiles of all items are cut into (fewer where an item would have more
-// than `splits` pieces; splits 1: an item goes to the run in which it begins).
-// With splits > 1: o_part / lse_part fp32 [T*hq*splits*128] / [T*hq*splits], pieces
-// [n_seqs * hkv * ceil(max_nodes / (128 / G))].
+// words]; max_nodes: the most nodes of a sequence. ctas: equal runs that all
+// items' units are cut into; o_part null: an item goes to the run in which it
+// begins. o_part / lse_part: fp32 [2*ctas*128*128] / [2*ctas*128], pieces
+// [2 * n_seqs * hkv * ceil(max_nodes / (128 / G))].
 extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, const void* v_cache, long long num_slots,
                             const int* q_start, const int* q_len, const int* ctx_len, const int* mask, int words,
                             int n_seqs, int max_nodes, const int* block_table, const int* bt_rows, int table_rows,
-                            int max_pages, int ld_table, int hq, int hkv, float scale, int ctas, int splits,
+                            int max_pages, int ld_table, int hq, int hkv, float scale, int ctas,
                             float* o_part, float* lse_part, int* pieces, void* out, int ldo, int* status, cudaStream_t stream) {
   using namespace ib200::atree;
   if (T <= 0 || n_seqs <= 0 || max_nodes <= 0) return 0;
-  if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 16 || splits < 1 || ctas < 1 || words < 1 || words > 8 ||
+  if (hkv <= 0 || hq % hkv != 0 || hq / hkv > 16 || ctas < 1 || words < 1 || words > 8 ||
       max_nodes > 32 * words || n_seqs > 65535 || (ldq % 8) != 0 || (ldo % 8) != 0 || num_slots < PAGE ||
-      num_slots % PAGE != 0 || max_pages < 0 || max_pages > (1 << 27) - 1 ||
+      num_slots % PAGE != 0 || max_pages < 0 || max_pages > (1 << 26) ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
     return -1;
-  if (splits > 1 && (o_part == nullptr || lse_part == nullptr || pieces == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0))
+  if (o_part != nullptr && (lse_part == nullptr || pieces == nullptr || (reinterpret_cast<uintptr_t>(o_part) & 15) != 0 ||
+                            (reinterpret_cast<uintptr_t>(pieces) & 7) != 0))
     return -1;
   try {
     const int kvw = hkv * D;
@@ -798,8 +806,8 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     p.nodes = BQ / p.G;
     p.blocks = (max_nodes + p.nodes - 1) / p.nodes;
     p.n_seqs = n_seqs;
-    p.splits = splits;
-    p.pieces = pieces;
+    p.cut = o_part != nullptr;
+    p.pieces = reinterpret_cast<int2*>(pieces);
     p.c = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);  // positive: masked scores are -inf times it
     p.q_flip = scale < 0.f ? 0x80008000u : 0u;
     p.q_keep = scale == 0.f ? 0u : ~0u;
@@ -820,13 +828,11 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     e = launch_pdl(tree_kernel, dim3(ctas), NUM_THREADS, SMEM_BYTES, stream, tk, tv, tk4, tv4, p);
     if (e != cudaSuccess) return static_cast<int>(e);
     const unsigned items = static_cast<unsigned>(n_seqs) * hkv * p.blocks;
-    // many pieces of few rows: a block a row (61 nodes of 32 heads in 20 pieces: 12 us with a warp each)
-    if (splits > MERGE_FEW && static_cast<long long>(T) * hq <= 16384)
-      e = launch_pdl(merge_kernel<MERGE_WARPS>, dim3(items, BQ), MERGE_WARPS * 32, 0, stream, p);
-    else if (splits > MERGE_FEW)
-      e = launch_pdl(merge_kernel<1>, dim3(items, BQ / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, p);
-    else if (splits > 1)
-      e = launch_pdl(merge_few_kernel, dim3(items, BQ / (4 * MERGE_ROWS)), 128, 0, stream, p);
+    // few items have many pieces: a block a row then (61 nodes of 32 heads over 100001 keys, 20 pieces)
+    if (p.cut && 4 * items <= static_cast<unsigned>(ctas))
+      e = launch_pdl(merge_kernel<8, 1>, dim3(items, BQ), 256, 0, stream, p);
+    else if (p.cut)
+      e = launch_pdl(merge_kernel<1, 8>, dim3(items, BQ / 8), 256, 0, stream, p);
     return static_cast<int>(e);
   } catch (...) {  // (no memory for a tensor map's entry)
     return -3;

@@ -18,9 +18,7 @@ struct Rows {
 // thread reports what does not fit.
 __device__ __forceinline__ Rows rows_of(const int* q_start, const int* q_len, int s, int T, int most, int* status) {
   const int start = q_start[s], n = max(q_len[s], 0);
-  int fit = min(n, most);
-  if (start < 0 || start > T) fit = 0;
-  fit = min(fit, T - start);
+  const int fit = start < 0 || start > T ? 0 : min(min(n, most), T - start);
   if (fit < n && threadIdx.x == 0) record_status_detail(status, kStatusBadIndex, 9, s, start < 0 || start > T ? start : n);
   return {start, fit};
 }

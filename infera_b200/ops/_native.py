@@ -138,8 +138,7 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
         "ib_kv_compact": [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_int, c_int,
                           c_vp, c_vp, c_int, c_vp, c_vp],
         "ib_attn_tree": [c_vp, c_int, c_int, c_vp, c_vp, c_ll, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp,
-                         c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp,
-                         c_vp],
+                         c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
         "ib_tree_mask": [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp],
         "ib_tree_accept": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp],
         "ib_gemm_set_trace": [c_vp],

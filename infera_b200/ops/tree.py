@@ -83,8 +83,7 @@ def tree_accept(tokens: torch.Tensor, target: torch.Tensor, parents: torch.Tenso
     if most < 1:
         raise ValueError(f"a path of at most {most} nodes")
     path = torch.empty(n, most, dtype=_I32, device=tokens.device)
-    both = torch.empty(2, n, dtype=_I32, device=tokens.device)
-    count, after = both[0], both[1]
+    count, after = torch.empty(2, n, dtype=_I32, device=tokens.device).unbind()
     if n == 0:
         return path, count, after
     if dev < 0:
@@ -113,18 +112,18 @@ def tree_accept(tokens: torch.Tensor, target: torch.Tensor, parents: torch.Tenso
 
 
 @lru_cache(maxsize=256)
-def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: int, num_sms: int) -> tuple[int, int]:
+def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: int, num_sms: int) -> tuple[int, bool]:
     per_item = 128 // group
     units = [3 + (-(-c // 64) or 1) for c in ctx_lens]  # an item's start and end cost some three tiles
     items = [-(-n // per_item) for n in q_lens]
     total = hkv * sum(i * u for i, u in zip(items, units))
     top, levels = max((u for i, u in zip(items, units) if i), default=4), max(1, max(items))
     ctas = max(1, min(2 * num_sms // levels * levels or levels, -(-total // 5)))
-    return ctas, 1 if top <= UNCUT + 3 else -(-top * ctas // total) + 1
+    return ctas, top > UNCUT + 3
 
 
-def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, int]:
-    """(CTAs, most pieces of an item) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each 128 rows of
+def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, bool]:
+    """(CTAs, whether an item may be shared by several) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each 128 rows of
     the longest tree, at least two tiles of 64 keys each; contexts of up to :data:`UNCUT` tiles are not cut."""
     return _plan(tuple(q_lens), tuple(ctx_lens), hq // hkv, hkv, num_sms)
 
@@ -132,7 +131,7 @@ def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms
 def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
               q_start: torch.Tensor, q_len: torch.Tensor, ctx_len: torch.Tensor, mask: torch.Tensor, hq: int, hkv: int,
               scale: float, out: torch.Tensor | None = None, host_meta: tuple[list[int], list[int]] | None = None,
-              bt_rows: torch.Tensor | None = None, plan: tuple[int, int] | None = None) -> torch.Tensor:
+              bt_rows: torch.Tensor | None = None, plan: tuple[int, bool] | None = None) -> torch.Tensor:
     """Attention of the nodes of trees whose K/V already sit in the bf16 cache. q: [T, >=hq*128] bf16; q_start / q_len
     / ctx_len: int32 [sequences], as of :func:`infera_b200.ops.kernels.attn_prefill`: a sequence's last ``q_len`` of
     ``ctx_len`` keys are its nodes, in order. A node sees all keys before them and the nodes whose bits ``mask`` int32
@@ -192,14 +191,14 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
         _attn_tree_cpu(q, k_cache, v_cache, block_table, q_start.tolist(), q_lens, ctx_lens, mask, hq, hkv, scale, out,
                        bt_rows)
         return out
-    ctas, splits = plan or tree_plan(q_lens, ctx_lens, hq, hkv, K._num_sms())
-    if splits < 1 or ctas < 1:
-        raise ValueError(f"plan {ctas}, {splits}")
+    ctas, cut = plan or tree_plan(q_lens, ctx_lens, hq, hkv, K._num_sms())
+    if not 1 <= ctas <= 65535:
+        raise ValueError(f"a plan of {ctas} CTAs")
     part = lse = pieces = None
-    if splits > 1:
+    if cut:
         # partials of this call: its own memory, so that calls on several streams and captured graphs share none
-        m = T * hq * splits
-        ws = torch.empty(m * (HEAD_DIM + 1) + n * hkv * -(-most // (128 // (hq // hkv))), dtype=torch.float32,
+        m = 2 * ctas * 128
+        ws = torch.empty(m * (HEAD_DIM + 1) + 2 * n * hkv * -(-most // (128 // (hq // hkv))), dtype=torch.float32,
                          device=q.device)
         part = ws.data_ptr()
         lse = part + 4 * m * HEAD_DIM
@@ -208,10 +207,10 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     rc = _native.kernels().ib_attn_tree(q.data_ptr(), T, ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
                                         q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), mask.data_ptr(),
                                         words, n, most, block_table.data_ptr(), K._ptr(bt_rows), block_table.shape[0],
-                                        places, block_table.stride(0), hq, hkv, scale, ctas, splits, part, lse,
-                                        pieces, out.data_ptr(), ldo, status, stream)
+                                        places, block_table.stride(0), hq, hkv, scale, ctas, part, lse, pieces,
+                                        out.data_ptr(), ldo, status, stream)
     _native.check(rc, "ib_attn_tree")
-    K._count(2 if splits > 1 else 1)
+    K._count(2 if cut else 1)
     return out
 
 

@@ -165,7 +165,8 @@ def test_decode_captured_with_other_lengths_and_into_the_queries():
 
 
 @pytest.mark.parametrize("keep,recent,sink", [(1, 0, 0), (7, 3, 2), (64, 64, 0), (64, 0, 64), (64, 8, 4), (3000, 100, 16)])
-@pytest.mark.parametrize("lens,hkv", [([1, 64, 0, 65, 100], 2), ([5000, 2999, 3001], 2), ([40001], 8), ([2048] * 20, 4)])
+@pytest.mark.parametrize("lens,hkv", [([1, 64, 0, 65, 100], 2), ([5000, 2999, 3001], 2), ([40001], 8), ([2048] * 20, 4),
+                                      ([50001] + [100] * 79, 1)])
 def test_selection(lens, hkv, keep, recent, sink):
     g = torch.Generator().manual_seed(keep + len(lens))
     cap = max(lens) + 5

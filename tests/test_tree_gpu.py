@@ -120,7 +120,7 @@ CASES = {
 }
 
 
-@pytest.mark.parametrize("plan", [None, (300, 1), (1, 3), (2, 9), (31, 5), (300, 40)])
+@pytest.mark.parametrize("plan", [None, (300, False), (7, False), (1, True), (2, True), (31, True), (300, True)])
 @pytest.mark.parametrize("name", CASES)
 def test_attention(name, plan):
     n, ctx, hq, hkv, words = CASES[name]
@@ -147,7 +147,7 @@ def test_any_mask_scale_and_stride(runs, scale):
 
 
 @pytest.mark.parametrize("n,hq", [(20, 4), (40, 4)])
-@pytest.mark.parametrize("plan", [(7, 1), (3, 9)])
+@pytest.mark.parametrize("plan", [(7, False), (3, True), (40, True)])
 def test_what_is_masked_may_be_anything(n, hq, plan):
     ctx = 250
     q, k, v, table, mask, masks = batch([n], [ctx], hq, 1, 2, 4)
@@ -179,7 +179,7 @@ def test_scores_of_very_different_size():
     size = torch.linspace(0.1, 40, ctx[0])
     for p in range(ctx[0]):
         k[int(table[0, p // 16]) * 16 + p % 16] *= size[p if p % 2 else ctx[0] - 1 - p]
-    for plan in ((2, 1), (9, 9)):
+    for plan in ((2, False), (9, True), (100, True)):
         out = tree.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32([0]), i32(n), i32(ctx), mask.cuda(), hq, 1,
                              SCALE, plan=plan)
         check(out.cpu(), q, k, v, table, masks, n, ctx, hq, 1)
@@ -219,16 +219,13 @@ def test_into_the_queries_and_on_another_stream():
     check(out.cpu()[:, : hq * 128], q, k, v, table, masks, n, ctx, hq, hkv)
 
 
-def test_captured_calls_follow_lengths_and_share_nothing():
+@pytest.mark.parametrize("planned", [[700, 300], [100, 30]])
+def test_captured_calls_follow_lengths_and_share_nothing(planned):
     hq, hkv, n = 8, 2, [20, 12]
-    ctx = [700, 300]
-    q, k, v, table, mask, masks = batch(n, ctx, hq, hkv, 1, 8)
-    wide = torch.zeros(2, 64, dtype=torch.int32)
-    wide[:, : table.shape[1]] = table
-    dev = [x.cuda() for x in (q, k, v, wide)]
-    lens, rows, m = i32(ctx), i32(n), mask.cuda()
-    call = lambda: tree.attn_tree(*dev, i32_starts, rows, lens, m, hq, hkv, SCALE, host_meta=(n, ctx))  # noqa: E731
-    i32_starts = i32(starts(n))
+    q, k, v, table, mask, masks = batch(n, [1300, 300], hq, hkv, 1, 8)
+    dev = [x.cuda() for x in (q, k, v, table)]
+    lens, rows, first, m = i32(planned), i32(n), i32(starts(n)), mask.cuda()
+    call = lambda: tree.attn_tree(*dev, first, rows, lens, m, hq, hkv, SCALE, host_meta=(n, planned))  # noqa: E731
     call()
     graphs = []
     for _ in range(2):
@@ -236,7 +233,7 @@ def test_captured_calls_follow_lengths_and_share_nothing():
         with torch.cuda.graph(graph):
             out = call()
         graphs.append((graph, out))
-    for c, r in (([700, 300], [20, 12]), ([40, 20], [20, 12]), ([520, 7], [17, 7])):
+    for c, r in ((planned, n), ([40, 20], n), ([1300, 300], n), ([520, 7], [17, 7])):
         lens.copy_(i32(c)), rows.copy_(i32(r))
         sub = [masks[s][: r[s]] for s in range(2)]
         streams = [torch.cuda.Stream() for _ in graphs]
@@ -248,6 +245,19 @@ def test_captured_calls_follow_lengths_and_share_nothing():
         for _, out in graphs:
             for s in range(2):
                 check(out.cpu()[20 * s:], q[20 * s:], k, v, table[s:], sub[s:s + 1], r[s:s + 1], c[s:s + 1], hq, hkv)
+    assert status()["code"] == 0
+
+
+def test_many_sequences_of_every_length():
+    # more than a warp's, some without nodes, some without keys of their own
+    g = torch.Generator().manual_seed(3)
+    n = torch.randint(0, 20, (75,), generator=g).tolist()
+    ctx = [m + int(torch.randint(0, 2, (1,), generator=g)) * int(torch.randint(0, 500, (1,), generator=g)) for m in n]
+    q, k, v, table, mask, masks = batch(n, ctx, 16, 1, 1, 9)
+    for plan in (None, (296, True), (5, False)):
+        out = tree.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(starts(n)), i32(n), i32(ctx), mask.cuda(), 16, 1,
+                             SCALE, plan=plan)
+        check(out.cpu(), q, k, v, table, masks, n, ctx, 16, 1)
     assert status()["code"] == 0
 
 
@@ -295,6 +305,27 @@ def test_latent_rows_and_entries_that_do_not_move():
         K.kv_compact(kc, v.cuda(), t.cuda(), i32([bad]), i32([5]), start=None if first is None else i32(first),
                      bt_rows=None if rows is None else i32(rows))
         assert torch.equal(kc.cpu(), k) and status()["code"] == 7
+
+
+@pytest.mark.parametrize("width,layers", [(256, 1), (1024, 3), (576, 2), (4608, 1)])
+def test_long_lists_of_whole_rows(width, layers):
+    g = torch.Generator().manual_seed(width)
+    lens = [1500, 700, 40]
+    table, pool = O.page_table(lens, 5)
+    k = torch.randn(layers, pool * 16, width, generator=g).to(torch.bfloat16)
+    v = torch.randn(layers, pool * 16, width, generator=g).to(torch.bfloat16) if width % 128 == 0 else torch.zeros(1, 1, 1).to(torch.bfloat16).expand(layers, 1, 1).contiguous()
+    src, start = torch.full((3, 600), -1, dtype=torch.int32), [3, 0, 17]
+    count = [600, 333, 23]
+    for s in range(3):
+        src[s, : count[s]] = torch.randperm(lens[s] - start[s], generator=g)[: count[s]].sort().values.to(torch.int32)
+    want_k, want_v = k, v
+    for s in range(3):
+        want_k = O.moved(want_k, table[s], src[s, : count[s]].tolist(), start[s], width, 0)
+        if v.shape == k.shape:
+            want_v = O.moved(want_v, table[s], src[s, : count[s]].tolist(), start[s], width, 0)
+    kc, vc = k.cuda(), v.cuda()
+    K.kv_compact(kc, vc, table.cuda(), src.cuda(), i32(count), start=i32(start))
+    assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v) and status()["code"] == 0
 
 
 def test_a_whole_step():
