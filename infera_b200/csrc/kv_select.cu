@@ -9,6 +9,11 @@
 // writes the places, each behind what lies before it. A cluster of CTAs shares a
 // list: each takes a run of places and adds up the others' histograms through
 // distributed shared memory.
+// Bound by its chain of steps (load, three digits, count, write, a barrier or two
+// after each) and, for long runs, by some 120 instructions for 32 weights: 8 lists
+// of 1025 weights 8.2 us, 96 ragged ones up to 9000 13.5, 32 of 100001 by clusters
+// of four 27 (12.8 MB of weights). Four copies of the first histogram against
+// equal exponents were slower (42 us: the others' are read through the cluster).
 //
 // The moves: rows src[i] -> i of a sequence's places, in place. src[i] >= i, so
 // a row is never written before a row that is read later lies there: places are
@@ -21,6 +26,11 @@
 //   batch_kernel   short lists over many layers (the accepted path of a tree):
 //                  the moves are listed once, and rows of several layers are
 //                  held in registers at a time
+// Long lists are bound by HBM: 8192 rows of 32 lists, K and V, 268 MB read and
+// written, 47 us (5.7 TB/s, 0.89 of the copy rate), 2048 rows of 56 lists 22 us (4.5
+// TB/s). Moved in batches of rows held in registers they took 79 and 37 us. The
+// accepted rows of 48 trees in 80 layers (35 MB in pieces of 2 KB) take 14 us: the
+// chain count, entry, page, row, and rows of 160 layers far apart.
 #include <cooperative_groups.h>
 
 #include <algorithm>
