@@ -689,36 +689,49 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
   }
 }
 
-// Merge the pieces of cut items, W warps a row (a lane has 4 dims),
+// Merge the pieces of cut items,
 //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M)
-// a warp's first AHEAD pieces at a time under way.
-template <int W, int ROWS>  // rows of a block, W warps each
-__global__ void __launch_bounds__(W * ROWS * 32) merge_kernel(const __grid_constant__ Params p) {
-  constexpr int AHEAD = 4;
+// LANES lanes a row, which have 4 dims of each 4 LANES, and W warps that share a row's pieces.
+template <int LANES, int W>
+__global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params p) {
+  constexpr int V = 32 / LANES;              // float4s a lane
+  constexpr int ROWS = 8 / W * V;            // of a block
+  constexpr int AHEAD = W > 1 ? 4 : 2;       // pieces under way
+  static_assert(W == 1 || (W == 8 && V == 1), "the barrier below is the row's");
   pdl_trigger();
   pdl_wait();
   const int item = blockIdx.x, s = item / (p.hkv * p.blocks), kvh = item / p.blocks % p.hkv, block = item % p.blocks;
   const int2 pc = p.pieces[item];  // (of an item that there is)
   const Seq sq = sequence(p, s, nullptr);
-  const int lane = threadIdx.x & 31, w0 = (threadIdx.x >> 5) % W, r = blockIdx.y * ROWS + (threadIdx.x >> 5) / W;
-  const int node = block * p.nodes + r / p.G;
-  if (r >= p.nodes * p.G || node >= sq.n || pc.y <= 1) return;  // (the same for a row's warps)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1);
+  const int w0 = warp % W, r = blockIdx.y * ROWS + warp / W * V + (threadIdx.x & 31) / LANES;
+  const int at = r / p.G, node = block * p.nodes + at;
+  if (at >= p.nodes || node >= sq.n || pc.y <= 1) return;  // (the same for a row's warps)
   auto part = [&](int k) { return (2 * static_cast<size_t>(pc.x + k) + (k == 0)) * BQ + r; };
-  float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f, top = -INFINITY;
+  float num[V][4] = {}, den = 0.f, top = -INFINITY;
   for (int k0 = w0; k0 < pc.y; k0 += AHEAD * W) {
     float lse[AHEAD];
-    float4 o[AHEAD];
+    float4 o[AHEAD][V];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int k = k0 + i * W;
-      lse[i] = k < pc.y ? p.lse_part[part(k)] : -INFINITY;
-      o[i] = k < pc.y ? reinterpret_cast<const float4*>(p.o_part + part(k) * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      lse[i] = -INFINITY;
+      if (k < pc.y) {
+        lse[i] = p.lse_part[part(k)];
+        const float4* src = reinterpret_cast<const float4*>(p.o_part + part(k) * D) + lane;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[i][v] = src[v * LANES];
+      }
     }
-    const float mx = fmaxf(fmaxf(fmaxf(lse[0], lse[1]), fmaxf(lse[2], lse[3])), top);
+    float mx = top;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) mx = fmaxf(mx, lse[i]);
     const float f = top == -INFINITY ? 0.f : exp2f(top - mx);
     den *= f;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) num[d] *= f;
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) num[v][d] *= f;
     top = mx;
     const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
@@ -726,42 +739,42 @@ __global__ void __launch_bounds__(W * ROWS * 32) merge_kernel(const __grid_const
       if (lse[i] == -INFINITY) continue;  // (a piece without keys wrote no more)
       const float w = fmaxf(exp2f(lse[i] - ref), FLT_MIN);  // (a NaN in a piece stays one)
       den += w;
-      num[0] += o[i].x * w;
-      num[1] += o[i].y * w;
-      num[2] += o[i].z * w;
-      num[3] += o[i].w * w;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        num[v][0] += o[i][v].x * w;
+        num[v][1] += o[i][v].y * w;
+        num[v][2] += o[i][v].z * w;
+        num[v][3] += o[i][v].w * w;
+      }
     }
   }
   if constexpr (W > 1) {
-    __shared__ float4 s_num[ROWS][W][32];
-    __shared__ float2 s_den[ROWS][W];
-    const int i = (threadIdx.x >> 5) / W;
-    s_num[i][w0][lane] = make_float4(num[0], num[1], num[2], num[3]);
-    if (lane == 0) s_den[i][w0] = make_float2(top, den);
-    static_assert(ROWS == 1, "the barrier below is the row's");
+    __shared__ float4 s_num[W][32];
+    __shared__ float2 s_den[W];
+    s_num[w0][lane] = make_float4(num[0][0], num[0][1], num[0][2], num[0][3]);
+    if (lane == 0) s_den[w0] = make_float2(top, den);
     __syncthreads();
     if (w0 != 0) return;
     float mx = -INFINITY;
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_den[i][w].x);
-    den = num[0] = num[1] = num[2] = num[3] = 0.f;
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_den[w].x);
+    den = num[0][0] = num[0][1] = num[0][2] = num[0][3] = 0.f;
     for (int w = 0; w < W; ++w) {
-      const float2 td = s_den[i][w];
+      const float2 td = s_den[w];
       if (td.x == -INFINITY && td.y == 0.f) continue;
       const float f = fmaxf(exp2f(td.x - mx), FLT_MIN);
-      const float4 v = s_num[i][w][lane];
+      const float4 v = s_num[w][lane];
       den += td.y * f;
-      num[0] += v.x * f;
-      num[1] += v.y * f;
-      num[2] += v.z * f;
-      num[3] += v.w * f;
+      num[0][0] += v.x * f;
+      num[0][1] += v.y * f;
+      num[0][2] += v.z * f;
+      num[0][3] += v.w * f;
     }
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  const int head = kvh * p.G + r % p.G;
-  uint2 w;
-  w.x = pack_bf16(num[0] * inv, num[1] * inv);
-  w.y = pack_bf16(num[2] * inv, num[3] * inv);
-  reinterpret_cast<uint2*>(p.out + static_cast<size_t>(sq.start + node) * p.ldo + head * D)[lane] = w;
+  uint2* dst = reinterpret_cast<uint2*>(p.out + static_cast<size_t>(sq.start + node) * p.ldo + (kvh * p.G + r - at * p.G) * D) + lane;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    dst[v * LANES] = make_uint2(pack_bf16(num[v][0] * inv, num[v][1] * inv), pack_bf16(num[v][2] * inv, num[v][3] * inv));
 }
 
 }  // namespace atree
@@ -845,9 +858,9 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     const unsigned items = static_cast<unsigned>(n_seqs) * hkv * p.blocks;
     // few items have many pieces: a block a row then (61 nodes of 32 heads over 100001 keys, 20 pieces)
     if (p.cut && 4 * items <= static_cast<unsigned>(ctas))
-      e = launch_pdl(merge_kernel<8, 1>, dim3(items, BQ), 256, 0, stream, p);
+      e = launch_pdl(merge_kernel<32, 8>, dim3(items, BQ), 256, 0, stream, p);
     else if (p.cut)
-      e = launch_pdl(merge_kernel<1, 8>, dim3(items, BQ / 8), 256, 0, stream, p);
+      e = launch_pdl(merge_kernel<8, 1>, dim3(items, BQ / 32), 256, 0, stream, p);
     return static_cast<int>(e);
   } catch (...) {  // (no memory for a tensor map's entry)
     return -3;
