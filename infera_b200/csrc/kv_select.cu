@@ -68,15 +68,12 @@ struct SelectParams {
   int* status;
 };
 
-// An unsigned number in the order of the weights: a NaN below all, -0 as 0; and back.
+// An unsigned number in the order of the weights: a NaN below all, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
   uint32_t u = __float_as_uint(x);
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
   if ((u << 1) == 0u) u = 0u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float weight_of(uint32_t k) {
-  return k == 0u ? NAN : __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
 // CACHED: a CTA's run of places fits into its shared memory; else they are read
@@ -154,6 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_kernel(const S
   struct Keys {
     uint32_t k[4];
   };
+  auto key = [&](int i, float v) { return i < lo || i >= hi ? STAYS : order_of(v); };
   // What lies before and behind the middle stays: above every weight's number.
   auto keys_of = [&](int i, const float4& v) -> Keys {
     Keys q{{order_of(v.x), order_of(v.y), order_of(v.z), order_of(v.w)}};
@@ -257,18 +255,40 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_kernel(const S
     known |= ((1u << bits) - 1) << shift;
   }
   if (known == 0) prefix = STAYS - 1;  // above the number of every weight
-  // places above the threshold, and at it, of which the first `want` stay
+  // A warp's places above the threshold, and at it, of which the list's first `want` stay: counted, and listed over
+  // the weights that have been looked at.
   uint32_t gt = 0, eq = 0;
-  for (int i = w0 + 4 * lane; i < w1; i += 128) {
-    const Keys k = keys(i);
+  uint32_t* listed = CACHED ? cached + (w0 - first) : nullptr;
+  const uint32_t below = (1u << lane) - 1;
+  uint32_t on = 0;
+  constexpr int GROUPS = 4;  // of 32 places whose loads are under way together
+  for (int i0 = w0; i0 < w1; i0 += 32 * GROUPS) {
+    uint32_t k[GROUPS];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      gt += k.k[c] > prefix && i + c < w1;
-      eq += k.k[c] == prefix && i + c < w1;
+    for (int a = 0; a < GROUPS; ++a) {
+      const int i = i0 + 32 * a + lane;
+      k[a] = 0;
+      if (i < w1) {
+        if constexpr (CACHED)
+          k[a] = cached[i - first];
+        else
+          k[a] = key(i, x[i]);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < GROUPS; ++a) {
+      const int i = i0 + 32 * a + lane;
+      const bool is = k[a] >= prefix && i < w1;
+      const uint32_t all_on = __ballot_sync(0xffffffffu, is);
+      if constexpr (CACHED)
+        if (is) listed[on + __popc(all_on & below)] = static_cast<uint32_t>(i);
+      on += __popc(all_on);
+      eq += is && k[a] == prefix;
     }
   }
-  gt = __reduce_add_sync(0xffffffffu, gt);
   eq = __reduce_add_sync(0xffffffffu, eq);
+  gt = on - eq;
+  const int n_listed = CACHED ? static_cast<int>(on) : w1 - w0;
   if (lane == 0) {
     wgt[warp] = gt;
     weq[warp] = eq;
@@ -292,37 +312,29 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_kernel(const S
     eq += __reduce_add_sync(0xffffffffu, b);
   }
   // a place goes behind all that stay before it
-  for (int i0 = w0; i0 < w1; i0 += 128) {
-    const int i = i0 + 4 * lane;
-    const Keys k = i < w1 ? keys(i) : Keys{};
-    uint32_t mine = 0;  // above the threshold in the low half, at it in the high one
+  for (int j0 = 0; j0 < n_listed; j0 += 32 * GROUPS) {
+    int place[GROUPS];
+    float v[GROUPS];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (i + c < w1) mine += (k.k[c] > prefix ? 1u : 0u) + (k.k[c] == prefix ? 0x10000u : 0u);
-    uint32_t sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
+    for (int a = 0; a < GROUPS; ++a) {
+      const int j = j0 + 32 * a + lane;
+      place[a] = j >= n_listed ? -1 : (CACHED ? static_cast<int>(listed[j]) : w0 + j);
+      v[a] = place[a] >= 0 ? x[place[a]] : 0.f;
     }
-    if (mine != 0) {
-      uint32_t g = gt + ((sum - mine) & 0xffffu), e = eq + ((sum - mine) >> 16);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (i + c >= w1) break;
-        const bool above = k.k[c] > prefix, same = k.k[c] == prefix;
-        if (above || (same && e < want)) {
-          const uint32_t to = g + min(e, want);
-          kept[to] = i + c;
-          kept_mass[to] = k.k[c] == STAYS ? x[i + c] : weight_of(k.k[c]);
-        }
-        g += above;
-        e += same;
+    for (int a = 0; a < GROUPS; ++a) {
+      if (j0 + 32 * a >= n_listed) break;
+      const uint32_t k = key(place[a], v[a]);
+      const uint32_t above = __ballot_sync(0xffffffffu, place[a] >= 0 && k > prefix);
+      const uint32_t same = __ballot_sync(0xffffffffu, place[a] >= 0 && k == prefix);
+      const uint32_t e = eq + __popc(same & below), to = gt + __popc(above & below) + min(e, want);
+      if ((above >> lane & 1) != 0 || ((same >> lane & 1) != 0 && e < want)) {
+        kept[to] = place[a];
+        kept_mass[to] = v[a];
       }
+      gt += __popc(above);
+      eq += __popc(same);
     }
-    const uint32_t total = __shfl_sync(0xffffffffu, sum, 31);
-    gt += total & 0xffffu;
-    eq += total >> 16;
   }
   if (C > 1 || p.update) sync_all();  // (no CTA leaves while another reads its totals)
   if (p.update) {
