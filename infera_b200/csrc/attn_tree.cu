@@ -29,20 +29,22 @@
 // such pieces, the end of an item and the beginning of one, so the workspace does
 // not depend on the batch.
 //
-// Up to 128 rows bound by HBM: captured calls of 40 ragged trees of up to 26 nodes
-// (32 heads over 8) over up to 5000 keys on scattered pages take 93 to 96 us, where
-// the bytes need 67: the CTAs read at 7.5 TB/s once they run, 7 us after the
-// launch; the last one ends 12 us after the mean, and the merge of two or three
-// pieces of each item takes 5. More rows are bound by the tensor core's operands:
-// a 128 x 64 tile reads 64 KB of Q and K from shared memory (384 cycles at 128 bytes
-// a cycle, next to 128 for V and 256 for the loads), and two CTAs need 1740 cycles
-// for a tile each where the products alone take 1024: 64 nodes of 64 heads (four
-// items) over 8192 keys, 16 sequences, 290 to 320 us (0.53 to 0.58 of the library's
-// bf16 rate), 61 nodes over 100001 keys 120 to 127 us. 8 nodes over 508 keys take 12
-// us: 4 to the first scores, 0.6 a tile, the merge's launch or eight tiles.
-// Tried and no faster: two query tiles a CTA that share the ring, with one MMA warp
-// or two (297 us); 128-key tiles with one pair of query tiles a CTA (321); eight
-// softmax warps a tile with a common maximum (375).
+// Up to 128 rows are bound by HBM: captured calls of 40 ragged trees of up to 26 nodes
+// (32 heads over 8) over up to 5000 keys on scattered pages take 91 us, where the
+// bytes need 67: the CTAs read at 7.5 TB/s once they run, 7 us after the launch; the
+// last one ends 12 us after the mean, and then two or three pieces of each item are
+// merged. With more rows two CTAs take 1640 cycles for a tile each, where their
+// products or their exponentials alone need 1024: a softmax takes 1170 (290 to the
+// maximum, 820 for the weights, with the other CTA's on the same units), and its next
+// scores queue 470 behind the other CTA's products. 64 nodes of 64 heads (four items)
+// over 8192 keys, 16 sequences, take 284 to 330 us (0.51 to 0.6 of the library's bf16
+// rate), 61 nodes over 100001 keys 117 to 128, at 1.4 to 1.5 GHz: the power limit's
+// clock, so that fewer cycles do not show in full. 8 nodes over 508 keys take 12 us:
+// 4 to the first scores, 0.6 a tile, the merge's launch or eight tiles.
+// Tried and no faster (the 16 sequences): two query tiles a CTA that share the ring,
+// with one MMA warp or two (297 us); 128-key tiles, one CTA to an SM (321) or two
+// (337); eight softmax warps a tile with a common maximum (375); all of Q (352) or
+// half of it (298, 1810 cycles) in tensor memory, with one S buffer.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -691,7 +693,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 
 // Merge the pieces of cut items,
 //   o = sum_k 2^(lse_k - M) o_k / sum_k 2^(lse_k - M)
-// LANES lanes a row, which have 4 dims of each 4 LANES, and W warps that share a row's pieces.
+// LANES lanes a row, which have 4 dims of each 4 LANES, and W warps that share a row's pieces. With two pieces a
+// row most instructions are the row's, not the pieces', so 8 lanes take a row, and a warp four (65536 rows of 16
+// sequences, 64 nodes, 64 heads: 12 us from cold caches; a warp a row 22).
 template <int LANES, int W>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params p) {
   constexpr int V = 32 / LANES;              // float4s a lane

@@ -5,15 +5,17 @@
 // the largest x (equal ones: the lowest place first), `keep` in all, as places
 // in ascending order. The weights are read once, into shared memory; the
 // threshold is found digit by digit (11, 11 and 10 bits of the weight as an
-// unsigned number of the same order) in histograms; a last pass counts and one
-// writes the places, each behind what lies before it. A cluster of CTAs shares a
+// unsigned number of the same order) in histograms; a last pass lists each warp's
+// places at or above it over the weights, and what is listed and stays is written
+// behind all that lies before it. A cluster of CTAs shares a
 // list: each takes a run of places and adds up the others' histograms through
 // distributed shared memory.
-// Bound by its chain of steps (load, three digits, count, write, a barrier or two
-// after each) and, for long runs, by some 120 instructions for 32 weights: 8 lists
-// of 1025 weights 8.2 us, 96 ragged ones up to 9000 13.5, 32 of 100001 by clusters
-// of four 27 (12.8 MB of weights). Four copies of the first histogram against
-// equal exponents were slower (42 us: the others' are read through the cluster).
+// Bound by its chain of steps (load, three digits, list, write, a barrier or two
+// after each) and, for long runs, by some 90 instructions for 32 weights: 8 lists
+// of 1025 weights 8 us, 96 ragged ones up to 9000 12.5, 32 of 100001 by clusters
+// of four 24 (12.8 MB of weights; 120 instructions and 27 us when one pass counted
+// and another wrote). Four copies of the first histogram against equal exponents
+// were slower (42 us: the others' are read through the cluster).
 //
 // The moves: rows src[i] -> i of a sequence's places, in place. src[i] >= i, so
 // a row is never written before a row that is read later lies there: places are
