@@ -38,7 +38,7 @@
 // maximum, 820 for the weights, with the other CTA's on the same units), and its next
 // scores queue 470 behind the other CTA's products. 64 nodes of 64 heads (four items)
 // over 8192 keys, 16 sequences, take 284 to 330 us (0.51 to 0.6 of the library's bf16
-// rate), 61 nodes over 100001 keys 117 to 128, at 1.4 to 1.5 GHz: the power limit's
+// rate), 61 nodes over 100001 keys 117 to 136, at 1.5 GHz and 990 W: the power limit's
 // clock, so that fewer cycles do not show in full. 8 nodes over 508 keys take 12 us:
 // 4 to the first scores, 0.6 a tile, the merge's launch or eight tiles.
 // Tried and no faster (the 16 sequences): two query tiles a CTA that share the ring,
