@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 #pragma unroll
         for (int i = 0; i < TILE_PAGES; ++i) {
           const int lp = (j_lo + j) * TILE_PAGES + i;
-          next[i] = __ldg(sq.bt + (lp < n_pages ? lp : 0));
+          next[i] = sq.bt[lp < n_pages ? lp : 0];
         }
       };
       auto load_tile = [&](int j, const int (&at)[TILE_PAGES], const CUtensorMap* tm1, const CUtensorMap* tm4) {

@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Move
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
       const int e = entry(k, i);
-      v[i] = e < q.count && lane + 32 * i < RW ? __ldg(src + e) : -1;
+      v[i] = e < q.count && lane + 32 * i < RW ? src[e] : -1;
     }
   };
   auto load_pages = [&](int k) {
@@ -442,8 +442,8 @@ __global__ void __launch_bounds__(STREAM_WARPS * 32, 2) stream_kernel(const Move
       at[i] = moves_at(p, q, s, e, v[i]) ? v[i] : -1;
       ga[i] = gb[i] = 0;
       if (at[i] >= 0) {
-        ga[i] = __ldg(q.bt + (q.start + at[i]) / kv8::PAGE);
-        gb[i] = __ldg(q.bt + (q.start + e) / kv8::PAGE);
+        ga[i] = q.bt[(q.start + at[i]) / kv8::PAGE];
+        gb[i] = q.bt[(q.start + e) / kv8::PAGE];
       }
     }
   };
@@ -665,6 +665,7 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
     p.shared = heads == 1;
     p.width = 256;
     p.heads = row_bytes / 256;
+    if (static_cast<long long>(n) * p.heads > INT32_MAX) return -1;
     const long long lists = static_cast<long long>(n) * p.heads * channels * layers;
     // a CTA moves some 50 GB/s: where the lists are few, two or four share their columns
     p.parts = lists >= 2 * num_sms ? 1 : (2 * lists >= 2 * num_sms ? 2 : 4);

@@ -69,6 +69,8 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     if len(shape) not in (2, 3) or v_cache.dim() != len(shape) or shape[-2] < PAGE or shape[-2] % PAGE:
         raise ValueError(f"caches {tuple(shape)} and {tuple(v_cache.shape)}: [(layers,) slots, width], whole pages of "
                          f"{PAGE} slots")
+    if not two and v_cache.shape[-2:] != (1, 1):  # (a latent cache's V is a placeholder)
+        raise ValueError(f"caches {tuple(shape)} and {tuple(v_cache.shape)}: K and V differ")
     if not k_cache.is_contiguous() or (two and not v_cache.is_contiguous()):
         raise ValueError("the caches have to be contiguous")
     if v_cache.get_device() != dev:

@@ -148,6 +148,7 @@ def test_moves_of_a_latent_cache_and_refusals():
                           (dict(k_cache=kc.float(), v_cache=vc.float()), ValueError), (dict(src=i32([1])), ValueError),
                           (dict(src=torch.tensor([[1]])), ValueError), (dict(count=i32([1, 1])), ValueError),
                           (dict(start=i32([1, 2])), ValueError), (dict(src=i32([[[1]] * 3])), ValueError),
-                          (dict(k_cache=kc[:-1], v_cache=vc[:-1]), ValueError), (dict(block_table=table[:0]), ValueError)]:
+                          (dict(k_cache=kc[:-1], v_cache=vc[:-1]), ValueError), (dict(block_table=table[:0]), ValueError),
+                          (dict(v_cache=vc[:-16]), ValueError), (dict(v_cache=vc[:, :64]), ValueError)]:
         with pytest.raises(error):
             K.kv_compact(**{**good, **change})
