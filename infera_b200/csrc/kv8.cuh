@@ -1,7 +1,7 @@
 // What the kernels of the 8-bit KV cache share: e4m3 conversions, powers of
 // two, the exponents of pages, and the merge of key shares. The attention
 // kernels of the bf16 cache that came after them use the tcgen05 issue, the
-// page checks and the merge too.
+// page checks and the reductions too.
 #pragma once
 
 #include <cuda_bf16.h>
