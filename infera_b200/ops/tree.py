@@ -117,14 +117,15 @@ def _plan(q_lens: tuple[int, ...], ctx_lens: tuple[int, ...], group: int, hkv: i
     units = [3 + (-(-c // 64) or 1) for c in ctx_lens]  # an item's start and end cost some three tiles
     items = [-(-n // per_item) for n in q_lens]
     total = hkv * sum(i * u for i, u in zip(items, units))
-    top, levels = max((u for i, u in zip(items, units) if i), default=4), max(1, max(items))
+    top, levels = max((u for i, u in zip(items, units) if i), default=4), max(1, max(items, default=1))
     ctas = max(1, min(2 * num_sms // levels * levels or levels, -(-total // 5)))
     return ctas, top > UNCUT + 3
 
 
 def tree_plan(q_lens: list[int], ctx_lens: list[int], hq: int, hkv: int, num_sms: int = 148) -> tuple[int, bool]:
-    """(CTAs, whether an item may be shared by several) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each 128 rows of
-    the longest tree, at least two tiles of 64 keys each; contexts of up to :data:`UNCUT` tiles are not cut."""
+    """(CTAs, whether several may share an item) of :func:`attn_tree`: one wave of two CTAs to an SM, as many for each
+    128 rows of the longest tree, at least two tiles of 64 keys each; contexts of up to :data:`UNCUT` tiles are not
+    cut."""
     return _plan(tuple(q_lens), tuple(ctx_lens), hq // hkv, hkv, num_sms)
 
 
