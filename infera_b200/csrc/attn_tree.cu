@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     float l_run = 0.f;
     for (int j = done; j < done + nk && ok; ++j) {
       const int k0 = (j_lo + j - done) * BKV;
-      const bool edge = k0 + BKV > sq.base;              // the tile has nodes, or ends behind the sequence
+      // the tile has nodes, or ends behind the sequence (whose nodes lie behind its keys where the table cuts it)
+      const bool edge = k0 + BKV > min(sq.base, sq.ctx);
       if (!mbar_wait_warp(&s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, p.status,
                           kStatusTimeoutTmemFull)) {
         ok = false;
