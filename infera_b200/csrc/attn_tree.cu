@@ -49,6 +49,7 @@
 
 #include "kv8.cuh"
 #include "tma_host.h"
+#include "tree_pieces.h"
 
 namespace ib200 {
 namespace atree {
@@ -95,6 +96,7 @@ struct Params {
   int hq, hkv, G, nodes;   // nodes: of an item, 128 / G
   int blocks;              // items of the longest tree and KV head
   bool cut;                // items may be cut; else one goes to the run in which it begins
+  int runs;                // CTAs of the first kernel
   float c;                 // |scale| * log2(e)
   uint32_t q_flip, q_keep;
   float* o_part;           // [2 * runs, 128 rows, 128]: of run w the piece that an item begins with in 2 w + 1, another in 2 w
@@ -711,8 +713,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LANES - 1);
   const int w0 = warp % W, r = blockIdx.y * ROWS + warp / W * V + (threadIdx.x & 31) / LANES;
   const int at = r / p.G, node = block * p.nodes + at;
-  if (at >= p.nodes || node >= sq.n || pc.y <= 1) return;  // (the same for a row's warps)
-  auto part = [&](int k) { return (2 * static_cast<size_t>(pc.x + k) + (k == 0)) * BQ + r; };
+  if (at >= p.nodes || node >= sq.n || pc.y <= 1 || !pieces_exist(pc.x, pc.y, p.runs)) return;  // (the same for a row's warps)
+  auto part = [&](int k) { return static_cast<size_t>(piece_at(pc.x, k)) * BQ + r; };
   float num[V][4] = {}, den = 0.f, top = -INFINITY;
   for (int k0 = w0; k0 < pc.y; k0 += AHEAD * W) {
     float lse[AHEAD];
@@ -840,6 +842,7 @@ extern "C" int ib_attn_tree(const void* q, int T, int ldq, const void* k_cache, 
     p.blocks = (max_nodes + p.nodes - 1) / p.nodes;
     p.n_seqs = n_seqs;
     p.cut = o_part != nullptr;
+    p.runs = ctas;
     p.pieces = reinterpret_cast<int2*>(pieces);
     p.c = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);  // positive: masked scores are -inf times it
     p.q_flip = scale < 0.f ? 0x80008000u : 0u;
