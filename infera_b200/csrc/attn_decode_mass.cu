@@ -64,6 +64,9 @@ constexpr int SMEM_BYTES = 1024 + SLOTS * TILE + 2 * QBLK + 2 * PBLK + 1024;
 constexpr uint32_t TMEM_COLS = 64;   // S0 [0,16) S1 [16,32) O [32,48)
 constexpr uint32_t O_COL = 32;
 constexpr float kLagLog2 = 8.0f;     // the running maximum may lag by this much
+// Weights that meet V, and their sums, carry a factor of 2^-32, which divides out: 2^24 of the lagging ones times bf16's
+// largest value are numbers of 32 bits.
+constexpr float kDown = 1.0f / 4294967296.0f;
 constexpr int FIN_THREADS = 256;
 constexpr int FIN_KEYS = 1024;       // keys of a block of the second kernel
 
@@ -82,7 +85,7 @@ struct Params {
   float* scores;                // [B, hkv, keys, GP] raw scores
   long long keys;
   float* o_part;                // [B, hq, splits, D], not divided by the sum
-  float2* ml;                   // [B, hq, splits] maximum (log2 units) and sum; (-inf, 0): no keys
+  float2* ml;                   // [B, hq, splits] maximum (log2 units) and sum (with kDown); (-inf, 0): no keys
   float* mass;                  // [mass_rows, hkv, cap]
   int mass_rows;
   long long cap;
@@ -165,7 +168,7 @@ __device__ __forceinline__ int covered(const Params& p, const Seq& sq) {
   return static_cast<int>(
       min(static_cast<long long>(sq.len), static_cast<long long>(p.splits) * p.tiles_per_split * BKV));
 }
-// M and 1 / L of the group's heads.
+// M and 1 / L of the group's heads (L with the factor kDown).
 template <int N>
 __device__ __forceinline__ void make_sums(const Params& p, int b, int kvh, float* s_m, float* s_inv) {
   const int lane = threadIdx.x & 31;
@@ -232,7 +235,7 @@ __device__ __forceinline__ void add_mass(const Params& p, const Seq& sq, int b, 
 #pragma unroll
   for (int h = 0; h < GP; ++h) {
     m[h] = h < G ? s_m[h] : 0.f;
-    inv[h] = h < G ? s_inv[h] : 0.f;
+    inv[h] = h < G ? s_inv[h] * kDown : 0.f;
   }
   const float* scores = p.scores + (static_cast<size_t>(b) * p.hkv + kvh) * static_cast<size_t>(p.keys) * GP;
   float* mass = p.mass + (static_cast<size_t>(sq.row) * p.hkv + kvh) * static_cast<size_t>(p.cap);
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       for (int i = 0; i < 4 * NC; ++i) d[i] = 0u;
 #pragma unroll
       for (int h = 0; h < GP; ++h) {
-        const float w = exp2f(fmaf(x[h], p.c, -m_run[h]));
+        const float w = exp2f(fmaf(x[h], p.c, -m_run[h])) * kDown;
         l_part[h] += w;
         const __nv_bfloat16 hi = __float2bfloat16(w);
         const __nv_bfloat16 lo = __float2bfloat16(w - __bfloat162float(hi));

@@ -2,7 +2,7 @@
 // bf16 paged KV cache, on tcgen05. A sequence's last q_len keys are its nodes;
 // node i sees the keys before them and node j where bit j of its mask is set.
 //
-//   S = Q K^T, O += W V,  w = 2^(c s - m) in bf16 (rounded, by up to 2^-8 of
+//   S = Q K^T, O += W V,  w = 2^(c s - m - 32) in bf16 (rounded, by up to 2^-8 of
 //   itself, as in the prompt kernel), the sum of the softmax over the fp32 weights
 //
 // The query heads of a KV head are packed: rows are (node, head) pairs. A CTA
@@ -76,6 +76,9 @@ constexpr int SMEM_BYTES = 1024 + 2 * QBLK + SLOTS * TILE;  // barriers in the f
 constexpr uint32_t TMEM_COLS = 256;   // S0 [0,64) S1 [64,128), W over them; O [128,256)
 constexpr uint32_t O_COL = 128;
 constexpr float kLagLog2 = 8.0f;      // the running maximum may lag by this much
+// Weights carry a factor of 2^-32, and a merge's one of 2^-16: 2^24 of the lagging ones, and 2^16 pieces, times bf16's
+// largest value are numbers of 32 bits. The sums carry it too, so it divides out (bf16 has the exponents for it).
+constexpr float kDownLog2 = 32.0f, kUp = 4294967296.0f, kMergeDownLog2 = 16.0f;
 constexpr int kStart = 3;             // what an item's start and end cost, in key tiles
 
 struct Params {
@@ -620,8 +623,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
           m_run = m_use;
         }
         const float m_ref = m_run == -INFINITY ? 0.f : m_run;
-        // w = 2^(c s - m) as bf16 pairs over the S columns just read
-        const uint64_t c2 = f2pack(p.c, p.c), b2 = f2pack(-m_ref, -m_ref);
+        // w = 2^(c s - m - 32) as bf16 pairs over the S columns just read
+        const uint64_t c2 = f2pack(p.c, p.c), b2 = f2pack(-m_ref - kDownLog2, -m_ref - kDownLog2);
         uint64_t l2[2] = {f2pack(0.f, 0.f), f2pack(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < BKV; i += 2) {
@@ -647,7 +650,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
     if (ok) {
       const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;   // a NaN stays one
       const bool merge = pieces > 1;
-      if (merge && live) p.lse_part[part] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run);
+      if (merge && live) p.lse_part[part] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run * kUp);
 #pragma unroll 1
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t o[32];
@@ -740,7 +743,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 #pragma unroll
       for (int d = 0; d < 4; ++d) num[v][d] *= f;
     top = mx;
-    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float ref = mx == -INFINITY ? 0.f : mx + kMergeDownLog2;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (lse[i] == -INFINITY) continue;  // (a piece without keys wrote no more)

@@ -29,3 +29,23 @@ def test_a_context_beyond_the_table_is_cut(pages, over, plan):
     seen = O.seen_of(masks[1], 6, ctx[1])[:, :room]
     want, bound, _, _ = O.attend(q[5:11, : hq * 128], kk, vv, seen, hq, hkv, SCALE, W_STEP)
     O.close(out[5:11], want, bound)
+
+
+@pytest.mark.parametrize("n,ctx", [(20, 260), (200, 700)])
+def test_values_near_the_largest(n, ctx):
+    """Sums of weighted values stay in range, however far the maximum lags and in however many pieces an item is cut."""
+    hq = 4
+    q, k, v, table, mask, masks = batch([n], [ctx], hq, 1, 8, 3)
+    slot = lambda p: int(table[0, p // 16]) * 16 + p % 16  # noqa: E731
+    for p in range(ctx):  # scores that grow by some 6 in log2 from tile to tile, under the lag
+        k[slot(p), 0] = p / 64
+        v[slot(p), 20] = 3.3e38
+        v[slot(p), 21] = -3.3e38 if p % 3 else 3.3e38
+        v[slot(p), 22] = 3.3e38 if p % 50 == 7 else 1.0
+    for h in range(hq):
+        q[:, 128 * h] = 48
+    args = [x.cuda() for x in (q, k, v, table)] + [i32([0]), i32([n]), i32([ctx]), mask.cuda()]
+    for plan in ((1, True), (2, False), (9, True), (40, True), (290, True)):
+        out = tree.attn_tree(*args, hq, 1, SCALE, plan=plan)
+        check(out.cpu(), q, k, v, table, masks, [n], [ctx], hq, 1)
+    assert status()["code"] == 0
