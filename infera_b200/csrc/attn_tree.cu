@@ -702,6 +702,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 // LANES lanes a row, which have 4 dims of each 4 LANES, and W warps that share a row's pieces. With two pieces a
 // row most instructions are the row's, not the pieces', so 8 lanes take a row, and a warp four (65536 rows of 16
 // sequences, 64 nodes, 64 heads: 12 us from cold caches; a warp a row 22).
+__device__ __forceinline__ float scaled(float x, float w) {  // w x, w >= 0; an infinity or a NaN stays one where w is 0
+  return fabsf(x) <= FLT_MAX ? x * w : x;
+}
 template <int LANES, int W>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params p) {
   constexpr int V = 32 / LANES;              // float4s a lane
@@ -741,20 +744,20 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int d = 0; d < 4; ++d) num[v][d] *= f;
+      for (int d = 0; d < 4; ++d) num[v][d] = scaled(num[v][d], f);
     top = mx;
     const float ref = mx == -INFINITY ? 0.f : mx + kMergeDownLog2;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (lse[i] == -INFINITY) continue;  // (a piece without keys wrote no more)
-      const float w = fmaxf(exp2f(lse[i] - ref), FLT_MIN);  // (a NaN in a piece stays one)
+      const float w = exp2f(lse[i] - ref);
       den += w;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        num[v][0] += o[i][v].x * w;
-        num[v][1] += o[i][v].y * w;
-        num[v][2] += o[i][v].z * w;
-        num[v][3] += o[i][v].w * w;
+        num[v][0] += scaled(o[i][v].x, w);
+        num[v][1] += scaled(o[i][v].y, w);
+        num[v][2] += scaled(o[i][v].z, w);
+        num[v][3] += scaled(o[i][v].w, w);
       }
     }
   }
@@ -771,13 +774,13 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Para
     for (int w = 0; w < W; ++w) {
       const float2 td = s_den[w];
       if (td.x == -INFINITY && td.y == 0.f) continue;
-      const float f = fmaxf(exp2f(td.x - mx), FLT_MIN);
+      const float f = exp2f(td.x - mx);
       const float4 v = s_num[w][lane];
       den += td.y * f;
-      num[0][0] += v.x * f;
-      num[0][1] += v.y * f;
-      num[0][2] += v.z * f;
-      num[0][3] += v.w * f;
+      num[0][0] += scaled(v.x, f);
+      num[0][1] += scaled(v.y, f);
+      num[0][2] += scaled(v.z, f);
+      num[0][3] += scaled(v.w, f);
     }
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;

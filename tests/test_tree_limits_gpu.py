@@ -49,3 +49,28 @@ def test_values_near_the_largest(n, ctx):
         out = tree.attn_tree(*args, hq, 1, SCALE, plan=plan)
         check(out.cpu(), q, k, v, table, masks, [n], [ctx], hq, 1)
     assert status()["code"] == 0
+
+
+@pytest.mark.parametrize("hq", [1, 4])
+def test_infinities_in_items_of_several_pieces(hq):
+    """A value that is not finite stays so however far above its piece's scores those of the pieces behind it are (the
+    weight of the whole piece is then 0 in 32 bits), and finite ones there count nothing."""
+    n, ctx = 256, 1000
+    q, k, v, table, mask, _ = batch([n], [ctx], hq, 1, 8, 2)
+    rows = O.mask_of(list(range(-1, n - 1)), 8)  # a chain: node i sees all nodes before it
+    mask[:n] = rows
+    slot = lambda p: int(table[0, p // 16]) * 16 + p % 16  # noqa: E731
+    base = ctx - n
+    for j, d, x in ((5, 11, float("inf")), (70, 12, float("-inf")), (100, 13, float("nan")), (130, 14, float("inf")), (6, 15, 3e38)):
+        v[slot(base + j), d] = x
+    for h in range(hq):
+        q[:, 128 * h] = 8
+    for p in range(ctx - 60, ctx):  # 300 above the others in log2
+        k[slot(p), 0] = 300
+    kk, vv = (O.rows_of(x, table[0], ctx, 1) for x in (k, v))
+    want, bound, _, _ = O.attend(q[:n, : hq * 128], kk, vv, O.seen_of(rows, n, ctx), hq, 1, SCALE, W_STEP)
+    args = [x.cuda() for x in (q, k, v, table)] + [i32([0]), i32([n]), i32([ctx]), mask.cuda()]
+    for ctas in range(1, 70):
+        out = tree.attn_tree(*args, hq, 1, SCALE, plan=(ctas, True))
+        O.close(out[:n].cpu(), want, bound, f"{ctas} CTAs")
+    assert status()["code"] == 0
