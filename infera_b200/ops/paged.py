@@ -112,13 +112,11 @@ def _kv_compact_cpu(k, v, block_table, src, count, start, bt_rows) -> None:
     (table_rows, places), pages = block_table.shape, k.shape[-2] // PAGE
     heads = src.shape[1] if src.dim() == 3 else 1
     src = src.view(src.shape[0], heads, -1).long()
-    taken: set[int] = set()
-    for s in range(src.shape[0]):
-        row = s if bt_rows is None else int(bt_rows[s])
+    rows = list(range(src.shape[0])) if bt_rows is None else bt_rows.tolist()
+    for s, row in enumerate(rows):
         first = 0 if start is None else int(start[s])
-        if not 0 <= row < table_rows or row in taken or first < 0:
+        if not 0 <= row < table_rows or row in rows[:s] or first < 0:
             continue
-        taken.add(row)
         m = min(max(int(count[s]), 0), src.shape[2])
         for h in range(heads):
             to = torch.arange(m)

@@ -34,3 +34,27 @@ def test_values_near_the_largest(hq):
                                 tiles_per_split=tps)
         check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, 1)
     assert status()["code"] == 0
+
+
+@pytest.mark.parametrize("heads,layers,m", [(1, 3, 9), (2, 1, 70), (1, 2, 100)])
+def test_a_table_row_named_twice_moves_once(heads, layers, m):
+    """By the first sequence that names it, whether that one's rows move or its start is refused."""
+    g = torch.Generator().manual_seed(m)
+    table, pool = O.page_table([300, 200], 5)
+    k, v = (torch.randn(layers, pool * 16, 256, generator=g).to(torch.bfloat16) for _ in range(2))
+    src = torch.stack([torch.randperm(150, generator=g)[:m].sort().values for _ in range(4 * heads)]).to(torch.int32)
+    src = src.view(4, heads, m) if heads > 1 else src
+    for start in ([0, 7, 3, 11], [-1, 7, 3, 11]):
+        want = [k, v]
+        for s, row in ((0, 0), (1, 1)):  # (the third and fourth come after them)
+            for h in range(heads):
+                if start[s] >= 0:
+                    w = 256 // heads
+                    want = [O.moved(x, table[row], src.view(4, heads, m)[s, h].tolist(), start[s], w, h * w) for x in want]
+        for dev in ("cuda", "cpu"):
+            kc, vc = (x.clone().to(dev) for x in (k, v))
+            K.kv_compact(kc, vc, table.to(dev), src.to(dev), torch.full((4,), m, dtype=torch.int32, device=dev),
+                         start=torch.tensor(start, dtype=torch.int32, device=dev),
+                         bt_rows=torch.tensor([0, 1, 0, 1], dtype=torch.int32, device=dev))
+            assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1]), dev
+        assert status()["code"] == 7
