@@ -58,3 +58,46 @@ def test_a_table_row_named_twice_moves_once(heads, layers, m):
                          bt_rows=torch.tensor([0, 1, 0, 1], dtype=torch.int32, device=dev))
             assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1]), dev
         assert status()["code"] == 7
+
+
+def test_fewer_places_in_the_mass_than_keys():
+    """Weights of places that the mass has are added, up to its end and not into the next row; the output is whole."""
+    lens, hq, hkv = [100, 300, 60, 151], 8, 2
+    q, k, v, table, mass = batch(lens, hq, hkv, 4)
+    for splits, tps in ((1, 0), (2, 0), (3, 1)):
+        got = mass[:, :, :150].contiguous().cuda()
+        out = evict.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lens), hq, hkv, SCALE, got, splits,
+                                tiles_per_split=tps).cpu()
+        assert status()["code"] == 7
+        for b, n in enumerate(lens):
+            kk, vv = (O.rows_of(x, table[b], n, hkv) for x in (k, v))
+            want, bound, w, wb = O.attend(q[b:b + 1, : hq * 128], kk, vv, torch.ones(1, n, dtype=torch.bool), hq, hkv, SCALE, W_STEP)
+            O.close(out[b:b + 1], want, bound)
+            cut = min(n, 150)
+            was = mass[b, :, :150].double()
+            bound_m = 2.0 ** -23 * was + 1e-37
+            was[:, :cut] += w[0].view(hkv, -1, n).sum(1)[:, :cut]
+            bound_m[:, :cut] += (wb + 2.0 ** -20 * w)[0].view(hkv, -1, n).sum(1)[:, :cut]
+            O.close(got[b], was, bound_m, f"mass {b}")
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3])
+def test_a_length_beyond_the_table_is_cut(splits):
+    lens, hq, hkv = [100, 304, 60], 4, 1
+    q, k, v, table, mass = batch(lens, hq, hkv, 4)
+    got = mass.cuda()
+    out = evict.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32([100, 5000, 60]), hq, hkv, SCALE, got, splits)
+    assert status()["code"] == 7
+    check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, hkv)
+
+
+@pytest.mark.parametrize("plan", ["plan", (1, 0), (235, 1)])
+def test_long_contexts_of_many_shares(plan):
+    lens, hq, hkv = [30011, 9001], 4, 1
+    q, k, v, table, mass = batch(lens, hq, hkv, 9)
+    splits, tps = evict.decode_plan(2, hkv, max(lens)) if plan == "plan" else plan
+    got = mass.cuda()
+    out = evict.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lens), hq, hkv, SCALE, got, splits,
+                            tiles_per_split=tps)
+    assert status()["code"] == 0
+    check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, hkv)

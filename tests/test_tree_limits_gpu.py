@@ -1,4 +1,5 @@
-"""Tree attention at the ends of its ranges on the GPU."""
+"""Tree attention at the ends of its ranges on the GPU: contexts that the table cuts, more nodes than fit, long contexts,
+values that are huge or not finite."""
 
 import math
 
@@ -74,3 +75,27 @@ def test_infinities_in_items_of_several_pieces(hq):
         out = tree.attn_tree(*args, hq, 1, SCALE, plan=(ctas, True))
         O.close(out[:n].cpu(), want, bound, f"{ctas} CTAs")
     assert status()["code"] == 0
+
+
+def test_more_nodes_than_fit():
+    """The first nodes, as far as the plan's rows and the queries' go, see what they would in the whole tree."""
+    n, ctx, hq = [6, 6, 6], [100, 200, 60], 4
+    q, k, v, table, mask, masks = batch(n, ctx, hq, 1, 1, 6)
+    args = [x.cuda() for x in (q, k, v, table)]
+    out = tree.attn_tree(*args, i32(starts(n)), i32([6, 6, 50]), i32(ctx), mask.cuda(), hq, 1, SCALE, host_meta=(n, ctx)).cpu()
+    assert status()["code"] == 7
+    check(out[:12], q, k, v, table, masks[:2], n[:2], ctx[:2], hq, 1)
+    kk, vv = (O.rows_of(x, table[2], 60, 1) for x in (k, v))
+    seen = O.seen_of(torch.cat([mask[12:], torch.zeros(42, 1, dtype=torch.int32)]), 50, 60)[:8]
+    want, bound, _, _ = O.attend(q[12:, : hq * 128], kk, vv, seen, hq, 1, SCALE, W_STEP)
+    O.close(out[12:], want, bound)
+
+
+@pytest.mark.parametrize("plan", [None, (296, True), (3, False)])
+def test_long_contexts(plan):
+    n, ctx, hq, hkv = [5, 40], [30011, 9001], 4, 1
+    q, k, v, table, mask, masks = batch(n, ctx, hq, hkv, 2, 12)
+    out = tree.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(starts(n)), i32(n), i32(ctx), mask.cuda(), hq, hkv,
+                         SCALE, plan=plan)
+    assert status()["code"] == 0
+    check(out.cpu(), q, k, v, table, masks, n, ctx, hq, hkv)
