@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) select_kernel(const S
     if (tid == 0 && rank == 0) record_status_detail(p.status, kStatusBadIndex, 6, s, static_cast<int>(n_keys));
     n_keys = p.cap;
   }
-  if (!bad && p.update && p.bt_rows != nullptr) {  // a row that an earlier sequence has is that one's to change
+  // a row that an earlier sequence has is that one's to change (those without keys, which pad a batch, may share one)
+  if (!bad && p.update && p.bt_rows != nullptr && n_keys > 0) {
     bool twice = false;
     for (int i = tid; i < s; i += THREADS) twice = twice || p.bt_rows[i] == row;
     if (__syncthreads_or(twice)) {
@@ -379,7 +380,8 @@ __device__ __forceinline__ MoveSeq move_seq(const MoveParams& p, int s) {
     if (threadIdx.x == 0) record_status_detail(p.status, kStatusBadIndex, 1, s, static_cast<int>(q.start));
     q.count = 0;
   }
-  if (p.bt_rows != nullptr) {  // a sequence whose places an earlier one has too stays as that one leaves it
+  // a sequence whose places an earlier one has too stays as that one leaves it (those without moves may share a row)
+  if (p.bt_rows != nullptr && q.count > 0) {
     bool twice = false;
     for (int i = threadIdx.x; i < s; i += blockDim.x) twice = twice || p.bt_rows[i] == row;
     if (__syncthreads_or(twice)) {

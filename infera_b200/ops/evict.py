@@ -70,7 +70,8 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     What the device finds wrong goes to the status word: keys that no split covers (they are left out), a length beyond
     the page table's places (cut there) or beyond ``mass``'s (no weights are added there), a ``bt_rows`` entry that is
     no row of the table (the sequence gets zeros) or of ``mass``, or that an earlier sequence has (both: no weights are
-    added). A page id outside the cache reads as zeros."""
+    added). Sequences of length 0 may share a row with others before them: so a batch is padded. A page id outside the
+    cache reads as zeros."""
     _check_heads(hq, hkv, 8)
     B, dev = seq_lens.shape[0], q.get_device()
     ldq = _check_rows("q", q, B, hq * HEAD_DIM, dev, 4)
@@ -156,7 +157,8 @@ def select_keys(mass: torch.Tensor, seq_lens: torch.Tensor, keep: int, recent: i
     the front, zero behind it.
 
     To the status word: a length beyond ``mass``'s places (cut there), a ``bt_rows`` entry that is no row of ``mass``
-    or, with ``update``, that an earlier sequence has (it keeps nothing)."""
+    or, with ``update``, that an earlier sequence has (it keeps nothing). Sequences of length 0 may share a row with others
+    before them."""
     if mass.dim() != 3:
         raise ValueError(f"mass: [rows, hkv, places], not {tuple(mass.shape)}")
     hkv, n, dev = mass.shape[1], seq_lens.shape[0], mass.get_device()

@@ -780,8 +780,8 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     what else reads them (a shared prefix) sees the moved rows. To the status
     word, and not moved: another entry below its index, one beyond the page
     table's places, a page id outside the cache; a ``bt_rows`` entry that is no
-    row of the table or that an earlier sequence has (whether or not that one's
-    rows move); a negative ``start``."""
+    row of the table, or that an earlier sequence has (whether or not that one's
+    rows move) while this one's ``count`` is not 0; a negative ``start``."""
     from infera_b200.ops import paged
 
     paged.kv_compact(k_cache, v_cache, block_table, src, count, start, bt_rows)

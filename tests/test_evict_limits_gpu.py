@@ -101,3 +101,52 @@ def test_long_contexts_of_many_shares(plan):
                             tiles_per_split=tps)
     assert status()["code"] == 0
     check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, hkv)
+
+
+def test_a_padded_batch():
+    """Sequences of length 0 that pad a batch share one row of the table: a captured eviction step over them reports nothing
+    and leaves the row, and what the others do, alone."""
+    lens, hq, hkv, keep = [200, 90, 150, 64], 4, 2, 60
+    q, k, v, table, mass = batch(lens, hq, hkv, 6)
+    k, v = k.nan_to_num(0.5), v.nan_to_num(0.5)
+    rows = [2, 0, 1, 3, 3, 3]
+    now = [lens[2], lens[0], lens[1], 0, 0, 0]
+    qp = torch.cat([q[rows[:3]], q[:3]])
+    dev = [qp.cuda(), k.cuda(), v.cuda(), table.cuda()]
+    got, lens_d, rows_d = mass.cuda(), i32(now), i32(rows)
+    start = i32([0] * 6)
+
+    def step():
+        out = evict.attn_decode(*dev, lens_d, hq, hkv, SCALE, got, 2, bt_rows=rows_d)
+        kept, _, count = evict.select_keys(got, lens_d, keep, recent=8, sink=2, bt_rows=rows_d, update=True)
+        K.kv_compact(dev[1], dev[2], dev[3], kept, count, start=start, bt_rows=rows_d)  # each KV head's columns by a list
+        K.kv_compact(dev[1], dev[2], dev[3], whole, moved, start=start, bt_rows=rows_d)  # whole rows
+        return out, kept, count
+
+    whole, moved = i32([[3, 9]] * 6), i32([0] * 6)
+    step()
+    assert status()["code"] == 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, kept, count = step()
+    for x, y in zip((dev[1], dev[2], got), (k, v, mass)):
+        x.copy_(y)
+    graph.replay()
+    assert status()["code"] == 0 and count.tolist() == [60, 60, 60, 0, 0, 0] and torch.all(kept[3:] == -1)
+    assert torch.all(out[3:] == 0) and torch.equal(got[3].cpu(), mass[3])
+    want_k, want_v = k, v
+    for s in range(3):
+        n, row = now[s], rows[s]
+        kk, vv = (O.rows_of(x, table[row], n, hkv) for x in (k, v))
+        want, bound, w, wb = O.attend(qp[s:s + 1, : hq * 128], kk, vv, torch.ones(1, n, dtype=torch.bool), hq, hkv, SCALE, W_STEP)
+        O.close(out[s:s + 1], want, bound)
+        was = mass[row, :, :n].double()
+        full = was + w[0].view(hkv, -1, n).sum(1)
+        bound_m = 2.0 ** -23 * was + (wb + 2.0 ** -20 * w)[0].view(hkv, -1, n).sum(1)
+        for h in range(hkv):
+            on = kept[s, h].tolist()
+            assert on[:2] == [0, 1] and on[-8:] == list(range(n - 8, n)) and on == sorted(set(on))
+            O.close(got[row, h, :60], full[h, on], bound_m[h, on])
+            assert torch.all(got[row, h, 60:n] == 0)
+            want_k, want_v = (O.moved(x, table[row], on, 0, 128, 128 * h) for x in (want_k, want_v))
+    assert torch.equal(dev[1].cpu(), want_k) and torch.equal(dev[2].cpu(), want_v)
