@@ -36,7 +36,9 @@
 // scores from L2; of 61 ragged ones up to 12000 keys on scattered pages (32 over
 // 8) 256 us, 240 (0.94) and 15; of one of 100 keys 7.3 us. Finishing in the CTA
 // that ends last in a (sequence, KV head), by a counter, was slower: it streams
-// nothing meanwhile, 12 KB of scores a round trip (287 and 201 us).
+// nothing meanwhile, 12 KB of scores a round trip (287 and 201 us). One sequence of
+// 100000 keys on one KV head (8 heads, 261 shares) takes 45 us, where its bytes need 8:
+// one CTA merges the shares in a loop; on 8 KV heads (64 heads, 36 shares) 78 of 65.
 #include "kv8.cuh"
 #include "tma_host.h"
 

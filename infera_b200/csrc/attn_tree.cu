@@ -5,6 +5,15 @@
 //   S = Q K^T, O += W V,  w = 2^(c s - m - 32) in bf16 (rounded, by up to 2^-8 of
 //   itself, as in the prompt kernel), the sum of the softmax over the fp32 weights
 //
+// One bf16 digit of W is a choice: outputs are off by 0.0020 to 0.0023 in the
+// 2-norm, where rounding the output alone gives 0.0017. A second digit in the
+// other half of S's columns, as the decode kernel with weights has, gives 0.0017
+// and takes 12.6 -> 14.2 us (8 nodes over 508 keys), 90 -> 95 (40 ragged trees),
+// 287 -> 357 (16 x 64 nodes) and 121 -> 148 (61 over 100001): too much for an error
+// that the prompt kernel's rows, which the cache comes from, have too. The sum over
+// the rounded weights gives 0.0033 instead of 0.0048 as the largest error of the 16
+// sequences, and takes 287 -> 315 us.
+//
 // The query heads of a KV head are packed: rows are (node, head) pairs. A CTA
 // takes 128 rows and walks its keys in tiles of 64 (4 pages), 16 KB of K and 16
 // KB of V in a ring of five slots that both take in turn:
@@ -33,12 +42,14 @@
 // (32 heads over 8) over up to 5000 keys on scattered pages take 91 us, where the
 // bytes need 67: the CTAs read at 7.5 TB/s once they run, 7 us after the launch; the
 // last one ends 12 us after the mean, and then two or three pieces of each item are
-// merged. With more rows two CTAs take 1640 cycles for a tile each, where their
-// products or their exponentials alone need 1024: a softmax takes 1170 (290 to the
+// merged. With more rows two CTAs take 1640 cycles for a tile each. Their products or
+// their exponentials alone need 1024, but shared memory 1536: a tile's scores read 48
+// KB of it (8 steps of 4 KB of Q and 2 KB of K), W V 16 KB, and TMA writes 32 KB, at
+// 128 bytes a cycle. A softmax takes 1170 cycles (290 to the
 // maximum, 820 for the weights, with the other CTA's on the same units), and its next
 // scores queue 470 behind the other CTA's products. 64 nodes of 64 heads (four items)
 // over 8192 keys, 16 sequences, take 284 to 330 us (0.51 to 0.6 of the library's bf16
-// rate), 61 nodes over 100001 keys 117 to 136, at 1.5 GHz and 990 W: the power limit's
+// rate), 61 nodes over 100001 keys 117 to 142, at 1.5 GHz and 990 W: the power limit's
 // clock, so that fewer cycles do not show in full. 8 nodes over 508 keys take 12 us:
 // 4 to the first scores, 0.6 a tile, the merge's launch or eight tiles.
 // Tried and no faster (the 16 sequences): two query tiles a CTA that share the ring,

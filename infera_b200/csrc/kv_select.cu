@@ -31,8 +31,9 @@
 // Long lists are bound by HBM: 8192 rows of 32 lists, K and V, 268 MB read and
 // written, 47 us (5.7 TB/s, 0.89 of the copy rate), 2048 rows of 56 lists 22 us (4.5
 // TB/s). Moved in batches of rows held in registers they took 79 and 37 us. The
-// accepted rows of 48 trees in 80 layers (35 MB in pieces of 2 KB) take 14 us: the
-// chain count, entry, page, row, and rows of 160 layers far apart.
+// accepted rows of 48 trees in 80 layers (35 MB in pieces of 2 KB) take 14 us: 1152
+// CTAs are 2.6 waves of those that the SMs hold, and each wave goes through the
+// chain count, entry, page, row, with the rows of 160 layers far apart.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -689,7 +690,8 @@ extern "C" int ib_kv_compact(void* k, void* v, int layers, long long num_slots, 
   p.shared = false;
   p.heads = heads;
   const long long lists = static_cast<long long>(n) * heads * channels;
-  // rows of more than 4 KB in parts; layers in as many groups as give the SMs eight CTAs each
+  // rows of more than 4 KB in parts; layers in as many groups as give each SM eight CTAs, three of which it holds at a
+  // time (75 registers)
   const int pieces = p.width / 16;
   p.parts = (pieces + MOVE_THREADS - 1) / MOVE_THREADS;
   p.lanes = (pieces + p.parts - 1) / p.parts;

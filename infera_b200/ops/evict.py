@@ -1,7 +1,9 @@
 """Eviction from the bf16 paged KV cache by accumulated attention weight.
 
 ``mass`` (fp32 [rows, hkv, places], a row for each row of the page table) holds what each cached key of a sequence has
-received: the softmax weights of a KV head's query heads, summed over the decode steps so far. It starts at zero.
+received: the softmax weights of a KV head's query heads, summed over the decode steps so far. It starts at zero, and
+the prompt calls add nothing to it: until some steps have, all keys of a prompt have the same 0, and of those the lowest
+places stay.
 
 * :func:`attn_decode` attends with one query token per sequence and adds the step's weights to ``mass``
   (:func:`infera_b200.ops.kernels.attn_decode` comes here when it is given ``mass``);
@@ -65,7 +67,8 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     ``splits`` and ``tiles_per_split`` come from :func:`decode_plan`: split s covers the 128-key tiles [s*T, (s+1)*T)
     of every sequence, so ``splits * tiles_per_split * 128`` must cover the longest one (``tiles_per_split=0``: enough
     tiles for every key that the page table has room for). The call keeps the raw scores in a workspace of 4 bytes a
-    key that the splits cover and query head (1, 2, 4 or 8 to a KV head).
+    key that the splits cover and query head (1, 2, 4 or 8 to a KV head), for every sequence as for the longest: 1.6 GB for
+    128 sequences and 32 heads over 8 where one has 100000 keys.
 
     What the device finds wrong goes to the status word: keys that no split covers (they are left out), a length beyond
     the page table's places (cut there) or beyond ``mass``'s (no weights are added there), a ``bt_rows`` entry that is

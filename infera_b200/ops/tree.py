@@ -26,8 +26,10 @@ from infera_b200.ops.kv8 import HEAD_DIM, PAGE, _check_heads, _check_i32, _check
 
 _BF16, _I32 = torch.bfloat16, torch.int32
 MAX_NODES = 256
-# Contexts of up to so many tiles of 64 keys are not cut: 8 nodes of 32 heads over 508 keys take 12 us either way on the
-# GPU, and one launch instead of two.
+# Contexts of up to so many tiles of 64 keys are not cut. Captured, uncut against cut: 8 nodes of 32 heads (over 8) in 6
+# tiles 11.9 against 13.8 us, in 8 13.8 against 13.4, in 10 15.7 against 13.6, in 14 19.4 against 13.6; 40 trees of 16 nodes
+# in 8 tiles 29.3 against 31.3, in 10 33.6 against 33.9, in 14 42.9 against 38.3. (Trees of several items gain from cuts
+# later, 4 of 64 nodes and 64 heads not before 20 tiles, 33.1 against 36.1.) Uncut is also one launch instead of two.
 UNCUT = 10
 
 
@@ -141,13 +143,16 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
 
     ``host_meta`` (q_len, ctx_len on the host; read back from the device without it) sizes the grid and the workspace
     (``plan``: :func:`tree_plan`). In a captured graph the lengths on the device may change from replay to replay: up
-    to the most nodes of ``host_meta``, and any context that the page table holds.
+    to the most nodes of ``host_meta``, and any context that the page table holds. What ``host_meta``'s contexts do not
+    cut (up to :data:`UNCUT` tiles) stays so, and an item of a far longer context is then one CTA's: plan a capture with
+    the longest contexts that it will see.
 
     A row that sees no key is zero; rows of no sequence are left as they are. What a masked key or value holds does not
     reach the row, an infinity or a NaN neither; where a node's value is not finite, rows that see it get it in that
     dim. Weights are rounded to bf16 for the product with V, as in the prompt attention. To the status word: more nodes
-    than fit (the first are computed), a context beyond the page table's places (cut there), a ``bt_rows`` entry that
-    is no row of the table (its rows are zero). A page id outside the cache reads as zeros."""
+    than fit (the first are computed), a context beyond the page table's places (cut there: the keys that it has are
+    seen as in the whole context), a ``bt_rows`` entry that is no row of the table (its rows are zero). A page id
+    outside the cache reads as zeros."""
     _check_heads(hq, hkv, 16)
     n, T, dev = q_len.shape[0], q.shape[0], q.get_device()
     ldq = _check_rows("q", q, T, hq * HEAD_DIM, dev, 16)
