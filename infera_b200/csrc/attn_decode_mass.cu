@@ -48,6 +48,7 @@ namespace dmass {
 using kv8::elect_one;
 using kv8::known_pages;
 using kv8::max_over_warp;
+using kv8::scaled;
 using kv8::table_row;
 using kv8::umma_bf16_if;
 using kv8::umma_commit_if;
@@ -75,6 +76,7 @@ constexpr int FIN_KEYS = 1024;       // keys of a block of the second kernel
 struct Params {
   const __nv_bfloat16* q;
   int ldq;
+  const __nv_bfloat16* v;
   int num_pages;
   const int* block_table;
   const int* bt_rows;
@@ -204,10 +206,10 @@ __device__ __forceinline__ void merge_parts(const Params& p, int b, int kvh, con
       if (m == -INFINITY) continue;  // a share without keys wrote nothing
       const float w = exp2f(m - s_m[h]);
       const float4 o = __ldcg(reinterpret_cast<const float4*>(p.o_part + (base + s) * D + d));
-      a[0] += o.x * w;
-      a[1] += o.y * w;
-      a[2] += o.z * w;
-      a[3] += o.w * w;
+      a[0] += scaled(o.x, w);
+      a[1] += scaled(o.y, w);
+      a[2] += scaled(o.z, w);
+      a[3] += scaled(o.w, w);
     }
     const float inv = s_inv[h];
     uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(b) * p.ldo + (kvh * p.G + h) * D + d);
@@ -282,6 +284,28 @@ __device__ __forceinline__ void end_share(const Params& p, const Seq& sq, int b,
   make_sums<NUM_THREADS>(p, b, kvh, s_m, s_inv);
   __syncthreads();
   add_mass<GP, NUM_THREADS>(p, sq, b, kvh, 0, sq.len, s_m, s_inv);
+}
+
+// The sum of what is not finite in one column (`v`, in a page's first row) of the values of keys k_lo .. k_hi: an
+// infinity, a NaN, or 0. An infinity times two digits of different sign, or one of 0, is a NaN in the product. Rare, so
+// nothing here is tuned.
+__device__ __noinline__ float values_not_finite(const __nv_bfloat16* v, int width, int num_pages, const int* bt, int k_lo,
+                                                int k_hi) {
+  float sum = 0.f;
+  for (int k0 = k_lo; k0 < k_hi && !isnan(sum); k0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + i, page = k < k_hi ? bt[k / PAGE] : -1;
+      x[i] = static_cast<unsigned>(page) >= static_cast<unsigned>(num_pages)
+                 ? 0.f
+                 : __bfloat162float(v[(static_cast<size_t>(page) * PAGE + k % PAGE) * width]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(fabsf(x[i]) <= FLT_MAX)) sum += x[i];
+  }
+  return sum;
 }
 
 template <int GP>  // query heads per KV head, rounded up to 1, 2, 4 or 8
@@ -587,11 +611,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
       if (lane == 0) red[q4 * GP + h] = v;
     }
     barrier_or(false);
+    float wild = 0.f;  // (every head sees every key)
+    bool odd = false;
+#pragma unroll
+    for (int h = 0; h < GP; ++h) {
+      const float o = __uint_as_float(ov[h]) + __uint_as_float(ov[GP + h]);
+      odd = odd || (h < G && isnan(o) && !isnan(red[h] + red[GP + h] + red[2 * GP + h] + red[3 * GP + h]));
+    }
+    if (odd && ok) wild = values_not_finite(p.v + kvh * D + r, p.hkv * D, p.num_pages, sq.bt, t0 * BKV, min(len, t1 * BKV));
 #pragma unroll
     for (int h = 0; h < GP; ++h) {
       if (h >= G || !ok) break;
       const float l = red[h] + red[GP + h] + red[2 * GP + h] + red[3 * GP + h];
-      const float o = __uint_as_float(ov[h]) + __uint_as_float(ov[GP + h]);
+      float o = __uint_as_float(ov[h]) + __uint_as_float(ov[GP + h]);
+      if (wild != 0.f) o = wild;
       const int head = kvh * G + h;
       const size_t slot = (static_cast<size_t>(b) * p.hq + head) * p.splits + split;
       if (r == 0) p.ml[slot] = make_float2(l == 0.f ? -INFINITY : m_run[h], l);
@@ -693,6 +726,7 @@ extern "C" int ib_attn_decode_mass(const void* q, int ldq, const void* k_cache, 
     Params p;
     p.q = static_cast<const __nv_bfloat16*>(q);
     p.ldq = ldq;
+    p.v = static_cast<const __nv_bfloat16*>(v_cache);
     p.num_pages = static_cast<int>(num_slots / PAGE);
     p.block_table = block_table;
     p.bt_rows = bt_rows;

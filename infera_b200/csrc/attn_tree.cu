@@ -67,6 +67,7 @@ namespace atree {
 
 using kv8::elect_one;
 using kv8::mbar_expect_tx_if;
+using kv8::scaled;
 using kv8::tma_load_2d_if;
 using kv8::umma_bf16_if;
 using kv8::umma_commit_if;
@@ -713,9 +714,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 // LANES lanes a row, which have 4 dims of each 4 LANES, and W warps that share a row's pieces. With two pieces a
 // row most instructions are the row's, not the pieces', so 8 lanes take a row, and a warp four (65536 rows of 16
 // sequences, 64 nodes, 64 heads: 12 us from cold caches; a warp a row 22).
-__device__ __forceinline__ float scaled(float x, float w) {  // w x, w >= 0; an infinity or a NaN stays one where w is 0
-  return fabsf(x) <= FLT_MAX ? x * w : x;
-}
 template <int LANES, int W>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Params p) {
   constexpr int V = 32 / LANES;              // float4s a lane

@@ -1,7 +1,7 @@
 // What the kernels of the 8-bit KV cache share: e4m3 conversions, powers of
 // two, the exponents of pages, and the merge of key shares. The attention
 // kernels of the bf16 cache that came after them use the tcgen05 issue, the
-// page checks and the reductions too.
+// page checks, the reductions and scaled() too.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -48,6 +48,9 @@ __device__ __forceinline__ float max_over_warp(float x) {  // a NaN counts as no
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
 }
+
+// w x for a weight w; what is not finite stays so where w is 0
+__device__ __forceinline__ float scaled(float x, float w) { return fabsf(x) <= FLT_MAX ? x * w : x; }
 
 // ---- tcgen05 issue by a whole warp
 // The MMA warp runs its loop with all lanes and issues under the elected

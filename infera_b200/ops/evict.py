@@ -74,7 +74,7 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     the page table's places (cut there) or beyond ``mass``'s (no weights are added there), a ``bt_rows`` entry that is
     no row of the table (the sequence gets zeros) or of ``mass``, or that an earlier sequence has (both: no weights are
     added). Sequences of length 0 may share a row with others before them: so a batch is padded. A page id outside the
-    cache reads as zeros."""
+    cache reads as zeros. An infinity among a sequence's values is the output's in its dim."""
     _check_heads(hq, hkv, 8)
     B, dev = seq_lens.shape[0], q.get_device()
     ldq = _check_rows("q", q, B, hq * HEAD_DIM, dev, 4)

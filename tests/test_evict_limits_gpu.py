@@ -150,3 +150,31 @@ def test_a_padded_batch():
             assert torch.all(got[row, h, 60:n] == 0)
             want_k, want_v = (O.moved(x, table[row], on, 0, 128, 128 * h) for x in (want_k, want_v))
     assert torch.equal(dev[1].cpu(), want_k) and torch.equal(dev[2].cpu(), want_v)
+
+
+@pytest.mark.parametrize("hq", [1, 2, 4, 8, 3])
+def test_infinite_values(hq):
+    """An infinity among the values is the output's, of both signs a NaN, whatever the weight's digits are."""
+    lens = [700, 300, 129]
+    q, k, v, table, mass = batch(lens, hq, 1, 8)
+    slot = lambda s, p: int(table[s, p // 16]) * 16 + p % 16  # noqa: E731
+    inf = float("inf")
+    for s, p, d, x in ((0, 3, 5, inf), (0, 650, 5, inf), (0, 130, 7, -inf), (0, 131, 9, inf), (0, 500, 9, -inf), (0, 699, 127, inf),
+                       (1, 0, 0, -inf), (1, 299, 64, inf), (1, 150, 65, float("nan")), (2, 128, 66, inf), (2, 5, 67, 3e38)):
+        v[slot(s, p), d] = x
+    for splits, tps in ((1, 0), (2, 0), (6, 1)):
+        got = mass.cuda()
+        out = evict.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lens), hq, 1, SCALE, got, splits,
+                                tiles_per_split=tps)
+        check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, 1)
+    # a share far below the others in weight
+    for p in range(600, 700):
+        k[slot(0, p), 0] = 300
+    for h in range(hq):
+        q[:, 128 * h] = 8
+    for splits, tps in ((1, 0), (2, 0), (6, 1)):
+        got = mass.cuda()
+        out = evict.attn_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lens), hq, 1, SCALE, got, splits,
+                                tiles_per_split=tps)
+        check(out.cpu(), got.cpu(), q, k, v, table, mass, lens, hq, 1)
+    assert status()["code"] == 0
