@@ -775,7 +775,7 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     :func:`infera_b200.ops.evict.select_keys` keeps); [n, m]: whole rows (the
     path of :func:`infera_b200.ops.tree.tree_accept`). ``start`` None: 0.
 
-    An entry is at least its index; -1 moves nothing. Rows move as if all were
+    ``count`` above m counts as m. An entry is at least its index; -1 moves nothing. Rows move as if all were
     read before the first is written. A sequence's pages have to be its own:
     what else reads them (a shared prefix) sees the moved rows. To the status
     word, and not moved: another entry below its index, one beyond the page

@@ -149,7 +149,8 @@ def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
 
     A row that sees no key is zero; rows of no sequence are left as they are. What a masked key or value holds does not
     reach the row, an infinity or a NaN neither; where a node's value is not finite, rows that see it get it in that
-    dim. Weights are rounded to bf16 for the product with V, as in the prompt attention. To the status word: more nodes
+    dim. (An infinity before the nodes makes the rows that dim's infinity, or a NaN where its weight is 0 in bf16.)
+    Weights are rounded to bf16 for the product with V, as in the prompt attention. To the status word: more nodes
     than fit (the first are computed), a context beyond the page table's places (cut there: the keys that it has are
     seen as in the whole context), a ``bt_rows`` entry that is no row of the table (its rows are zero). A page id
     outside the cache reads as zeros."""
