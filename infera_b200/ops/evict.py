@@ -128,7 +128,8 @@ def _attn_decode_cpu(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, scale,
         kb, vb = (paged.cpu_keys(x, bt[b], n, hkv) for x in (k, v))
         s = q[b, : hq * HEAD_DIM].float().view(hkv, -1, HEAD_DIM) @ kb.transpose(1, 2) * scale
         w = torch.softmax(s, -1)
-        y[b] = (w @ vb).flatten()
+        wild = ~vb.isfinite()  # (reaches the row, and not by a weight of zero)
+        y[b] = (w @ vb.masked_fill(wild, 0.0) + torch.where(wild, vb, 0.0).sum(1, keepdim=True)).flatten()
         if rows[b] < mass.shape[0] and rows[b] not in rows[:b]:
             cut = min(n, mass.shape[2])
             mass[rows[b], :, :cut] += w.sum(1)[:, :cut]

@@ -775,13 +775,14 @@ def kv_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.
     :func:`infera_b200.ops.evict.select_keys` keeps); [n, m]: whole rows (the
     path of :func:`infera_b200.ops.tree.tree_accept`). ``start`` None: 0.
 
-    ``count`` above m counts as m. An entry is at least its index; -1 moves nothing. Rows move as if all were
-    read before the first is written. A sequence's pages have to be its own:
-    what else reads them (a shared prefix) sees the moved rows. To the status
-    word, and not moved: another entry below its index, one beyond the page
-    table's places, a page id outside the cache; a ``bt_rows`` entry that is no
-    row of the table, or that an earlier sequence has (whether or not that one's
-    rows move) while this one's ``count`` is not 0; a negative ``start``."""
+    An entry is at least its index; -1 moves nothing; ``count`` above m counts
+    as m. Rows move as if all were read before the first is written. A
+    sequence's pages have to be its own: what else reads them (a shared prefix)
+    sees the moved rows. To the status word, and not moved: another entry below
+    its index, one beyond the page table's places, a page id outside the cache;
+    a ``bt_rows`` entry that is no row of the table, or that an earlier sequence
+    has (whether or not that one's rows move) while this one's ``count`` is not
+    0; a negative ``start``."""
     from infera_b200.ops import paged
 
     paged.kv_compact(k_cache, v_cache, block_table, src, count, start, bt_rows)
